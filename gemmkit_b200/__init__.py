@@ -27,7 +27,7 @@ __all__ = [
     "gemm_i8_packed_b_requant", "gemm_i8_requant_batched", "gemm_i8_requant_batched_ptr",
     "gemm_half_f32", "gemm_bf16_f32_unchecked", "gemm_f16_f32_unchecked",
     "gemm_half_f32_batched", "gemm_half_f32_fused", "gemm_i8_fused", "gemm_i8_fused_unchecked", "Activation", "quantize_f32_i8", "gemm_i8_noalloc_unchecked", "set_tile_n", "knob_names", "knob_get",
-    "knob_set", "device_status", "selftest_wait_timeout",
+    "gemm_half_grouped", "gemm_half_grouped_wgrad", "knob_set", "device_status", "selftest_wait_timeout",
 ]
 
 
@@ -511,6 +511,90 @@ def gemm_half_f32_batched(is_f16, batch, m, k, n, alpha, a, rsa, csa, a_bs, b, r
     _check(_lib.load().gk_gemm_half_f32_batched_unchecked(
         _ws(ws), int(is_f16), batch, m, k, n, alpha, a, rsa, csa, a_bs, b, rsb, csb, b_bs, beta,
         c, rsc, csc, c_bs, par.c(), _stream(stream)))
+
+
+# ---- products of rows grouped by expert ------------------------------------------------------
+
+def _elem_type(data, default: int) -> int:
+    """The C ABI's element type of a tensor (``default`` for a (pointer, length) pair, or for the
+    int16 / uint16 tensors that carry 16-bit floats)."""
+    if isinstance(data, tuple):
+        return default
+    name = str(data.dtype)
+    types = {"torch.float32": _lib.DT_F32, "torch.float16": _lib.DT_F16,
+             "torch.bfloat16": _lib.DT_BF16, "torch.int16": default, "torch.uint16": default}
+    if name not in types:
+        raise GemmkitError(GK_EINVAL, f"gemmkit: elements of type {name} are not supported here")
+    return types[name]
+
+
+def _same_device(**tensors) -> None:
+    """The engine launches on the current device: refuse tensors that lie elsewhere."""
+    import torch
+    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for name, t in tensors.items():
+        if t is None or isinstance(t, tuple):
+            continue
+        if not t.is_cuda:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: {name} is not in device memory")
+        if t.device.index != cur:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: {name} is on cuda:{t.device.index}, the "
+                                          f"current device is cuda:{cur}")
+
+
+def _offsets(offsets):
+    """(pointer, groups) of an int32 offsets tensor or a (pointer, groups + 1) pair."""
+    if isinstance(offsets, tuple):
+        return int(offsets[0]), int(offsets[1]) - 1
+    if str(offsets.dtype) != "torch.int32" or offsets.dim() != 1 or not offsets.is_contiguous():
+        raise GemmkitError(GK_EINVAL, "gemmkit: offsets must be a contiguous 1-D int32 tensor")
+    return int(offsets.data_ptr()), int(offsets.numel()) - 1
+
+
+def _grouped_args(a, b, offsets, c, is_f16):
+    half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
+    _same_device(A=a.data, B=b.data, C=c.data, offsets=offsets)
+    for name, d in (("A", a.data), ("B", b.data)):
+        if _elem_type(d, half) != half:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold "
+                                          f"{'f16' if is_f16 else 'bf16'} elements")
+    ptr, groups = _offsets(offsets)
+    if groups < 0:
+        groups = 0
+    return ptr, groups, _elem_type(c.data, half)
+
+
+def gemm_half_grouped(alpha: float, a: MatRef, b: MatRef, b_gs: int, offsets, beta: float,
+                      c: MatMut, is_f16=False, par: Parallelism = SERIAL, stream=None,
+                      sync: bool = True) -> None:
+    """The experts' products (extension): C[i, :] <- alpha*A[i, :]*B[g] + beta*C[i, :] for the rows
+    offsets[g] <= i < offsets[g + 1]. A (rows x k) holds bf16 (f16 with is_f16), `b` views group 0's
+    k x n matrix inside a slice that holds all groups at stride b_gs (elements, 0 = shared);
+    `offsets` is an int32 device tensor of groups + 1 entries that the host never reads. C holds
+    f32 or the operands' type, by its tensor's dtype (16-bit for a (pointer, length) pair). Rows
+    outside the groups are left as they are. With C's gradient as A and B viewed transposed the
+    same call is the gradient of A."""
+    ptr, groups, out = _grouped_args(a, b, offsets, c, is_f16)
+    _check(_lib.load().gk_gemm_half_grouped(int(is_f16), groups, ptr, float(alpha), a.c(), b.c(),
+                                            int(b_gs), float(beta), c.c(), out, par.c(),
+                                            _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+def gemm_half_grouped_wgrad(alpha: float, a: MatRef, b: MatRef, offsets, beta: float, c: MatMut,
+                            c_gs: int, is_f16=False, par: Parallelism = SERIAL, stream=None,
+                            sync: bool = True) -> None:
+    """The experts' weight gradients (extension): C[g] <- alpha*A_g^T*B_g + beta*C[g] with A (rows x
+    m) and B (rows x n) grouped by `offsets` as in gemm_half_grouped; `c` views group 0's m x n
+    matrix inside a slice that holds all groups at stride c_gs. An empty group's C[g] becomes
+    beta*C[g]."""
+    ptr, groups, out = _grouped_args(a, b, offsets, c, is_f16)
+    _check(_lib.load().gk_gemm_half_grouped_wgrad(int(is_f16), groups, ptr, float(alpha), a.c(),
+                                                  b.c(), float(beta), c.c(), int(c_gs), out,
+                                                  par.c(), _stream(stream)))
+    if sync:
+        _sync(stream)
 
 
 # ---- i8 -> i32 without allocation ---------------------------------------------------------

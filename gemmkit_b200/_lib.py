@@ -13,6 +13,7 @@ from . import _build
 GK_OK, GK_EINVAL, GK_ENOMEM, GK_ECUDA, GK_ETIMEOUT, GK_ENODEV = range(6)
 AXIS_NONE, AXIS_ROW, AXIS_COL = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 sz, pd, vp, i32, u32, f32 = C.c_size_t, C.c_ssize_t, C.c_void_p, C.c_int32, C.c_uint32, C.c_float
 
@@ -115,6 +116,10 @@ SIGNATURES = {
     "gk_gemm_i8_fused": (i32, [vp, i32, MatRefC, MatRefC, i32, MatMutC, vp, sz, C.c_int, C.c_int,
                                Parallelism, vp]),
     "gk_quantize_f32_i8_unchecked": (i32, [sz, sz, vp, pd, pd, vp, pd, pd, f32, i32, vp, vp]),
+    "gk_gemm_half_grouped": (i32, [C.c_int, sz, vp, f32, MatRefC, MatRefC, pd, f32, MatMutC,
+                                   C.c_int, Parallelism, vp]),
+    "gk_gemm_half_grouped_wgrad": (i32, [C.c_int, sz, vp, f32, MatRefC, MatRefC, f32, MatMutC, pd,
+                                         C.c_int, Parallelism, vp]),
     "gk_set_tile_n": (i32, [C.c_int]),
     "gk_knob_names": (C.c_char_p, []),
     "gk_knob_get": (i32, [C.c_char_p, C.POINTER(C.c_int64)]),

@@ -657,6 +657,31 @@ int check_scale_value(float s) {
 namespace gk {
 // Records `text` as this thread's gk_last_error() message (for entries in other files).
 int set_last_error(int code, const char* text) { return set_err(code, "%s", text); }
+
+// The checks and settings of this file for the entries of other files.
+int api_err(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int api_check_device(int* dev) { return check_device(dev); }
+int api_check_view(size_t len, size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs,
+                   const char* name) {
+    return check_view(len, rows, cols, rs, cs, name);
+}
+int api_validate_gemm_views(const gk_matref& a, const gk_matref& b, const gk_matmut& c, size_t si,
+                            size_t so) {
+    return validate_gemm_views(a, b, c, si, so);
+}
+bool api_self_aliases(size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs) {
+    return self_aliases(rows, cols, rs, cs);
+}
+bool api_overlaps(const void* pa, size_t bytes_a, const void* pb, size_t bytes_b) {
+    return overlaps_bytes(pa, bytes_a, 1, pb, bytes_b, 1);
+}
+int api_pdl_enabled() { return pdl_enabled() ? 1 : 0; }
 }  // namespace gk
 
 // ==========================================================================================

@@ -12,6 +12,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "gemmkit_cuda.h"
+
 namespace gk {
 
 enum class Kind : int { I8 = 0, F16 = 1, BF16 = 2 };
@@ -198,5 +200,16 @@ int launch_quantize_rows(const float* x, int64_t rsx, int64_t csx, int64_t rows,
 
 // Sets this thread's gk_last_error() text (gk_api.cu); returns `code`.
 int set_last_error(int code, const char* text);
+
+// The C ABI's checks and settings (gk_api.cu) for entries that live in other files.
+int api_err(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int api_check_device(int* dev);
+int api_check_view(size_t len, size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs,
+                   const char* name);
+int api_validate_gemm_views(const gk_matref& a, const gk_matref& b, const gk_matmut& c, size_t si,
+                            size_t so);
+bool api_self_aliases(size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs);
+bool api_overlaps(const void* pa, size_t bytes_a, const void* pb, size_t bytes_b);
+int api_pdl_enabled();
 
 }  // namespace gk

@@ -1,0 +1,511 @@
+// gk_grouped.cu -- bf16 / f16 products of rows grouped by expert, forward and both gradients.
+//
+//   forward / input gradient   C[i, :] = alpha A[i, :] B[g] + beta C[i, :],  off[g] <= i < off[g+1]
+//   weight gradient            C[g]    = alpha A_g^T B_g + beta C[g]         (contraction over rows)
+//
+// Both are lowered to D[i, j] = sum_p P[i, p] Q[j, p] per group: P on the 128 TMEM lanes, Q on
+// the MMA's N. P is always the side along C's columns (the weights' n, or B's columns), so a
+// warp stores 32 consecutive elements of a row of C per instruction; Q is the ragged side of the
+// forward product (the rows of A), so a group's last tile runs with N rounded up to 16 of its
+// rows instead of a whole tile of rows.
+//
+// One persistent kernel: warp 1 issues tcgen05.mma kind::f16 (M = 128, N <= BN, f32
+// accumulators, two TMEM buffers), the epilogue warps drain one accumulator while the next tile
+// is computed, and the loader warps fill a ring of shared-memory stages of 64 contraction
+// elements in the 128-byte swizzle. The tile schedule is computed on the device from the offsets
+// (gk_group.cuh), so the host never waits for them.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "gemmkit_cuda.h"
+#include "gk_engine.h"
+#include "gk_group.cuh"
+#include "gk_sm100.cuh"
+#include "gk_tc_common.cuh"
+
+namespace gk {
+
+namespace {
+
+constexpr int GBK = 64;  // contraction elements per stage (one 128-byte swizzle row)
+
+// An operand as the loaders read it: element (row r, contraction index p) of group g at
+// ptr + g * gs + r * rs + p * ps.
+struct GOperand {
+    const uint16_t* ptr;
+    int64_t rs, ps, gs;
+};
+
+struct GroupedParams {
+    GOperand P, Q;
+    int64_t np;               // rows of the P side (columns of C)
+    int64_t nq;               // weight gradient: rows of the Q side; else unused
+    int32_t kdim;             // forward: contraction length
+    int32_t wgrad;            // 1: the contraction is ragged
+    int32_t zero;             // 1: no product (k == 0 or alpha == 0): C <- beta C
+    int32_t groups, rows, tiles_p, tiles_q;  // tiles_q: weight gradient only
+    const int32_t* offsets;
+    void* c;
+    int64_t ldq, ldp, gsc;    // strides of C along the Q side, the P side and the groups
+    float alpha, beta;
+    int32_t f16;              // operands are f16 (else bf16)
+    int32_t out_f32;
+    uint64_t timeout_ns;
+    unsigned int* status;
+};
+
+template <int BN>
+struct GroupedCfg {
+    static constexpr int NEPI = BN >= 64 ? 8 : 4;
+    static constexpr int NLOAD = 8;
+    static constexpr int EPI_W0 = 4;
+    static constexpr int LOAD_W0 = EPI_W0 + NEPI;
+    static constexpr int THREADS = 32 * (LOAD_W0 + NLOAD);
+    static constexpr int WCOLS = BN / (NEPI / 4);
+    static constexpr int P_BYTES = BM * BKB;
+    static constexpr int Q_BYTES = BN * BKB;
+    static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
+    static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
+    static constexpr int BAR_BYTES = 256;
+    static constexpr int RAW_STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    static constexpr int STAGES = RAW_STAGES > 10 ? 10 : RAW_STAGES;
+    static constexpr int OFF_BARS = STAGES * STAGE_BYTES;
+    static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
+    static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
+    static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static_assert(BN == 32 || BN == 64 || BN == 128 || BN == 256, "tile width");
+    static_assert(STAGES >= 2 && SMEM <= SMEM_LIMIT, "shared memory budget");
+    static_assert((2 * STAGES + 7) * 8 <= BAR_BYTES, "barrier area");
+};
+
+// One tile of the schedule as every role sees it.
+struct GTile {
+    int g, p0, q0;        // group, first row on the P and Q sides (inside the group)
+    int qn;               // rows of the Q side left from q0
+    int64_t qbase;        // first row of the Q operand / of C along the Q side
+    int k0, nk;           // first contraction row (weight gradient) and contraction length
+};
+
+template <int BN>
+__device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, GTile& t) {
+    int tp, tq;
+    if (!w.next(p.tiles_p, tp, tq)) return false;
+    t.g = w.g;
+    t.p0 = tp * BM;
+    t.q0 = tq * BN;
+    const int o0 = w.off[t.g], m = w.off[t.g + 1] - o0;
+    if (p.wgrad) {
+        t.qn = static_cast<int>(p.nq) - t.q0;
+        t.qbase = t.q0;
+        t.k0 = o0;
+        t.nk = p.zero ? 0 : m;
+    } else {
+        t.qn = m - t.q0;
+        t.qbase = static_cast<int64_t>(o0) + t.q0;
+        t.k0 = 0;
+        t.nk = p.zero ? 0 : p.kdim;
+    }
+    return true;
+}
+
+// Gathers rows [r0, r0 + R) x contraction [k0, k0 + 64) of an operand with any strides into a
+// K-major 128-byte-swizzled stage (16-byte piece j of row r at piece j ^ (r mod 8)); rows at or
+// past `nr` and contraction indices at or past `nk` are zero. `t` of `nt` threads.
+template <int R>
+__device__ __forceinline__ void gather_stage(uint8_t* dst, const uint16_t* src, int64_t rs,
+                                             int64_t ps, int nr, int nk, int t, int nt) {
+    const bool kfast = ps == 1;  // neighbouring threads read neighbouring addresses
+    for (int i = t; i < R * 8; i += nt) {
+        const int r = kfast ? i >> 3 : i % R;
+        const int j = kfast ? i & 7 : i / R;
+        uint16_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = j * 8 + e;
+            v[e] = (r < nr && k < nk) ? __ldg(src + r * rs + k * ps) : static_cast<uint16_t>(0);
+        }
+        uint4 q;
+        q.x = v[0] | (static_cast<uint32_t>(v[1]) << 16);
+        q.y = v[2] | (static_cast<uint32_t>(v[3]) << 16);
+        q.z = v[4] | (static_cast<uint32_t>(v[5]) << 16);
+        q.w = v[6] | (static_cast<uint32_t>(v[7]) << 16);
+        *reinterpret_cast<uint4*>(dst + r * 128 + ((j ^ (r & 7)) << 4)) = q;
+    }
+}
+
+// alpha * acc + beta * C of one element, rounded once to the output type.
+__device__ __forceinline__ void store_elem(const GroupedParams& p, int64_t at, float acc) {
+    float v = p.alpha * acc;
+    if (p.out_f32) {
+        float* c = static_cast<float*>(p.c) + at;
+        if (p.beta != 0.0f) v = fmaf(p.beta, *c, v);
+        *c = v;
+    } else if (p.f16) {
+        __half* c = static_cast<__half*>(p.c) + at;
+        if (p.beta != 0.0f) v = fmaf(p.beta, __half2float(*c), v);
+        *c = __float2half_rn(v);
+    } else {
+        __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c) + at;
+        if (p.beta != 0.0f) v = fmaf(p.beta, __bfloat162float(*c), v);
+        *c = __float2bfloat16_rn(v);
+    }
+}
+
+template <int BN>
+__global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
+    grouped_half_kernel(const GroupedParams p) {
+    using C = GroupedCfg<BN>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sP = smem;
+    uint8_t* sQ = smem + STAGES * C::P_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
+    int* tile0 = off + GROUP_TABLE_INTS;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t tmo = p.timeout_ns;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], C::NLOAD);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], C::NEPI);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    griddep_wait();  // the offsets, operands and C may belong to the previous kernel
+    load_groups(p.offsets, p.groups, p.rows, off, tile0, blockIdx.x == 0 ? p.status : nullptr,
+                [&](int m) {
+                    return p.wgrad ? p.tiles_p * p.tiles_q : (m + BN - 1) / BN * p.tiles_p;
+                });
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    GroupWalk walk(off, tile0, p.groups, blockIdx.x, gridDim.x);
+    GTile t;
+
+    if (warp >= C::LOAD_W0) {
+        // ---------------- loaders: any strides, one stage at a time ----------------
+        const int lt = threadIdx.x - 32 * C::LOAD_W0;
+        constexpr int NT = 32 * C::NLOAD;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        while (ok && next_tile<BN>(walk, p, t)) {
+            // the Q side's rows are absolute (ragged) in the forward product; the contraction
+            // starts at the group's first row in the weight gradient
+            const uint16_t* ps = p.P.ptr + t.g * p.P.gs + t.p0 * p.P.rs +
+                                 static_cast<int64_t>(t.k0) * p.P.ps;
+            const uint16_t* qs = p.Q.ptr + t.qbase * p.Q.rs + static_cast<int64_t>(t.k0) * p.Q.ps;
+            const int pn = static_cast<int>(min(static_cast<int64_t>(BM), p.np - t.p0));
+            const int qn = min(BN, t.qn);
+            for (int kb = 0; kb < t.nk; kb += GBK) {
+                if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                    ok = false;
+                    break;
+                }
+                gather_stage<BM>(sP + stage * C::P_BYTES, ps + kb * p.P.ps, p.P.rs, p.P.ps, pn,
+                                 t.nk - kb, lt, NT);
+                gather_stage<BN>(sQ + stage * C::Q_BYTES, qs + kb * p.Q.ps, p.Q.rs, p.Q.ps, qn,
+                                 t.nk - kb, lt, NT);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[stage]);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer ----------------
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int local = 0; ok && next_tile<BN>(walk, p, t); ++local) {
+                const int acc = local & 1;
+                const uint32_t aph = (local >> 1) & 1;
+                if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                               tmo))
+                    break;
+                tc_fence_after();
+                const uint32_t idesc =
+                    idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0);
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                for (int kb = 0; kb < t.nk; kb += GBK) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                                   tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
+                    const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
+#pragma unroll
+                    for (int ks = 0; ks < BKB / MMA_KB; ++ks)
+                        mma_f16(d, sdesc_kmajor_sw128(a0 + ks * MMA_KB),
+                                sdesc_kmajor_sw128(b0 + ks * MMA_KB), idesc,
+                                (kb | ks) != 0 ? 1u : 0u);
+                    mma_commit(&empty[stage]);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit(&tfull[acc]);
+            }
+            mma_commit(drain);  // every issued MMA has finished before TMEM is freed
+            int dummy = 0;
+            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (warp >= C::EPI_W0) {
+        // ---------------- epilogue ----------------
+        const int q = warp & 3;
+        const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
+        for (int local = 0; next_tile<BN>(walk, p, t); ++local) {
+            const int acc = local & 1;
+            const uint32_t aph = (local >> 1) & 1;
+            if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
+                break;
+            tc_fence_after();
+            const int i = t.p0 + q * 32 + lane;
+            const bool row_ok = i < p.np;
+            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i * p.ldp;
+            const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                static_cast<uint32_t>(acc * BN + cbase);
+            for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
+                uint32_t v[32];
+                tmem_ld_x32(tb + c, v);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int j = cbase + c + e;
+                    if (row_ok && j < t.qn)
+                        store_elem(p, at + j * p.ldq,
+                                   t.nk > 0 ? __uint_as_float(v[e]) : 0.0f);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+}
+
+template <int BN>
+int launch_grouped(GroupedParams p, int grid, int pdl, cudaStream_t stream, char* err,
+                   size_t errlen) {
+    using C = GroupedCfg<BN>;
+    auto kern = grouped_half_kernel<BN>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(static_cast<unsigned>(grid));
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl ? 1 : 0;
+        e = cudaLaunchKernelEx(&cfg, kern, p);
+    }
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        snprintf(err, errlen, "gemmkit: grouped kernel launch failed: %s", cudaGetErrorString(e));
+        return GK_ECUDA;
+    }
+    return GK_OK;
+}
+
+// Tile width along the Q side. Forward: the mean rows of a group; a group's last tile costs only
+// its own rows on the tensor cores, so a wide tile loses little on short groups, but its stages
+// are larger and fewer fit.
+int grouped_bn(int64_t q) { return q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256; }
+
+int run_grouped(GroupedParams p, cudaStream_t stream) {
+    int dev = 0;
+    int rc = api_check_device(&dev);
+    if (rc) return rc;
+    const int64_t mean = (static_cast<int64_t>(p.rows) + p.groups - 1) / p.groups;
+    const int bn = grouped_bn(p.wgrad ? p.nq : mean);
+    const int64_t tp = (p.np + BM - 1) / BM;
+    // an upper bound of the tiles (the device computes the true number from the offsets)
+    const int64_t tq = p.wgrad ? (p.nq + bn - 1) / bn * p.groups
+                               : (static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups;
+    if (tp * tq > INT32_MAX / 2)
+        return set_last_error(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    p.tiles_p = static_cast<int>(tp);
+    p.tiles_q = static_cast<int>((p.nq + bn - 1) / bn);
+    p.timeout_ns = 4000000000ull;
+    p.status = device_status_ptr();
+    const int sms = sm_count();
+    const int grid = static_cast<int>(tp * tq < sms ? tp * tq : sms);
+    const int pdl = api_pdl_enabled();
+    char err[256] = "";
+    switch (bn) {
+        case 32: rc = launch_grouped<32>(p, grid, pdl, stream, err, sizeof(err)); break;
+        case 64: rc = launch_grouped<64>(p, grid, pdl, stream, err, sizeof(err)); break;
+        case 128: rc = launch_grouped<128>(p, grid, pdl, stream, err, sizeof(err)); break;
+        default: rc = launch_grouped<256>(p, grid, pdl, stream, err, sizeof(err)); break;
+    }
+    return rc ? set_last_error(rc, err) : GK_OK;
+}
+
+// The checks that both grouped entries share.
+int check_groups(size_t groups, const int32_t* offsets, size_t rows, int is_f16, int out_type) {
+    if (groups < 1 || groups > MAX_GROUPS)
+        return api_err(GK_EINVAL, "gemmkit: grouped products take 1 to %d groups (groups = %zu)",
+                       MAX_GROUPS, groups);
+    if (!offsets) return api_err(GK_EINVAL, "gemmkit: null offsets");
+    if (rows > INT32_MAX / 2)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    if (out_type != GK_F32 && out_type != (is_f16 ? GK_F16 : GK_BF16))
+        return api_err(GK_EINVAL, "gemmkit: a grouped product writes f32 or its operands' type");
+    return GK_OK;
+}
+
+// A stack of `groups` views at stride gs (elements): the slice must hold all of them.
+int check_stack(size_t len, size_t groups, size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs,
+                ptrdiff_t gs, const char* name) {
+    int rc = api_check_view(len, rows, cols, rs, cs, name);
+    if (rc) return rc;
+    if (gs < 0)
+        return api_err(GK_EINVAL, "gemmkit: %s group stride (%td) must not be negative", name, gs);
+    if (groups > 1 && rows && cols) {
+        const __int128 last = static_cast<__int128>(groups - 1) * gs + 1 +
+                              static_cast<__int128>(rows - 1) * rs +
+                              static_cast<__int128>(cols - 1) * cs;
+        if (last > static_cast<__int128>(len))
+            return api_err(GK_EINVAL,
+                           "gemmkit: %s stack of %zu views %zux%zu (strides %td,%td, group stride "
+                           "%td) does not fit its slice of %zu elements",
+                           name, groups, rows, cols, rs, cs, gs, len);
+    }
+    return GK_OK;
+}
+
+}  // namespace
+
+}  // namespace gk
+
+using namespace gk;
+
+extern "C" {
+
+int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t* offsets, float alpha,
+                         gk_matref a, gk_matref b, ptrdiff_t b_gs, float beta, gk_matmut c,
+                         int out_type, gk_parallelism par, gk_stream_t stream) {
+    (void)par;
+    int rc = check_groups(groups, offsets, a.rows, is_f16, out_type);
+    if (rc) return rc;
+    const size_t so = out_type == GK_F32 ? 4 : 2;
+    if ((rc = api_validate_gemm_views(a, b, c, 2, so))) return rc;
+    if ((rc = check_stack(b.len, groups, b.rows, b.cols, b.rs, b.cs, b_gs, "B"))) return rc;
+    if (a.cols > INT32_MAX / 2 || b.cols > INT32_MAX / 2)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    if (c.rows == 0 || c.cols == 0) return GK_OK;
+    if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    const bool zero = a.cols == 0 || alpha == 0.0f;
+    if (!zero && (!a.data || !b.data)) return api_err(GK_EINVAL, "gemmkit: null A or B");
+    GroupedParams p;
+    memset(&p, 0, sizeof(p));
+    p.P = GOperand{static_cast<const uint16_t*>(b.data), b.cs, b.rs, b_gs};
+    p.Q = GOperand{static_cast<const uint16_t*>(a.data), a.rs, a.cs, 0};
+    p.np = static_cast<int64_t>(b.cols);
+    p.kdim = static_cast<int32_t>(a.cols);
+    p.zero = zero;
+    p.groups = static_cast<int>(groups);
+    p.rows = static_cast<int>(a.rows);
+    p.offsets = offsets;
+    p.c = c.data;
+    p.ldq = c.rs;
+    p.ldp = c.cs;
+    p.alpha = alpha;
+    p.beta = beta;
+    p.f16 = is_f16 != 0;
+    p.out_f32 = out_type == GK_F32;
+    return run_grouped(p, static_cast<cudaStream_t>(stream));
+}
+
+int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t* offsets, float alpha,
+                               gk_matref a, gk_matref b, float beta, gk_matmut c, ptrdiff_t c_gs,
+                               int out_type, gk_parallelism par, gk_stream_t stream) {
+    (void)par;
+    int rc = check_groups(groups, offsets, a.rows, is_f16, out_type);
+    if (rc) return rc;
+    const size_t so = out_type == GK_F32 ? 4 : 2;
+    // A^T B in gemmkit's frame: (A.cols x rows) (rows x B.cols)
+    const gk_matref at{a.data, a.len, a.cols, a.rows, a.cs, a.rs};
+    if ((rc = api_validate_gemm_views(at, b, c, 2, so))) return rc;
+    const gk_matref cr{c.data, c.len, c.rows, c.cols, c.rs, c.cs};
+    if ((rc = check_stack(cr.len, groups, cr.rows, cr.cols, cr.rs, cr.cs, c_gs, "C"))) return rc;
+    if (a.cols > INT32_MAX / 2 || b.cols > INT32_MAX / 2)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    if (c.rows == 0 || c.cols == 0) return GK_OK;
+    if (groups > 1) {  // no element of one group's C may be an element of another's
+        size_t need = static_cast<size_t>((c.rows - 1) * c.rs + (c.cols - 1) * c.cs) + 1;
+        if (static_cast<size_t>(c_gs) < need)
+            return api_err(GK_EINVAL,
+                           "gemmkit: the groups of C overlap (group stride %td, a group spans %zu "
+                           "elements)",
+                           c_gs, need);
+    }
+    if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    const bool zero = a.rows == 0 || alpha == 0.0f;
+    if (!zero && (!a.data || !b.data)) return api_err(GK_EINVAL, "gemmkit: null A or B");
+    GroupedParams p;
+    memset(&p, 0, sizeof(p));
+    p.P = GOperand{static_cast<const uint16_t*>(b.data), b.cs, b.rs, 0};
+    p.Q = GOperand{static_cast<const uint16_t*>(a.data), a.cs, a.rs, 0};
+    p.np = static_cast<int64_t>(b.cols);
+    p.nq = static_cast<int64_t>(a.cols);
+    p.wgrad = 1;
+    p.zero = zero;
+    p.groups = static_cast<int>(groups);
+    p.rows = static_cast<int>(a.rows);
+    p.offsets = offsets;
+    p.c = c.data;
+    p.ldq = c.rs;
+    p.ldp = c.cs;
+    p.gsc = c_gs;
+    p.alpha = alpha;
+    p.beta = beta;
+    p.f16 = is_f16 != 0;
+    p.out_f32 = out_type == GK_F32;
+    return run_grouped(p, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

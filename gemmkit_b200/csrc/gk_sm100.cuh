@@ -16,6 +16,7 @@ enum : unsigned int {
     GK_DEV_TIMEOUT_EPILOGUE = 1u << 2,
     GK_DEV_TIMEOUT_DRAIN = 1u << 3,
     GK_DEV_TIMEOUT_SELFTEST = 1u << 4,
+    GK_DEV_BAD_OFFSETS = 1u << 5,  // a grouped call's offsets were not ascending inside the rows
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -97,8 +97,11 @@ typedef struct {
 const char *gk_version(void);
 /* Thread-local text of the last error returned by an entry on this thread. */
 const char *gk_last_error(void);
-/* Read (and with clear != 0 reset) the device status word of `device`: nonzero bits mean a
- * bounded in-kernel wait gave up (GK_ETIMEOUT). Synchronizes the device. */
+/* Read (and with clear != 0 reset) the device status word of `device`. GK_STATUS_OFFSETS means a
+ * grouped call's offsets did not ascend inside its rows (the call ran on the offsets made safe,
+ * see gk_gemm_half_grouped); any other bit that a bounded in-kernel wait gave up (GK_ETIMEOUT).
+ * Synchronizes the device. */
+#define GK_STATUS_OFFSETS (1u << 5)
 int gk_device_status(int device, int clear, uint32_t *status);
 
 int gk_workspace_create(gk_workspace **out);
@@ -305,6 +308,38 @@ int gk_gemm_i8_fused_unchecked(gk_workspace *ws, size_t m, size_t k, size_t n, i
 int gk_gemm_i8_fused(gk_workspace *ws, int32_t alpha, gk_matref a, gk_matref b, int32_t beta,
                      gk_matmut c, const int32_t *bias, size_t bias_len, int bias_dim, int act,
                      gk_parallelism par, gk_stream_t stream);
+
+/* ---- products of rows grouped by expert (no counterpart in gemmkit) -------------------- */
+
+/* Element types of the entries below. */
+typedef enum { GK_F32 = 0, GK_F16 = 1, GK_BF16 = 2 } gk_dtype;
+
+/* The experts' products of a mixture-of-experts layer: the rows of A and C are sorted by group
+ * (expert), group g being the rows offsets[g] <= i < offsets[g + 1], and
+ *   C[i, :] <- alpha * A[i, :] * B[g] + beta * C[i, :].
+ * `offsets` is a DEVICE array of groups + 1 int32 (1 <= groups <= 1024) that the host never reads,
+ * so a router may still be writing it on the same stream. It must ascend inside [0, A.rows];
+ * the kernels use its running maximum clamped to that range, so no offset reaches outside the
+ * buffers, and an array that had to be changed sets GK_STATUS_OFFSETS in the device status word.
+ * A group may be empty; rows of C before the first and past the last offset are left as they are.
+ * A (rows x k) and B (k x n, group g at + g * b_gs elements; b_gs == 0: one B for every group)
+ * are bf16, or f16 with is_f16; C is f32 or the operands' type (out_type), computed in f32 and
+ * rounded once. beta == 0 never reads C; k == 0 or alpha == 0 is C <- beta * C on the groups'
+ * rows and reads neither A nor B. Any non-negative strides; A with unit column stride and B with a
+ * unit row or column stride, 16-byte aligned with every other stride a multiple of 16 bytes,
+ * take the fast path. The gradient of A is the same call with C's gradient as A and B
+ * viewed transposed. Needs no workspace, allocates nothing and may be captured. */
+int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t *offsets, float alpha,
+                         gk_matref a, gk_matref b, ptrdiff_t b_gs, float beta, gk_matmut c,
+                         int out_type, gk_parallelism par, gk_stream_t stream);
+/* The weight gradient: C[g] <- alpha * A_g^T * B_g + beta * C[g] with A (rows x m) and B (rows x
+ * n) grouped as above, A_g the rows of group g, and C[g] (m x n) at + g * c_gs elements. The
+ * contraction runs over the group's rows; an empty group's C[g] becomes beta * C[g] (zeros when
+ * beta == 0). Rows of A and B outside the groups are never used, whatever they hold. The
+ * groups of C must not overlap. */
+int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t *offsets, float alpha,
+                               gk_matref a, gk_matref b, float beta, gk_matmut c, ptrdiff_t c_gs,
+                               int out_type, gk_parallelism par, gk_stream_t stream);
 
 /* ---- producer step: f32 activations -> i8 (no counterpart in gemmkit) ---------------- */
 

@@ -350,3 +350,47 @@ def test_gemv_entry_row_range():
     for m in (0, 65):
         expect_err(lambda: gk.gemv_i8_requant(m, 0, 1, 1, _NoPack(), req, 0, 1, 1),
                    "gemv takes 1 to 64 activation rows")
+
+
+def test_grouped_validation_without_gpu():
+    """The grouped entries' refusals, all before any device work."""
+    off = (4096, 3)
+    a = gk.MatRef.new((16, 12), 4, 3, 3, 1)
+    b = gk.MatRef.new((256, 30), 3, 5, 5, 1)
+    c = gk.MatMut.new((1024, 20), 4, 5, 5, 1)
+
+    def fwd(a=a, b=b, b_gs=15, offsets=off, c=c):
+        return lambda: gk.gemm_half_grouped(1.0, a, b, b_gs, offsets, 0.0, c)
+
+    expect_err(fwd(offsets=(4096, 1)), "1 to 1024 groups")
+    expect_err(fwd(offsets=(4096, 1026)), "1 to 1024 groups")
+    expect_err(fwd(offsets=(0, 3)), "null offsets")
+    expect_err(fwd(b_gs=16), "B stack of 2 views 3x5")
+    expect_err(fwd(b_gs=-1), "must not be negative")
+    expect_err(fwd(b=gk.MatRef.new((256, 40), 4, 5, 5, 1)), "A.cols (3) != B.rows (4)")
+    expect_err(fwd(c=gk.MatMut.new((1024, 19), 4, 5, 5, 1)), "C view of 4x5")
+    expect_err(fwd(c=gk.MatMut.new((1024, 20), 4, 5, 0, 1)), "aliases itself")
+    expect_err(fwd(c=gk.MatMut.new((20, 20), 4, 5, 5, 1)), "C aliases A or B")
+    expect_err(fwd(a=gk.MatRef.new((16, 12), 4, 3, -3, 1)), "negative strides")
+    expect_err(fwd(a=gk.MatRef.new((0, 12), 4, 3, 3, 1)), "null A or B")
+    lib = _lib.load()
+    args = (0, 2, C.c_void_p(4096), 1.0, a.c(), b.c(), 15, 0.0, c.c())
+    assert lib.gk_gemm_half_grouped(*args, 1, gk.SERIAL.c(), None) == gk.GK_EINVAL  # f16 C of bf16
+    assert b"f32 or its operands" in lib.gk_last_error()
+    assert lib.gk_gemm_half_grouped(*args, 7, gk.SERIAL.c(), None) == gk.GK_EINVAL
+    # empty outputs are accepted without a device
+    none = gk.MatMut.new((1024, 0), 4, 0, 5, 1)
+    gk.gemm_half_grouped(1.0, a, gk.MatRef.new((256, 30), 3, 0, 5, 1), 15, off, 0.0, none, sync=False)
+
+    x = gk.MatRef.new((16, 12), 4, 3, 3, 1)
+    y = gk.MatRef.new((256, 20), 4, 5, 5, 1)
+    w = gk.MatMut.new((1024, 30), 3, 5, 5, 1)
+
+    def wgrad(x=x, y=y, w=w, gs=15):
+        return lambda: gk.gemm_half_grouped_wgrad(1.0, x, y, off, 0.0, w, gs)
+
+    expect_err(wgrad(gs=14), "the groups of C overlap")
+    expect_err(wgrad(gs=0), "the groups of C overlap")
+    expect_err(wgrad(gs=16), "C stack of 2 views 3x5")
+    expect_err(wgrad(y=gk.MatRef.new((256, 25), 5, 5, 5, 1)), "A.cols (4) != B.rows (5)")
+    expect_err(wgrad(w=gk.MatMut.new((1024, 40), 4, 5, 5, 1)), "A.rows (3) != C.rows (4)")
