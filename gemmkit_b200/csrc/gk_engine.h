@@ -8,6 +8,7 @@
 // (gemmkit/src/dispatch.rs:395), so that the output's contiguous axis is j.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -161,6 +162,12 @@ int launch_tc_gemm_planned(const TcProblem& p, const TcPlan& plan, char* err, si
 // Launch the tcgen05 GEMM for `p` (all operands already TMA-compatible). Returns a GK_*
 // status and fills `err` on failure.
 int launch_tc_gemm(const TcProblem& p, char* err, size_t errlen);
+
+// A 3-D tensor map of 16-bit elements (dimension 0 contiguous, ld1 / ld2 the element strides of
+// dimensions 1 and 2), boxes of box0 x box1 elements in the 128-byte swizzle (box0 * 2 == 128).
+// Encoded on every call: nothing is kept by address. Returns a GK_* status and fills `err`.
+int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, int64_t d2,
+                    int64_t ld1, int64_t ld2, int box0, int box1, char* err, size_t errlen);
 
 // Device status word for the current device (bounded-wait give-ups are or-ed into it).
 unsigned int* device_status_ptr();

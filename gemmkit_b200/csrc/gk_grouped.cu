@@ -11,9 +11,17 @@
 //
 // One persistent kernel: warp 1 issues tcgen05.mma kind::f16 (M = 128, N <= BN, f32
 // accumulators, two TMEM buffers), the epilogue warps drain one accumulator while the next tile
-// is computed, and the loader warps fill a ring of shared-memory stages of 64 contraction
-// elements in the 128-byte swizzle. The tile schedule is computed on the device from the offsets
-// (gk_group.cuh), so the host never waits for them.
+// is computed, and a ring of shared-memory stages of 64 contraction elements in the 128-byte
+// swizzle is filled by TMA (one producer thread), or, for operands that TMA cannot address, by
+// eight loader warps that gather any strides. The tile schedule is computed on the device from
+// the offsets (gk_group.cuh), so the host never waits for them.
+//
+// Operands lie K-major (the contraction contiguous: rows of A, weights stored n x k) or MN-major
+// (weights stored k x n, both operands of the weight gradient); the MMA reads either from the
+// boxes as they land. In the weight gradient the contraction ends where the group ends, in the
+// middle of a stage: the stage's later MMAs are skipped, and warp 2 zeroes the rows between the
+// end and the next multiple of 16 in both operands (they belong to other groups and may hold
+// anything) before the MMA thread may read them.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -32,6 +40,23 @@ namespace gk {
 namespace {
 
 constexpr int GBK = 64;  // contraction elements per stage (one 128-byte swizzle row)
+// MN-major stages: boxes of 64 rows (128 bytes) x 64 contraction indices, one after the other
+// along the rows; an MMA reads 16 contraction indices = 16 lines of 128 bytes.
+constexpr int MN_BOX = GBK * 128;
+constexpr int MN_STEP = 16 * 128;
+
+// Shared-memory matrix descriptor of an MN-major operand in such boxes: 128-byte swizzle atoms of
+// 64 elements x 8 contraction indices; the next 64 elements are a box away (leading offset), the
+// next 8 contraction indices 1024 bytes (stride offset).
+__device__ __forceinline__ uint64_t sdesc_mn128(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(MN_BOX >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
 
 // An operand as the loaders read it: element (row r, contraction index p) of group g at
 // ptr + g * gs + r * rs + p * ps.
@@ -52,16 +77,18 @@ struct GroupedParams {
     void* c;
     int64_t ldq, ldp, gsc;    // strides of C along the Q side, the P side and the groups
     float alpha, beta;
+    int32_t p_mn, q_mn;       // TMA: the operand is MN-major
+    int32_t p_z;              // TMA: 1 = the P operand has a group dimension
     int32_t f16;              // operands are f16 (else bf16)
     int32_t out_f32;
     uint64_t timeout_ns;
     unsigned int* status;
 };
 
-template <int BN>
+template <int BN, bool TMA>
 struct GroupedCfg {
     static constexpr int NEPI = BN >= 64 ? 8 : 4;
-    static constexpr int NLOAD = 8;
+    static constexpr int NLOAD = TMA ? 0 : 8;
     static constexpr int EPI_W0 = 4;
     static constexpr int LOAD_W0 = EPI_W0 + NEPI;
     static constexpr int THREADS = 32 * (LOAD_W0 + NLOAD);
@@ -79,7 +106,7 @@ struct GroupedCfg {
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
     static_assert(BN == 32 || BN == 64 || BN == 128 || BN == 256, "tile width");
     static_assert(STAGES >= 2 && SMEM <= SMEM_LIMIT, "shared memory budget");
-    static_assert((2 * STAGES + 7) * 8 <= BAR_BYTES, "barrier area");
+    static_assert((2 * STAGES + 8) * 8 <= BAR_BYTES, "barrier area");
 };
 
 // One tile of the schedule as every role sees it.
@@ -137,28 +164,39 @@ __device__ __forceinline__ void gather_stage(uint8_t* dst, const uint16_t* src, 
     }
 }
 
-// alpha * acc + beta * C of one element, rounded once to the output type.
-__device__ __forceinline__ void store_elem(const GroupedParams& p, int64_t at, float acc) {
-    float v = p.alpha * acc;
-    if (p.out_f32) {
-        float* c = static_cast<float*>(p.c) + at;
-        if (p.beta != 0.0f) v = fmaf(p.beta, *c, v);
-        *c = v;
-    } else if (p.f16) {
-        __half* c = static_cast<__half*>(p.c) + at;
-        if (p.beta != 0.0f) v = fmaf(p.beta, __half2float(*c), v);
-        *c = __float2half_rn(v);
+__device__ __forceinline__ float from_out(float x) { return x; }
+__device__ __forceinline__ float from_out(__half x) { return __half2float(x); }
+__device__ __forceinline__ float from_out(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void to_out(float* p, float x) { *p = x; }
+__device__ __forceinline__ void to_out(__half* p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void to_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// One thread's 32 accumulators (its lane's P row, 32 consecutive Q rows, `n` of them in C):
+// alpha * acc + beta * C in f32, rounded once to the output type. A warp's stores of one Q row
+// are 32 consecutive elements when C's P stride is 1.
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* c, int64_t ldq, const uint32_t (&v)[32], int n,
+                                            float alpha, float beta) {
+    if (beta != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (e < n)
+                to_out(c + e * ldq, fmaf(beta, from_out(c[e * ldq]), alpha * __uint_as_float(v[e])));
+    } else if (n >= 32) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) to_out(c + e * ldq, alpha * __uint_as_float(v[e]));
     } else {
-        __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c) + at;
-        if (p.beta != 0.0f) v = fmaf(p.beta, __bfloat162float(*c), v);
-        *c = __float2bfloat16_rn(v);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (e < n) to_out(c + e * ldq, alpha * __uint_as_float(v[e]));
     }
 }
 
-template <int BN>
-__global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
-    grouped_half_kernel(const GroupedParams p) {
-    using C = GroupedCfg<BN>;
+template <int BN, bool TMA>
+__global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
+    grouped_half_kernel(const __grid_constant__ CUtensorMap tmP,
+                        const __grid_constant__ CUtensorMap tmQ, const GroupedParams p) {
+    using C = GroupedCfg<BN, TMA>;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -169,7 +207,9 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     uint64_t* tfull = empty + STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* fixreq = drain + 1;  // the stage holding a group's ragged end has landed
+    uint64_t* fixdone = drain + 2; // ... and its rows past the end are zero
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 3);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
     int* tile0 = off + GROUP_TABLE_INTS;
@@ -178,7 +218,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     const uint64_t tmo = p.timeout_ns;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], C::NLOAD);
+            mbar_init(&full[s], TMA ? 1 : C::NLOAD);
             mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -186,8 +226,14 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
             mbar_init(&tempty[a], C::NEPI);
         }
         mbar_init(drain, 1);
+        mbar_init(fixreq, 1);
+        mbar_init(fixdone, 1);
         *abort_flag = 0;
         fence_mbar_init();
+    }
+    if (TMA && threadIdx.x == 0) {
+        prefetch_tmap(&tmP);
+        prefetch_tmap(&tmQ);
     }
     if (warp == 1) {
         tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -205,10 +251,85 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     GroupWalk walk(off, tile0, p.groups, blockIdx.x, gridDim.x);
     GTile t;
 
-    if (warp >= C::LOAD_W0) {
+    if (TMA && warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer ----------------
+            int stage = 0;
+            uint32_t phase = 0, issued = 0, last_par = 0;
+            bool ok = true;
+            while (ok && next_tile<BN>(walk, p, t)) {
+                const int pz = p.p_z ? t.g : 0;
+                const int qb = static_cast<int>(t.qbase);
+                for (int kb = 0; kb < t.nk; kb += GBK) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    uint64_t* fb = &full[stage];
+                    uint8_t* dp = sP + stage * C::P_BYTES;
+                    uint8_t* dq = sQ + stage * C::Q_BYTES;
+                    mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+                    const int k = t.k0 + kb;
+                    if (p.p_mn) {
+#pragma unroll
+                        for (int c = 0; c < BM / 64; ++c)
+                            tma_load_3d(dp + c * MN_BOX, &tmP, fb, t.p0 + 64 * c, k, pz);
+                    } else {
+                        tma_load_3d(dp, &tmP, fb, k, t.p0, pz);
+                    }
+                    if (p.q_mn) {
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c)
+                            tma_load_3d(dq + c * MN_BOX, &tmQ, fb, qb + 64 * c, k, 0);
+                    } else {
+                        tma_load_3d(dq, &tmQ, fb, k, qb, 0);
+                    }
+                    issued |= 1u << stage;
+                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            griddep_launch_dependents();
+            // every issued copy has landed before the CTA may exit
+            int dummy = 0;
+            for (int s = 0; s < STAGES; ++s)
+                if (issued & (1u << s))
+                    mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
+                              GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (TMA && warp == 2) {
+        // ---------------- the contraction's ragged end (weight gradient) ----------------
+        if (p.wgrad) {
+            int blocks = 0;  // stages filled so far
+            uint32_t par = 0;
+            while (next_tile<BN>(walk, p, t)) {
+                blocks += (t.nk + GBK - 1) / GBK;
+                if ((t.nk & 15) == 0) continue;
+                const int stage = (blocks - 1) % STAGES;
+                if (!warp_wait(fixreq, par, abort_flag, p.status, GK_DEV_TIMEOUT_PRODUCER, tmo))
+                    break;
+                par ^= 1u;
+                const int v = t.nk & (GBK - 1), zrows = 16 - (t.nk & 15);  // rows [v, v + zrows)
+                constexpr int CH = (BM + BN) / 64;
+                for (int i = lane; i < CH * zrows * 8; i += 32) {
+                    const int c = i / (zrows * 8), r = i % (zrows * 8);
+                    uint8_t* box = c < BM / 64 ? sP + stage * C::P_BYTES + c * MN_BOX
+                                               : sQ + stage * C::Q_BYTES + (c - BM / 64) * MN_BOX;
+                    *reinterpret_cast<uint4*>(box + v * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(fixdone);
+            }
+        }
+    } else if (!TMA && warp >= C::LOAD_W0) {
         // ---------------- loaders: any strides, one stage at a time ----------------
         const int lt = threadIdx.x - 32 * C::LOAD_W0;
-        constexpr int NT = 32 * C::NLOAD;
+        constexpr int NT = TMA ? 32 : 32 * C::NLOAD;
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -243,7 +364,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
         if (lane == 0) {
             // ---------------- MMA issuer ----------------
             int stage = 0;
-            uint32_t phase = 0;
+            uint32_t phase = 0, fixpar = 0;
             bool ok = true;
             for (int local = 0; ok && next_tile<BN>(walk, p, t); ++local) {
                 const int acc = local & 1;
@@ -252,8 +373,10 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                                tmo))
                     break;
                 tc_fence_after();
-                const uint32_t idesc =
-                    idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0);
+                uint32_t idesc = idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0);
+                if constexpr (TMA)
+                    idesc |= (static_cast<uint32_t>(p.p_mn) << 15) |
+                             (static_cast<uint32_t>(p.q_mn) << 16);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 for (int kb = 0; kb < t.nk; kb += GBK) {
                     if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
@@ -264,11 +387,34 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                     tc_fence_after();
                     const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
                     const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
+                    if constexpr (TMA) {
+                        int steps = GBK / 16;
+                        if (p.wgrad && t.nk - kb < GBK) {
+                            steps = (t.nk - kb + 15) >> 4;
+                            if (t.nk & 15) {
+                                mbar_arrive(fixreq);
+                                if (!mbar_wait(fixdone, fixpar, abort_flag, p.status,
+                                               GK_DEV_TIMEOUT_MMA, tmo)) {
+                                    ok = false;
+                                    break;
+                                }
+                                fixpar ^= 1u;
+                                tc_fence_after();
+                            }
+                        }
+                        for (int ks = 0; ks < steps; ++ks)
+                            mma_f16(d, p.p_mn ? sdesc_mn128(a0 + ks * MN_STEP)
+                                              : sdesc_kmajor_sw128(a0 + ks * MMA_KB),
+                                    p.q_mn ? sdesc_mn128(b0 + ks * MN_STEP)
+                                           : sdesc_kmajor_sw128(b0 + ks * MMA_KB),
+                                    idesc, (kb | ks) != 0 ? 1u : 0u);
+                    } else {
 #pragma unroll
-                    for (int ks = 0; ks < BKB / MMA_KB; ++ks)
-                        mma_f16(d, sdesc_kmajor_sw128(a0 + ks * MMA_KB),
-                                sdesc_kmajor_sw128(b0 + ks * MMA_KB), idesc,
-                                (kb | ks) != 0 ? 1u : 0u);
+                        for (int ks = 0; ks < BKB / MMA_KB; ++ks)
+                            mma_f16(d, sdesc_kmajor_sw128(a0 + ks * MMA_KB),
+                                    sdesc_kmajor_sw128(b0 + ks * MMA_KB), idesc,
+                                    (kb | ks) != 0 ? 1u : 0u);
+                    }
                     mma_commit(&empty[stage]);
                     if (++stage == STAGES) {
                         stage = 0;
@@ -299,14 +445,21 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                                 static_cast<uint32_t>(acc * BN + cbase);
             for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
                 uint32_t v[32];
-                tmem_ld_x32(tb + c, v);
+                if (t.nk > 0) {
+                    tmem_ld_x32(tb + c, v);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int j = cbase + c + e;
-                    if (row_ok && j < t.qn)
-                        store_elem(p, at + j * p.ldq,
-                                   t.nk > 0 ? __uint_as_float(v[e]) : 0.0f);
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }
+                if (!row_ok) continue;
+                const int64_t o = at + (cbase + c) * p.ldq;
+                const int n = t.qn - cbase - c;
+                if (p.out_f32)
+                    store_chunk(static_cast<float*>(p.c) + o, p.ldq, v, n, p.alpha, p.beta);
+                else if (p.f16)
+                    store_chunk(static_cast<__half*>(p.c) + o, p.ldq, v, n, p.alpha, p.beta);
+                else
+                    store_chunk(static_cast<__nv_bfloat16*>(p.c) + o, p.ldq, v, n, p.alpha, p.beta);
             }
             tc_fence_before();
             __syncwarp();
@@ -322,11 +475,11 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     }
 }
 
-template <int BN>
-int launch_grouped(GroupedParams p, int grid, int pdl, cudaStream_t stream, char* err,
-                   size_t errlen) {
-    using C = GroupedCfg<BN>;
-    auto kern = grouped_half_kernel<BN>;
+template <int BN, bool TMA>
+int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p, int grid,
+                   int pdl, cudaStream_t stream, char* err, size_t errlen) {
+    using C = GroupedCfg<BN, TMA>;
+    auto kern = grouped_half_kernel<BN, TMA>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg;
@@ -340,7 +493,7 @@ int launch_grouped(GroupedParams p, int grid, int pdl, cudaStream_t stream, char
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = pdl ? 1 : 0;
-        e = cudaLaunchKernelEx(&cfg, kern, p);
+        e = cudaLaunchKernelEx(&cfg, kern, tp, tq, p);
     }
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) {
@@ -348,6 +501,28 @@ int launch_grouped(GroupedParams p, int grid, int pdl, cudaStream_t stream, char
         return GK_ECUDA;
     }
     return GK_OK;
+}
+
+// Whether TMA can address a 16-bit operand of `rows` rows x `len` contraction indices x `groups`
+// (1: no group dimension), and how it lies: 0 = K-major, 1 = MN-major, -1 = not at all. A stride
+// along a dimension of one element says nothing.
+int tma_major(const GOperand& o, int64_t rows, int64_t len, int64_t groups, bool mn_ok, bool k_ok) {
+    if (reinterpret_cast<uintptr_t>(o.ptr) & 15) return -1;
+    if (groups > 1 && (o.gs <= 0 || o.gs % 8)) return -1;
+    const bool r1 = rows <= 1, p1 = len <= 1;
+    if (k_ok && (o.ps == 1 || p1) && (r1 || (o.rs > 0 && o.rs % 8 == 0))) return 0;
+    if (mn_ok && (o.rs == 1 || r1) && (p1 || (o.ps > 0 && o.ps % 8 == 0))) return 1;
+    return -1;
+}
+
+// The tensor map of such an operand: 64 contiguous elements x `box` lines (a power of two) of one
+// group. Strides along dimensions of one element are replaced by any valid one.
+int encode_goperand(CUtensorMap* map, const GOperand& o, int major, int64_t rows, int64_t len,
+                    int64_t groups, int box, char* err, size_t errlen) {
+    const int64_t inner = major ? rows : len, outer = major ? len : rows;
+    const int64_t ld = outer > 1 ? (major ? o.ps : o.rs) : (inner + 7) / 8 * 8;
+    const int64_t gs = groups > 1 ? o.gs : ld;
+    return encode_tmap_u16(map, o.ptr, inner, outer, groups, ld, gs, 64, box, err, errlen);
 }
 
 // Tile width along the Q side. Forward: the mean rows of a group; a group's last tile costs only
@@ -360,7 +535,7 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
     int rc = api_check_device(&dev);
     if (rc) return rc;
     const int64_t mean = (static_cast<int64_t>(p.rows) + p.groups - 1) / p.groups;
-    const int bn = grouped_bn(p.wgrad ? p.nq : mean);
+    const int bn = p.wgrad ? grouped_bn(p.nq < 64 ? 64 : p.nq) : grouped_bn(mean);
     const int64_t tp = (p.np + BM - 1) / BM;
     // an upper bound of the tiles (the device computes the true number from the offsets)
     const int64_t tq = p.wgrad ? (p.nq + bn - 1) / bn * p.groups
@@ -375,11 +550,38 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
     const int grid = static_cast<int>(tp * tq < sms ? tp * tq : sms);
     const int pdl = api_pdl_enabled();
     char err[256] = "";
+    // TMA needs unit strides and 16-byte multiples; the forward product's Q rows start anywhere
+    // (K-major only: their coordinate is the slow one), and so does the weight gradient's
+    // contraction (MN-major only).
+    const int64_t gp = p.P.gs != 0 ? p.groups : 1;
+    const int64_t plen = p.wgrad ? p.rows : p.kdim;
+    const int64_t qrows = p.wgrad ? p.nq : p.rows;
+    p.p_mn = tma_major(p.P, p.np, plen, gp, true, !p.wgrad);
+    p.q_mn = tma_major(p.Q, qrows, plen, 1, p.wgrad != 0, !p.wgrad);
+    p.p_z = gp > 1;
+    CUtensorMap tmp, tmq;
+    memset(&tmp, 0, sizeof(tmp));
+    memset(&tmq, 0, sizeof(tmq));
+    const bool tma = !p.zero && p.p_mn >= 0 && p.q_mn >= 0;
+    if (tma) {
+        rc = encode_goperand(&tmp, p.P, p.p_mn, p.np, plen, gp, p.p_mn ? GBK : BM, err, sizeof(err));
+        if (!rc)
+            rc = encode_goperand(&tmq, p.Q, p.q_mn, qrows, plen, 1, p.q_mn ? GBK : bn, err,
+                                 sizeof(err));
+        if (rc) return set_last_error(rc, err);
+    } else {
+        p.p_mn = p.q_mn = 0;
+    }
+    auto go = [&](auto bn_tag) {
+        constexpr int BN = decltype(bn_tag)::value;
+        return tma ? launch_grouped<BN, true>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err))
+                   : launch_grouped<BN, false>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
+    };
     switch (bn) {
-        case 32: rc = launch_grouped<32>(p, grid, pdl, stream, err, sizeof(err)); break;
-        case 64: rc = launch_grouped<64>(p, grid, pdl, stream, err, sizeof(err)); break;
-        case 128: rc = launch_grouped<128>(p, grid, pdl, stream, err, sizeof(err)); break;
-        default: rc = launch_grouped<256>(p, grid, pdl, stream, err, sizeof(err)); break;
+        case 32: rc = go(std::integral_constant<int, 32>{}); break;
+        case 64: rc = go(std::integral_constant<int, 64>{}); break;
+        case 128: rc = go(std::integral_constant<int, 128>{}); break;
+        default: rc = go(std::integral_constant<int, 256>{}); break;
     }
     return rc ? set_last_error(rc, err) : GK_OK;
 }

@@ -686,6 +686,28 @@ int encode_tiled_operand(CUtensorMap* map, const Operand& op, int64_t K, int box
     return 0;
 }
 
+int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, int64_t d2,
+                    int64_t ld1, int64_t ld2, int box0, int box1, char* err, size_t errlen) {
+    PFN_tmapEncodeTiled enc = get_encode();
+    if (!enc) {
+        snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled is unavailable (driver too old?)");
+        return 5;
+    }
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(d0), static_cast<cuuint64_t>(d1),
+                          static_cast<cuuint64_t>(d2)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld1) * 2, static_cast<cuuint64_t>(ld2) * 2};
+    cuuint32_t box[3] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(box1), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(ptr), dims, strides,
+                     box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+        return 3;
+    }
+    return 0;
+}
+
 static int encode_operand_uncached(CUtensorMap* map, const Operand& op, int64_t K, int64_t batch,
                                    int es, int box_rows, char* err, size_t errlen) {
     PFN_tmapEncodeTiled enc = get_encode();
