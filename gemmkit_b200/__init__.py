@@ -15,7 +15,7 @@ from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
 from . import _lib
-from ._lib import (AXIS_COL, AXIS_NONE, AXIS_ROW, GK_EINVAL, GK_ENODEV, GK_ENOMEM, GK_ETIMEOUT,
+from ._lib import (AXIS_COL, AXIS_NONE, AXIS_ROW, FP4_MX, FP4_NV, GK_EINVAL, GK_ENODEV, GK_ENOMEM, GK_ETIMEOUT,
                    GK_OK, MatMutC, MatRefC, ProblemC, RequantC)
 
 __all__ = [
@@ -27,7 +27,8 @@ __all__ = [
     "gemm_i8_packed_b_requant", "gemm_i8_requant_batched", "gemm_i8_requant_batched_ptr",
     "gemm_half_f32", "gemm_bf16_f32_unchecked", "gemm_f16_f32_unchecked",
     "gemm_half_f32_batched", "gemm_half_f32_fused", "gemm_i8_fused", "gemm_i8_fused_unchecked", "Activation", "quantize_f32_i8", "gemm_i8_noalloc_unchecked", "set_tile_n", "knob_names", "knob_get",
-    "gemm_half_grouped", "gemm_half_grouped_wgrad", "knob_set", "device_status", "selftest_wait_timeout",
+    "gemm_half_grouped", "gemm_half_grouped_wgrad", "Fp4Matrix", "quantize_fp4", "dequantize_fp4",
+    "gemm_fp4", "FP4_MX", "FP4_NV", "knob_set", "device_status", "selftest_wait_timeout",
 ]
 
 
@@ -593,6 +594,124 @@ def gemm_half_grouped_wgrad(alpha: float, a: MatRef, b: MatRef, offsets, beta: f
     _check(_lib.load().gk_gemm_half_grouped_wgrad(int(is_f16), groups, ptr, float(alpha), a.c(),
                                                   b.c(), float(beta), c.c(), int(c_gs), out,
                                                   par.c(), _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+# ---- microscaled 4-bit floating point --------------------------------------------------------
+
+class Fp4Matrix:
+    """A rows x cols matrix in microscaled 4-bit floats (extension; see gk_fp4_matrix in the C
+    header): e2m1 codes with a scale per 32 (FP4_MX) or 16 (FP4_NV) elements of a row. Made by
+    quantize_fp4, from_codes, or empty; holds its device tensors `data` and `scales`.
+
+    `groups` equal groups make a stack of matrices (rows / groups rows each); `offsets` (an int32
+    device tensor of groups + 1 entries) ragged groups. `scale` is the FP4_NV format's matrix
+    scale (1 for FP4_MX)."""
+
+    def __init__(self, rows: int, cols: int, fmt: int, scale: float, groups: int, offsets, data,
+                 scales):
+        self.rows, self.cols, self.fmt, self.scale = int(rows), int(cols), fmt, float(scale)
+        self.groups, self.offsets, self.data, self.scales = groups, offsets, data, scales
+        c = _lib.Fp4MatrixC()
+        c.fmt, c.scale, c.groups = fmt, self.scale, groups
+        c.rows, c.cols = self.rows, self.cols
+        if offsets is not None:
+            c.offsets = _offsets(offsets)[0]
+        (c.data, c.data_len), (c.scales, c.scales_len) = _flat(data), _flat(scales)
+        self.c = c
+
+    @staticmethod
+    def empty(rows: int, cols: int, fmt: int, scale: float = 1.0, groups: int = 1, offsets=None,
+              device=None) -> "Fp4Matrix":
+        """An unwritten matrix on the current device (a destination for quantize_fp4)."""
+        import torch
+        if offsets is not None:
+            groups = _offsets(offsets)[1]
+        if fmt not in (FP4_MX, FP4_NV) or groups < 1 or rows < 0 or cols < 0:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: no 4-bit matrix of {rows}x{cols}, format {fmt}, "
+                                          f"{groups} groups")
+        # one allocation: codes, then scales (both parts whole 16-byte pieces)
+        nd, ns = _fp4_sizes(rows, cols, fmt, groups, offsets is not None)
+        buf = torch.empty(nd + ns, dtype=torch.uint8, device=device or "cuda")
+        return Fp4Matrix(rows, cols, fmt, scale, groups, offsets, buf[:nd], buf[nd:])
+
+    @staticmethod
+    def from_codes(codes, block_scales, rows: int, cols: int, fmt: int, scale: float = 1.0,
+                   groups: int = 1, offsets=None, stream=None, sync: bool = True) -> "Fp4Matrix":
+        """A matrix from plain row-major parts, as checkpoints hold them: uint8 tensors of codes
+        (rows x ceil(cols / 2), the first element of a pair in the low nibble) and of block scales
+        (rows x blocks: e8m0 or e4m3 bytes), both with contiguous rows."""
+        _same_device(codes=codes, block_scales=block_scales, offsets=offsets)
+        for name, t in (("codes", codes), ("block_scales", block_scales)):
+            if t.dim() != 2 or t.shape[0] != rows or t.element_size() != 1 or \
+                    (t.shape[1] > 1 and t.stride(1) != 1):
+                raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold {rows} contiguous rows of "
+                                              "bytes")
+        q = Fp4Matrix.empty(rows, cols, fmt, scale, groups, offsets, codes.device)
+
+        def part(t):
+            ld = t.stride(0) if rows > 1 else t.shape[1]
+            return t.data_ptr(), (rows - 1) * ld + t.shape[1] if rows else 0, ld
+        _check(_lib.load().gk_fp4_import(*part(codes), *part(block_scales), C.byref(q.c),
+                                         _stream(stream)))
+        if sync:
+            _sync(stream)
+        return q
+
+
+def _fp4_sizes(rows, cols, fmt, groups, ragged):
+    lib = _lib.load()
+    return (lib.gk_fp4_data_bytes(rows, cols),
+            lib.gk_fp4_scale_bytes(fmt, groups, int(ragged), rows, cols))
+
+
+def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: int = 1,
+                 x_gs: int = 0, x_type: Optional[int] = None, out: Optional[Fp4Matrix] = None,
+                 stream=None, sync: bool = True) -> Fp4Matrix:
+    """x (f32, f16 or bf16) in 4 bits along its columns (extension): e2m1 codes, a scale per 32
+    (FP4_MX) or 16 (FP4_NV, times `scale`) consecutive elements of a row. Activations (rows x k) as
+    they are; weights with a column per output as the transposed view (n x k). With `offsets` the
+    rows form ragged groups; with groups > 1 `x` views the first of `groups` matrices that lie
+    x_gs elements apart. `out` reuses a matrix of the same shape, format and groups (its scale and
+    groups then hold); x_type names the element type of a (pointer, length) pair."""
+    _same_device(X=x.data, offsets=offsets)
+    if out is None:
+        stacked = offsets is None and groups > 1
+        out = Fp4Matrix.empty(x.rows * groups if stacked else x.rows, x.cols, fmt, scale, groups,
+                              offsets)
+    elif out.fmt != fmt:
+        raise GemmkitError(GK_EINVAL, "gemmkit: the output is held in another 4-bit format")
+    if x_type is None:
+        x_type = _elem_type(x.data, -1)
+    _check(_lib.load().gk_quantize_fp4(x.c(), x_type, x_gs, C.byref(out.c), _stream(stream)))
+    if sync:
+        _sync(stream)
+    return out
+
+
+def dequantize_fp4(q: Fp4Matrix, out: MatMut, stream=None, sync: bool = True) -> None:
+    """The f32 values that a 4-bit matrix stands for (extension)."""
+    _same_device(Q=q.data, C=out.data)
+    if _elem_type(out.data, _lib.DT_F32) != _lib.DT_F32:
+        raise GemmkitError(GK_EINVAL, "gemmkit: C must hold f32 elements")
+    _check(_lib.load().gk_dequantize_fp4(C.byref(q.c), out.c(), _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+def gemm_fp4(alpha: float, a: Fp4Matrix, b: Fp4Matrix, beta: float, c: MatMut,
+             c_type: Optional[int] = None, par: Parallelism = SERIAL, stream=None,
+             sync: bool = True) -> None:
+    """C <- alpha*A*B^T + beta*C with both operands in 4 bits (extension): A (rows x k), B (n x k),
+    C f32, f16 or bf16 by its tensor's dtype (c_type for a (pointer, length) pair). With groups,
+    row i of A's group g is multiplied by B's g-th matrix: A ragged (offsets) or equal groups, B a
+    stack of as many."""
+    _same_device(A=a.data, B=b.data, C=c.data)
+    if c_type is None:
+        c_type = _elem_type(c.data, -1)
+    _check(_lib.load().gk_gemm_fp4(float(alpha), C.byref(a.c), C.byref(b.c), float(beta), c.c(),
+                                   c_type, par.c(), _stream(stream)))
     if sync:
         _sync(stream)
 

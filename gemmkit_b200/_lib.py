@@ -14,6 +14,7 @@ GK_OK, GK_EINVAL, GK_ENOMEM, GK_ECUDA, GK_ETIMEOUT, GK_ENODEV = range(6)
 AXIS_NONE, AXIS_ROW, AXIS_COL = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+FP4_MX, FP4_NV = 0, 1
 
 sz, pd, vp, i32, u32, f32 = C.c_size_t, C.c_ssize_t, C.c_void_p, C.c_int32, C.c_uint32, C.c_float
 
@@ -44,6 +45,11 @@ class ProblemC(C.Structure):
     _fields_ = [("m", sz), ("k", sz), ("n", sz), ("a", vp), ("rsa", pd), ("csa", pd),
                 ("b", vp), ("rsb", pd), ("csb", pd), ("c", vp), ("rsc", pd), ("csc", pd),
                 ("req", RequantC)]
+
+
+class Fp4MatrixC(C.Structure):
+    _fields_ = [("fmt", i32), ("scale", f32), ("groups", sz), ("offsets", vp), ("rows", sz),
+                ("cols", sz), ("data", vp), ("data_len", sz), ("scales", vp), ("scales_len", sz)]
 
 
 SIGNATURES = {
@@ -120,6 +126,13 @@ SIGNATURES = {
                                    C.c_int, Parallelism, vp]),
     "gk_gemm_half_grouped_wgrad": (i32, [C.c_int, sz, vp, f32, MatRefC, MatRefC, f32, MatMutC, pd,
                                          C.c_int, Parallelism, vp]),
+    "gk_fp4_data_bytes": (sz, [sz, sz]),
+    "gk_fp4_scale_bytes": (sz, [C.c_int, sz, C.c_int, sz, sz]),
+    "gk_quantize_fp4": (i32, [MatRefC, C.c_int, pd, C.POINTER(Fp4MatrixC), vp]),
+    "gk_dequantize_fp4": (i32, [C.POINTER(Fp4MatrixC), MatMutC, vp]),
+    "gk_fp4_import": (i32, [vp, sz, sz, vp, sz, sz, C.POINTER(Fp4MatrixC), vp]),
+    "gk_gemm_fp4": (i32, [f32, C.POINTER(Fp4MatrixC), C.POINTER(Fp4MatrixC), f32, MatMutC, C.c_int,
+                          Parallelism, vp]),
     "gk_set_tile_n": (i32, [C.c_int]),
     "gk_knob_names": (C.c_char_p, []),
     "gk_knob_get": (i32, [C.c_char_p, C.POINTER(C.c_int64)]),

@@ -1,0 +1,1003 @@
+// gk_fp4.cu -- microscaled 4-bit floats: quantisation, the values back, and the product.
+//
+// A row is cut into blocks of consecutive elements that share one scale; the elements are e2m1
+// (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the first in the low nibble.
+//   mx  blocks of 32, the scale a power of two (e8m0):   2^(floor(log2 amax) - 2)
+//   nv  blocks of 16, the scale e4m3 times a per-matrix f32 scale s:  e4m3(amax / (6 s))
+//   element = e2m1(x / (block scale [* s])), ties to even, saturating at 6
+// A block that holds an infinity or a NaN gets a NaN scale and zero elements.
+//
+// Layout. Elements: row-major, rows at a pitch of whole 16-byte pieces. Scales: the order in which
+// the tensor cores take them from TMEM. A group of rows is cut into blocks of 128 rows (every
+// group starts a new one); per block and 4 consecutive scales one 512-byte atom, the scale j of
+// row r at (r % 32) * 16 + (r / 32 % 4) * 4 + j. An atom is copied to TMEM by one tcgen05.cp
+// (32 lanes x 16 bytes, replicated to the four lane quarters): column r / 32 then holds the four
+// scales of row r in lane r % 32. The atoms of a block follow each other along the row and cover
+// a whole number of 256-element stages.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "gemmkit_cuda.h"
+#include "gk_engine.h"
+#include "gk_group.cuh"
+#include "gk_sm100.cuh"
+#include "gk_store.cuh"
+#include "gk_tc_common.cuh"
+
+namespace gk {
+
+namespace {
+
+constexpr int FBK = 256;  // elements per stage (128 bytes of codes)
+
+template <int FMT>
+struct Fp4 {
+    static constexpr int BS = FMT == GK_FP4_MX ? 32 : 16;      // elements per scale
+    static constexpr int ATOMS = FBK / (4 * BS);               // scale atoms per stage: 2 / 4
+    static constexpr int SF_BYTES = ATOMS * 512;               // scales of 128 rows, one stage
+};
+
+// ---- conversions -------------------------------------------------------------------------------
+
+// Eight f32 to e2m1 (round to nearest even, saturating), x[0] in the low nibble.
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float (&x)[8]) {
+    uint32_t w;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(w)
+        : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+    return w;
+}
+
+// Two f32 to e4m3 (round to nearest even, saturating): lo in the low byte.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+    uint16_t h;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(hi), "f"(lo));
+    return h;
+}
+
+__device__ __forceinline__ float e4m3_to_float(uint32_t b) {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(b & 0xFFu)));
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
+}
+
+// The value of an e2m1 code (0..15).
+__device__ __forceinline__ float e2m1_to_float(uint32_t c) {
+    const uint32_t m = c & 7u;
+    // 1 + m % 2 / 2 scaled by 2^(m / 2 - 1) from its exponent and mantissa bits; 0 and 0.5 apart
+    const uint32_t bits = m < 2 ? (m ? 0x3F000000u : 0u)
+                                : (((m >> 1) + 126u) << 23) | ((m & 1u) << 22);
+    return __uint_as_float(bits | ((c & 8u) << 28));
+}
+
+// 2^(b - 127), b = 255: NaN
+__device__ __forceinline__ float e8m0_to_float(uint32_t b) {
+    return __uint_as_float(b == 255u ? 0x7FFFFFFFu : b == 0u ? 0x00400000u : b << 23);
+}
+
+struct NvScale {
+    float s, inv6;  // the matrix scale, and 1 / (6 s) in f32
+};
+
+// The nv block scale, exactly: e4m3 of amax / (6 s). f32 gives the quotient within 2^-22; where
+// both ends of that interval round alike, so does the exact quotient. Otherwise it lies next to
+// the border between two codes, and amax is compared with border * 6 s, which f64 holds exactly
+// (the border has 5 significant bits, 6 s has 26).
+__device__ __forceinline__ uint32_t nv_block_scale(float amax, const NvScale& n) {
+    const float q = amax * n.inv6;
+    const uint32_t two = cvt_e4m3x2(q * (1.0f - 0x1p-21f), q * (1.0f + 0x1p-21f));
+    const uint32_t lo = two & 0xFFu, hi = two >> 8;
+    if (lo == hi) return lo;
+    const double mid = 0.5 * (static_cast<double>(e4m3_to_float(lo)) + e4m3_to_float(hi));
+    const double border = mid * (6.0 * static_cast<double>(n.s));
+    const double a = static_cast<double>(amax);
+    return a < border ? lo : a > border ? hi : (lo & 1u) ? hi : lo;
+}
+
+// Eight elements over d = sb * s, exactly as nv_block_scale: the quotient in f32 within 2^-21,
+// and next to a border the comparison |x| with border * sb * s in f64 (4 + 4 + 24 bits).
+__device__ __forceinline__ uint32_t nv_elements(const float (&x)[8], float r, float sb, float s) {
+    float lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float y = x[i] * r;
+        lo[i] = y * (1.0f - 0x1p-20f);
+        hi[i] = y * (1.0f + 0x1p-20f);
+    }
+    uint32_t w = cvt_e2m1x8(lo);
+    const uint32_t w2 = cvt_e2m1x8(hi);
+    if (w != w2) {
+        const double d = static_cast<double>(sb) * static_cast<double>(s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t c = (w >> (4 * i)) & 15u, c2 = (w2 >> (4 * i)) & 15u;
+            if (c == c2) continue;
+            const double mid = 0.5 * (fabs(static_cast<double>(e2m1_to_float(c))) +
+                                      fabs(static_cast<double>(e2m1_to_float(c2))));
+            const double a = fabs(static_cast<double>(x[i])), border = mid * d;
+            const bool up = a > border || (a == border && (c & 1u));
+            if (up) w = (w & ~(15u << (4 * i))) | (c2 << (4 * i));
+        }
+    }
+    return w;
+}
+
+__device__ __forceinline__ float load_f(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_f(const __half* p) { return __half2float(__ldg(p)); }
+__device__ __forceinline__ float load_f(const __nv_bfloat16* p) {
+    return __bfloat162float(__ldg(p));
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+        v[2 * i] = __low2float(h);
+        v[2 * i + 1] = __high2float(h);
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+
+// ---- where a row lies ----------------------------------------------------------------------------
+
+struct Fp4View {
+    uint8_t* data;
+    uint8_t* scales;
+    int64_t pitch;  // bytes between rows of codes
+    int32_t rows, cols, groups, stages;  // stages: 256-element stages per row
+    const int32_t* offsets;
+    unsigned int* status;
+};
+
+// The group tables of a view in shared memory (blocks of 128 rows before each group); a single
+// group without offsets needs none.
+struct RowMap {
+    int off[GROUP_TABLE_INTS];
+    int blk[GROUP_TABLE_INTS];
+};
+
+__device__ __forceinline__ bool one_group(const Fp4View& v) { return v.groups == 1 && !v.offsets; }
+
+// The 128-row scale block and the row inside it of row r, and r's group and place in the group;
+// false for a row of no group.
+__device__ __forceinline__ bool find_row(const Fp4View& v, const RowMap& m, int r, int& block,
+                                         int& in, int& g, int& at) {
+    if (one_group(v)) {
+        g = 0;
+        at = r;
+        block = r >> 7;
+        in = r & 127;
+        return true;
+    }
+    if (r < m.off[0] || r >= m.off[v.groups]) return false;
+    int lo = 0, hi = v.groups;  // off[lo] <= r < off[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (m.off[mid] <= r)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    g = lo;
+    at = r - m.off[lo];
+    block = m.blk[lo] + (at >> 7);
+    in = at & 127;
+    return true;
+}
+
+template <int FMT>
+__device__ __forceinline__ uint8_t* scale_ptr(const Fp4View& v, int block, int in, int sf) {
+    return v.scales + (static_cast<int64_t>(block) * v.stages * Fp4<FMT>::ATOMS + (sf >> 2)) * 512 +
+           (in & 31) * 16 + (in >> 5) * 4 + (sf & 3);
+}
+
+// ---- quantisation --------------------------------------------------------------------------------
+
+// One block's scale from the largest magnitude's bits (as f32): the scale byte, and what the
+// elements are multiplied with.
+template <int FMT>
+__device__ __forceinline__ uint32_t block_scale(uint32_t amax_bits, const NvScale& nv, float& mul,
+                                                float& sb) {
+    sb = 0.0f;
+    if constexpr (FMT == GK_FP4_MX) {
+        const uint32_t e = amax_bits >> 23;
+        const uint32_t b = e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+        mul = __uint_as_float((254u - b) << 23);  // 2^(127 - b); b <= 252 or 255 (unused then)
+        return b;
+    } else {
+        if (amax_bits >= 0x7F800000u) {
+            mul = 0.0f;
+            return 0x7Fu;
+        }
+        const uint32_t b = nv_block_scale(__uint_as_float(amax_bits), nv);
+        sb = e4m3_to_float(b);
+        mul = b ? 1.0f / (sb * nv.s) : 0.0f;
+        return b;
+    }
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t block_codes(const float (&x)[8], uint32_t amax_bits, float mul,
+                                                float sb, const NvScale& nv) {
+    if (amax_bits >= 0x7F800000u) return 0u;
+    if constexpr (FMT == GK_FP4_MX) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[i] * mul;  // a power of two: exact
+        return cvt_e2m1x8(y);
+    } else {
+        return nv_elements(x, mul, sb, nv.s);
+    }
+}
+
+// Rows with contiguous elements (or any column stride, slower). A warp takes 256 elements of a
+// row (one stage), a lane eight: loads of 16 bytes (two for f32), the block's maximum by
+// shuffles, four bytes of codes stored. Elements past the row are zero, and so are the scales of
+// blocks past it (the product reads whole stages).
+template <int FMT, typename T>
+__global__ void __launch_bounds__(256)
+    quantize_fp4_kernel(const T* __restrict__ x, int64_t rs, int64_t cs, int64_t gs, int vec,
+                        Fp4View v, NvScale nv) {
+    __shared__ RowMap map;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (!one_group(v))
+        load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
+                    blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
+    const int lane = threadIdx.x & 31;
+    constexpr int LPB = Fp4<FMT>::BS / 8;  // lanes per block
+    const int64_t units = static_cast<int64_t>(v.rows) * v.stages;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+         u < units; u += step) {
+        const int r = static_cast<int>(u / v.stages), st = static_cast<int>(u - static_cast<int64_t>(r) * v.stages);
+        int block, in, g, at;
+        if (!find_row(v, map, r, block, in, g, at)) continue;
+        const int k = st * FBK + lane * 8;
+        // a stack's groups lie gs apart; ragged groups and a single one lie row after row
+        const T* src = x + (v.offsets ? static_cast<int64_t>(r) * rs : g * gs + at * rs);
+        float e[8];
+        if (vec && k + 8 <= v.cols) {
+            load8(src + k, e);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                e[i] = k + i < v.cols ? load_f(src + static_cast<int64_t>(k + i) * cs) : 0.0f;
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(e[i]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int d = 1; d < LPB; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        float mul, sb;
+        const uint32_t b = block_scale<FMT>(m, nv, mul, sb);
+        const uint32_t w = block_codes<FMT>(e, m, mul, sb, nv);
+        const int64_t byte = static_cast<int64_t>(st) * (FBK / 2) + lane * 4;
+        if (byte < v.pitch)
+            *reinterpret_cast<uint32_t*>(v.data + static_cast<int64_t>(r) * v.pitch + byte) = w;
+        if (lane % LPB == 0)
+            *scale_ptr<FMT>(v, block, in, st * (32 / LPB) + lane / LPB) =
+                static_cast<uint8_t>(k < v.cols ? b : 0u);
+    }
+}
+
+// The values back, in f32: code * block scale (exact) [* s, rounded once].
+template <int FMT>
+__global__ void __launch_bounds__(256)
+    dequantize_fp4_kernel(Fp4View v, float s, float* __restrict__ out, int64_t rs, int64_t cs,
+                          int vec) {
+    __shared__ RowMap map;
+    griddep_wait();
+    if (!one_group(v))
+        load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
+                    blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
+    const int lane = threadIdx.x & 31;
+    const int64_t units = static_cast<int64_t>(v.rows) * v.stages;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+         u < units; u += step) {
+        const int r = static_cast<int>(u / v.stages), st = static_cast<int>(u - static_cast<int64_t>(r) * v.stages);
+        int block, in, g, at;
+        if (!find_row(v, map, r, block, in, g, at)) continue;
+        const int k = st * FBK + lane * 8;
+        if (k >= v.cols) continue;
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(
+            v.data + static_cast<int64_t>(r) * v.pitch + static_cast<int64_t>(st) * (FBK / 2) +
+            lane * 4);
+        const uint32_t b = *scale_ptr<FMT>(v, block, in, k / Fp4<FMT>::BS);
+        const float sb = FMT == GK_FP4_MX ? e8m0_to_float(b) : e4m3_to_float(b);
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            y[i] = e2m1_to_float(w >> (4 * i)) * sb;
+            if (FMT != GK_FP4_MX) y[i] *= s;
+        }
+        float* dst = out + r * rs + k * cs;
+        if (vec && k + 8 <= v.cols) {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k + i < v.cols) dst[i * cs] = y[i];
+        }
+    }
+}
+
+// Row-major codes (two a byte) and scales (one byte a block) into the layout above.
+template <int FMT>
+__global__ void __launch_bounds__(256)
+    import_fp4_kernel(const uint8_t* __restrict__ codes, int64_t codes_ld,
+                      const uint8_t* __restrict__ scales, int64_t scales_ld, Fp4View v) {
+    __shared__ RowMap map;
+    griddep_wait();
+    if (!one_group(v))
+        load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
+                    blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
+    const int lane = threadIdx.x & 31;
+    const int64_t units = static_cast<int64_t>(v.rows) * v.stages;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+         u < units; u += step) {
+        const int r = static_cast<int>(u / v.stages), st = static_cast<int>(u - static_cast<int64_t>(r) * v.stages);
+        int block, in, g, at;
+        if (!find_row(v, map, r, block, in, g, at)) continue;
+        const int64_t byte = static_cast<int64_t>(st) * (FBK / 2) + lane * 4;
+        if (byte < v.pitch) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t k = (byte + i) * 2;
+                uint32_t c = k < v.cols ? codes[r * codes_ld + byte + i] : 0u;
+                if (k + 1 >= v.cols) c &= 15u;
+                w |= c << (8 * i);
+            }
+            *reinterpret_cast<uint32_t*>(v.data + static_cast<int64_t>(r) * v.pitch + byte) = w;
+        }
+        constexpr int NSF = 4 * Fp4<FMT>::ATOMS;  // scales of a stage
+        if (lane < NSF) {
+            const int sf = st * NSF + lane;
+            const bool in_row = sf * Fp4<FMT>::BS < v.cols;
+            *scale_ptr<FMT>(v, block, in, sf) = in_row ? scales[r * scales_ld + sf] : 0;
+        }
+    }
+}
+
+// ---- the product -----------------------------------------------------------------------------------
+
+struct Fp4GemmParams {
+    const uint8_t* psf;       // scales of P (the weights) and Q (the rows of A)
+    const uint8_t* qsf;
+    int32_t np, npb;          // rows of P in a group, its 128-row scale blocks
+    int32_t kdim, stages;     // contraction length, in 256-element stages
+    int32_t zero;
+    int32_t groups, rows, tiles_p;
+    const int32_t* offsets;   // of A's rows (nullptr: equal groups)
+    void* c;
+    int64_t ldq, ldp;
+    float alpha, beta;
+    int32_t out_type;
+    uint64_t timeout_ns;
+    unsigned int* status;
+};
+
+// BN: rows of A per tile. A tile's scales start at a TMEM column of their own only where a 128-row
+// scale block starts, so tiles of fewer rows serve calls that have no more rows than that (one
+// tile per group); every other call takes tiles of 128 rows.
+template <int FMT, int BN>
+struct Fp4Cfg {
+    static constexpr int NEPI = BN >= 64 ? 8 : 4;
+    static constexpr int EPI_W0 = 4;
+    static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
+    static constexpr int WCOLS = BN / (NEPI / 4);
+    static constexpr int SF = Fp4<FMT>::SF_BYTES;
+    static constexpr int P_BYTES = BM * BKB;
+    static constexpr int Q_BYTES = BN * BKB;
+    static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + 2 * SF;
+    static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
+    static constexpr int BAR_BYTES = 256;
+    static constexpr int RAW_STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    // TMEM: two accumulators, then each stage's scales (its own columns: they are free again when
+    // the stage is)
+    static constexpr int SF_COLS = 2 * 4 * Fp4<FMT>::ATOMS;
+    static constexpr int TMEM_STAGES = (512 - 2 * BN) / SF_COLS;
+    static constexpr int STAGES0 = RAW_STAGES > 10 ? 10 : RAW_STAGES;
+    static constexpr int STAGES = STAGES0 > TMEM_STAGES ? TMEM_STAGES : STAGES0;
+    // P | Q | scales of P | scales of Q | barriers | tables
+    static constexpr int OFF_Q = STAGES * P_BYTES;
+    static constexpr int OFF_SF = OFF_Q + STAGES * Q_BYTES;
+    static constexpr int OFF_BARS = OFF_SF + STAGES * 2 * SF;
+    static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
+    static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
+    static constexpr int TMEM_COLS = 512;
+    static_assert(BN == 32 || BN == 64 || BN == 128, "tile width");
+    static_assert(STAGES >= 2 && SMEM <= SMEM_LIMIT, "shared memory budget");
+    static_assert((2 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
+};
+
+// Instruction descriptor of kind::mxf4 / mxf4nvf4: both operands e2m1 (1 at bits 7 and 10), K-major,
+// N >> 3 at bit 17, the scales' type at bit 23 (1 = e8m0), M >> 4 at bit 24. The ids at bits 4
+// and 29 pick the bytes of a scale column that an instruction of 64 elements uses: with a
+// scale per 32, bytes 0-1 or 2-3 (ids 0, 2); with a scale per 16 all four (id 0).
+template <int FMT>
+__device__ __forceinline__ uint32_t idesc_fp4(int m, int n, int id) {
+    return (static_cast<uint32_t>(id) << 4) | (1u << 7) | (1u << 10) |
+           (static_cast<uint32_t>(n >> 3) << 17) | ((FMT == GK_FP4_MX ? 1u : 0u) << 23) |
+           (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(id) << 29);
+}
+
+template <int FMT>
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc,
+                                        uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (FMT == GK_FP4_MX)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+            "[%5], p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb),
+            "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, "
+            "[%4], [%5], p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb),
+            "r"(accumulate)
+            : "memory");
+}
+
+// One 512-byte scale atom (32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart) to four
+// TMEM columns, replicated to the four lane quarters. Executes in order with the later MMAs of
+// this thread.
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
+    const uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) |
+                       (static_cast<uint64_t>(128u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+template <int FMT, int BN>
+__global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
+                    const __grid_constant__ CUtensorMap tmQ32, const Fp4GemmParams p) {
+    using C = Fp4Cfg<FMT, BN>;
+    constexpr int STAGES = C::STAGES;
+    constexpr int ATOMS = Fp4<FMT>::ATOMS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sP = smem;
+    uint8_t* sQ = smem + C::OFF_Q;
+    uint8_t* sSF = smem + C::OFF_SF;  // per stage: P's scales, then Q's
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
+    int* tile0 = off + GROUP_TABLE_INTS;
+    int* qblk = tile0 + GROUP_TABLE_INTS;  // scale blocks of Q before each group
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t tmo = p.timeout_ns;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], C::NEPI);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        if (!p.zero) {
+            prefetch_tmap(&tmP);
+            prefetch_tmap(&tmQ);
+            prefetch_tmap(&tmQ32);
+        }
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    griddep_wait();
+    load_groups(p.offsets, p.groups, p.rows, off, qblk, blockIdx.x == 0 ? p.status : nullptr,
+                [](int m) { return (m + 127) >> 7; });
+    if (warp == 0)
+        sum_groups(off, p.groups, tile0, [&](int m) { return (m + BN - 1) / BN * p.tiles_p; });
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    GroupWalk walk(off, tile0, p.groups, blockIdx.x, gridDim.x);
+    int tp, tq;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- producer ----------------
+            int stage = 0;
+            uint32_t phase = 0, issued = 0, last_par = 0;
+            bool ok = true;
+            while (ok && walk.next(p.tiles_p, tp, tq)) {
+                const int g = walk.g, q0 = tq * BN;
+                const int64_t pb = static_cast<int64_t>(g) * p.npb + tp;
+                const int64_t qb = static_cast<int64_t>(qblk[g]) + (q0 >> 7);
+                const int prow = g * p.np + tp * BM, qrow = off[g] + q0;
+                const int ns = p.zero ? 0 : p.stages;
+                // a short tile loads its rows in pieces of 32 (the same bytes in shared memory)
+                const int qn = off[g + 1] - off[g] - q0;
+                const int pieces = qn > BN - 32 ? 0 : (qn + 31) >> 5;
+                const uint32_t bytes = C::STAGE_BYTES - (pieces ? C::Q_BYTES - pieces * 32 * BKB : 0);
+                for (int kb = 0; kb < ns; ++kb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    uint64_t* fb = &full[stage];
+                    mbar_arrive_expect_tx(fb, bytes);
+                    tma_load_3d(sP + stage * C::P_BYTES, &tmP, fb, kb * (FBK / 4), prow, 0);
+                    uint8_t* dq = sQ + stage * C::Q_BYTES;
+                    if (pieces == 0) tma_load_3d(dq, &tmQ, fb, kb * (FBK / 4), qrow, 0);
+                    for (int i = 0; i < pieces; ++i)
+                        tma_load_3d(dq + i * 32 * BKB, &tmQ32, fb, kb * (FBK / 4), qrow + 32 * i, 0);
+                    uint8_t* sf = sSF + stage * 2 * C::SF;
+                    bulk_load(sf, p.psf + (pb * p.stages + kb) * C::SF, C::SF, fb);
+                    bulk_load(sf + C::SF, p.qsf + (qb * p.stages + kb) * C::SF, C::SF, fb);
+                    issued |= 1u << stage;
+                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            griddep_launch_dependents();
+            int dummy = 0;
+            for (int s = 0; s < STAGES; ++s)
+                if (issued & (1u << s))
+                    mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
+                              GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer ----------------
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int local = 0; ok && walk.next(p.tiles_p, tp, tq); ++local) {
+                const int acc = local & 1;
+                const uint32_t aph = (local >> 1) & 1;
+                if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                               tmo))
+                    break;
+                tc_fence_after();
+                const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
+                const int n = min(BN, (qn + 15) & ~15);
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                const int ns = p.zero ? 0 : p.stages;
+                for (int kb = 0; kb < ns; ++kb) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                                   tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sf = smem_u32(sSF + stage * 2 * C::SF);
+                    const uint32_t tsf = tmem_base + static_cast<uint32_t>(2 * BN + stage * C::SF_COLS);
+#pragma unroll
+                    for (int a = 0; a < 2 * ATOMS; ++a) copy_scales(tsf + 4 * a, sf + 512 * a);
+                    const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
+                    const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
+                    const int steps = min(4, (p.kdim - kb * FBK + 63) >> 6);
+                    for (int ks = 0; ks < steps; ++ks) {
+                        const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
+                        const int id = FMT == GK_FP4_MX ? (ks & 1) * 2 : 0;
+                        mma_fp4<FMT>(d, sdesc_kmajor_sw128(a0 + ks * 32),
+                                     sdesc_kmajor_sw128(b0 + ks * 32), idesc_fp4<FMT>(BM, n, id),
+                                     tsf + 4 * atom, tsf + 4 * (ATOMS + atom),
+                                     (kb | ks) != 0 ? 1u : 0u);
+                    }
+                    mma_commit(&empty[stage]);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit(&tfull[acc]);
+            }
+            mma_commit(drain);
+            int dummy = 0;
+            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (warp >= C::EPI_W0) {
+        // ---------------- epilogue ----------------
+        const int q = warp & 3;
+        const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
+        for (int local = 0; walk.next(p.tiles_p, tp, tq); ++local) {
+            const int acc = local & 1;
+            const uint32_t aph = (local >> 1) & 1;
+            if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
+                break;
+            tc_fence_after();
+            const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
+            const int i = tp * BM + q * 32 + lane;
+            const bool row_ok = i < p.np;
+            const int64_t at = (static_cast<int64_t>(off[walk.g]) + q0) * p.ldq + i * p.ldp;
+            const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                static_cast<uint32_t>(acc * BN + cbase);
+            const bool have = !p.zero;
+            for (int c = 0; c < C::WCOLS && cbase + c < qn; c += 32) {
+                uint32_t v[32];
+                if (have) {
+                    tmem_ld_x32(tb + c, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                }
+                if (!row_ok) continue;
+                store_any(p.c, p.out_type, at + (cbase + c) * p.ldq, p.ldq, v, qn - cbase - c,
+                          p.alpha, p.beta);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------
+
+int64_t fp4_pitch(int64_t cols) { return ((cols + 1) / 2 + 15) / 16 * 16; }
+int64_t fp4_stages(int64_t cols) { return (cols + FBK - 1) / FBK; }
+int fp4_sf_bytes(int fmt) { return fmt == GK_FP4_MX ? Fp4<GK_FP4_MX>::SF_BYTES : Fp4<GK_FP4_NV>::SF_BYTES; }
+
+// The checks of a 4-bit matrix; `name` in the messages.
+int check_fp4(const gk_fp4_matrix* q, const char* name) {
+    if (!q) return api_err(GK_EINVAL, "gemmkit: null 4-bit matrix %s", name);
+    if (q->fmt != GK_FP4_MX && q->fmt != GK_FP4_NV)
+        return api_err(GK_EINVAL, "gemmkit: %s: unknown 4-bit format %d", name, q->fmt);
+    if (q->groups < 1 || q->groups > MAX_GROUPS)
+        return api_err(GK_EINVAL, "gemmkit: %s: 1 to %d groups (groups = %zu)", name, MAX_GROUPS,
+                       q->groups);
+    if (q->rows > INT32_MAX / 2 || q->cols > INT32_MAX / 2)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    if (!q->offsets && q->rows % q->groups)
+        return api_err(GK_EINVAL, "gemmkit: %s: %zu rows do not split into %zu equal groups", name,
+                       q->rows, q->groups);
+    // 2^-100 .. 2^100 keeps every quotient and product of the scales inside f32
+    if (!(q->scale >= 0x1p-100f && q->scale <= 0x1p100f) || (q->fmt == GK_FP4_MX && q->scale != 1.0f))
+        return api_err(GK_EINVAL, q->fmt == GK_FP4_MX
+                                      ? "gemmkit: %s: the mx format has no matrix scale (must be 1)"
+                                      : "gemmkit: %s: the matrix scale must lie in [2^-100, 2^100]",
+                       name);
+    if (q->rows == 0 || q->cols == 0) return GK_OK;
+    if (!q->data || !q->scales) return api_err(GK_EINVAL, "gemmkit: %s: null data or scales", name);
+    if ((reinterpret_cast<uintptr_t>(q->data) | reinterpret_cast<uintptr_t>(q->scales)) & 15)
+        return api_err(GK_EINVAL, "gemmkit: %s: data and scales must be 16-byte aligned", name);
+    const size_t nd = gk_fp4_data_bytes(q->rows, q->cols);
+    const size_t ns = gk_fp4_scale_bytes(q->fmt, q->groups, q->offsets != nullptr, q->rows, q->cols);
+    if (q->data_len < nd || q->scales_len < ns)
+        return api_err(GK_EINVAL,
+                       "gemmkit: %s: %zux%zu in 4 bits needs %zu bytes of data and %zu of scales "
+                       "(has %zu and %zu)",
+                       name, q->rows, q->cols, nd, ns, q->data_len, q->scales_len);
+    return GK_OK;
+}
+
+Fp4View view_of(const gk_fp4_matrix* q) {
+    Fp4View v;
+    memset(&v, 0, sizeof(v));
+    v.data = q->data;
+    v.scales = q->scales;
+    v.pitch = fp4_pitch(static_cast<int64_t>(q->cols));
+    v.rows = static_cast<int>(q->rows);
+    v.cols = static_cast<int>(q->cols);
+    v.groups = static_cast<int>(q->groups);
+    v.stages = static_cast<int>(fp4_stages(static_cast<int64_t>(q->cols)));
+    v.offsets = q->offsets;
+    v.status = device_status_ptr();
+    return v;
+}
+
+// A launch that may start while the previous kernel of the stream drains (the kernels wait for it
+// before they touch memory).
+template <typename... Args>
+int launch_overlapped(void (*kern)(Args...), int grid, int threads, size_t smem, cudaStream_t st,
+                      Args... args) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = api_pdl_enabled() ? 1 : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess)
+        return api_err(GK_ECUDA, "gemmkit: 4-bit kernel launch failed: %s", cudaGetErrorString(e));
+    return GK_OK;
+}
+
+// Blocks of 8 warps for `units` warp-sized units: up to 8 resident blocks on every SM.
+int unit_grid(int64_t units) {
+    const int64_t b = (units + 7) / 8, most = static_cast<int64_t>(sm_count()) * 8;
+    return static_cast<int>(b < most ? b : most);
+}
+
+template <int FMT, int BN>
+int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tq32,
+                    const Fp4GemmParams& p, int grid, cudaStream_t st) {
+    using C = Fp4Cfg<FMT, BN>;
+    auto kern = fp4_gemm_kernel<FMT, BN>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess)
+        return api_err(GK_ECUDA, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, Fp4GemmParams>(
+        kern, grid, C::THREADS, C::SMEM, st, tp, tq, tq32, p);
+}
+
+template <int FMT>
+int run_fp4_gemm(Fp4GemmParams p, const gk_fp4_matrix* a, const gk_fp4_matrix* b, cudaStream_t st) {
+    const int bn = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
+    const int64_t tp = (p.np + BM - 1) / BM;
+    const int64_t tq = (static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups;
+    if (tp * tq > INT32_MAX / 2)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    p.tiles_p = static_cast<int>(tp);
+    const int sms = sm_count();
+    const int grid = static_cast<int>(tp * tq < sms ? tp * tq : sms);
+    CUtensorMap tmp, tmq, tmq32;
+    memset(&tmp, 0, sizeof(tmp));
+    memset(&tmq, 0, sizeof(tmq));
+    memset(&tmq32, 0, sizeof(tmq32));
+    if (!p.zero) {
+        // codes as 16-bit elements: four codes each, the pitch a multiple of 16 bytes
+        const int64_t pe = fp4_pitch(p.kdim) / 2;
+        char err[256] = "";
+        int rc = encode_tmap_u16(&tmp, b->data, pe, static_cast<int64_t>(b->rows), 1, pe, pe, 64, BM,
+                                 err, sizeof(err));
+        if (!rc)
+            rc = encode_tmap_u16(&tmq, a->data, pe, p.rows, 1, pe, pe, 64, bn, err, sizeof(err));
+        if (!rc)
+            rc = encode_tmap_u16(&tmq32, a->data, pe, p.rows, 1, pe, pe, 64, 32, err, sizeof(err));
+        if (rc) return set_last_error(rc, err);
+    }
+    switch (bn) {
+        case 32: return launch_fp4_gemm<FMT, 32>(tmp, tmq, tmq32, p, grid, st);
+        case 64: return launch_fp4_gemm<FMT, 64>(tmp, tmq, tmq32, p, grid, st);
+        default: return launch_fp4_gemm<FMT, 128>(tmp, tmq, tmq32, p, grid, st);
+    }
+}
+
+template <int FMT, typename T>
+int run_quantize(const void* x, int64_t rs, int64_t cs, int64_t gs, const Fp4View& v, float scale,
+                 cudaStream_t st) {
+    // 16-byte loads: contiguous rows whose starts are all 16-byte aligned
+    const int64_t es = sizeof(T);
+    const bool rows1 = v.rows <= 1;
+    const int vec = cs == 1 && !(reinterpret_cast<uintptr_t>(x) & 15) &&
+                    (rows1 || (rs * es) % 16 == 0) &&
+                    (v.offsets || v.groups == 1 || (gs * es) % 16 == 0);
+    const NvScale nv{scale, 1.0f / (6.0f * scale)};
+    return launch_overlapped<const T*, int64_t, int64_t, int64_t, int, Fp4View, NvScale>(
+        quantize_fp4_kernel<FMT, T>, unit_grid(static_cast<int64_t>(v.rows) * v.stages), 256, 0, st,
+        static_cast<const T*>(x), rs, cs, gs, vec, v, nv);
+}
+
+}  // namespace
+
+}  // namespace gk
+
+using namespace gk;
+
+extern "C" {
+
+size_t gk_fp4_data_bytes(size_t rows, size_t cols) {
+    return rows * static_cast<size_t>(fp4_pitch(static_cast<int64_t>(cols)));
+}
+
+size_t gk_fp4_scale_bytes(int fmt, size_t groups, int ragged, size_t rows, size_t cols) {
+    if (groups == 0) groups = 1;
+    const size_t blocks = ragged ? (rows + 127) / 128 + groups : groups * ((rows / groups + 127) / 128);
+    return blocks * static_cast<size_t>(fp4_stages(static_cast<int64_t>(cols))) *
+           static_cast<size_t>(fp4_sf_bytes(fmt));
+}
+
+int gk_quantize_fp4(gk_matref x, int x_type, ptrdiff_t x_gs, const gk_fp4_matrix* dst,
+                    gk_stream_t stream) {
+    int rc = check_fp4(dst, "the destination");
+    if (rc) return rc;
+    if (x_type != GK_F32 && x_type != GK_F16 && x_type != GK_BF16)
+        return api_err(GK_EINVAL, "gemmkit: unknown element type %d", x_type);
+    const bool stacked = !dst->offsets && dst->groups > 1;
+    const size_t rows = stacked ? dst->rows / dst->groups : dst->rows;
+    if (x.rows != rows || x.cols != dst->cols)
+        return api_err(GK_EINVAL, "gemmkit: the source is %zux%zu, the 4-bit matrix holds %zux%zu%s",
+                       x.rows, x.cols, rows, dst->cols, stacked ? " per group" : "");
+    if ((rc = api_check_view(x.len, x.rows, x.cols, x.rs, x.cs, "X"))) return rc;
+    if (x.rows == 0 || x.cols == 0) return GK_OK;
+    if (!x.data) return api_err(GK_EINVAL, "gemmkit: null X");
+    if (stacked) {
+        const __int128 last = static_cast<__int128>(dst->groups - 1) * x_gs + 1 +
+                              static_cast<__int128>(x.rows - 1) * x.rs +
+                              static_cast<__int128>(x.cols - 1) * x.cs;
+        if (x_gs < 0 || last > static_cast<__int128>(x.len))
+            return api_err(GK_EINVAL, "gemmkit: X stack of %zu views %zux%zu (group stride %td) does "
+                                      "not fit its slice of %zu elements",
+                           dst->groups, x.rows, x.cols, x_gs, x.len);
+    }
+    const size_t es = x_type == GK_F32 ? 4 : 2;
+    if (api_overlaps(x.data, x.len * es, dst->data, dst->data_len) ||
+        api_overlaps(x.data, x.len * es, dst->scales, dst->scales_len) ||
+        api_overlaps(dst->data, dst->data_len, dst->scales, dst->scales_len))
+        return api_err(GK_EINVAL, "gemmkit: the 4-bit matrix aliases its source or itself");
+    if ((rc = api_check_device(nullptr))) return rc;
+    const Fp4View v = view_of(dst);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto go = [&](auto fmt) {
+        constexpr int F = decltype(fmt)::value;
+        if (x_type == GK_F32)
+            return run_quantize<F, float>(x.data, x.rs, x.cs, x_gs, v, dst->scale, st);
+        if (x_type == GK_F16)
+            return run_quantize<F, __half>(x.data, x.rs, x.cs, x_gs, v, dst->scale, st);
+        return run_quantize<F, __nv_bfloat16>(x.data, x.rs, x.cs, x_gs, v, dst->scale, st);
+    };
+    return dst->fmt == GK_FP4_MX ? go(std::integral_constant<int, GK_FP4_MX>{})
+                                 : go(std::integral_constant<int, GK_FP4_NV>{});
+}
+
+int gk_dequantize_fp4(const gk_fp4_matrix* q, gk_matmut out, gk_stream_t stream) {
+    int rc = check_fp4(q, "the source");
+    if (rc) return rc;
+    if (out.rows != q->rows || out.cols != q->cols)
+        return api_err(GK_EINVAL, "gemmkit: the 4-bit matrix holds %zux%zu, the output is %zux%zu",
+                       q->rows, q->cols, out.rows, out.cols);
+    if ((rc = api_check_view(out.len, out.rows, out.cols, out.rs, out.cs, "C"))) return rc;
+    if (api_self_aliases(out.rows, out.cols, out.rs, out.cs))
+        return api_err(GK_EINVAL, "gemmkit: C view aliases itself");
+    if (out.rows == 0 || out.cols == 0) return GK_OK;
+    if (!out.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    if (api_overlaps(out.data, out.len * 4, q->data, q->data_len) ||
+        api_overlaps(out.data, out.len * 4, q->scales, q->scales_len))
+        return api_err(GK_EINVAL, "gemmkit: C aliases the 4-bit matrix");
+    if ((rc = api_check_device(nullptr))) return rc;
+    const Fp4View v = view_of(q);
+    const int vec = out.cs == 1 && !(reinterpret_cast<uintptr_t>(out.data) & 15) &&
+                    (v.rows <= 1 || out.rs % 4 == 0);
+    const int grid = unit_grid(static_cast<int64_t>(v.rows) * v.stages);
+    auto kern = q->fmt == GK_FP4_MX ? dequantize_fp4_kernel<GK_FP4_MX>
+                                    : dequantize_fp4_kernel<GK_FP4_NV>;
+    return launch_overlapped<Fp4View, float, float*, int64_t, int64_t, int>(
+        kern, grid, 256, 0, static_cast<cudaStream_t>(stream), v, q->scale,
+        static_cast<float*>(out.data), out.rs, out.cs, vec);
+}
+
+int gk_fp4_import(const uint8_t* codes, size_t codes_len, size_t codes_ld, const uint8_t* scales,
+                  size_t scales_len, size_t scales_ld, const gk_fp4_matrix* dst,
+                  gk_stream_t stream) {
+    int rc = check_fp4(dst, "the destination");
+    if (rc) return rc;
+    if (dst->rows == 0 || dst->cols == 0) return GK_OK;
+    const size_t bs = dst->fmt == GK_FP4_MX ? 32 : 16;
+    const size_t cb = (dst->cols + 1) / 2, sb = (dst->cols + bs - 1) / bs;
+    if (!codes || !scales) return api_err(GK_EINVAL, "gemmkit: null codes or scales");
+    if (codes_ld < cb || scales_ld < sb || codes_len < (dst->rows - 1) * codes_ld + cb ||
+        scales_len < (dst->rows - 1) * scales_ld + sb)
+        return api_err(GK_EINVAL,
+                       "gemmkit: %zux%zu in 4 bits takes rows of %zu code bytes and %zu scales (has "
+                       "%zu at pitch %zu and %zu at pitch %zu)",
+                       dst->rows, dst->cols, cb, sb, codes_len, codes_ld, scales_len, scales_ld);
+    if (api_overlaps(codes, codes_len, dst->data, dst->data_len) ||
+        api_overlaps(codes, codes_len, dst->scales, dst->scales_len) ||
+        api_overlaps(scales, scales_len, dst->data, dst->data_len) ||
+        api_overlaps(scales, scales_len, dst->scales, dst->scales_len) ||
+        api_overlaps(dst->data, dst->data_len, dst->scales, dst->scales_len))
+        return api_err(GK_EINVAL, "gemmkit: the 4-bit matrix aliases its source or itself");
+    if ((rc = api_check_device(nullptr))) return rc;
+    const Fp4View v = view_of(dst);
+    const int grid = unit_grid(static_cast<int64_t>(v.rows) * v.stages);
+    auto kern = dst->fmt == GK_FP4_MX ? import_fp4_kernel<GK_FP4_MX> : import_fp4_kernel<GK_FP4_NV>;
+    return launch_overlapped<const uint8_t*, int64_t, const uint8_t*, int64_t, Fp4View>(
+        kern, grid, 256, 0, static_cast<cudaStream_t>(stream), codes,
+        static_cast<int64_t>(codes_ld), scales, static_cast<int64_t>(scales_ld), v);
+}
+
+int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, float beta, gk_matmut c,
+                int out_type, gk_parallelism par, gk_stream_t stream) {
+    (void)par;
+    int rc;
+    if ((rc = check_fp4(a, "A")) || (rc = check_fp4(b, "B"))) return rc;
+    if (out_type != GK_F32 && out_type != GK_F16 && out_type != GK_BF16)
+        return api_err(GK_EINVAL, "gemmkit: unknown element type %d", out_type);
+    if (a->fmt != b->fmt)
+        return api_err(GK_EINVAL, "gemmkit: A and B are held in different 4-bit formats");
+    if (b->offsets) return api_err(GK_EINVAL, "gemmkit: B's groups must be equal (no offsets)");
+    if (a->groups != b->groups)
+        return api_err(GK_EINVAL, "gemmkit: A has %zu groups, B has %zu", a->groups, b->groups);
+    const size_t n = b->rows / b->groups;
+    if (a->cols != b->cols)
+        return api_err(GK_EINVAL, "gemmkit: A.cols (%zu) != B.cols (%zu) (4-bit operands share k)",
+                       a->cols, b->cols);
+    if (a->rows != c.rows)
+        return api_err(GK_EINVAL, "gemmkit: A.rows (%zu) != C.rows (%zu)", a->rows, c.rows);
+    if (n != c.cols)
+        return api_err(GK_EINVAL, "gemmkit: B.rows per group (%zu) != C.cols (%zu)", n, c.cols);
+    if ((rc = api_check_view(c.len, c.rows, c.cols, c.rs, c.cs, "C"))) return rc;
+    if (api_self_aliases(c.rows, c.cols, c.rs, c.cs))
+        return api_err(GK_EINVAL,
+                       "gemmkit: C view aliases itself (strides %td,%td map distinct elements to "
+                       "the same memory); C must address each (i,j) uniquely",
+                       c.rs, c.cs);
+    const size_t cb = c.len * (out_type == GK_F32 ? 4 : 2);
+    for (const gk_fp4_matrix* o : {a, b})
+        if (o->rows && o->cols &&
+            (api_overlaps(c.data, cb, o->data, o->data_len) ||
+             api_overlaps(c.data, cb, o->scales, o->scales_len)))
+            return api_err(GK_EINVAL, "gemmkit: C aliases A or B");
+    if (c.rows == 0 || c.cols == 0) return GK_OK;
+    if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    if ((rc = api_check_device(nullptr))) return rc;
+    Fp4GemmParams p;
+    memset(&p, 0, sizeof(p));
+    p.psf = b->scales;
+    p.qsf = a->scales;
+    p.np = static_cast<int>(n);
+    p.npb = static_cast<int>((n + 127) / 128);
+    p.kdim = static_cast<int>(a->cols);
+    p.stages = static_cast<int>(fp4_stages(static_cast<int64_t>(a->cols)));
+    p.zero = a->cols == 0 || alpha == 0.0f;
+    p.groups = static_cast<int>(a->groups);
+    p.rows = static_cast<int>(a->rows);
+    p.offsets = a->offsets;
+    p.c = c.data;
+    p.ldq = c.rs;
+    p.ldp = c.cs;
+    p.alpha = static_cast<float>(static_cast<double>(alpha) * a->scale * b->scale);
+    p.beta = beta;
+    p.out_type = out_type;
+    p.timeout_ns = 4000000000ull;
+    p.status = device_status_ptr();
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a->fmt == GK_FP4_MX ? run_fp4_gemm<GK_FP4_MX>(p, a, b, st)
+                               : run_fp4_gemm<GK_FP4_NV>(p, a, b, st);
+}
+
+}  // extern "C"

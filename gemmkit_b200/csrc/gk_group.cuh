@@ -69,6 +69,26 @@ __device__ __forceinline__ void load_groups(const int32_t* offsets, int groups, 
     __syncthreads();
 }
 
+// Running sums of f(rows of the group) over sanitised offsets, by one warp: acc[0 .. groups].
+template <typename F>
+__device__ __forceinline__ void sum_groups(const int* off, int groups, int* acc, F f) {
+    const int lane = threadIdx.x & 31;
+    int sum = 0;
+    for (int base = 0; base < groups; base += 32) {
+        const int i = base + lane;
+        int s = i < groups ? f(off[i + 1] - off[i]) : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, s, d);
+            if (lane >= d) s += u;
+        }
+        s += sum;
+        if (i < groups) acc[i + 1] = s;
+        sum = __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) acc[0] = 0;
+}
+
 // Walks one block's tiles t = first, first + step, ... of a group schedule. Inside a group the
 // tiles run in bands of BAND tiles of the q side, q fastest: the blocks that work at one time
 // share the p operand's tiles, and the band's q operand stays in L2.

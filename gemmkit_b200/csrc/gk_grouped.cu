@@ -33,6 +33,7 @@
 #include "gk_engine.h"
 #include "gk_group.cuh"
 #include "gk_sm100.cuh"
+#include "gk_store.cuh"
 #include "gk_tc_common.cuh"
 
 namespace gk {
@@ -80,7 +81,7 @@ struct GroupedParams {
     int32_t p_mn, q_mn;       // TMA: the operand is MN-major
     int32_t p_z;              // TMA: 1 = the P operand has a group dimension
     int32_t f16;              // operands are f16 (else bf16)
-    int32_t out_f32;
+    int32_t out_type;         // gk_dtype of C
     uint64_t timeout_ns;
     unsigned int* status;
 };
@@ -161,34 +162,6 @@ __device__ __forceinline__ void gather_stage(uint8_t* dst, const uint16_t* src, 
         q.z = v[4] | (static_cast<uint32_t>(v[5]) << 16);
         q.w = v[6] | (static_cast<uint32_t>(v[7]) << 16);
         *reinterpret_cast<uint4*>(dst + r * 128 + ((j ^ (r & 7)) << 4)) = q;
-    }
-}
-
-__device__ __forceinline__ float from_out(float x) { return x; }
-__device__ __forceinline__ float from_out(__half x) { return __half2float(x); }
-__device__ __forceinline__ float from_out(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void to_out(float* p, float x) { *p = x; }
-__device__ __forceinline__ void to_out(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void to_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-
-// One thread's 32 accumulators (its lane's P row, 32 consecutive Q rows, `n` of them in C):
-// alpha * acc + beta * C in f32, rounded once to the output type. A warp's stores of one Q row
-// are 32 consecutive elements when C's P stride is 1.
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* c, int64_t ldq, const uint32_t (&v)[32], int n,
-                                            float alpha, float beta) {
-    if (beta != 0.0f) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (e < n)
-                to_out(c + e * ldq, fmaf(beta, from_out(c[e * ldq]), alpha * __uint_as_float(v[e])));
-    } else if (n >= 32) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) to_out(c + e * ldq, alpha * __uint_as_float(v[e]));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (e < n) to_out(c + e * ldq, alpha * __uint_as_float(v[e]));
     }
 }
 
@@ -454,12 +427,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                 if (!row_ok) continue;
                 const int64_t o = at + (cbase + c) * p.ldq;
                 const int n = t.qn - cbase - c;
-                if (p.out_f32)
-                    store_chunk(static_cast<float*>(p.c) + o, p.ldq, v, n, p.alpha, p.beta);
-                else if (p.f16)
-                    store_chunk(static_cast<__half*>(p.c) + o, p.ldq, v, n, p.alpha, p.beta);
-                else
-                    store_chunk(static_cast<__nv_bfloat16*>(p.c) + o, p.ldq, v, n, p.alpha, p.beta);
+                store_any(p.c, p.out_type, o, p.ldq, v, n, p.alpha, p.beta);
             }
             tc_fence_before();
             __syncwarp();
@@ -658,7 +626,7 @@ int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t* offsets, floa
     p.alpha = alpha;
     p.beta = beta;
     p.f16 = is_f16 != 0;
-    p.out_f32 = out_type == GK_F32;
+    p.out_type = out_type;
     return run_grouped(p, static_cast<cudaStream_t>(stream));
 }
 
@@ -706,7 +674,7 @@ int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t* offsets
     p.alpha = alpha;
     p.beta = beta;
     p.f16 = is_f16 != 0;
-    p.out_f32 = out_type == GK_F32;
+    p.out_type = out_type;
     return run_grouped(p, static_cast<cudaStream_t>(stream));
 }
 

@@ -341,6 +341,64 @@ int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t *offsets
                                gk_matref a, gk_matref b, float beta, gk_matmut c, ptrdiff_t c_gs,
                                int out_type, gk_parallelism par, gk_stream_t stream);
 
+/* ---- microscaled 4-bit floating point (no counterpart in gemmkit) ----------------------- */
+
+/* Formats: e2m1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives) in blocks of consecutive
+ * elements of a row that share a scale.
+ *   GK_FP4_MX  blocks of 32, scale 2^(floor(log2 amax) - 2) (e8m0);
+ *   GK_FP4_NV  blocks of 16, scale e4m3(amax / (6 * s)) times a per-matrix f32 scale s.
+ * An element is x / (block scale [* s]) rounded to the nearest e2m1 value, ties to even, saturating
+ * at 6; decisions are exact (as if in infinite precision). A block that holds an infinity or a NaN
+ * gets a NaN scale: its values, and every product with them, are NaN. */
+typedef enum { GK_FP4_MX = 0, GK_FP4_NV = 1 } gk_fp4_format;
+
+/* A rows x cols matrix in 4 bits, quantised along its columns (the contraction of a product), in
+ * device memory that the caller owns: `data` holds the codes, `scales` the scales in the engine's
+ * tile order (both 16-byte aligned; sizes from gk_fp4_data_bytes / gk_fp4_scale_bytes).
+ * The rows form `groups` groups: equal ones (a stack of matrices, offsets == NULL; groups == 1 for
+ * a plain matrix), or ragged ones given by a device array of groups + 1 offsets as in
+ * gk_gemm_half_grouped. The scales are laid out per group, so a matrix must be read with the
+ * groups it was written with. `scale` is the nv format's s (2^-100 .. 2^100); 1 for mx. */
+typedef struct {
+    int32_t fmt;            /* gk_fp4_format */
+    float scale;
+    size_t groups;
+    const int32_t *offsets; /* device, groups + 1 entries, or NULL */
+    size_t rows, cols;
+    uint8_t *data;
+    size_t data_len;        /* bytes */
+    uint8_t *scales;
+    size_t scales_len;      /* bytes */
+} gk_fp4_matrix;
+
+size_t gk_fp4_data_bytes(size_t rows, size_t cols);
+/* ragged: nonzero when the rows are grouped by offsets. */
+size_t gk_fp4_scale_bytes(int fmt, size_t groups, int ragged, size_t rows, size_t cols);
+
+/* Quantize x (f32, f16 or bf16 by x_type, a gk_dtype; any non-negative strides) into dst. For a
+ * stack x views group 0's rows and the groups lie x_gs elements apart; otherwise x_gs is
+ * unused. Rows outside ragged groups are neither read nor written. */
+int gk_quantize_fp4(gk_matref x, int x_type, ptrdiff_t x_gs, const gk_fp4_matrix *dst,
+                    gk_stream_t stream);
+/* The f32 values that q stands for (one rounding, by s, in the nv format). */
+int gk_dequantize_fp4(const gk_fp4_matrix *q, gk_matmut out, gk_stream_t stream);
+/* A 4-bit matrix from plain row-major parts, as checkpoints hold them: codes two a byte (the
+ * first in the low nibble) at codes_ld bytes a row, one scale byte a block (e8m0, or e4m3 without
+ * sign) at scales_ld bytes a row. */
+int gk_fp4_import(const uint8_t *codes, size_t codes_len, size_t codes_ld, const uint8_t *scales,
+                  size_t scales_len, size_t scales_ld, const gk_fp4_matrix *dst,
+                  gk_stream_t stream);
+
+/* C <- alpha * A * B^T + beta * C with A (rows x k) and B (n x k per group) in 4 bits and the same
+ * format, on the block-scaled tensor cores with f32 accumulation; C (rows x n) is f32, f16 or bf16
+ * (out_type, a gk_dtype), rounded once. With groups, row i of A's group g is multiplied by B's
+ * g-th matrix: A's groups may be ragged (a device array, as in gk_gemm_half_grouped, with the same
+ * rules for its contents and for rows outside the groups) or equal, B's are equal; both have the
+ * same number. beta == 0 never reads C; k == 0 or alpha == 0 is C <- beta * C. Needs no
+ * workspace, allocates nothing and may be captured. */
+int gk_gemm_fp4(float alpha, const gk_fp4_matrix *a, const gk_fp4_matrix *b, float beta,
+                gk_matmut c, int out_type, gk_parallelism par, gk_stream_t stream);
+
 /* ---- producer step: f32 activations -> i8 (no counterpart in gemmkit) ---------------- */
 
 /* Quantize a rows x cols f32 view (element (i, j) at x[i*rsx + j*csx]) into i8 (q[i*rsq +

@@ -394,3 +394,69 @@ def test_grouped_validation_without_gpu():
     expect_err(wgrad(gs=16), "C stack of 2 views 3x5")
     expect_err(wgrad(y=gk.MatRef.new((256, 25), 5, 5, 5, 1)), "A.cols (4) != B.rows (5)")
     expect_err(wgrad(w=gk.MatMut.new((1024, 40), 4, 5, 5, 1)), "A.rows (3) != C.rows (4)")
+
+
+def fp4(rows, cols, fmt=gk.FP4_MX, scale=1.0, groups=1, offsets=None, at=1 << 20, data_len=None,
+        scales_len=None):
+    """A 4-bit matrix over made-up device addresses (the refusals come before any device work)."""
+    nd, ns = gk._fp4_sizes(rows, cols, fmt if fmt in (0, 1) else 0, groups, offsets is not None)
+    return gk.Fp4Matrix(rows, cols, fmt, scale, groups, offsets,
+                        (at, nd if data_len is None else data_len),
+                        (at + (1 << 16), ns if scales_len is None else scales_len))
+
+
+def test_fp4_sizes():
+    assert gk._fp4_sizes(3, 31, gk.FP4_MX, 1, False) == (48, 1024)
+    assert gk._fp4_sizes(129, 257, gk.FP4_NV, 1, False) == (129 * 144, 2 * 2 * 2048)
+    assert gk._fp4_sizes(260, 256, gk.FP4_MX, 2, False) == (260 * 128, 4 * 1024)
+    assert gk._fp4_sizes(260, 256, gk.FP4_MX, 2, True) == (260 * 128, 5 * 1024)
+
+
+def test_fp4_validation_without_gpu():
+    x = gk.MatRef.new((64, 32), 4, 8, 8, 1)
+
+    def quant(x=x, out=None, x_type=0, **kw):
+        return lambda: gk.quantize_fp4(x, (out or fp4(4, 8)).fmt, out=out or fp4(4, 8), x_type=x_type,
+                                       sync=False, **kw)
+
+    expect_err(quant(out=fp4(4, 8, fmt=7)), "unknown 4-bit format 7")
+    expect_err(quant(out=fp4(4, 8, scale=2.0)), "the mx format has no matrix scale")
+    for s in (0.0, -1.0, float("nan"), float("inf"), 2.0 ** 101, 2.0 ** -101):
+        expect_err(quant(out=fp4(4, 8, fmt=gk.FP4_NV, scale=s)), "the matrix scale must lie in")
+    expect_err(quant(out=fp4(4, 8, groups=3)), "4 rows do not split into 3 equal groups")
+    expect_err(quant(out=fp4(4, 8, groups=0)), "1 to 1024 groups")
+    expect_err(quant(out=fp4(5, 8)), "the source is 4x8, the 4-bit matrix holds 5x8")
+    expect_err(quant(out=fp4(4, 8, at=8)), "16-byte aligned")
+    expect_err(quant(out=fp4(4, 8, data_len=63)), "needs 64 bytes of data")
+    expect_err(quant(out=fp4(4, 8, scales_len=1023)), "and 1024 of scales")
+    expect_err(quant(out=fp4(4, 8, at=96)), "aliases its source")
+    expect_err(quant(x_type=9), "unknown element type 9")
+    expect_err(quant(x=gk.MatRef.new((64, 31), 4, 8, 8, 1)), "X view of 4x8")
+    expect_err(quant(x=gk.MatRef.new((0, 32), 4, 8, 8, 1)), "null X")
+    expect_err(quant(out=fp4(8, 8, groups=2), x_gs=-1), "X stack of 2 views")
+    expect_err(quant(out=fp4(8, 8, groups=2), x_gs=1), "X stack of 2 views")
+
+    out = gk.MatMut.new((64, 32), 4, 8, 8, 1)
+    expect_err(lambda: gk.dequantize_fp4(fp4(5, 8), out), "holds 5x8, the output is 4x8")
+    expect_err(lambda: gk.dequantize_fp4(fp4(4, 8, at=96), out), "C aliases the 4-bit matrix")
+
+    a, b, c = fp4(4, 8), fp4(6, 8, at=1 << 22), gk.MatMut.new((64, 24), 4, 6, 6, 1)
+
+    def gemm(a=a, b=b, c=c, t=0):
+        return lambda: gk.gemm_fp4(1.0, a, b, 0.0, c, c_type=t, sync=False)
+
+    expect_err(gemm(t=3), "unknown element type 3")
+    expect_err(gemm(a=fp4(4, 8, fmt=gk.FP4_NV)), "different 4-bit formats")
+    expect_err(gemm(b=fp4(6, 9, at=1 << 22)), "A.cols (8) != B.cols (9)")
+    expect_err(gemm(b=fp4(6, 8, groups=2, at=1 << 22)), "A has 1 groups, B has 2")
+    expect_err(gemm(b=fp4(6, 8, groups=1, offsets=(4096, 2), at=1 << 22)), "B's groups must be equal")
+    expect_err(gemm(a=fp4(5, 8)), "A.rows (5) != C.rows (4)")
+    expect_err(gemm(b=fp4(7, 8, at=1 << 22)), "B.rows per group (7) != C.cols (6)")
+    expect_err(gemm(c=gk.MatMut.new((64, 24), 4, 6, 6, 0)), "aliases itself")
+    expect_err(gemm(c=gk.MatMut.new((64, 23), 4, 6, 6, 1)), "C view of 4x6")
+    expect_err(gemm(c=gk.MatMut.new((1 << 20, 24), 4, 6, 6, 1)), "C aliases A or B")
+    lib = _lib.load()
+    assert lib.gk_gemm_fp4(1.0, None, C.byref(b.c), 0.0, c.c(), 0, gk.SERIAL.c(), None) == gk.GK_EINVAL
+    assert b"null 4-bit matrix A" in lib.gk_last_error()
+    assert lib.gk_fp4_import(64, 15, 4, 128, 4, 1, C.byref(a.c), None) == gk.GK_EINVAL
+    assert b"takes rows of 4 code bytes and 1 scales" in lib.gk_last_error()
