@@ -118,12 +118,12 @@ struct GTile {
     int k0, nk;           // first contraction row (weight gradient) and contraction length
 };
 
-template <int BN>
+template <int BN, int TM = BM>
 __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, GTile& t) {
     int tp, tq;
     if (!w.next(p.tiles_p, tp, tq)) return false;
     t.g = w.g;
-    t.p0 = tp * BM;
+    t.p0 = tp * TM;
     t.q0 = tq * BN;
     const int o0 = w.off[t.g], m = w.off[t.g + 1] - o0;
     if (p.wgrad) {
@@ -443,6 +443,310 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
     }
 }
 
+// ---- the CTA-pair form ----------------------------------------------------------------------------
+//
+// Two CTAs of a cluster compute a tile of 256 P rows x up to 256 Q rows with tcgen05 cta_group::2:
+// each loads its 128 rows of P and half of the Q rows (the peer's half is read from its shared
+// memory by the MMA), so an SM moves a third less operand data per MAC than the one-CTA kernel's
+// 128 x 256 tile, whose rate the shared-memory traffic holds at about 55 % of the peak. The leader
+// (even CTA) issues every MMA; barriers as in the engine's other pair kernel: full[] and tempty[]
+// live in the leader, empty[] and tfull[] in both (one multicast commit each).
+
+struct GPairCfg {
+    static constexpr int BN = 256;
+    static constexpr int NEPI = 8;
+    static constexpr int EPI_W0 = 4;
+    static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
+    static constexpr int WCOLS = BN / 2;
+    static constexpr int P_BYTES = BM * BKB;
+    static constexpr int Q_BYTES = BN / 2 * BKB;
+    static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
+    static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
+    static constexpr int BAR_BYTES = 256;
+    static constexpr int STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    static constexpr int OFF_BARS = STAGES * STAGE_BYTES;
+    static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
+    static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
+    static_assert(STAGES >= 4 && (2 * STAGES + 8) * 8 <= BAR_BYTES, "barrier area");
+};
+
+__global__ void __launch_bounds__(GPairCfg::THREADS, 1)
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap tmP,
+                        const __grid_constant__ CUtensorMap tmQ, const GroupedParams p) {
+    using C = GPairCfg;
+    constexpr int STAGES = C::STAGES, BN = C::BN, TM = 2 * BM;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sP = smem;
+    uint8_t* sQ = smem + STAGES * C::P_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint64_t* fixreq = drain + 1;
+    uint64_t* fixdone = drain + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 3);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
+    int* tile0 = off + GROUP_TABLE_INTS;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const uint64_t tmo = p.timeout_ns;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);  // the leader's producer; the peer's copies only add bytes
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], 2 * C::NEPI);  // every epilogue warp of both CTAs
+        }
+        mbar_init(drain, 1);
+        mbar_init(fixreq, 1);
+        mbar_init(fixdone, 2);  // both CTAs' warps
+        *abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmP);
+        prefetch_tmap(&tmQ);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    griddep_wait();
+    load_groups(p.offsets, p.groups, p.rows, off, tile0, blockIdx.x == 0 ? p.status : nullptr,
+                [&](int m) {
+                    return p.wgrad ? p.tiles_p * p.tiles_q : (m + BN - 1) / BN * p.tiles_p;
+                });
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t full_l = mapa_shared(smem_u32(&full[0]), 0);
+    const uint32_t tempty_l = mapa_shared(smem_u32(&tempty[0]), 0);
+    GroupWalk walk(off, tile0, p.groups, blockIdx.x >> 1, gridDim.x >> 1);
+    GTile t;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer (both CTAs) ----------------
+            int stage = 0;
+            uint32_t phase = 0, issued = 0, last_par = 0;
+            bool ok = true;
+            while (ok && next_tile<BN, TM>(walk, p, t)) {
+                const int pz = p.p_z ? t.g : 0;
+                const int p0 = t.p0 + static_cast<int>(rank) * BM;
+                // the MMA's N, and this CTA's half of its rows
+                const int n = min(BN, (t.qn + 31) & ~31);
+                const int qb = static_cast<int>(t.qbase) + static_cast<int>(rank) * (n >> 1);
+                for (int kb = 0; kb < t.nk; kb += GBK) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = full_l + 8u * stage;
+                    uint8_t* dp = sP + stage * C::P_BYTES;
+                    uint8_t* dq = sQ + stage * C::Q_BYTES;
+                    if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
+                    const int k = t.k0 + kb;
+                    if (p.p_mn) {
+#pragma unroll
+                        for (int c = 0; c < BM / 64; ++c)
+                            tma_load_3d_pair(dp + c * MN_BOX, &tmP, fb, p0 + 64 * c, k, pz);
+                    } else {
+                        tma_load_3d_pair(dp, &tmP, fb, k, p0, pz);
+                    }
+                    if (p.q_mn) {
+#pragma unroll
+                        for (int c = 0; c < BN / 128; ++c)
+                            tma_load_3d_pair(dq + c * MN_BOX, &tmQ, fb, qb + 64 * c, k, 0);
+                    } else {
+                        tma_load_3d_pair(dq, &tmQ, fb, k, qb, 0);
+                    }
+                    issued |= 1u << stage;
+                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            griddep_launch_dependents();
+            if (leader) {  // its full barriers count both CTAs' copies
+                int dummy = 0;
+                for (int s = 0; s < STAGES; ++s)
+                    if (issued & (1u << s))
+                        mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
+                                  GK_DEV_TIMEOUT_DRAIN, tmo);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ---------------- MMA issuer (leader) ----------------
+            const uint32_t fixreq0 = mapa_shared(smem_u32(fixreq), 0);
+            const uint32_t fixreq1 = mapa_shared(smem_u32(fixreq), 1);
+            int stage = 0;
+            uint32_t phase = 0, fixpar = 0;
+            bool ok = true;
+            for (int local = 0; ok && next_tile<BN, TM>(walk, p, t); ++local) {
+                const int acc = local & 1;
+                const uint32_t aph = (local >> 1) & 1;
+                if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                               tmo))
+                    break;
+                tc_fence_after();
+                const uint32_t idesc = idesc_f16(TM, min(BN, (t.qn + 31) & ~31), p.f16 == 0) |
+                                       (static_cast<uint32_t>(p.p_mn) << 15) |
+                                       (static_cast<uint32_t>(p.q_mn) << 16);
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                for (int kb = 0; kb < t.nk; kb += GBK) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                                   tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
+                    const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
+                    int steps = GBK / 16;
+                    if (p.wgrad && t.nk - kb < GBK) {
+                        steps = (t.nk - kb + 15) >> 4;
+                        if (t.nk & 15) {
+                            mbar_arrive_cluster(fixreq0);
+                            mbar_arrive_cluster(fixreq1);
+                            if (!mbar_wait_cluster(fixdone, fixpar, abort_flag, p.status,
+                                                   GK_DEV_TIMEOUT_MMA, tmo)) {
+                                ok = false;
+                                break;
+                            }
+                            fixpar ^= 1u;
+                            tc_fence_after();
+                        }
+                    }
+                    for (int ks = 0; ks < steps; ++ks)
+                        mma_f16_pair(d, p.p_mn ? sdesc_mn128(a0 + ks * MN_STEP)
+                                               : sdesc_kmajor_sw128(a0 + ks * MMA_KB),
+                                     p.q_mn ? sdesc_mn128(b0 + ks * MN_STEP)
+                                            : sdesc_kmajor_sw128(b0 + ks * MMA_KB),
+                                     idesc, (kb | ks) != 0 ? 1u : 0u);
+                    mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+            }
+            mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            int dummy = 0;
+            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (warp == 2) {
+        // ---------------- the contraction's ragged end (both CTAs) ----------------
+        if (p.wgrad) {
+            const uint32_t done = mapa_shared(smem_u32(fixdone), 0);
+            int blocks = 0;
+            uint32_t par = 0;
+            while (next_tile<BN, TM>(walk, p, t)) {
+                blocks += (t.nk + GBK - 1) / GBK;
+                if ((t.nk & 15) == 0) continue;
+                const int stage = (blocks - 1) % STAGES;
+                const bool ok = mbar_wait_cluster(fixreq, par, abort_flag, p.status,
+                                                  GK_DEV_TIMEOUT_PRODUCER, tmo);
+                if (__any_sync(0xffffffffu, !ok)) break;
+                par ^= 1u;
+                const int v = t.nk & (GBK - 1), zrows = 16 - (t.nk & 15);
+                constexpr int CH = (BM + BN / 2) / 64;
+                for (int i = lane; i < CH * zrows * 8; i += 32) {
+                    const int c = i / (zrows * 8), r = i % (zrows * 8);
+                    uint8_t* box = c < BM / 64 ? sP + stage * C::P_BYTES + c * MN_BOX
+                                               : sQ + stage * C::Q_BYTES + (c - BM / 64) * MN_BOX;
+                    *reinterpret_cast<uint4*>(box + v * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(done);
+            }
+        }
+    } else if (warp >= C::EPI_W0) {
+        // ---------------- epilogue (both CTAs) ----------------
+        const int q = warp & 3;
+        const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
+        for (int local = 0; next_tile<BN, TM>(walk, p, t); ++local) {
+            const int acc = local & 1;
+            const uint32_t aph = (local >> 1) & 1;
+            if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
+                break;
+            tc_fence_after();
+            const int i = t.p0 + static_cast<int>(rank) * BM + q * 32 + lane;
+            const bool row_ok = i < p.np;
+            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i * p.ldp;
+            const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                static_cast<uint32_t>(acc * BN + cbase);
+            for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
+                uint32_t v[32];
+                if (t.nk > 0) {
+                    tmem_ld_x32(tb + c, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                }
+                if (row_ok)
+                    store_any(p.c, p.out_type, at + (cbase + c) * p.ldq, p.ldq, v,
+                              t.qn - cbase - c, p.alpha, p.beta);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(tempty_l + 8u * acc);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // neither CTA leaves while the other may still use its barriers or operands
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+int launch_grouped_pair(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p,
+                        int grid, int pdl, cudaStream_t stream, char* err, size_t errlen) {
+    using C = GPairCfg;
+    cudaError_t e = cudaFuncSetAttribute(grouped_pair_kernel,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(static_cast<unsigned>(grid));
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl ? 2 : 1;
+        e = cudaLaunchKernelEx(&cfg, grouped_pair_kernel, tp, tq, p);
+    }
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        snprintf(err, errlen, "gemmkit: grouped kernel launch failed: %s", cudaGetErrorString(e));
+        return GK_ECUDA;
+    }
+    return GK_OK;
+}
+
 template <int BN, bool TMA>
 int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p, int grid,
                    int pdl, cudaStream_t stream, char* err, size_t errlen) {
@@ -498,26 +802,41 @@ int encode_goperand(CUtensorMap* map, const GOperand& o, int major, int64_t rows
 // are larger and fewer fit.
 int grouped_bn(int64_t q) { return q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256; }
 
+// Clusters of the pair kernel that are resident at once on the current device.
+int pair_clusters() {
+    static int cache[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int& n = cache[dev & 63];
+    if (n == 0) {
+        cudaLaunchConfig_t q;
+        memset(&q, 0, sizeof(q));
+        q.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
+        q.blockDim = dim3(GPairCfg::THREADS);
+        q.dynamicSmemBytes = GPairCfg::SMEM;
+        cudaLaunchAttribute a[1];
+        a[0].id = cudaLaunchAttributeClusterDimension;
+        a[0].val.clusterDim.x = 2;
+        a[0].val.clusterDim.y = 1;
+        a[0].val.clusterDim.z = 1;
+        q.attrs = a;
+        q.numAttrs = 1;
+        int c = 0;
+        if (cudaFuncSetAttribute(grouped_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 GPairCfg::SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&c, grouped_pair_kernel, &q) != cudaSuccess || c <= 0) {
+            cudaGetLastError();
+            c = sm_count() / 2;
+        }
+        n = c;
+    }
+    return n;
+}
+
 int run_grouped(GroupedParams p, cudaStream_t stream) {
     int dev = 0;
     int rc = api_check_device(&dev);
     if (rc) return rc;
-    const int64_t mean = (static_cast<int64_t>(p.rows) + p.groups - 1) / p.groups;
-    const int bn = p.wgrad ? grouped_bn(p.nq < 64 ? 64 : p.nq) : grouped_bn(mean);
-    const int64_t tp = (p.np + BM - 1) / BM;
-    // an upper bound of the tiles (the device computes the true number from the offsets)
-    const int64_t tq = p.wgrad ? (p.nq + bn - 1) / bn * p.groups
-                               : (static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups;
-    if (tp * tq > INT32_MAX / 2)
-        return set_last_error(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
-    p.tiles_p = static_cast<int>(tp);
-    p.tiles_q = static_cast<int>((p.nq + bn - 1) / bn);
-    p.timeout_ns = 4000000000ull;
-    p.status = device_status_ptr();
-    const int sms = sm_count();
-    const int grid = static_cast<int>(tp * tq < sms ? tp * tq : sms);
-    const int pdl = api_pdl_enabled();
-    char err[256] = "";
     // TMA needs unit strides and 16-byte multiples; the forward product's Q rows start anywhere
     // (K-major only: their coordinate is the slow one), and so does the weight gradient's
     // contraction (MN-major only).
@@ -527,19 +846,51 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
     p.p_mn = tma_major(p.P, p.np, plen, gp, true, !p.wgrad);
     p.q_mn = tma_major(p.Q, qrows, plen, 1, p.wgrad != 0, !p.wgrad);
     p.p_z = gp > 1;
+    const bool tma = !p.zero && p.p_mn >= 0 && p.q_mn >= 0;
+    if (!tma) p.p_mn = p.q_mn = 0;
+
+    const int64_t mean = (static_cast<int64_t>(p.rows) + p.groups - 1) / p.groups;
+    const int64_t qside = p.wgrad ? p.nq : mean;
+    // an upper bound of the tiles (the device computes the true number from the offsets)
+    auto tiles_bound = [&](int64_t tm, int64_t bn) {
+        const int64_t tq = p.wgrad ? (p.nq + bn - 1) / bn * p.groups
+                                   : (static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups;
+        return (p.np + tm - 1) / tm * tq;
+    };
+    const int clusters = pair_clusters();
+    // The pair kernel where its 256 x 256 tiles are mostly full on both sides and keep every
+    // cluster busy (a forward group that fills no whole tile still counts one in the bound)
+    const int64_t pair_tiles = tiles_bound(2 * BM, 256) - (p.wgrad ? 0 : p.groups);
+    const bool pair = tma && p.np > BM && qside > BM && pair_tiles >= clusters;
+    const int bn = pair ? 256 : grouped_bn(p.wgrad && qside < 64 ? 64 : qside);
+    const int tm = pair ? 2 * BM : BM;
+    const int64_t tiles = tiles_bound(tm, bn);
+    if (tiles > INT32_MAX / 2)
+        return set_last_error(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    p.tiles_p = static_cast<int>((p.np + tm - 1) / tm);
+    p.tiles_q = static_cast<int>((p.nq + bn - 1) / bn);
+    p.timeout_ns = 4000000000ull;
+    p.status = device_status_ptr();
+    const int pdl = api_pdl_enabled();
+    char err[256] = "";
     CUtensorMap tmp, tmq;
     memset(&tmp, 0, sizeof(tmp));
     memset(&tmq, 0, sizeof(tmq));
-    const bool tma = !p.zero && p.p_mn >= 0 && p.q_mn >= 0;
     if (tma) {
+        const int qbox = pair ? bn / 2 : bn;
         rc = encode_goperand(&tmp, p.P, p.p_mn, p.np, plen, gp, p.p_mn ? GBK : BM, err, sizeof(err));
         if (!rc)
-            rc = encode_goperand(&tmq, p.Q, p.q_mn, qrows, plen, 1, p.q_mn ? GBK : bn, err,
+            rc = encode_goperand(&tmq, p.Q, p.q_mn, qrows, plen, 1, p.q_mn ? GBK : qbox, err,
                                  sizeof(err));
         if (rc) return set_last_error(rc, err);
-    } else {
-        p.p_mn = p.q_mn = 0;
     }
+    if (pair) {
+        const int grid = 2 * static_cast<int>(tiles < clusters ? tiles : clusters);
+        rc = launch_grouped_pair(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
+        return rc ? set_last_error(rc, err) : GK_OK;
+    }
+    const int sms = sm_count();
+    const int grid = static_cast<int>(tiles < sms ? tiles : sms);
     auto go = [&](auto bn_tag) {
         constexpr int BN = decltype(bn_tag)::value;
         return tma ? launch_grouped<BN, true>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err))

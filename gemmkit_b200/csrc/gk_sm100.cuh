@@ -409,6 +409,41 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t caddr) {
                  : "memory");
 }
 
+// An arrival (release, cluster scope) on an mbarrier of this cluster that publishes the thread's
+// earlier shared-memory writes to the CTA that waits on it with mbar_wait_cluster().
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr)
+                 : "memory");
+}
+
+// mbar_wait with acquire at cluster scope (for arrivals from the peer CTA that publish writes).
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
+                                                  volatile int* abort_flag, unsigned int* status,
+                                                  unsigned int where, uint64_t timeout_ns) {
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (uint32_t i = 0;; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (i == 0) t0 = globaltimer_ns();
+        if ((i & 31u) == 31u) {
+            if (*abort_flag) return false;
+            if (globaltimer_ns() - t0 > timeout_ns) {
+                *abort_flag = 1;
+                if (status) atomicOr(status, where);
+                return false;
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t caddr, uint32_t bytes) {
     asm volatile(
         "mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(caddr),

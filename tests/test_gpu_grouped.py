@@ -443,3 +443,20 @@ def test_wide_rows_pass_32_bits():
     run_fwd(a, b, off, big, "bf16")
     want = a[-3:].double() @ b[0].double()
     assert torch.equal(big[-3:].double(), want) and not bool(big[:-3].any())
+
+
+PAIR_SIZES = [([1000, 0, 700, 255, 257, 1, 2083], 2, 5), ([4096], 0, 0), ([31, 4000, 33], 0, 1)]
+
+
+@pytest.mark.parametrize("sizes,lead,tail", PAIR_SIZES)
+@pytest.mark.parametrize("k,n,major", [(136, 1512, "k"), (72, 2048, "n"), (1, 4096, "n"),
+                                       (520, 1288, "n")])
+def test_forward_exact_large(sizes, lead, tail, k, n, major):
+    """Sizes that the CTA-pair kernel takes: whole and cut tiles on both sides."""
+    test_forward_exact(sizes, lead, tail, k, n, major)
+
+
+@pytest.mark.parametrize("sizes,lead,tail", PAIR_SIZES + [([16, 1, 0, 15, 17, 64, 63, 65], 0, 3)])
+@pytest.mark.parametrize("m,n", [(1032, 1512), (2048, 2304), (264, 4104)])
+def test_wgrad_exact_large(sizes, lead, tail, m, n):
+    test_wgrad_exact(sizes, lead, tail, m, n)
