@@ -587,6 +587,9 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
     } else if (warp == 1) {
         if (lane == 0) {
             // ---------------- MMA issuer ----------------
+            const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
+            const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
+            constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);  // both scale ids 2
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -598,7 +601,7 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
                     break;
                 tc_fence_after();
                 const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
-                const int n = min(BN, (qn + 15) & ~15);
+                const uint32_t idesc = idesc_fp4<FMT>(BM, min(BN, (qn + 15) & ~15), 0);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 const int ns = p.zero ? 0 : p.stages;
                 for (int kb = 0; kb < ns; ++kb) {
@@ -612,16 +615,24 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
                     const uint32_t tsf = tmem_base + static_cast<uint32_t>(2 * BN + stage * C::SF_COLS);
 #pragma unroll
                     for (int a = 0; a < 2 * ATOMS; ++a) copy_scales(tsf + 4 * a, sf + 512 * a);
-                    const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
-                    const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
-                    const int steps = min(4, (p.kdim - kb * FBK + 63) >> 6);
-                    for (int ks = 0; ks < steps; ++ks) {
+                    const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
+                    const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
+                    // slice ks: 64 elements = 32 bytes; its scales
+                    auto slice = [&](int ks) {
                         const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
-                        const int id = FMT == GK_FP4_MX ? (ks & 1) * 2 : 0;
-                        mma_fp4<FMT>(d, sdesc_kmajor_sw128(a0 + ks * 32),
-                                     sdesc_kmajor_sw128(b0 + ks * 32), idesc_fp4<FMT>(BM, n, id),
+                        mma_fp4<FMT>(d, ad + ks * 2, bd + ks * 2,
+                                     idesc + (FMT == GK_FP4_MX ? (ks & 1) * idesc_id2 : 0u),
                                      tsf + 4 * atom, tsf + 4 * (ATOMS + atom),
                                      (kb | ks) != 0 ? 1u : 0u);
+                    };
+                    const int steps = (p.kdim - kb * FBK + 63) >> 6;
+                    if (steps >= 4) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) slice(ks);
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < 3; ++ks)
+                            if (ks < steps) slice(ks);
                     }
                     mma_commit(&empty[stage]);
                     if (++stage == STAGES) {

@@ -59,6 +59,21 @@ __device__ __forceinline__ uint64_t sdesc_mn128(uint32_t saddr) {
     return d;
 }
 
+// The descriptors of an operand's stage 0 and the distances (in the descriptor's 16-byte units)
+// between its MMAs' 16-element slices. The issuing thread has about 128 cycles per MMA: building
+// the descriptors anew for each one held the products at 0.65 of what the tensor cores give.
+struct OperandDesc {
+    uint64_t base;
+    uint32_t step;
+    __device__ __forceinline__ OperandDesc(uint32_t saddr, int mn)
+        : base(mn ? sdesc_mn128(saddr) : sdesc_kmajor_sw128(saddr)),
+          step((mn ? MN_STEP : MMA_KB) >> 4) {}
+    // slice ks of the stage that lies `off` bytes after stage 0
+    __device__ __forceinline__ uint64_t at(uint32_t off, int ks) const {
+        return base + (off >> 4) + static_cast<uint32_t>(ks) * step;
+    }
+};
+
 // An operand as the loaders read it: element (row r, contraction index p) of group g at
 // ptr + g * gs + r * rs + p * ps.
 struct GOperand {
@@ -338,6 +353,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
             // ---------------- MMA issuer ----------------
             int stage = 0;
             uint32_t phase = 0, fixpar = 0;
+            const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
             bool ok = true;
             for (int local = 0; ok && next_tile<BN>(walk, p, t); ++local) {
                 const int acc = local & 1;
@@ -346,10 +362,9 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                                tmo))
                     break;
                 tc_fence_after();
-                uint32_t idesc = idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0);
-                if constexpr (TMA)
-                    idesc |= (static_cast<uint32_t>(p.p_mn) << 15) |
-                             (static_cast<uint32_t>(p.q_mn) << 16);
+                const uint32_t idesc = idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0) |
+                                       (static_cast<uint32_t>(p.p_mn) << 15) |
+                                       (static_cast<uint32_t>(p.q_mn) << 16);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 for (int kb = 0; kb < t.nk; kb += GBK) {
                     if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
@@ -358,35 +373,26 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
-                    const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
-                    if constexpr (TMA) {
-                        int steps = GBK / 16;
-                        if (p.wgrad && t.nk - kb < GBK) {
-                            steps = (t.nk - kb + 15) >> 4;
-                            if (t.nk & 15) {
-                                mbar_arrive(fixreq);
-                                if (!mbar_wait(fixdone, fixpar, abort_flag, p.status,
-                                               GK_DEV_TIMEOUT_MMA, tmo)) {
-                                    ok = false;
-                                    break;
-                                }
-                                fixpar ^= 1u;
-                                tc_fence_after();
+                    const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
+                    if (TMA && p.wgrad && t.nk - kb < GBK) {
+                        // the group's end: the rows past it up to a multiple of 16 are zeroed
+                        if (t.nk & 15) {
+                            mbar_arrive(fixreq);
+                            if (!mbar_wait(fixdone, fixpar, abort_flag, p.status,
+                                           GK_DEV_TIMEOUT_MMA, tmo)) {
+                                ok = false;
+                                break;
                             }
+                            fixpar ^= 1u;
+                            tc_fence_after();
                         }
+                        const int steps = (t.nk - kb + 15) >> 4;
                         for (int ks = 0; ks < steps; ++ks)
-                            mma_f16(d, p.p_mn ? sdesc_mn128(a0 + ks * MN_STEP)
-                                              : sdesc_kmajor_sw128(a0 + ks * MMA_KB),
-                                    p.q_mn ? sdesc_mn128(b0 + ks * MN_STEP)
-                                           : sdesc_kmajor_sw128(b0 + ks * MMA_KB),
-                                    idesc, (kb | ks) != 0 ? 1u : 0u);
+                            mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, (kb | ks) != 0 ? 1u : 0u);
                     } else {
 #pragma unroll
-                        for (int ks = 0; ks < BKB / MMA_KB; ++ks)
-                            mma_f16(d, sdesc_kmajor_sw128(a0 + ks * MMA_KB),
-                                    sdesc_kmajor_sw128(b0 + ks * MMA_KB), idesc,
-                                    (kb | ks) != 0 ? 1u : 0u);
+                        for (int ks = 0; ks < GBK / 16; ++ks)
+                            mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, (kb | ks) != 0 ? 1u : 0u);
                     }
                     mma_commit(&empty[stage]);
                     if (++stage == STAGES) {
@@ -592,6 +598,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
             const uint32_t fixreq1 = mapa_shared(smem_u32(fixreq), 1);
             int stage = 0;
             uint32_t phase = 0, fixpar = 0;
+            const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
             bool ok = true;
             for (int local = 0; ok && next_tile<BN, TM>(walk, p, t); ++local) {
                 const int acc = local & 1;
@@ -611,11 +618,8 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(sP + stage * C::P_BYTES);
-                    const uint32_t b0 = smem_u32(sQ + stage * C::Q_BYTES);
-                    int steps = GBK / 16;
+                    const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
                     if (p.wgrad && t.nk - kb < GBK) {
-                        steps = (t.nk - kb + 15) >> 4;
                         if (t.nk & 15) {
                             mbar_arrive_cluster(fixreq0);
                             mbar_arrive_cluster(fixreq1);
@@ -627,13 +631,16 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                             fixpar ^= 1u;
                             tc_fence_after();
                         }
+                        const int steps = (t.nk - kb + 15) >> 4;
+                        for (int ks = 0; ks < steps; ++ks)
+                            mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
+                                         (kb | ks) != 0 ? 1u : 0u);
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < GBK / 16; ++ks)
+                            mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
+                                         (kb | ks) != 0 ? 1u : 0u);
                     }
-                    for (int ks = 0; ks < steps; ++ks)
-                        mma_f16_pair(d, p.p_mn ? sdesc_mn128(a0 + ks * MN_STEP)
-                                               : sdesc_kmajor_sw128(a0 + ks * MMA_KB),
-                                     p.q_mn ? sdesc_mn128(b0 + ks * MN_STEP)
-                                            : sdesc_kmajor_sw128(b0 + ks * MMA_KB),
-                                     idesc, (kb | ks) != 0 ? 1u : 0u);
                     mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
                     if (++stage == STAGES) {
                         stage = 0;
