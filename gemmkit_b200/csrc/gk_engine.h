@@ -169,6 +169,10 @@ int launch_tc_gemm(const TcProblem& p, char* err, size_t errlen);
 int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, int64_t d2,
                     int64_t ld1, int64_t ld2, int box0, int box1, char* err, size_t errlen);
 
+// A tensor map of `lines` contiguous lines of 1024 bytes, boxes of `box` lines, not swizzled.
+int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int box, char* err,
+                      size_t errlen);
+
 // Device status word for the current device (bounded-wait give-ups are or-ed into it).
 unsigned int* device_status_ptr();
 

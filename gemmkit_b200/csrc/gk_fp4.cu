@@ -469,13 +469,18 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t ad, uint64_t bd, ui
             : "memory");
 }
 
-// One 512-byte scale atom (32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart) to four
-// TMEM columns, replicated to the four lane quarters. Executes in order with the later MMAs of
-// this thread.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
-    const uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) |
-                       (static_cast<uint64_t>(128u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+// The descriptor of a 512-byte scale atom: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes
+// apart.
+__device__ __forceinline__ uint64_t sdesc_scales(uint32_t saddr) {
+    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) |
+           (static_cast<uint64_t>(128u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
+}
+
+// One scale atom to four TMEM columns, replicated to the four lane quarters. Executes in order
+// with the later MMAs of this thread.
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
 }
 
 template <int FMT, int BN>
@@ -589,6 +594,7 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
             // ---------------- MMA issuer ----------------
             const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
             const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
+            const uint64_t dS = sdesc_scales(smem_u32(sSF));
             constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);  // both scale ids 2
             int stage = 0;
             uint32_t phase = 0;
@@ -611,10 +617,10 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sf = smem_u32(sSF + stage * 2 * C::SF);
+                    const uint64_t sd = dS + ((stage * 2 * C::SF) >> 4);
                     const uint32_t tsf = tmem_base + static_cast<uint32_t>(2 * BN + stage * C::SF_COLS);
 #pragma unroll
-                    for (int a = 0; a < 2 * ATOMS; ++a) copy_scales(tsf + 4 * a, sf + 512 * a);
+                    for (int a = 0; a < 2 * ATOMS; ++a) copy_scales(tsf + 4 * a, sd + 32 * a);
                     const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
                     const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
                     // slice ks: 64 elements = 32 bytes; its scales
@@ -690,6 +696,341 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
     }
 }
 
+// ---- the CTA-pair form -----------------------------------------------------------------------------
+//
+// Two CTAs compute 256 P rows x up to 256 Q rows with cta_group::2, each loading its 128 rows of P
+// and half of the Q rows (an SM then takes in 64 bytes of operands per cycle of MMA; the 128 x 128
+// tile of the kernel above takes 128, all that shared memory gives). Each SM computes its 128
+// rows times all Q rows, so both hold all of Q's scales.
+//
+// TMEM. Two 256-column accumulators and the scales need more than 512 columns, so the accumulators
+// overlap by OVER columns: accumulator 0 is columns [0, 256), accumulator 1 [256 - OVER, 512 -
+// OVER), the scales lie in the last OVER columns. The epilogue reads the shared columns first and
+// hands them over (thead) before it stores anything; the next tile's MMAs wait for that, not for
+// the rest. The scales have SLOTS slots; a slot is refilled once the MMAs of the stage that used it
+// last have finished (their commit on empty[]).
+
+template <int FMT>
+struct Fp4PairCfg {
+    static constexpr int BN = 256;
+    static constexpr int NEPI = 8;
+    static constexpr int EPI_W0 = 4;
+    static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
+    static constexpr int ATOMS = Fp4<FMT>::ATOMS;
+    static constexpr int SF = Fp4<FMT>::SF_BYTES;
+    static constexpr int P_BYTES = BM * BKB;
+    static constexpr int Q_BYTES = BN / 2 * BKB;
+    static constexpr int SF_STAGE = 3 * SF;  // P's block, Q's two blocks
+    static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + SF_STAGE;
+    static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
+    static constexpr int BAR_BYTES = 256;
+    static constexpr int STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    static constexpr int OFF_Q = STAGES * P_BYTES;
+    static constexpr int OFF_SF = OFF_Q + STAGES * Q_BYTES;
+    static constexpr int OFF_BARS = OFF_SF + STAGES * SF_STAGE;
+    static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
+    static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
+    static constexpr int OVER = 96;
+    static constexpr int SF_COLS = 12 * ATOMS;         // 4 of P, 8 of Q per atom
+    static constexpr int SLOTS = OVER / SF_COLS;       // mx 4, nv 2
+    static constexpr int SF_COL0 = 512 - OVER;
+    static_assert(SLOTS >= 2 && SLOTS <= STAGES && OVER % 32 == 0, "TMEM budget");
+    static_assert((2 * STAGES + 8) * 8 <= BAR_BYTES && SMEM <= SMEM_LIMIT, "shared memory budget");
+};
+
+template <int FMT>
+__device__ __forceinline__ void mma_fp4_pair(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc,
+                                             uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (FMT == GK_FP4_MX)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+            "[%5], p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb),
+            "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, "
+            "[%4], [%5], p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb),
+            "r"(accumulate)
+            : "memory");
+}
+
+// copy_scales in both CTAs of the pair, each from its own shared memory to its own TMEM.
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
+    fp4_pair_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
+                    const __grid_constant__ CUtensorMap tmQ32,
+                    const __grid_constant__ CUtensorMap tmPS,
+                    const __grid_constant__ CUtensorMap tmQS, const Fp4GemmParams p) {
+    using C = Fp4PairCfg<FMT>;
+    constexpr int STAGES = C::STAGES, BN = C::BN, ATOMS = C::ATOMS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sP = smem;
+    uint8_t* sQ = smem + C::OFF_Q;
+    uint8_t* sSF = smem + C::OFF_SF;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* thead = tempty + 2;
+    uint64_t* drain = thead + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
+    int* tile0 = off + GROUP_TABLE_INTS;
+    int* qblk = tile0 + GROUP_TABLE_INTS;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const uint64_t tmo = p.timeout_ns;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], 2 * C::NEPI);
+            mbar_init(&thead[a], 2 * C::NEPI);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmP);
+        prefetch_tmap(&tmQ);
+        prefetch_tmap(&tmQ32);
+        prefetch_tmap(&tmPS);
+        prefetch_tmap(&tmQS);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    griddep_wait();
+    load_groups(p.offsets, p.groups, p.rows, off, qblk, blockIdx.x == 0 ? p.status : nullptr,
+                [](int m) { return (m + 127) >> 7; });
+    if (warp == 0)
+        sum_groups(off, p.groups, tile0, [&](int m) { return (m + BN - 1) / BN * p.tiles_p; });
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t full_l = mapa_shared(smem_u32(&full[0]), 0);
+    const uint32_t tempty_l = mapa_shared(smem_u32(&tempty[0]), 0);
+    const uint32_t thead_l = mapa_shared(smem_u32(&thead[0]), 0);
+    GroupWalk walk(off, tile0, p.groups, blockIdx.x >> 1, gridDim.x >> 1);
+    int tp, tq;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- producer (both CTAs) ----------------
+            int stage = 0;
+            uint32_t phase = 0, issued = 0, last_par = 0;
+            bool ok = true;
+            while (ok && walk.next(p.tiles_p, tp, tq)) {
+                const int g = walk.g, q0 = tq * BN;
+                const int qn = off[g + 1] - off[g] - q0;
+                const int half = min(BN, (qn + 31) & ~31) >> 1;  // Q rows of each CTA
+                const int pieces = half > 96 ? 0 : (half + 31) >> 5;
+                const uint32_t bytes =
+                    2 * (C::STAGE_BYTES - (pieces ? C::Q_BYTES - pieces * 32 * BKB : 0));
+                const int prow = g * p.np + tp * 2 * BM + static_cast<int>(rank) * BM;
+                const int qrow = off[g] + q0 + static_cast<int>(rank) * half;
+                // lines of the scale maps: one stage of a 128-row block is SL lines (blocks that
+                // do not exist belong to rows that are not stored)
+                constexpr int SL = C::SF / 1024;
+                const int pl = (g * p.npb + tp * 2 + static_cast<int>(rank)) * p.stages * SL;
+                const int ql = (qblk[g] + (q0 >> 7)) * p.stages * SL;
+                for (int kb = 0; kb < p.stages; ++kb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = full_l + 8u * stage;
+                    if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
+                    uint8_t* dq = sQ + stage * C::Q_BYTES;
+                    uint8_t* sf = sSF + stage * C::SF_STAGE;
+                    tma_load_3d_pair(sP + stage * C::P_BYTES, &tmP, fb, kb * (FBK / 4), prow, 0);
+                    if (pieces == 0) tma_load_3d_pair(dq, &tmQ, fb, kb * (FBK / 4), qrow, 0);
+                    for (int i = 0; i < pieces; ++i)
+                        tma_load_3d_pair(dq + i * 32 * BKB, &tmQ32, fb, kb * (FBK / 4),
+                                         qrow + 32 * i, 0);
+                    tma_load_3d_pair(sf, &tmPS, fb, 0, pl + kb * SL, 0);
+                    tma_load_3d_pair(sf + C::SF, &tmQS, fb, 0, ql + kb * SL, 0);
+                    tma_load_3d_pair(sf + 2 * C::SF, &tmQS, fb, 0, ql + (p.stages + kb) * SL, 0);
+                    issued |= 1u << stage;
+                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            griddep_launch_dependents();
+            if (leader) {
+                int dummy = 0;
+                for (int s = 0; s < STAGES; ++s)
+                    if (issued & (1u << s))
+                        mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
+                                  GK_DEV_TIMEOUT_DRAIN, tmo);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ---------------- MMA issuer (leader) ----------------
+            const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
+            const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
+            const uint64_t dS = sdesc_scales(smem_u32(sSF));
+            constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);
+            int stage = 0, slot = 0, oldest = 0;  // oldest: the stage that used `slot` last
+            uint32_t phase = 0, oldest_phase = 0, used = 0;
+            bool ok = true;
+            for (int local = 0; ok && walk.next(p.tiles_p, tp, tq); ++local) {
+                const int acc = local & 1;
+                if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_MMA, tmo) ||
+                    (local > 0 && !mbar_wait(&thead[acc ^ 1], ((local - 1) >> 1) & 1, abort_flag,
+                                             p.status, GK_DEV_TIMEOUT_MMA, tmo)))
+                    break;
+                tc_fence_after();
+                const int qn = off[walk.g + 1] - off[walk.g] - tq * BN;
+                const uint32_t idesc = idesc_fp4<FMT>(2 * BM, min(BN, (qn + 31) & ~31), 0);
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * (BN - C::OVER));
+                for (int kb = 0; kb < p.stages; ++kb) {
+                    // the slot's last user has finished
+                    if (used == C::SLOTS) {
+                        if (!mbar_wait(&empty[oldest], oldest_phase, abort_flag, p.status,
+                                       GK_DEV_TIMEOUT_MMA, tmo)) {
+                            ok = false;
+                            break;
+                        }
+                        if (++oldest == STAGES) {
+                            oldest = 0;
+                            oldest_phase ^= 1u;
+                        }
+                    } else {
+                        ++used;
+                    }
+                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                                   tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t tsf =
+                        tmem_base + static_cast<uint32_t>(C::SF_COL0 + slot * C::SF_COLS);
+                    const uint64_t sd = dS + ((stage * C::SF_STAGE) >> 4);
+#pragma unroll
+                    for (int a = 0; a < ATOMS; ++a) {
+                        copy_scales_pair(tsf + 4 * a, sd + a * 32);
+                        copy_scales_pair(tsf + 4 * ATOMS + 8 * a, sd + ((C::SF >> 4) + a * 32));
+                        copy_scales_pair(tsf + 4 * ATOMS + 8 * a + 4,
+                                         sd + ((2 * C::SF >> 4) + a * 32));
+                    }
+                    const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
+                    const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
+                    auto slice = [&](int ks) {
+                        const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
+                        mma_fp4_pair<FMT>(d, ad + ks * 2, bd + ks * 2,
+                                          idesc + (FMT == GK_FP4_MX ? (ks & 1) * idesc_id2 : 0u),
+                                          tsf + 4 * atom, tsf + 4 * ATOMS + 8 * atom,
+                                          (kb | ks) != 0 ? 1u : 0u);
+                    };
+                    const int steps = (p.kdim - kb * FBK + 63) >> 6;
+                    if (steps >= 4) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) slice(ks);
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < 3; ++ks)
+                            if (ks < steps) slice(ks);
+                    }
+                    mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    if (++slot == C::SLOTS) slot = 0;
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+            }
+            mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            int dummy = 0;
+            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (warp >= C::EPI_W0) {
+        // ---------------- epilogue (both CTAs) ----------------
+        const int q = warp & 3;
+        const int h = (warp - C::EPI_W0) >> 2;  // which half of the columns
+        constexpr int HO = C::OVER / 2, HR = (BN - C::OVER) / 2;  // shared, other columns per warp
+        static_assert(HO % 16 == 0 && HR % 16 == 0, "chunks of 16 columns");
+        for (int local = 0; walk.next(p.tiles_p, tp, tq); ++local) {
+            const int acc = local & 1;
+            const uint32_t aph = (local >> 1) & 1;
+            if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
+                break;
+            tc_fence_after();
+            const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
+            const int i = (tp * 2 + static_cast<int>(rank)) * BM + q * 32 + lane;
+            const bool row_ok = i < p.np;
+            const int64_t at = (static_cast<int64_t>(off[walk.g]) + q0) * p.ldq + i * p.ldp;
+            const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                static_cast<uint32_t>(acc * (BN - C::OVER));
+            // first the columns that the next accumulator shares: accumulator 0's last, 1's first
+            const int s0 = (acc ? 0 : BN - C::OVER) + h * HO;
+            uint32_t v[HO / 16][32];
+#pragma unroll
+            for (int c = 0; c < HO / 16; ++c) tmem_ld_chunk<16>(tb + s0 + 16 * c, v[c]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < HO / 16; ++c) reg_fence<16>(v[c]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(thead_l + 8u * acc);
+            if (row_ok) {
+#pragma unroll
+                for (int c = 0; c < HO / 16; ++c) {
+                    const int j = s0 + 16 * c;
+                    if (j < qn)
+                        store_any<16>(p.c, p.out_type, at + j * p.ldq, p.ldq, v[c], qn - j, p.alpha,
+                                      p.beta);
+                }
+            }
+            const int r0 = (acc ? C::OVER : 0) + h * HR;
+#pragma unroll 1
+            for (int c = 0; c < HR && r0 + c < qn; c += 16) {
+                tmem_ld_x16(tb + r0 + c, v[0]);
+                if (row_ok)
+                    store_any<16>(p.c, p.out_type, at + (r0 + c) * p.ldq, p.ldq, v[0], qn - r0 - c,
+                                  p.alpha, p.beta);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(tempty_l + 8u * acc);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------
 
 int64_t fp4_pitch(int64_t cols) { return ((cols + 1) / 2 + 15) / 16 * 16; }
@@ -747,7 +1088,7 @@ Fp4View view_of(const gk_fp4_matrix* q) {
 // A launch that may start while the previous kernel of the stream drains (the kernels wait for it
 // before they touch memory).
 template <typename... Args>
-int launch_overlapped(void (*kern)(Args...), int grid, int threads, size_t smem, cudaStream_t st,
+int launch_overlapped(int cluster, void (*kern)(Args...), int grid, int threads, size_t smem, cudaStream_t st,
                       Args... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
@@ -755,11 +1096,22 @@ int launch_overlapped(void (*kern)(Args...), int grid, int threads, size_t smem,
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[n].val.clusterDim.y = 1;
+        attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (api_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = api_pdl_enabled() ? 1 : 0;
+    cfg.numAttrs = n;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess)
@@ -782,35 +1134,102 @@ int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensor
     if (e != cudaSuccess)
         return api_err(GK_ECUDA, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, Fp4GemmParams>(
-        kern, grid, C::THREADS, C::SMEM, st, tp, tq, tq32, p);
+        1, kern, grid, C::THREADS, C::SMEM, st, tp, tq, tq32, p);
+}
+
+// Clusters of the pair kernel that are resident at once on the current device (0 on failure).
+template <int FMT>
+int fp4_pair_clusters() {
+    using C = Fp4PairCfg<FMT>;
+    static int cache[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int& n = cache[dev & 63];
+    if (n == 0) {
+        cudaLaunchConfig_t q;
+        memset(&q, 0, sizeof(q));
+        q.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
+        q.blockDim = dim3(C::THREADS);
+        q.dynamicSmemBytes = C::SMEM;
+        cudaLaunchAttribute a[1];
+        a[0].id = cudaLaunchAttributeClusterDimension;
+        a[0].val.clusterDim.x = 2;
+        a[0].val.clusterDim.y = 1;
+        a[0].val.clusterDim.z = 1;
+        q.attrs = a;
+        q.numAttrs = 1;
+        int c = 0;
+        if (cudaFuncSetAttribute(fp4_pair_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&c, fp4_pair_kernel<FMT>, &q) != cudaSuccess || c <= 0) {
+            cudaGetLastError();
+            c = sm_count() / 2;
+        }
+        n = c;
+    }
+    return n;
 }
 
 template <int FMT>
 int run_fp4_gemm(Fp4GemmParams p, const gk_fp4_matrix* a, const gk_fp4_matrix* b, cudaStream_t st) {
-    const int bn = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
-    const int64_t tp = (p.np + BM - 1) / BM;
-    const int64_t tq = (static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups;
-    if (tp * tq > INT32_MAX / 2)
+    // an upper bound of the tiles (the device computes the true number from the offsets)
+    auto tiles_bound = [&](int64_t tm, int64_t bn) {
+        return (p.np + tm - 1) / tm * ((static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups);
+    };
+    const int64_t mean = (static_cast<int64_t>(p.rows) + p.groups - 1) / p.groups;
+    const int clusters = fp4_pair_clusters<FMT>();
+    // The pair kernel where its 256 x 256 tiles are mostly full on both sides and keep every
+    // cluster busy (a group that fills no whole tile still counts one in the bound).
+    const bool pair = !p.zero && p.np > BM && mean > BM &&
+                      tiles_bound(2 * BM, 256) - p.groups >= clusters;
+    const int bn = pair ? 256 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
+    const int tm = pair ? 2 * BM : BM;
+    const int64_t tiles = tiles_bound(tm, bn);
+    const int64_t lines = fp4_sf_bytes(FMT) / 1024;
+    const int64_t ablocks = (static_cast<int64_t>(p.rows) + 127) / 128 + p.groups;
+    const int64_t bblocks = static_cast<int64_t>(p.groups) * p.npb;
+    if (tiles > INT32_MAX / 2 || ablocks * p.stages * lines > INT32_MAX / 2 ||
+        bblocks * p.stages * lines > INT32_MAX / 2 ||
+        static_cast<int64_t>(p.groups) * p.np > INT32_MAX / 2)
         return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
-    p.tiles_p = static_cast<int>(tp);
-    const int sms = sm_count();
-    const int grid = static_cast<int>(tp * tq < sms ? tp * tq : sms);
+    p.tiles_p = static_cast<int>((p.np + tm - 1) / tm);
     CUtensorMap tmp, tmq, tmq32;
     memset(&tmp, 0, sizeof(tmp));
     memset(&tmq, 0, sizeof(tmq));
     memset(&tmq32, 0, sizeof(tmq32));
+    char err[256] = "";
+    int rc = 0;
     if (!p.zero) {
         // codes as 16-bit elements: four codes each, the pitch a multiple of 16 bytes
         const int64_t pe = fp4_pitch(p.kdim) / 2;
-        char err[256] = "";
-        int rc = encode_tmap_u16(&tmp, b->data, pe, static_cast<int64_t>(b->rows), 1, pe, pe, 64, BM,
-                                 err, sizeof(err));
+        rc = encode_tmap_u16(&tmp, b->data, pe, static_cast<int64_t>(b->rows), 1, pe, pe, 64, BM,
+                             err, sizeof(err));
         if (!rc)
-            rc = encode_tmap_u16(&tmq, a->data, pe, p.rows, 1, pe, pe, 64, bn, err, sizeof(err));
-        if (!rc)
+            rc = encode_tmap_u16(&tmq, a->data, pe, p.rows, 1, pe, pe, 64, pair ? 128 : bn, err,
+                                 sizeof(err));
+        if (!rc && bn > 32)
             rc = encode_tmap_u16(&tmq32, a->data, pe, p.rows, 1, pe, pe, 64, 32, err, sizeof(err));
         if (rc) return set_last_error(rc, err);
+        if (bn == 32) tmq32 = tmq;
     }
+    if (pair) {
+        using C = Fp4PairCfg<FMT>;
+        // the scale buffers as lines of 1024 bytes (both sizes are whole lines)
+        CUtensorMap tps, tqs;
+        rc = encode_tmap_lines(&tps, b->scales, bblocks * p.stages * lines, static_cast<int>(lines),
+                               err, sizeof(err));
+        const int64_t qb = static_cast<int64_t>(gk_fp4_scale_bytes(
+                               FMT, a->groups, a->offsets != nullptr, a->rows, a->cols)) / 1024;
+        if (!rc)
+            rc = encode_tmap_lines(&tqs, a->scales, qb, static_cast<int>(lines), err, sizeof(err));
+        if (rc) return set_last_error(rc, err);
+        const int grid = 2 * static_cast<int>(tiles < clusters ? tiles : clusters);
+        return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap,
+                                 Fp4GemmParams>(2, fp4_pair_kernel<FMT>, grid, C::THREADS, C::SMEM,
+                                                st, tmp, tmq, tmq32, tps, tqs, p);
+    }
+    const int sms = sm_count();
+    const int grid = static_cast<int>(tiles < sms ? tiles : sms);
     switch (bn) {
         case 32: return launch_fp4_gemm<FMT, 32>(tmp, tmq, tmq32, p, grid, st);
         case 64: return launch_fp4_gemm<FMT, 64>(tmp, tmq, tmq32, p, grid, st);
@@ -829,7 +1248,7 @@ int run_quantize(const void* x, int64_t rs, int64_t cs, int64_t gs, const Fp4Vie
                     (v.offsets || v.groups == 1 || (gs * es) % 16 == 0);
     const NvScale nv{scale, 1.0f / (6.0f * scale)};
     return launch_overlapped<const T*, int64_t, int64_t, int64_t, int, Fp4View, NvScale>(
-        quantize_fp4_kernel<FMT, T>, unit_grid(static_cast<int64_t>(v.rows) * v.stages), 256, 0, st,
+        1, quantize_fp4_kernel<FMT, T>, unit_grid(static_cast<int64_t>(v.rows) * v.stages), 256, 0, st,
         static_cast<const T*>(x), rs, cs, gs, vec, v, nv);
 }
 
@@ -917,7 +1336,7 @@ int gk_dequantize_fp4(const gk_fp4_matrix* q, gk_matmut out, gk_stream_t stream)
     auto kern = q->fmt == GK_FP4_MX ? dequantize_fp4_kernel<GK_FP4_MX>
                                     : dequantize_fp4_kernel<GK_FP4_NV>;
     return launch_overlapped<Fp4View, float, float*, int64_t, int64_t, int>(
-        kern, grid, 256, 0, static_cast<cudaStream_t>(stream), v, q->scale,
+        1, kern, grid, 256, 0, static_cast<cudaStream_t>(stream), v, q->scale,
         static_cast<float*>(out.data), out.rs, out.cs, vec);
 }
 
@@ -947,7 +1366,7 @@ int gk_fp4_import(const uint8_t* codes, size_t codes_len, size_t codes_ld, const
     const int grid = unit_grid(static_cast<int64_t>(v.rows) * v.stages);
     auto kern = dst->fmt == GK_FP4_MX ? import_fp4_kernel<GK_FP4_MX> : import_fp4_kernel<GK_FP4_NV>;
     return launch_overlapped<const uint8_t*, int64_t, const uint8_t*, int64_t, Fp4View>(
-        kern, grid, 256, 0, static_cast<cudaStream_t>(stream), codes,
+        1, kern, grid, 256, 0, static_cast<cudaStream_t>(stream), codes,
         static_cast<int64_t>(codes_ld), scales, static_cast<int64_t>(scales_ld), v);
 }
 

@@ -708,6 +708,28 @@ int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, i
     return 0;
 }
 
+int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int box, char* err,
+                      size_t errlen) {
+    PFN_tmapEncodeTiled enc = get_encode();
+    if (!enc) {
+        snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled is unavailable (driver too old?)");
+        return 5;
+    }
+    cuuint64_t dims[3] = {256, static_cast<cuuint64_t>(lines), 1};
+    cuuint64_t strides[2] = {1024, 1024};
+    cuuint32_t boxd[3] = {256, static_cast<cuuint32_t>(box), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), dims, strides,
+                     boxd, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled (scales) failed (%d)",
+                 static_cast<int>(r));
+        return 3;
+    }
+    return 0;
+}
+
 static int encode_operand_uncached(CUtensorMap* map, const Operand& op, int64_t K, int64_t batch,
                                    int es, int box_rows, char* err, size_t errlen) {
     PFN_tmapEncodeTiled enc = get_encode();

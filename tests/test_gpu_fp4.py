@@ -478,3 +478,24 @@ def test_long_matrix_passes_32_bits():
     product(q, b, c)
     assert torch.equal(c[base:base + 300].double(), tv @ bv.T)
     assert not bool(c[:base].any())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,k,n", [(2560, 320, 2560), (1300, 1000, 5000), (4097, 64, 1288),
+                                   (300, 2304, 19000)])
+def test_product_exact_large(fmt, m, k, n):
+    """Sizes that the CTA-pair kernel takes: whole and cut tiles, short and long contractions."""
+    torch = torch_cuda()
+    a, av = grid_operand(m + k, m, k, fmt)
+    b, bv = grid_operand(n + k + 1, n, k, fmt)
+    c = torch.full((m, n), float("nan"), device="cuda")
+    product(a, b, c)
+    assert torch.equal(c.double(), av @ bv.T)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("sizes,lead,tail", [([1000, 0, 700, 255, 257, 1, 2083], 2, 5),
+                                             ([31, 4000, 33], 0, 1), ([300, 129, 160, 513], 0, 0)])
+@pytest.mark.parametrize("k,n", [(320, 2600), (1000, 4224)])
+def test_product_by_expert_large(fmt, sizes, lead, tail, k, n):
+    test_product_by_expert(fmt, sizes, lead, tail, k, n)
