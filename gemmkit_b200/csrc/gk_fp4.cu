@@ -708,7 +708,9 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
 // OVER), the scales lie in the last OVER columns. The epilogue reads the shared columns first and
 // hands them over (thead) before it stores anything; the next tile's MMAs wait for that, not for
 // the rest. The scales have SLOTS slots; a slot is refilled once the MMAs of the stage that used it
-// last have finished (their commit on empty[]).
+// last have finished (their commit on empty[]). Warp 3 issues the copies of scales to TMEM ahead of
+// the MMA warp: issued between the MMAs by the same thread, the 12 (nv) or 6 (mx) copies of a
+// stage took MMA issue time.
 
 template <int FMT>
 struct Fp4PairCfg {
@@ -735,7 +737,8 @@ struct Fp4PairCfg {
     static constexpr int SLOTS = OVER / SF_COLS;       // mx 4, nv 2
     static constexpr int SF_COL0 = 512 - OVER;
     static_assert(SLOTS >= 2 && SLOTS <= STAGES && OVER % 32 == 0, "TMEM budget");
-    static_assert((2 * STAGES + 8) * 8 <= BAR_BYTES && SMEM <= SMEM_LIMIT, "shared memory budget");
+    static_assert((2 * STAGES + SLOTS + 10) * 8 <= BAR_BYTES && SMEM <= SMEM_LIMIT,
+                  "shared memory budget");
 };
 
 template <int FMT>
@@ -781,8 +784,9 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
     uint64_t* tfull = empty + STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* thead = tempty + 2;
-    uint64_t* drain = thead + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* sfull = thead + 2;  // a slot's scales are in TMEM
+    uint64_t* drain = sfull + C::SLOTS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
     int* tile0 = off + GROUP_TABLE_INTS;
@@ -802,7 +806,9 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
             mbar_init(&tempty[a], 2 * C::NEPI);
             mbar_init(&thead[a], 2 * C::NEPI);
         }
+        for (int s = 0; s < C::SLOTS; ++s) mbar_init(&sfull[s], 1);
         mbar_init(drain, 1);
+        mbar_init(drain + 1, 1);
         *abort_flag = 0;
         fence_mbar_init();
         prefetch_tmap(&tmP);
@@ -891,10 +897,9 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
             // ---------------- MMA issuer (leader) ----------------
             const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
             const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
-            const uint64_t dS = sdesc_scales(smem_u32(sSF));
             constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);
-            int stage = 0, slot = 0, oldest = 0;  // oldest: the stage that used `slot` last
-            uint32_t phase = 0, oldest_phase = 0, used = 0;
+            int stage = 0, slot = 0;
+            uint32_t phase = 0, slot_phase = 0;
             bool ok = true;
             for (int local = 0; ok && walk.next(p.tiles_p, tp, tq); ++local) {
                 const int acc = local & 1;
@@ -908,7 +913,61 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                 const uint32_t idesc = idesc_fp4<FMT>(2 * BM, min(BN, (qn + 31) & ~31), 0);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * (BN - C::OVER));
                 for (int kb = 0; kb < p.stages; ++kb) {
-                    // the slot's last user has finished
+                    if (!mbar_wait(&sfull[slot], slot_phase, abort_flag, p.status,
+                                   GK_DEV_TIMEOUT_MMA, tmo) ||
+                        !mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                                   tmo)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t tsf =
+                        tmem_base + static_cast<uint32_t>(C::SF_COL0 + slot * C::SF_COLS);
+                    const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
+                    const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
+                    auto slice = [&](int ks) {
+                        const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
+                        mma_fp4_pair<FMT>(d, ad + ks * 2, bd + ks * 2,
+                                          idesc + (FMT == GK_FP4_MX ? (ks & 1) * idesc_id2 : 0u),
+                                          tsf + 4 * atom, tsf + 4 * ATOMS + 8 * atom,
+                                          (kb | ks) != 0 ? 1u : 0u);
+                    };
+                    const int steps = (p.kdim - kb * FBK + 63) >> 6;
+                    if (steps >= 4) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) slice(ks);
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < 3; ++ks)
+                            if (ks < steps) slice(ks);
+                    }
+                    mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    if (++slot == C::SLOTS) {
+                        slot = 0;
+                        slot_phase ^= 1u;
+                    }
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+            }
+            mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            int dummy = 0;
+            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+        }
+    } else if (warp == 3) {
+        if (lane == 0 && leader) {
+            // ---------------- scales to TMEM (leader, for both CTAs) ----------------
+            const uint64_t dS = sdesc_scales(smem_u32(sSF));
+            int stage = 0, slot = 0, oldest = 0;  // oldest: the stage that used `slot` last
+            uint32_t phase = 0, oldest_phase = 0, used = 0;
+            bool ok = true;
+            while (ok && walk.next(p.tiles_p, tp, tq)) {
+                for (int kb = 0; kb < p.stages; ++kb) {
+                    // the MMAs of the slot's last user have finished
                     if (used == C::SLOTS) {
                         if (!mbar_wait(&empty[oldest], oldest_phase, abort_flag, p.status,
                                        GK_DEV_TIMEOUT_MMA, tmo)) {
@@ -938,37 +997,17 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                         copy_scales_pair(tsf + 4 * ATOMS + 8 * a + 4,
                                          sd + ((2 * C::SF >> 4) + a * 32));
                     }
-                    const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
-                    const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
-                    auto slice = [&](int ks) {
-                        const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
-                        mma_fp4_pair<FMT>(d, ad + ks * 2, bd + ks * 2,
-                                          idesc + (FMT == GK_FP4_MX ? (ks & 1) * idesc_id2 : 0u),
-                                          tsf + 4 * atom, tsf + 4 * ATOMS + 8 * atom,
-                                          (kb | ks) != 0 ? 1u : 0u);
-                    };
-                    const int steps = (p.kdim - kb * FBK + 63) >> 6;
-                    if (steps >= 4) {
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) slice(ks);
-                    } else {
-#pragma unroll
-                        for (int ks = 0; ks < 3; ++ks)
-                            if (ks < steps) slice(ks);
-                    }
-                    mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    mma_commit_pair(mapa_shared(smem_u32(&sfull[slot]), 0));
                     if (++slot == C::SLOTS) slot = 0;
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
-                if (!ok) break;
-                mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
             }
-            mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            mma_commit_pair(mapa_shared(smem_u32(drain + 1), 0));
             int dummy = 0;
-            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+            mbar_wait(drain + 1, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp >= C::EPI_W0) {
         // ---------------- epilogue (both CTAs) ----------------
