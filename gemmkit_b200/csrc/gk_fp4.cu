@@ -107,12 +107,12 @@ __device__ __forceinline__ uint32_t nv_block_scale(float amax, const NvScale& n)
 // Eight elements over d = sb * s, exactly as nv_block_scale: the quotient in f32 within 2^-21,
 // and next to a border the comparison |x| with border * sb * s in f64 (4 + 4 + 24 bits).
 __device__ __forceinline__ uint32_t nv_elements(const float (&x)[8], float r, float sb, float s) {
+    const float rlo = r * (1.0f - 0x1p-20f), rhi = r * (1.0f + 0x1p-20f);
     float lo[8], hi[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float y = x[i] * r;
-        lo[i] = y * (1.0f - 0x1p-20f);
-        hi[i] = y * (1.0f + 0x1p-20f);
+        lo[i] = x[i] * rlo;
+        hi[i] = x[i] * rhi;
     }
     uint32_t w = cvt_e2m1x8(lo);
     const uint32_t w2 = cvt_e2m1x8(hi);
@@ -130,36 +130,6 @@ __device__ __forceinline__ uint32_t nv_elements(const float (&x)[8], float r, fl
         }
     }
     return w;
-}
-
-__device__ __forceinline__ float load_f(const float* p) { return __ldg(p); }
-__device__ __forceinline__ float load_f(const __half* p) { return __half2float(__ldg(p)); }
-__device__ __forceinline__ float load_f(const __nv_bfloat16* p) {
-    return __bfloat162float(__ldg(p));
-}
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
-        v[2 * i] = __low2float(h);
-        v[2 * i + 1] = __high2float(h);
-    }
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
 }
 
 // ---- where a row lies ----------------------------------------------------------------------------
@@ -254,11 +224,40 @@ __device__ __forceinline__ uint32_t block_codes(const float (&x)[8], uint32_t am
     }
 }
 
-// Rows with contiguous elements (or any column stride, slower). A warp takes 256 elements of a
-// row (one stage), a lane eight: loads of 16 bytes (two for f32), the block's maximum by
-// shuffles, four bytes of codes stored. Elements past the row are zero, and so are the scales of
-// blocks past it (the product reads whole stages).
-template <int FMT, typename T>
+// Eight elements of a row as loaded: 16 bytes of 16-bit floats, or 32 of f32.
+template <typename T>
+struct Raw8 {
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+            q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    // element by element: any stride, zero at or past column `cols`
+    __device__ __forceinline__ void load(const T* src, int64_t cs, int k, int cols) {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = k + i < cols ? src[static_cast<int64_t>(k + i) * cs] : T(0.0f);
+        memcpy(q, v, sizeof(v));
+    }
+    __device__ __forceinline__ void values(float (&x)[8]) const {
+        T v[8];
+        memcpy(v, q, sizeof(v));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f(v[i]);
+    }
+    static __device__ __forceinline__ float to_f(float v) { return v; }
+    static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+};
+
+// A warp takes up to QU stages (256 elements each) of a row, a lane eight elements of each: loads
+// of 16 bytes (two for f32), the block's maximum by shuffles, four bytes of codes stored.
+// Elements past the row are zero, and so are the scales of blocks past it (the product reads
+// whole stages). QU is 4 where that still gives every SM's warps a unit, so that enough loads are
+// in flight, else 1: for one row of 4096 the four would only follow each other.
+template <int FMT, typename T, int QU>
 __global__ void __launch_bounds__(256)
     quantize_fp4_kernel(const T* __restrict__ x, int64_t rs, int64_t cs, int64_t gs, int vec,
                         Fp4View v, NvScale nv) {
@@ -270,38 +269,53 @@ __global__ void __launch_bounds__(256)
                     blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
     const int lane = threadIdx.x & 31;
     constexpr int LPB = Fp4<FMT>::BS / 8;  // lanes per block
-    const int64_t units = static_cast<int64_t>(v.rows) * v.stages;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-         u < units; u += step) {
-        const int r = static_cast<int>(u / v.stages), st = static_cast<int>(u - static_cast<int64_t>(r) * v.stages);
+    const uint32_t chunks = static_cast<uint32_t>(v.stages + QU - 1) / QU;  // of a row
+    // units (row, chunk), counted in 64 bits only where 32 do not hold them
+    const uint64_t units = static_cast<uint64_t>(v.rows) * chunks;
+    const uint32_t step = gridDim.x * (blockDim.x >> 5);
+    for (uint64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
+        const int r = units >> 32 ? static_cast<int>(u / chunks)
+                                  : static_cast<int>(static_cast<uint32_t>(u) / chunks);
+        const int st0 = static_cast<int>(u - static_cast<uint64_t>(r) * chunks) * QU;
         int block, in, g, at;
         if (!find_row(v, map, r, block, in, g, at)) continue;
-        const int k = st * FBK + lane * 8;
         // a stack's groups lie gs apart; ragged groups and a single one lie row after row
         const T* src = x + (v.offsets ? static_cast<int64_t>(r) * rs : g * gs + at * rs);
-        float e[8];
-        if (vec && k + 8 <= v.cols) {
-            load8(src + k, e);
+        uint8_t* dst = v.data + static_cast<int64_t>(r) * v.pitch + lane * 4;
+        Raw8<T> raw[QU];
+        if (vec && (st0 + QU) * FBK <= v.cols) {
+#pragma unroll
+            for (int i = 0; i < QU; ++i) raw[i].load(src + (st0 + i) * FBK + lane * 8);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                e[i] = k + i < v.cols ? load_f(src + static_cast<int64_t>(k + i) * cs) : 0.0f;
+            for (int i = 0; i < QU; ++i) {
+                const int k = (st0 + i) * FBK + lane * 8;
+                if (vec && k + 8 <= v.cols)
+                    raw[i].load(src + k);
+                else
+                    raw[i].load(src, cs, k, v.cols);
+            }
         }
-        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(e[i]) & 0x7FFFFFFFu);
+        for (int i = 0; i < QU; ++i) {
+            const int st = st0 + i;
+            if (st >= v.stages) break;
+            float e[8];
+            raw[i].values(e);
+            uint32_t m = 0;
 #pragma unroll
-        for (int d = 1; d < LPB; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        float mul, sb;
-        const uint32_t b = block_scale<FMT>(m, nv, mul, sb);
-        const uint32_t w = block_codes<FMT>(e, m, mul, sb, nv);
-        const int64_t byte = static_cast<int64_t>(st) * (FBK / 2) + lane * 4;
-        if (byte < v.pitch)
-            *reinterpret_cast<uint32_t*>(v.data + static_cast<int64_t>(r) * v.pitch + byte) = w;
-        if (lane % LPB == 0)
-            *scale_ptr<FMT>(v, block, in, st * (32 / LPB) + lane / LPB) =
-                static_cast<uint8_t>(k < v.cols ? b : 0u);
+            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(e[j]) & 0x7FFFFFFFu);
+#pragma unroll
+            for (int d = 1; d < LPB; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+            float mul, sb;
+            const uint32_t b = block_scale<FMT>(m, nv, mul, sb);
+            const uint32_t w = block_codes<FMT>(e, m, mul, sb, nv);
+            const int byte = st * (FBK / 2);
+            if (byte + lane * 4 < v.pitch) *reinterpret_cast<uint32_t*>(dst + byte) = w;
+            if (lane % LPB == 0)
+                *scale_ptr<FMT>(v, block, in, st * (32 / LPB) + lane / LPB) =
+                    static_cast<uint8_t>(st * FBK + lane * 8 < v.cols ? b : 0u);
+        }
     }
 }
 
@@ -316,11 +330,13 @@ __global__ void __launch_bounds__(256)
         load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
                     blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
     const int lane = threadIdx.x & 31;
-    const int64_t units = static_cast<int64_t>(v.rows) * v.stages;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-         u < units; u += step) {
-        const int r = static_cast<int>(u / v.stages), st = static_cast<int>(u - static_cast<int64_t>(r) * v.stages);
+    const uint32_t stages = static_cast<uint32_t>(v.stages);
+    const uint64_t units = static_cast<uint64_t>(v.rows) * stages;
+    const uint32_t step = gridDim.x * (blockDim.x >> 5);
+    for (uint64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
+        const int r = units >> 32 ? static_cast<int>(u / stages)
+                                  : static_cast<int>(static_cast<uint32_t>(u) / stages);
+        const int st = static_cast<int>(u - static_cast<uint64_t>(r) * stages);
         int block, in, g, at;
         if (!find_row(v, map, r, block, in, g, at)) continue;
         const int k = st * FBK + lane * 8;
@@ -359,11 +375,13 @@ __global__ void __launch_bounds__(256)
         load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
                     blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
     const int lane = threadIdx.x & 31;
-    const int64_t units = static_cast<int64_t>(v.rows) * v.stages;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-         u < units; u += step) {
-        const int r = static_cast<int>(u / v.stages), st = static_cast<int>(u - static_cast<int64_t>(r) * v.stages);
+    const uint32_t stages = static_cast<uint32_t>(v.stages);
+    const uint64_t units = static_cast<uint64_t>(v.rows) * stages;
+    const uint32_t step = gridDim.x * (blockDim.x >> 5);
+    for (uint64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
+        const int r = units >> 32 ? static_cast<int>(u / stages)
+                                  : static_cast<int>(static_cast<uint32_t>(u) / stages);
+        const int st = static_cast<int>(u - static_cast<uint64_t>(r) * stages);
         int block, in, g, at;
         if (!find_row(v, map, r, block, in, g, at)) continue;
         const int64_t byte = static_cast<int64_t>(st) * (FBK / 2) + lane * 4;
@@ -732,12 +750,12 @@ struct Fp4PairCfg {
     static constexpr int OFF_BARS = OFF_SF + STAGES * SF_STAGE;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
-    static constexpr int OVER = 96;
+    static constexpr int OVER = FMT == GK_FP4_MX ? 96 : 160;
     static constexpr int SF_COLS = 12 * ATOMS;         // 4 of P, 8 of Q per atom
-    static constexpr int SLOTS = OVER / SF_COLS;       // mx 4, nv 2
+    static constexpr int SLOTS = OVER / SF_COLS;       // mx 4, nv 3
     static constexpr int SF_COL0 = 512 - OVER;
     static_assert(SLOTS >= 2 && SLOTS <= STAGES && OVER % 32 == 0, "TMEM budget");
-    static_assert((2 * STAGES + SLOTS + 10) * 8 <= BAR_BYTES && SMEM <= SMEM_LIMIT,
+    static_assert((2 * STAGES + SLOTS + 11) * 8 <= BAR_BYTES && SMEM <= SMEM_LIMIT,
                   "shared memory budget");
 };
 
@@ -786,7 +804,7 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
     uint64_t* thead = tempty + 2;
     uint64_t* sfull = thead + 2;  // a slot's scales are in TMEM
     uint64_t* drain = sfull + C::SLOTS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 3);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
     int* tile0 = off + GROUP_TABLE_INTS;
@@ -809,6 +827,7 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
         for (int s = 0; s < C::SLOTS; ++s) mbar_init(&sfull[s], 1);
         mbar_init(drain, 1);
         mbar_init(drain + 1, 1);
+        mbar_init(drain + 2, 1);
         *abort_flag = 0;
         fence_mbar_init();
         prefetch_tmap(&tmP);
@@ -893,8 +912,8 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
-            // ---------------- MMA issuer (leader) ----------------
+        if (leader) {
+            // ---------------- MMA issuer (leader; the whole warp, one lane issues) ----------------
             const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
             const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
             constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);
@@ -903,9 +922,9 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
             bool ok = true;
             for (int local = 0; ok && walk.next(p.tiles_p, tp, tq); ++local) {
                 const int acc = local & 1;
-                if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1u, abort_flag, p.status,
+                if (!warp_wait(&tempty[acc], ((local >> 1) & 1) ^ 1u, abort_flag, p.status,
                                GK_DEV_TIMEOUT_MMA, tmo) ||
-                    (local > 0 && !mbar_wait(&thead[acc ^ 1], ((local - 1) >> 1) & 1, abort_flag,
+                    (local > 0 && !warp_wait(&thead[acc ^ 1], ((local - 1) >> 1) & 1, abort_flag,
                                              p.status, GK_DEV_TIMEOUT_MMA, tmo)))
                     break;
                 tc_fence_after();
@@ -913,9 +932,9 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                 const uint32_t idesc = idesc_fp4<FMT>(2 * BM, min(BN, (qn + 31) & ~31), 0);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * (BN - C::OVER));
                 for (int kb = 0; kb < p.stages; ++kb) {
-                    if (!mbar_wait(&sfull[slot], slot_phase, abort_flag, p.status,
+                    if (!warp_wait(&sfull[slot], slot_phase, abort_flag, p.status,
                                    GK_DEV_TIMEOUT_MMA, tmo) ||
-                        !mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                        !warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
                                    tmo)) {
                         ok = false;
                         break;
@@ -933,15 +952,18 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                                           (kb | ks) != 0 ? 1u : 0u);
                     };
                     const int steps = (p.kdim - kb * FBK + 63) >> 6;
-                    if (steps >= 4) {
+                    if (elect_one()) {
+                        if (steps >= 4) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) slice(ks);
-                    } else {
+                            for (int ks = 0; ks < 4; ++ks) slice(ks);
+                        } else {
 #pragma unroll
-                        for (int ks = 0; ks < 3; ++ks)
-                            if (ks < steps) slice(ks);
+                            for (int ks = 0; ks < 3; ++ks)
+                                if (ks < steps) slice(ks);
+                        }
+                        mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
                     }
-                    mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    __syncwarp();
                     if (++slot == C::SLOTS) {
                         slot = 0;
                         slot_phase ^= 1u;
@@ -952,52 +974,56 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                     }
                 }
                 if (!ok) break;
-                mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+                if (elect_one()) mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+                __syncwarp();
             }
-            mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            if (elect_one()) mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            __syncwarp();
             int dummy = 0;
             mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
         }
-    } else if (warp == 3) {
-        if (lane == 0 && leader) {
+    } else if (warp == 2 || warp == 3) {
+        if (leader) {
             // ---------------- scales to TMEM (leader, for both CTAs) ----------------
+            // warp 2 takes the even stages of the ring's order, warp 3 the odd ones
             const uint64_t dS = sdesc_scales(smem_u32(sSF));
+            uint64_t* done = drain + (warp - 1);
             int stage = 0, slot = 0, oldest = 0;  // oldest: the stage that used `slot` last
-            uint32_t phase = 0, oldest_phase = 0, used = 0;
+            uint32_t phase = 0, oldest_phase = 0, count = 0;
             bool ok = true;
             while (ok && walk.next(p.tiles_p, tp, tq)) {
-                for (int kb = 0; kb < p.stages; ++kb) {
-                    // the MMAs of the slot's last user have finished
-                    if (used == C::SLOTS) {
-                        if (!mbar_wait(&empty[oldest], oldest_phase, abort_flag, p.status,
+                for (int kb = 0; kb < p.stages; ++kb, ++count) {
+                    if ((count & 1u) == static_cast<uint32_t>(warp - 2)) {
+                        // the MMAs of the slot's last user have finished
+                        if ((count >= C::SLOTS &&
+                             !warp_wait(&empty[oldest], oldest_phase, abort_flag, p.status,
+                                        GK_DEV_TIMEOUT_MMA, tmo)) ||
+                            !warp_wait(&full[stage], phase, abort_flag, p.status,
                                        GK_DEV_TIMEOUT_MMA, tmo)) {
                             ok = false;
                             break;
                         }
-                        if (++oldest == STAGES) {
-                            oldest = 0;
-                            oldest_phase ^= 1u;
-                        }
-                    } else {
-                        ++used;
-                    }
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
-                                   tmo)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t tsf =
-                        tmem_base + static_cast<uint32_t>(C::SF_COL0 + slot * C::SF_COLS);
-                    const uint64_t sd = dS + ((stage * C::SF_STAGE) >> 4);
+                        tc_fence_after();
+                        const uint32_t tsf =
+                            tmem_base + static_cast<uint32_t>(C::SF_COL0 + slot * C::SF_COLS);
+                        const uint64_t sd = dS + ((stage * C::SF_STAGE) >> 4);
+                        if (elect_one()) {
 #pragma unroll
-                    for (int a = 0; a < ATOMS; ++a) {
-                        copy_scales_pair(tsf + 4 * a, sd + a * 32);
-                        copy_scales_pair(tsf + 4 * ATOMS + 8 * a, sd + ((C::SF >> 4) + a * 32));
-                        copy_scales_pair(tsf + 4 * ATOMS + 8 * a + 4,
-                                         sd + ((2 * C::SF >> 4) + a * 32));
+                            for (int a = 0; a < ATOMS; ++a) {
+                                copy_scales_pair(tsf + 4 * a, sd + a * 32);
+                                copy_scales_pair(tsf + 4 * ATOMS + 8 * a,
+                                                 sd + ((C::SF >> 4) + a * 32));
+                                copy_scales_pair(tsf + 4 * ATOMS + 8 * a + 4,
+                                                 sd + ((2 * C::SF >> 4) + a * 32));
+                            }
+                            mma_commit_pair(mapa_shared(smem_u32(&sfull[slot]), 0));
+                        }
+                        __syncwarp();
                     }
-                    mma_commit_pair(mapa_shared(smem_u32(&sfull[slot]), 0));
+                    if (count >= C::SLOTS && ++oldest == STAGES) {
+                        oldest = 0;
+                        oldest_phase ^= 1u;
+                    }
                     if (++slot == C::SLOTS) slot = 0;
                     if (++stage == STAGES) {
                         stage = 0;
@@ -1005,9 +1031,10 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                     }
                 }
             }
-            mma_commit_pair(mapa_shared(smem_u32(drain + 1), 0));
+            if (elect_one()) mma_commit_pair(mapa_shared(smem_u32(done), 0));
+            __syncwarp();
             int dummy = 0;
-            mbar_wait(drain + 1, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+            mbar_wait(done, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp >= C::EPI_W0) {
         // ---------------- epilogue (both CTAs) ----------------
@@ -1286,9 +1313,15 @@ int run_quantize(const void* x, int64_t rs, int64_t cs, int64_t gs, const Fp4Vie
                     (rows1 || (rs * es) % 16 == 0) &&
                     (v.offsets || v.groups == 1 || (gs * es) % 16 == 0);
     const NvScale nv{scale, 1.0f / (6.0f * scale)};
-    return launch_overlapped<const T*, int64_t, int64_t, int64_t, int, Fp4View, NvScale>(
-        1, quantize_fp4_kernel<FMT, T>, unit_grid(static_cast<int64_t>(v.rows) * v.stages), 256, 0, st,
-        static_cast<const T*>(x), rs, cs, gs, vec, v, nv);
+    auto go = [&](auto qu_tag) {
+        constexpr int QU = decltype(qu_tag)::value;
+        return launch_overlapped<const T*, int64_t, int64_t, int64_t, int, Fp4View, NvScale>(
+            1, quantize_fp4_kernel<FMT, T, QU>,
+            unit_grid(static_cast<int64_t>(v.rows) * ((v.stages + QU - 1) / QU)), 256, 0, st,
+            static_cast<const T*>(x), rs, cs, gs, vec, v, nv);
+    };
+    const bool large = static_cast<int64_t>(v.rows) * v.stages >= 4 * 32 * static_cast<int64_t>(sm_count());
+    return large ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 1>{});
 }
 
 }  // namespace

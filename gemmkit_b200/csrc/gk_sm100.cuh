@@ -29,6 +29,16 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
     return t;
 }
 
+// One lane of a converged warp (the same one every time), chosen so that the compiler sees the
+// code around it as warp-uniform: operands of the tensor-core instructions then stay in uniform
+// registers instead of being moved there before each one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p != 0;
+}
+
 // ---- mbarrier --------------------------------------------------------------------------
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
