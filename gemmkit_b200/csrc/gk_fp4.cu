@@ -437,7 +437,7 @@ struct Fp4Cfg {
     static constexpr int Q_BYTES = BN * BKB;
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + 2 * SF;
     static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
-    static constexpr int BAR_BYTES = 256;
+    static constexpr int BAR_BYTES = 512;
     static constexpr int RAW_STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
     // TMEM: two accumulators, then each stage's scales (its own columns: they are free again when
     // the stage is)
@@ -454,7 +454,7 @@ struct Fp4Cfg {
     static constexpr int TMEM_COLS = 512;
     static_assert(BN == 32 || BN == 64 || BN == 128, "tile width");
     static_assert(STAGES >= 2 && SMEM <= SMEM_LIMIT, "shared memory budget");
-    static_assert((2 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
+    static_assert((3 * STAGES + 7) * 8 <= BAR_BYTES, "barrier area");
 };
 
 // Instruction descriptor of kind::mxf4 / mxf4nvf4: both operands e2m1 (1 at bits 7 and 10), K-major,
@@ -515,10 +515,11 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
     uint8_t* sSF = smem + C::OFF_SF;  // per stage: P's scales, then Q's
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
     uint64_t* empty = full + STAGES;
-    uint64_t* tfull = empty + STAGES;
+    uint64_t* sfull = empty + STAGES;  // a stage's scales are in TMEM
+    uint64_t* tfull = sfull + STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
     int* tile0 = off + GROUP_TABLE_INTS;
@@ -530,12 +531,14 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+            mbar_init(&sfull[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
             mbar_init(&tempty[a], C::NEPI);
         }
         mbar_init(drain, 1);
+        mbar_init(drain + 1, 1);
         *abort_flag = 0;
         fence_mbar_init();
         if (!p.zero) {
@@ -608,48 +611,42 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
                               GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ---------------- MMA issuer ----------------
-            const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
-            const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
-            const uint64_t dS = sdesc_scales(smem_u32(sSF));
-            constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);  // both scale ids 2
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int local = 0; ok && walk.next(p.tiles_p, tp, tq); ++local) {
-                const int acc = local & 1;
-                const uint32_t aph = (local >> 1) & 1;
-                if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
-                               tmo))
+        // ---------------- MMA issuer (the whole warp, one lane issues) ----------------
+        const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
+        const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
+        constexpr uint32_t idesc_id2 = (2u << 4) | (2u << 29);  // both scale ids 2
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int local = 0; ok && walk.next(p.tiles_p, tp, tq); ++local) {
+            const int acc = local & 1;
+            const uint32_t aph = (local >> 1) & 1;
+            if (!warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo))
+                break;
+            tc_fence_after();
+            const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
+            const uint32_t idesc = idesc_fp4<FMT>(BM, min(BN, (qn + 15) & ~15), 0);
+            const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+            const int ns = p.zero ? 0 : p.stages;
+            for (int kb = 0; kb < ns; ++kb) {
+                if (!warp_wait(&sfull[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo) ||
+                    !warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
+                    ok = false;
                     break;
+                }
                 tc_fence_after();
-                const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
-                const uint32_t idesc = idesc_fp4<FMT>(BM, min(BN, (qn + 15) & ~15), 0);
-                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-                const int ns = p.zero ? 0 : p.stages;
-                for (int kb = 0; kb < ns; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
-                                   tmo)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint64_t sd = dS + ((stage * 2 * C::SF) >> 4);
-                    const uint32_t tsf = tmem_base + static_cast<uint32_t>(2 * BN + stage * C::SF_COLS);
-#pragma unroll
-                    for (int a = 0; a < 2 * ATOMS; ++a) copy_scales(tsf + 4 * a, sd + 32 * a);
-                    const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
-                    const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
-                    // slice ks: 64 elements = 32 bytes; its scales
-                    auto slice = [&](int ks) {
-                        const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
-                        mma_fp4<FMT>(d, ad + ks * 2, bd + ks * 2,
-                                     idesc + (FMT == GK_FP4_MX ? (ks & 1) * idesc_id2 : 0u),
-                                     tsf + 4 * atom, tsf + 4 * (ATOMS + atom),
-                                     (kb | ks) != 0 ? 1u : 0u);
-                    };
-                    const int steps = (p.kdim - kb * FBK + 63) >> 6;
+                const uint32_t tsf = tmem_base + static_cast<uint32_t>(2 * BN + stage * C::SF_COLS);
+                const uint64_t ad = dP + ((stage * C::P_BYTES) >> 4);
+                const uint64_t bd = dQ + ((stage * C::Q_BYTES) >> 4);
+                // slice ks: 64 elements = 32 bytes; its scales
+                auto slice = [&](int ks) {
+                    const int atom = FMT == GK_FP4_MX ? ks >> 1 : ks;
+                    mma_fp4<FMT>(d, ad + ks * 2, bd + ks * 2,
+                                 idesc + (FMT == GK_FP4_MX ? (ks & 1) * idesc_id2 : 0u),
+                                 tsf + 4 * atom, tsf + 4 * (ATOMS + atom), (kb | ks) != 0 ? 1u : 0u);
+                };
+                const int steps = (p.kdim - kb * FBK + 63) >> 6;
+                if (elect_one()) {
                     if (steps >= 4) {
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) slice(ks);
@@ -659,18 +656,55 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
                             if (ks < steps) slice(ks);
                     }
                     mma_commit(&empty[stage]);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
                 }
-                if (!ok) break;
-                mma_commit(&tfull[acc]);
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
-            mma_commit(drain);
-            int dummy = 0;
-            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+            if (!ok) break;
+            if (elect_one()) mma_commit(&tfull[acc]);
+            __syncwarp();
         }
+        if (elect_one()) mma_commit(drain);
+        __syncwarp();
+        int dummy = 0;
+        mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+    } else if (warp == 2) {
+        // ---------------- scales to TMEM ----------------
+        // A stage's columns are its own: they are free when its shared memory was, which the
+        // producer waited for before it filled the stage again.
+        const uint64_t dS = sdesc_scales(smem_u32(sSF));
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        while (ok && walk.next(p.tiles_p, tp, tq)) {
+            const int ns = p.zero ? 0 : p.stages;
+            for (int kb = 0; kb < ns; ++kb) {
+                if (!warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t sd = dS + ((stage * 2 * C::SF) >> 4);
+                const uint32_t tsf = tmem_base + static_cast<uint32_t>(2 * BN + stage * C::SF_COLS);
+                if (elect_one()) {
+#pragma unroll
+                    for (int a = 0; a < 2 * ATOMS; ++a) copy_scales(tsf + 4 * a, sd + 32 * a);
+                    mma_commit(&sfull[stage]);
+                }
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (elect_one()) mma_commit(drain + 1);
+        __syncwarp();
+        int dummy = 0;
+        mbar_wait(drain + 1, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
     } else if (warp >= C::EPI_W0) {
         // ---------------- epilogue ----------------
         const int q = warp & 3;

@@ -349,43 +349,41 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ---------------- MMA issuer ----------------
-            int stage = 0;
-            uint32_t phase = 0, fixpar = 0;
-            const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
-            bool ok = true;
-            for (int local = 0; ok && next_tile<BN>(walk, p, t); ++local) {
-                const int acc = local & 1;
-                const uint32_t aph = (local >> 1) & 1;
-                if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
-                               tmo))
+        // ---------------- MMA issuer (the whole warp, one lane issues) ----------------
+        int stage = 0;
+        uint32_t phase = 0, fixpar = 0;
+        const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
+        bool ok = true;
+        for (int local = 0; ok && next_tile<BN>(walk, p, t); ++local) {
+            const int acc = local & 1;
+            const uint32_t aph = (local >> 1) & 1;
+            if (!warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo))
+                break;
+            tc_fence_after();
+            const uint32_t idesc = idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0) |
+                                   (static_cast<uint32_t>(p.p_mn) << 15) |
+                                   (static_cast<uint32_t>(p.q_mn) << 16);
+            const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+            for (int kb = 0; kb < t.nk; kb += GBK) {
+                if (!warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
+                    ok = false;
                     break;
+                }
                 tc_fence_after();
-                const uint32_t idesc = idesc_f16(BM, min(BN, (t.qn + 15) & ~15), p.f16 == 0) |
-                                       (static_cast<uint32_t>(p.p_mn) << 15) |
-                                       (static_cast<uint32_t>(p.q_mn) << 16);
-                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-                for (int kb = 0; kb < t.nk; kb += GBK) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
-                                   tmo)) {
+                const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
+                // the group's end: the rows past it up to a multiple of 16 are zeroed
+                const bool cut = TMA && p.wgrad && t.nk - kb < GBK;
+                if (cut && (t.nk & 15)) {
+                    if (lane == 0) mbar_arrive(fixreq);
+                    if (!warp_wait(fixdone, fixpar, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
                         ok = false;
                         break;
                     }
+                    fixpar ^= 1u;
                     tc_fence_after();
-                    const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
-                    if (TMA && p.wgrad && t.nk - kb < GBK) {
-                        // the group's end: the rows past it up to a multiple of 16 are zeroed
-                        if (t.nk & 15) {
-                            mbar_arrive(fixreq);
-                            if (!mbar_wait(fixdone, fixpar, abort_flag, p.status,
-                                           GK_DEV_TIMEOUT_MMA, tmo)) {
-                                ok = false;
-                                break;
-                            }
-                            fixpar ^= 1u;
-                            tc_fence_after();
-                        }
+                }
+                if (elect_one()) {
+                    if (cut) {
                         const int steps = (t.nk - kb + 15) >> 4;
                         for (int ks = 0; ks < steps; ++ks)
                             mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, (kb | ks) != 0 ? 1u : 0u);
@@ -395,18 +393,21 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                             mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, (kb | ks) != 0 ? 1u : 0u);
                     }
                     mma_commit(&empty[stage]);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
                 }
-                if (!ok) break;
-                mma_commit(&tfull[acc]);
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
-            mma_commit(drain);  // every issued MMA has finished before TMEM is freed
-            int dummy = 0;
-            mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
+            if (!ok) break;
+            if (elect_one()) mma_commit(&tfull[acc]);
+            __syncwarp();
         }
+        if (elect_one()) mma_commit(drain);  // every issued MMA has finished before TMEM is freed
+        __syncwarp();
+        int dummy = 0;
+        mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
     } else if (warp >= C::EPI_W0) {
         // ---------------- epilogue ----------------
         const int q = warp & 3;
@@ -592,8 +593,8 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
-            // ---------------- MMA issuer (leader) ----------------
+        if (leader) {
+            // ---------------- MMA issuer (leader; the whole warp, one lane issues) ----------------
             const uint32_t fixreq0 = mapa_shared(smem_u32(fixreq), 0);
             const uint32_t fixreq1 = mapa_shared(smem_u32(fixreq), 1);
             int stage = 0;
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
             for (int local = 0; ok && next_tile<BN, TM>(walk, p, t); ++local) {
                 const int acc = local & 1;
                 const uint32_t aph = (local >> 1) & 1;
-                if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                if (!warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
                                tmo))
                     break;
                 tc_fence_after();
@@ -612,45 +613,54 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                                        (static_cast<uint32_t>(p.q_mn) << 16);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 for (int kb = 0; kb < t.nk; kb += GBK) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
+                    if (!warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
                                    tmo)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
-                    if (p.wgrad && t.nk - kb < GBK) {
-                        if (t.nk & 15) {
+                    const bool cut = p.wgrad && t.nk - kb < GBK;
+                    if (cut && (t.nk & 15)) {
+                        if (lane == 0) {
                             mbar_arrive_cluster(fixreq0);
                             mbar_arrive_cluster(fixreq1);
-                            if (!mbar_wait_cluster(fixdone, fixpar, abort_flag, p.status,
-                                                   GK_DEV_TIMEOUT_MMA, tmo)) {
-                                ok = false;
-                                break;
-                            }
-                            fixpar ^= 1u;
-                            tc_fence_after();
                         }
-                        const int steps = (t.nk - kb + 15) >> 4;
-                        for (int ks = 0; ks < steps; ++ks)
-                            mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
-                                         (kb | ks) != 0 ? 1u : 0u);
-                    } else {
-#pragma unroll
-                        for (int ks = 0; ks < GBK / 16; ++ks)
-                            mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
-                                         (kb | ks) != 0 ? 1u : 0u);
+                        const bool fixed = mbar_wait_cluster(fixdone, fixpar, abort_flag, p.status,
+                                                             GK_DEV_TIMEOUT_MMA, tmo);
+                        if (__any_sync(0xffffffffu, !fixed)) {
+                            ok = false;
+                            break;
+                        }
+                        fixpar ^= 1u;
+                        tc_fence_after();
                     }
-                    mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    if (elect_one()) {
+                        if (cut) {
+                            const int steps = (t.nk - kb + 15) >> 4;
+                            for (int ks = 0; ks < steps; ++ks)
+                                mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
+                                             (kb | ks) != 0 ? 1u : 0u);
+                        } else {
+#pragma unroll
+                            for (int ks = 0; ks < GBK / 16; ++ks)
+                                mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
+                                             (kb | ks) != 0 ? 1u : 0u);
+                        }
+                        mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                    }
+                    __syncwarp();
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+                if (elect_one()) mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+                __syncwarp();
             }
-            mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            if (elect_one()) mma_commit_pair(mapa_shared(smem_u32(drain), rank));
+            __syncwarp();
             int dummy = 0;
             mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
         }
