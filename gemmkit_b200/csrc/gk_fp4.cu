@@ -419,6 +419,7 @@ struct Fp4GemmParams {
     int64_t ldq, ldp;
     float alpha, beta;
     int32_t out_type;
+    int32_t pieces;           // C leaves in 16-byte pieces (c_in_pieces)
     uint64_t timeout_ns;
     unsigned int* status;
 };
@@ -438,7 +439,9 @@ struct Fp4Cfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + 2 * SF;
     static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int RAW_STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int RAW_STAGES =
+        (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     // TMEM: two accumulators, then each stage's scales (its own columns: they are free again when
     // the stage is)
     static constexpr int SF_COLS = 2 * 4 * Fp4<FMT>::ATOMS;
@@ -448,7 +451,8 @@ struct Fp4Cfg {
     // P | Q | scales of P | scales of Q | barriers | tables
     static constexpr int OFF_Q = STAGES * P_BYTES;
     static constexpr int OFF_SF = OFF_Q + STAGES * Q_BYTES;
-    static constexpr int OFF_BARS = OFF_SF + STAGES * 2 * SF;
+    static constexpr int OFF_EPI = OFF_SF + STAGES * 2 * SF;
+    static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
     static constexpr int TMEM_COLS = 512;
@@ -709,6 +713,7 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
         // ---------------- epilogue ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
         for (int local = 0; walk.next(p.tiles_p, tp, tq); ++local) {
             const int acc = local & 1;
             const uint32_t aph = (local >> 1) & 1;
@@ -716,23 +721,28 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
                 break;
             tc_fence_after();
             const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
-            const int i = tp * BM + q * 32 + lane;
-            const bool row_ok = i < p.np;
-            const int64_t at = (static_cast<int64_t>(off[walk.g]) + q0) * p.ldq + i * p.ldp;
+            const int i0 = tp * BM + q * 32;  // the warp's first P row
+            const int64_t at = (static_cast<int64_t>(off[walk.g]) + q0) * p.ldq + i0 * p.ldp;
             const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                 static_cast<uint32_t>(acc * BN + cbase);
             const bool have = !p.zero;
-            for (int c = 0; c < C::WCOLS && cbase + c < qn; c += 32) {
-                uint32_t v[32];
-                if (have) {
-                    tmem_ld_x32(tb + c, v);
-                } else {
+            const int pn = min(32, p.np - i0);
+            if (p.pieces) {
+                store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
+                             qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, have);
+            } else {
+                for (int c = 0; c < C::WCOLS && cbase + c < qn; c += 32) {
+                    uint32_t v[32];
+                    if (have) {
+                        tmem_ld_x32(tb + c, v);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                        for (int e = 0; e < 32; ++e) v[e] = 0u;
+                    }
+                    if (lane < pn)
+                        store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
+                                  qn - cbase - c, p.alpha, p.beta);
                 }
-                if (!row_ok) continue;
-                store_any(p.c, p.out_type, at + (cbase + c) * p.ldq, p.ldq, v, qn - cbase - c,
-                          p.alpha, p.beta);
             }
             tc_fence_before();
             __syncwarp();
@@ -778,10 +788,13 @@ struct Fp4PairCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + SF_STAGE;
     static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int STAGES =
+        (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     static constexpr int OFF_Q = STAGES * P_BYTES;
     static constexpr int OFF_SF = OFF_Q + STAGES * Q_BYTES;
-    static constexpr int OFF_BARS = OFF_SF + STAGES * SF_STAGE;
+    static constexpr int OFF_EPI = OFF_SF + STAGES * SF_STAGE;
+    static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
     static constexpr int OVER = FMT == GK_FP4_MX ? 96 : 160;
@@ -1074,6 +1087,7 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
         // ---------------- epilogue (both CTAs) ----------------
         const int q = warp & 3;
         const int h = (warp - C::EPI_W0) >> 2;  // which half of the columns
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
         constexpr int HO = C::OVER / 2, HR = (BN - C::OVER) / 2;  // shared, other columns per warp
         static_assert(HO % 16 == 0 && HR % 16 == 0, "chunks of 16 columns");
         for (int local = 0; walk.next(p.tiles_p, tp, tq); ++local) {
@@ -1083,38 +1097,64 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                 break;
             tc_fence_after();
             const int q0 = tq * BN, qn = off[walk.g + 1] - off[walk.g] - q0;
-            const int i = (tp * 2 + static_cast<int>(rank)) * BM + q * 32 + lane;
-            const bool row_ok = i < p.np;
-            const int64_t at = (static_cast<int64_t>(off[walk.g]) + q0) * p.ldq + i * p.ldp;
+            const int i0 = (tp * 2 + static_cast<int>(rank)) * BM + q * 32;  // its first P row
+            const int64_t at = (static_cast<int64_t>(off[walk.g]) + q0) * p.ldq + i0 * p.ldp;
             const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                 static_cast<uint32_t>(acc * (BN - C::OVER));
+            const int pn = min(32, p.np - i0);
             // first the columns that the next accumulator shares: accumulator 0's last, 1's first
             const int s0 = (acc ? 0 : BN - C::OVER) + h * HO;
-            uint32_t v[HO / 16][32];
-#pragma unroll
-            for (int c = 0; c < HO / 16; ++c) tmem_ld_chunk<16>(tb + s0 + 16 * c, v[c]);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < HO / 16; ++c) reg_fence<16>(v[c]);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(thead_l + 8u * acc);
-            if (row_ok) {
-#pragma unroll
-                for (int c = 0; c < HO / 16; ++c) {
-                    const int j = s0 + 16 * c;
-                    if (j < qn)
-                        store_any<16>(p.c, p.out_type, at + j * p.ldq, p.ldq, v[c], qn - j, p.alpha,
-                                      p.beta);
-                }
-            }
             const int r0 = (acc ? C::OVER : 0) + h * HR;
+            auto shared_read = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(thead_l + 8u * acc);
+            };
+            if (p.pieces) {
+                uint16_t* c = static_cast<uint16_t*>(p.c) + at;
+                uint32_t v[HO / 16][16];
+#pragma unroll
+                for (int k = 0; k < HO / 16; ++k) tmem_ld_frag16(tb + s0 + 16 * k, v[k]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < HO / 16; ++k) frag_fence(v[k]);
+                shared_read();
+#pragma unroll
+                for (int k = 0; k < HO / 16; ++k) {
+                    const int j = s0 + 16 * k;
+                    if (j < qn)
+                        store_frag16(c + j * p.ldq, p.ldq, v[k], qn - j, pn, p.alpha, p.out_type,
+                                     ebuf, lane);
+                }
+                store_cols16(tb + r0, HR, c + r0 * p.ldq, p.ldq, qn - r0, pn, p.alpha, p.out_type,
+                             ebuf, lane, true);
+            } else {
+                const int64_t al = at + lane * p.ldp;
+                uint32_t v[HO / 16][32];
+#pragma unroll
+                for (int k = 0; k < HO / 16; ++k) tmem_ld_chunk<16>(tb + s0 + 16 * k, v[k]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < HO / 16; ++k) reg_fence<16>(v[k]);
+                shared_read();
+                if (lane < pn) {
+#pragma unroll
+                    for (int k = 0; k < HO / 16; ++k) {
+                        const int j = s0 + 16 * k;
+                        if (j < qn)
+                            store_any<16>(p.c, p.out_type, al + j * p.ldq, p.ldq, v[k], qn - j,
+                                          p.alpha, p.beta);
+                    }
+                }
+                __syncwarp();
 #pragma unroll 1
-            for (int c = 0; c < HR && r0 + c < qn; c += 16) {
-                tmem_ld_x16(tb + r0 + c, v[0]);
-                if (row_ok)
-                    store_any<16>(p.c, p.out_type, at + (r0 + c) * p.ldq, p.ldq, v[0], qn - r0 - c,
-                                  p.alpha, p.beta);
+                for (int k = 0; k < HR && r0 + k < qn; k += 16) {
+                    tmem_ld_x16(tb + r0 + k, v[0]);
+                    if (lane < pn)
+                        store_any<16>(p.c, p.out_type, al + (r0 + k) * p.ldq, p.ldq, v[0],
+                                      qn - r0 - k, p.alpha, p.beta);
+                    __syncwarp();
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -1529,6 +1569,7 @@ int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, flo
     p.alpha = static_cast<float>(static_cast<double>(alpha) * a->scale * b->scale);
     p.beta = beta;
     p.out_type = out_type;
+    p.pieces = c_in_pieces(c.data, out_type, c.rs, c.cs, 0, static_cast<int64_t>(n), beta);
     p.timeout_ns = 4000000000ull;
     p.status = device_status_ptr();
     cudaStream_t st = static_cast<cudaStream_t>(stream);

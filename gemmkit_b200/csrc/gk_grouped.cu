@@ -97,6 +97,7 @@ struct GroupedParams {
     int32_t p_z;              // TMA: 1 = the P operand has a group dimension
     int32_t f16;              // operands are f16 (else bf16)
     int32_t out_type;         // gk_dtype of C
+    int32_t pieces;           // C leaves in 16-byte pieces (c_in_pieces)
     uint64_t timeout_ns;
     unsigned int* status;
 };
@@ -114,9 +115,12 @@ struct GroupedCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int RAW_STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
+    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int RAW_STAGES =
+        (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     static constexpr int STAGES = RAW_STAGES > 10 ? 10 : RAW_STAGES;
-    static constexpr int OFF_BARS = STAGES * STAGE_BYTES;
+    static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
+    static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
@@ -412,29 +416,34 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
         // ---------------- epilogue ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
         for (int local = 0; next_tile<BN>(walk, p, t); ++local) {
             const int acc = local & 1;
             const uint32_t aph = (local >> 1) & 1;
             if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
                 break;
             tc_fence_after();
-            const int i = t.p0 + q * 32 + lane;
-            const bool row_ok = i < p.np;
-            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i * p.ldp;
+            const int i0 = t.p0 + q * 32;  // the warp's first P row
+            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i0 * p.ldp;
             const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                 static_cast<uint32_t>(acc * BN + cbase);
-            for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
-                uint32_t v[32];
-                if (t.nk > 0) {
-                    tmem_ld_x32(tb + c, v);
-                } else {
+            const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+            if (p.pieces) {
+                store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
+                             t.qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, t.nk > 0);
+            } else {
+                for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
+                    uint32_t v[32];
+                    if (t.nk > 0) {
+                        tmem_ld_x32(tb + c, v);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                        for (int e = 0; e < 32; ++e) v[e] = 0u;
+                    }
+                    if (lane < pn)
+                        store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
+                                  t.qn - cbase - c, p.alpha, p.beta);
                 }
-                if (!row_ok) continue;
-                const int64_t o = at + (cbase + c) * p.ldq;
-                const int n = t.qn - cbase - c;
-                store_any(p.c, p.out_type, o, p.ldq, v, n, p.alpha, p.beta);
             }
             tc_fence_before();
             __syncwarp();
@@ -470,8 +479,11 @@ struct GPairCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int STAGES = (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES) / STAGE_BYTES;
-    static constexpr int OFF_BARS = STAGES * STAGE_BYTES;
+    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int STAGES =
+        (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
+    static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
+    static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
     static_assert(STAGES >= 4 && (2 * STAGES + 8) * 8 <= BAR_BYTES, "barrier area");
@@ -695,28 +707,34 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
         // ---------------- epilogue (both CTAs) ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
         for (int local = 0; next_tile<BN, TM>(walk, p, t); ++local) {
             const int acc = local & 1;
             const uint32_t aph = (local >> 1) & 1;
             if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
                 break;
             tc_fence_after();
-            const int i = t.p0 + static_cast<int>(rank) * BM + q * 32 + lane;
-            const bool row_ok = i < p.np;
-            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i * p.ldp;
+            const int i0 = t.p0 + static_cast<int>(rank) * BM + q * 32;  // the warp's first P row
+            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i0 * p.ldp;
             const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                 static_cast<uint32_t>(acc * BN + cbase);
-            for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
-                uint32_t v[32];
-                if (t.nk > 0) {
-                    tmem_ld_x32(tb + c, v);
-                } else {
+            const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+            if (p.pieces) {
+                store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
+                             t.qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, t.nk > 0);
+            } else {
+                for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
+                    uint32_t v[32];
+                    if (t.nk > 0) {
+                        tmem_ld_x32(tb + c, v);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                        for (int e = 0; e < 32; ++e) v[e] = 0u;
+                    }
+                    if (lane < pn)
+                        store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
+                                  t.qn - cbase - c, p.alpha, p.beta);
                 }
-                if (row_ok)
-                    store_any(p.c, p.out_type, at + (cbase + c) * p.ldq, p.ldq, v,
-                              t.qn - cbase - c, p.alpha, p.beta);
             }
             tc_fence_before();
             __syncwarp();
@@ -886,6 +904,7 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
         return set_last_error(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
     p.tiles_p = static_cast<int>((p.np + tm - 1) / tm);
     p.tiles_q = static_cast<int>((p.nq + bn - 1) / bn);
+    p.pieces = c_in_pieces(p.c, p.out_type, p.ldq, p.ldp, p.gsc, p.np, p.beta);
     p.timeout_ns = 4000000000ull;
     p.status = device_status_ptr();
     const int pdl = api_pdl_enabled();

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "gemmkit_cuda.h"
+#include "gk_sm100.cuh"
 
 namespace gk {
 
@@ -48,6 +49,119 @@ __device__ __forceinline__ void store_any(void* c, int type, int64_t at, int64_t
         store_chunk<CH>(static_cast<__half*>(c) + at, ldq, v, n, alpha, beta);
     else
         store_chunk<CH>(static_cast<__nv_bfloat16*>(c) + at, ldq, v, n, alpha, beta);
+}
+
+// ---- 16-bit rows of C in 16-byte pieces ------------------------------------------------------------
+//
+// The path for 16-bit C with P stride 1, 16-byte rows and no beta. A lane of the plain TMEM load
+// holds one P row, so its stores are 2 bytes wide and a 32 x 32 block takes 32 of them, each with
+// its address, conversion and product (a 256 x 256 tile: about 6000 cycles of an SM, more than the
+// MMAs of an expert's weight gradient over 700 rows). Here the accumulators are loaded in
+// the 16x256b layout (lane t: rows t / 4 and t / 4 + 8, two columns each), rounded in pairs,
+// transposed through 1 KB of shared memory per warp by stmatrix, and leave in 16-byte pieces.
+
+// 16 accumulator columns of the warp's 32 TMEM lanes, not waited for: r[0..7] lanes 0-15, r[8..15]
+// lanes 16-31; of each eight, four registers per 8 columns.
+__device__ __forceinline__ void tmem_ld_frag16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr + (16u << 16))
+        : "memory");
+}
+
+// After tcgen05.wait::ld: no use of the registers may be scheduled before it.
+__device__ __forceinline__ void frag_fence(uint32_t (&r)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        asm volatile(""
+                     : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]),
+                       "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+
+__device__ __forceinline__ uint32_t round_pair(uint32_t lo, uint32_t hi, float alpha, int type) {
+    const float a = alpha * __uint_as_float(lo), b = alpha * __uint_as_float(hi);
+    uint32_t w;
+    if (type == GK_F16)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
+}
+
+// alpha * acc of 16 Q rows (n of them in C) and the warp's 32 P rows (the first `pn` of them in
+// C, a multiple of 8 when fewer than 32), rounded to `type` and stored at c (the first Q row's
+// first element of the warp's 32), Q rows at a pitch of ldq elements. buf: the warp's 1 KB.
+__device__ __forceinline__ void store_frag16(uint16_t* c, int64_t ldq, const uint32_t (&r)[16], int n,
+                                             int pn, float alpha, int type, uint8_t* buf, int lane) {
+    const uint32_t sb = smem_u32(buf);
+    // Q row q of the block: 64 bytes at q * 64, its 16-byte piece m (8 P rows) at m ^ (q / 2 % 4):
+    // both the transposing stores and the loads below touch every bank once
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+        const int q = o * 8 + (lane & 7), m = lane >> 3;
+        const uint32_t addr = sb + static_cast<uint32_t>(q * 64 + ((m ^ ((q >> 1) & 3)) << 4));
+        const uint32_t w0 = round_pair(r[4 * o], r[4 * o + 1], alpha, type);
+        const uint32_t w1 = round_pair(r[4 * o + 2], r[4 * o + 3], alpha, type);
+        const uint32_t w2 = round_pair(r[8 + 4 * o], r[8 + 4 * o + 1], alpha, type);
+        const uint32_t w3 = round_pair(r[8 + 4 * o + 2], r[8 + 4 * o + 3], alpha, type);
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                         addr),
+                     "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                     : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+        const int q = o * 8 + (lane >> 2), m = lane & 3;
+        const uint4 v = ld_shared_v4(sb + static_cast<uint32_t>(q * 64 + ((m ^ ((q >> 1) & 3)) << 4)));
+        if (q < n && m * 8 < pn) st_global_v4(c + q * ldq + m * 8, v.x, v.y, v.z, v.w);
+    }
+    __syncwarp();  // the buffer is read before the next block is written
+}
+
+// `cols` accumulator columns (a multiple of 16) from TMEM address tb, of which the first n exist in
+// C: load (two blocks in flight), round, transpose, store. have == false: zeros, TMEM not read.
+__device__ __forceinline__ void store_cols16(uint32_t tb, int cols, uint16_t* c, int64_t ldq, int n,
+                                             int pn, float alpha, int type, uint8_t* buf, int lane,
+                                             bool have) {
+    const int nb = (min(cols, n) + 15) >> 4;  // blocks with anything to store
+    uint32_t a[16], b[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a[i] = b[i] = 0u;
+    if (have && nb > 0) tmem_ld_frag16(tb, a);
+    for (int k = 0; k < nb; k += 2) {
+        if (have) {
+            tmem_wait_ld();
+            frag_fence(a);
+            if (k + 1 < nb) tmem_ld_frag16(tb + 16 * (k + 1), b);
+        }
+        store_frag16(c + 16 * k * ldq, ldq, a, n - 16 * k, pn, alpha, type, buf, lane);
+        if (k + 1 < nb) {
+            if (have) {
+                tmem_wait_ld();
+                frag_fence(b);
+                if (k + 2 < nb) tmem_ld_frag16(tb + 16 * (k + 2), a);
+            }
+            store_frag16(c + 16 * (k + 1) * ldq, ldq, b, n - 16 * (k + 1), pn, alpha, type, buf,
+                         lane);
+        }
+    }
+}
+
+// Whether C takes that path: 16-bit, P stride 1, every row start 16-byte aligned, the P side a whole
+// number of pieces, no beta.
+inline bool c_in_pieces(const void* c, int type, int64_t ldq, int64_t ldp, int64_t gsc, int64_t np,
+                        float beta) {
+    return type != GK_F32 && ldp == 1 && ldq % 8 == 0 && gsc % 8 == 0 && np % 8 == 0 &&
+           (reinterpret_cast<uintptr_t>(c) & 15) == 0 && beta == 0.0f;
 }
 
 }  // namespace gk

@@ -499,3 +499,28 @@ def test_product_exact_large(fmt, m, k, n):
 @pytest.mark.parametrize("k,n", [(320, 2600), (1000, 4224)])
 def test_product_by_expert_large(fmt, sizes, lead, tail, k, n):
     test_product_by_expert(fmt, sizes, lead, tail, k, n)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes,lead,tail,k,n", [([5, 0, 37, 2], 3, 4, 64, 136), ([20], 0, 0, 96, 40),
+                                                 ([130, 0, 1, 255], 0, 2, 72, 264),
+                                                 ([1000, 0, 700, 257], 2, 5, 320, 2600)])
+def test_product_exact_16_bit(fmt, out, sizes, lead, tail, k, n):
+    """16-bit C (whole 16-byte pieces, and rows that are not): the exact value rounded once."""
+    torch = torch_cuda()
+    rows, g = lead + sum(sizes) + tail, len(sizes)
+    off = torch.tensor(np.cumsum([lead] + sizes), dtype=torch.int32, device="cuda")
+    a, av = grid_operand(1, rows, k, fmt, offsets=off)
+    b, bv = grid_operand(2, g * n, k, fmt, groups=g)
+    buf = torch.full((rows, n + 16), 7.0, device="cuda", dtype=tdt(out))
+    for c in (buf[:, 8:8 + n], buf[:, 3:3 + n]):
+        buf.fill_(7.0)
+        product(a, b, c, alpha=0.125)
+        want = torch.full((rows, n), 7.0, device="cuda", dtype=torch.float64)
+        o = off.tolist()
+        for e in range(g):
+            want[o[e]:o[e + 1]] = 0.125 * (av[o[e]:o[e + 1]] @ bv[e * n:(e + 1) * n].T)
+        assert torch.equal(c, want.to(tdt(out)))
+        at = c.storage_offset()
+        assert bool((buf[:, :at] == 7).all()) and bool((buf[:, at + n:] == 7).all())

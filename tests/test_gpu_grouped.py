@@ -460,3 +460,39 @@ def test_forward_exact_large(sizes, lead, tail, k, n, major):
 @pytest.mark.parametrize("m,n", [(1032, 1512), (2048, 2304), (264, 4104)])
 def test_wgrad_exact_large(sizes, lead, tail, m, n):
     test_wgrad_exact(sizes, lead, tail, m, n)
+
+
+HALF_SHAPES = [([5, 0, 37, 2], 3, 4, 64, 136), ([130, 0, 1, 255], 0, 2, 72, 264),
+               ([3] * 70, 0, 0, 40, 8), ([64, 200, 16], 1, 0, 33, 72),
+               ([1000, 0, 700, 255, 257, 1, 2083], 2, 5, 72, 1512), ([31, 4000, 33], 0, 1, 24, 2056)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes,lead,tail,k,n", HALF_SHAPES)
+def test_forward_exact_16_bit(dtype, sizes, lead, tail, k, n):
+    """16-bit C (whole 16-byte pieces): the f64 value rounded once; rows outside the groups stay."""
+    torch = torch_cuda()
+    rows, off = lead + sum(sizes) + tail, offsets_of(sizes, lead)
+    a, b = data(1, (rows, k), dtype), data(2, (len(sizes), k, n), dtype)
+    buf = torch.full((rows, n + 16), 7.0, device="cuda", dtype=tdt(dtype))
+    for c in (buf[:, 8:8 + n], buf[:, 3:3 + n]):  # aligned pieces, and not
+        buf.fill_(7.0)
+        run_fwd(a, b, off, c, dtype, alpha=0.5)
+        want, _ = want_fwd(a, b, off, torch.full((rows, n), 7.0, device="cuda"), 0.5, 0.0)
+        assert torch.equal(c, want.to(tdt(dtype)))
+        at = c.storage_offset()
+        assert bool((buf[:, :at] == 7).all()) and bool((buf[:, at + n:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes,m,n", [([5, 0, 37, 2], 40, 136), ([130, 0, 1, 255], 264, 72),
+                                       ([1000, 0, 700, 17], 1032, 1512)])
+def test_wgrad_exact_16_bit(dtype, sizes, m, n):
+    torch = torch_cuda()
+    off = offsets_of(sizes)
+    a, b = data(1, (sum(sizes), m), dtype), data(2, (sum(sizes), n), dtype)
+    c = torch.full((len(sizes), m + 1, n + 8), 7.0, device="cuda", dtype=tdt(dtype))
+    run_wgrad(a, b, off, c[:, :m, :n], dtype, alpha=0.25)
+    want, _ = want_wgrad(a, b, off, c, 0.25, 0.0)
+    assert torch.equal(c[:, :m, :n], want.to(tdt(dtype)))
+    assert bool((c[:, m:] == 7).all()) and bool((c[:, :, n:] == 7).all())
