@@ -68,16 +68,33 @@ class Parallelism:
 SERIAL = Parallelism.Serial()
 
 
+_cuda = None  # (torch, current-device call, raw-stream call), once torch has a CUDA context
+
+
+def _cuda_calls():
+    """torch's current-device and current-stream calls, without building a Stream object per
+    call (that and torch.cuda.is_available() cost several microseconds); None without CUDA."""
+    global _cuda
+    if _cuda is None:
+        try:
+            import torch
+        except ImportError:
+            return None
+        if not torch.cuda.is_available():
+            return None
+        torch.cuda.init()
+        dev = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda d: torch.cuda.current_stream(d).cuda_stream)
+        _cuda = (torch, dev, raw)
+    return _cuda
+
+
 def _stream(stream):
     if stream is not None:
         return C.c_void_p(int(stream))
-    try:
-        import torch
-        if torch.cuda.is_available():
-            return C.c_void_p(torch.cuda.current_stream().cuda_stream)
-    except ImportError:
-        pass
-    return C.c_void_p(0)
+    calls = _cuda or _cuda_calls()
+    return C.c_void_p(calls[2](calls[1]()) if calls else 0)
 
 
 def _sync(stream) -> None:
@@ -516,45 +533,52 @@ def gemm_half_f32_batched(is_f16, batch, m, k, n, alpha, a, rsa, csa, a_bs, b, r
 
 # ---- products of rows grouped by expert ------------------------------------------------------
 
+_ELEM = {"torch.float32": _lib.DT_F32, "torch.float16": _lib.DT_F16,
+         "torch.bfloat16": _lib.DT_BF16, "torch.int16": None, "torch.uint16": None}
+_elem = {}  # the same by dtype object, filled as they are met
+
+
 def _elem_type(data, default: int) -> int:
     """The C ABI's element type of a tensor (``default`` for a (pointer, length) pair, or for the
     int16 / uint16 tensors that carry 16-bit floats)."""
     if isinstance(data, tuple):
         return default
-    name = str(data.dtype)
-    types = {"torch.float32": _lib.DT_F32, "torch.float16": _lib.DT_F16,
-             "torch.bfloat16": _lib.DT_BF16, "torch.int16": default, "torch.uint16": default}
-    if name not in types:
-        raise GemmkitError(GK_EINVAL, f"gemmkit: elements of type {name} are not supported here")
-    return types[name]
+    dt = data.dtype
+    if dt not in _elem:
+        if str(dt) not in _ELEM:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: elements of type {dt} are not supported here")
+        _elem[dt] = _ELEM[str(dt)]
+    t = _elem[dt]
+    return default if t is None else t
 
 
-def _same_device(**tensors) -> None:
-    """The engine launches on the current device: refuse tensors that lie elsewhere."""
-    import torch
-    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for name, t in tensors.items():
-        if t is None or isinstance(t, tuple):
+def _same_device(*named) -> None:
+    """The engine launches on the current device: refuse tensors that lie elsewhere. Takes names
+    and tensors in turn; (pointer, length) pairs and None are not looked at."""
+    calls = _cuda or _cuda_calls()
+    cur = calls[1]() if calls else -2
+    for i in range(1, len(named), 2):
+        t = named[i]
+        if t is None or isinstance(t, tuple) or t.get_device() == cur:
             continue
-        if not t.is_cuda:
-            raise GemmkitError(GK_EINVAL, f"gemmkit: {name} is not in device memory")
-        if t.device.index != cur:
-            raise GemmkitError(GK_EINVAL, f"gemmkit: {name} is on cuda:{t.device.index}, the "
-                                          f"current device is cuda:{cur}")
+        if t.get_device() < 0:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: {named[i - 1]} is not in device memory")
+        raise GemmkitError(GK_EINVAL, f"gemmkit: {named[i - 1]} is on cuda:{t.get_device()}, the "
+                                      f"current device is cuda:{cur}")
 
 
 def _offsets(offsets):
     """(pointer, groups) of an int32 offsets tensor or a (pointer, groups + 1) pair."""
     if isinstance(offsets, tuple):
         return int(offsets[0]), int(offsets[1]) - 1
-    if str(offsets.dtype) != "torch.int32" or offsets.dim() != 1 or not offsets.is_contiguous():
+    if offsets.dim() != 1 or str(offsets.dtype) != "torch.int32" or not offsets.is_contiguous():
         raise GemmkitError(GK_EINVAL, "gemmkit: offsets must be a contiguous 1-D int32 tensor")
-    return int(offsets.data_ptr()), int(offsets.numel()) - 1
+    return offsets.data_ptr(), offsets.numel() - 1
 
 
 def _grouped_args(a, b, offsets, c, is_f16):
     half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
-    _same_device(A=a.data, B=b.data, C=c.data, offsets=offsets)
+    _same_device("A", a.data, "B", b.data, "C", c.data, "offsets", offsets)
     for name, d in (("A", a.data), ("B", b.data)):
         if _elem_type(d, half) != half:
             raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold "
@@ -612,29 +636,46 @@ class Fp4Matrix:
     def __init__(self, rows: int, cols: int, fmt: int, scale: float, groups: int, offsets, data,
                  scales):
         self.rows, self.cols, self.fmt, self.scale = int(rows), int(cols), fmt, float(scale)
-        self.groups, self.offsets, self.data, self.scales = groups, offsets, data, scales
-        c = _lib.Fp4MatrixC()
-        c.fmt, c.scale, c.groups = fmt, self.scale, groups
-        c.rows, c.cols = self.rows, self.cols
-        if offsets is not None:
-            c.offsets = _offsets(offsets)[0]
-        (c.data, c.data_len), (c.scales, c.scales_len) = _flat(data), _flat(scales)
-        self.c = c
+        self.groups, self.offsets = groups, offsets
+        self._data, self._scales = data, scales
+        off = None if offsets is None else _offsets(offsets)[0]
+        self.c = _lib.Fp4MatrixC(fmt, self.scale, groups, off, self.rows, self.cols, *_flat(data),
+                                 *_flat(scales))
+
+    @property
+    def data(self):
+        """The codes (uint8): rows at a pitch of whole 16-byte pieces."""
+        d = self._data
+        return d if self._scales is not None else d[:self.c.data_len]
+
+    @property
+    def scales(self):
+        """The block scales (uint8) in the engine's tile order."""
+        return self._scales if self._scales is not None else self._data[self.c.data_len:]
 
     @staticmethod
     def empty(rows: int, cols: int, fmt: int, scale: float = 1.0, groups: int = 1, offsets=None,
               device=None) -> "Fp4Matrix":
         """An unwritten matrix on the current device (a destination for quantize_fp4)."""
-        import torch
+        calls = _cuda or _cuda_calls()
+        if calls is None:
+            raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
+        torch = calls[0]
+        off = None
         if offsets is not None:
-            groups = _offsets(offsets)[1]
+            off, groups = _offsets(offsets)
         if fmt not in (FP4_MX, FP4_NV) or groups < 1 or rows < 0 or cols < 0:
             raise GemmkitError(GK_EINVAL, f"gemmkit: no 4-bit matrix of {rows}x{cols}, format {fmt}, "
                                           f"{groups} groups")
         # one allocation: codes, then scales (both parts whole 16-byte pieces)
         nd, ns = _fp4_sizes(rows, cols, fmt, groups, offsets is not None)
-        buf = torch.empty(nd + ns, dtype=torch.uint8, device=device or "cuda")
-        return Fp4Matrix(rows, cols, fmt, scale, groups, offsets, buf[:nd], buf[nd:])
+        buf = torch.empty(nd + ns, dtype=torch.uint8, device=device or torch.device("cuda", calls[1]()))
+        q = Fp4Matrix.__new__(Fp4Matrix)
+        q.rows, q.cols, q.fmt, q.scale = rows, cols, fmt, float(scale)
+        q.groups, q.offsets, q._data, q._scales = groups, offsets, buf, None
+        at = buf.data_ptr()
+        q.c = _lib.Fp4MatrixC(fmt, q.scale, groups, off, rows, cols, at, nd, at + nd, ns)
+        return q
 
     @staticmethod
     def from_codes(codes, block_scales, rows: int, cols: int, fmt: int, scale: float = 1.0,
@@ -642,7 +683,7 @@ class Fp4Matrix:
         """A matrix from plain row-major parts, as checkpoints hold them: uint8 tensors of codes
         (rows x ceil(cols / 2), the first element of a pair in the low nibble) and of block scales
         (rows x blocks: e8m0 or e4m3 bytes), both with contiguous rows."""
-        _same_device(codes=codes, block_scales=block_scales, offsets=offsets)
+        _same_device("codes", codes, "block_scales", block_scales, "offsets", offsets)
         for name, t in (("codes", codes), ("block_scales", block_scales)):
             if t.dim() != 2 or t.shape[0] != rows or t.element_size() != 1 or \
                     (t.shape[1] > 1 and t.stride(1) != 1):
@@ -661,9 +702,11 @@ class Fp4Matrix:
 
 
 def _fp4_sizes(rows, cols, fmt, groups, ragged):
-    lib = _lib.load()
-    return (lib.gk_fp4_data_bytes(rows, cols),
-            lib.gk_fp4_scale_bytes(fmt, groups, int(ragged), rows, cols))
+    """gk_fp4_data_bytes and gk_fp4_scale_bytes."""
+    groups = max(groups, 1)
+    blocks = (rows + 127) // 128 + groups if ragged else groups * ((rows // groups + 127) // 128)
+    pitch = ((cols + 1) // 2 + 15) // 16 * 16
+    return rows * pitch, blocks * ((cols + 255) // 256) * (1024 if fmt == FP4_MX else 2048)
 
 
 def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: int = 1,
@@ -675,7 +718,7 @@ def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: 
     rows form ragged groups; with groups > 1 `x` views the first of `groups` matrices that lie
     x_gs elements apart. `out` reuses a matrix of the same shape, format and groups (its scale and
     groups then hold); x_type names the element type of a (pointer, length) pair."""
-    _same_device(X=x.data, offsets=offsets)
+    _same_device("X", x.data, "offsets", offsets, "out", None if out is None else out._data)
     if out is None:
         stacked = offsets is None and groups > 1
         out = Fp4Matrix.empty(x.rows * groups if stacked else x.rows, x.cols, fmt, scale, groups,
@@ -692,7 +735,7 @@ def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: 
 
 def dequantize_fp4(q: Fp4Matrix, out: MatMut, stream=None, sync: bool = True) -> None:
     """The f32 values that a 4-bit matrix stands for (extension)."""
-    _same_device(Q=q.data, C=out.data)
+    _same_device("Q", q._data, "C", out.data)
     if _elem_type(out.data, _lib.DT_F32) != _lib.DT_F32:
         raise GemmkitError(GK_EINVAL, "gemmkit: C must hold f32 elements")
     _check(_lib.load().gk_dequantize_fp4(C.byref(q.c), out.c(), _stream(stream)))
@@ -707,7 +750,7 @@ def gemm_fp4(alpha: float, a: Fp4Matrix, b: Fp4Matrix, beta: float, c: MatMut,
     C f32, f16 or bf16 by its tensor's dtype (c_type for a (pointer, length) pair). With groups,
     row i of A's group g is multiplied by B's g-th matrix: A ragged (offsets) or equal groups, B a
     stack of as many."""
-    _same_device(A=a.data, B=b.data, C=c.data)
+    _same_device("A", a._data, "B", b._data, "C", c.data)
     if c_type is None:
         c_type = _elem_type(c.data, -1)
     _check(_lib.load().gk_gemm_fp4(float(alpha), C.byref(a.c), C.byref(b.c), float(beta), c.c(),

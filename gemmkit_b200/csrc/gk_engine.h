@@ -13,6 +13,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "gemmkit_cuda.h"
 
 namespace gk {
@@ -208,6 +210,20 @@ int launch_selftest_timeout(uint64_t timeout_ns, cudaStream_t s);
 int launch_quantize_rows(const float* x, int64_t rsx, int64_t csx, int64_t rows, int64_t cols,
                          int8_t* q, int64_t rsq, int64_t csq, float scale, int32_t zp,
                          float* scales, cudaStream_t s);
+
+// Allows `kern` its dynamic shared memory on the current device, once per device (`done` holds a
+// bit per device and belongs to the kernel).
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = uint64_t{1} << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // Sets this thread's gk_last_error() text (gk_api.cu); returns `code`.
 int set_last_error(int code, const char* text);

@@ -439,7 +439,7 @@ struct Fp4Cfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + 2 * SF;
     static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int EPI_BYTES = NEPI * EPI_BUF;
     static constexpr int RAW_STAGES =
         (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     // TMEM: two accumulators, then each stage's scales (its own columns: they are free again when
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
         // ---------------- epilogue ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
-        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * EPI_BUF;
         for (int local = 0; walk.next(p.tiles_p, tp, tq); ++local) {
             const int acc = local & 1;
             const uint32_t aph = (local >> 1) & 1;
@@ -788,7 +788,7 @@ struct Fp4PairCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + SF_STAGE;
     static constexpr int TAB_BYTES = (3 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int EPI_BYTES = NEPI * EPI_BUF;
     static constexpr int STAGES =
         (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     static constexpr int OFF_Q = STAGES * P_BYTES;
@@ -1087,7 +1087,7 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
         // ---------------- epilogue (both CTAs) ----------------
         const int q = warp & 3;
         const int h = (warp - C::EPI_W0) >> 2;  // which half of the columns
-        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * EPI_BUF;
         constexpr int HO = C::OVER / 2, HR = (BN - C::OVER) / 2;  // shared, other columns per warp
         static_assert(HO % 16 == 0 && HR % 16 == 0, "chunks of 16 columns");
         for (int local = 0; walk.next(p.tiles_p, tp, tq); ++local) {
@@ -1122,10 +1122,15 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < HO / 16; ++k) {
                     const int j = s0 + 16 * k;
-                    if (j < qn)
-                        store_frag16(c + j * p.ldq, p.ldq, v[k], qn - j, pn, p.alpha, p.out_type,
-                                     ebuf, lane);
+                    if (j >= qn) continue;
+                    const uint32_t sb = smem_u32(ebuf) + (k & 1) * 1024;
+                    Block16 x;
+                    x.round(v[k], p.alpha, p.out_type);
+                    x.stage(sb, lane);
+                    __syncwarp();
+                    copy_out(sb, c + j * p.ldq, p.ldq, qn - j, pn, lane);
                 }
+                __syncwarp();
                 store_cols16(tb + r0, HR, c + r0 * p.ldq, p.ldq, qn - r0, pn, p.alpha, p.out_type,
                              ebuf, lane, true);
             } else {
@@ -1270,7 +1275,8 @@ int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensor
                     const Fp4GemmParams& p, int grid, cudaStream_t st) {
     using C = Fp4Cfg<FMT, BN>;
     auto kern = fp4_gemm_kernel<FMT, BN>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(kern, C::SMEM, done);
     if (e != cudaSuccess)
         return api_err(GK_ECUDA, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, Fp4GemmParams>(

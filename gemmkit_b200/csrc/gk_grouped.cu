@@ -115,7 +115,7 @@ struct GroupedCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int EPI_BYTES = NEPI * EPI_BUF;
     static constexpr int RAW_STAGES =
         (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     static constexpr int STAGES = RAW_STAGES > 10 ? 10 : RAW_STAGES;
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
         // ---------------- epilogue ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
-        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * EPI_BUF;
         for (int local = 0; next_tile<BN>(walk, p, t); ++local) {
             const int acc = local & 1;
             const uint32_t aph = (local >> 1) & 1;
@@ -479,7 +479,7 @@ struct GPairCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int EPI_BYTES = NEPI * 1024;
+    static constexpr int EPI_BYTES = NEPI * EPI_BUF;
     static constexpr int STAGES =
         (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
         // ---------------- epilogue (both CTAs) ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
-        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * 1024;
+        uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * EPI_BUF;
         for (int local = 0; next_tile<BN, TM>(walk, p, t); ++local) {
             const int acc = local & 1;
             const uint32_t aph = (local >> 1) & 1;
@@ -754,8 +754,8 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
 int launch_grouped_pair(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p,
                         int grid, int pdl, cudaStream_t stream, char* err, size_t errlen) {
     using C = GPairCfg;
-    cudaError_t e = cudaFuncSetAttribute(grouped_pair_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(grouped_pair_kernel, C::SMEM, done);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
@@ -787,7 +787,8 @@ int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedPa
                    int pdl, cudaStream_t stream, char* err, size_t errlen) {
     using C = GroupedCfg<BN, TMA>;
     auto kern = grouped_half_kernel<BN, TMA>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(kern, C::SMEM, done);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));

@@ -58,7 +58,7 @@ __device__ __forceinline__ void store_any(void* c, int type, int64_t at, int64_t
 // its address, conversion and product (a 256 x 256 tile: about 6000 cycles of an SM, more than the
 // MMAs of an expert's weight gradient over 700 rows). Here the accumulators are loaded in
 // the 16x256b layout (lane t: rows t / 4 and t / 4 + 8, two columns each), rounded in pairs,
-// transposed through 1 KB of shared memory per warp by stmatrix, and leave in 16-byte pieces.
+// transposed through shared memory (2 KB per warp) by stmatrix, and leave in 16-byte pieces.
 
 // 16 accumulator columns of the warp's 32 TMEM lanes, not waited for: r[0..7] lanes 0-15, r[8..15]
 // lanes 16-31; of each eight, four registers per 8 columns.
@@ -96,63 +96,84 @@ __device__ __forceinline__ uint32_t round_pair(uint32_t lo, uint32_t hi, float a
     return w;
 }
 
-// alpha * acc of 16 Q rows (n of them in C) and the warp's 32 P rows (the first `pn` of them in
-// C, a multiple of 8 when fewer than 32), rounded to `type` and stored at c (the first Q row's
-// first element of the warp's 32), Q rows at a pitch of ldq elements. buf: the warp's 1 KB.
-__device__ __forceinline__ void store_frag16(uint16_t* c, int64_t ldq, const uint32_t (&r)[16], int n,
-                                             int pn, float alpha, int type, uint8_t* buf, int lane) {
-    const uint32_t sb = smem_u32(buf);
-    // Q row q of the block: 64 bytes at q * 64, its 16-byte piece m (8 P rows) at m ^ (q / 2 % 4):
-    // both the transposing stores and the loads below touch every bank once
+// A block of 16 Q rows x 32 P rows rounded to 16 bits, as stmatrix takes it.
+struct Block16 {
+    uint32_t w[8];
+    __device__ __forceinline__ void round(const uint32_t (&r)[16], float alpha, int type) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-        const int q = o * 8 + (lane & 7), m = lane >> 3;
-        const uint32_t addr = sb + static_cast<uint32_t>(q * 64 + ((m ^ ((q >> 1) & 3)) << 4));
-        const uint32_t w0 = round_pair(r[4 * o], r[4 * o + 1], alpha, type);
-        const uint32_t w1 = round_pair(r[4 * o + 2], r[4 * o + 3], alpha, type);
-        const uint32_t w2 = round_pair(r[8 + 4 * o], r[8 + 4 * o + 1], alpha, type);
-        const uint32_t w3 = round_pair(r[8 + 4 * o + 2], r[8 + 4 * o + 3], alpha, type);
-        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
-                         addr),
-                     "r"(w0), "r"(w1), "r"(w2), "r"(w3)
-                     : "memory");
+        for (int o = 0; o < 2; ++o) {
+            w[4 * o] = round_pair(r[4 * o], r[4 * o + 1], alpha, type);
+            w[4 * o + 1] = round_pair(r[4 * o + 2], r[4 * o + 3], alpha, type);
+            w[4 * o + 2] = round_pair(r[8 + 4 * o], r[8 + 4 * o + 1], alpha, type);
+            w[4 * o + 3] = round_pair(r[8 + 4 * o + 2], r[8 + 4 * o + 3], alpha, type);
+        }
     }
-    __syncwarp();
+    // Into the 1 KB at shared address sb, transposed: Q row q at q * 64, its 16-byte piece m (8 P
+    // rows) at m ^ (q / 2 % 4), so that these stores and the loads of copy_out touch every
+    // bank once.
+    __device__ __forceinline__ void stage(uint32_t sb, int lane) const {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const int q = o * 8 + (lane & 7), m = lane >> 3;
+            asm volatile(
+                "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                    sb + static_cast<uint32_t>(q * 64 + ((m ^ ((q >> 1) & 3)) << 4))),
+                "r"(w[4 * o]), "r"(w[4 * o + 1]), "r"(w[4 * o + 2]), "r"(w[4 * o + 3])
+                : "memory");
+        }
+    }
+};
+
+// A staged block to C: n of its Q rows exist in C, and the first pn of the warp's 32 P rows (a
+// multiple of 8 when fewer than 32); c is the first Q row's first element, ldq the pitch.
+__device__ __forceinline__ void copy_out(uint32_t sb, uint16_t* c, int64_t ldq, int n, int pn,
+                                         int lane) {
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
         const int q = o * 8 + (lane >> 2), m = lane & 3;
         const uint4 v = ld_shared_v4(sb + static_cast<uint32_t>(q * 64 + ((m ^ ((q >> 1) & 3)) << 4)));
         if (q < n && m * 8 < pn) st_global_v4(c + q * ldq + m * 8, v.x, v.y, v.z, v.w);
     }
-    __syncwarp();  // the buffer is read before the next block is written
 }
 
+constexpr int EPI_BUF = 2048;  // shared memory per epilogue warp: two staged blocks
+
 // `cols` accumulator columns (a multiple of 16) from TMEM address tb, of which the first n exist in
-// C: load (two blocks in flight), round, transpose, store. have == false: zeros, TMEM not read.
+// C: two blocks at a time, the next two loaded while these are stored. have == false: zeros, TMEM
+// not read.
 __device__ __forceinline__ void store_cols16(uint32_t tb, int cols, uint16_t* c, int64_t ldq, int n,
                                              int pn, float alpha, int type, uint8_t* buf, int lane,
                                              bool have) {
     const int nb = (min(cols, n) + 15) >> 4;  // blocks with anything to store
+    const uint32_t sb = smem_u32(buf);
     uint32_t a[16], b[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) a[i] = b[i] = 0u;
-    if (have && nb > 0) tmem_ld_frag16(tb, a);
+    if (have) {
+        if (nb > 0) tmem_ld_frag16(tb, a);
+        if (nb > 1) tmem_ld_frag16(tb + 16, b);
+    }
+#pragma unroll 1
     for (int k = 0; k < nb; k += 2) {
+        Block16 x, y;
         if (have) {
             tmem_wait_ld();
             frag_fence(a);
-            if (k + 1 < nb) tmem_ld_frag16(tb + 16 * (k + 1), b);
+            frag_fence(b);
         }
-        store_frag16(c + 16 * k * ldq, ldq, a, n - 16 * k, pn, alpha, type, buf, lane);
-        if (k + 1 < nb) {
-            if (have) {
-                tmem_wait_ld();
-                frag_fence(b);
-                if (k + 2 < nb) tmem_ld_frag16(tb + 16 * (k + 2), a);
-            }
-            store_frag16(c + 16 * (k + 1) * ldq, ldq, b, n - 16 * (k + 1), pn, alpha, type, buf,
-                         lane);
+        x.round(a, alpha, type);
+        y.round(b, alpha, type);
+        if (have) {
+            if (k + 2 < nb) tmem_ld_frag16(tb + 16 * (k + 2), a);
+            if (k + 3 < nb) tmem_ld_frag16(tb + 16 * (k + 3), b);
         }
+        x.stage(sb, lane);
+        y.stage(sb + 1024, lane);
+        __syncwarp();
+        copy_out(sb, c + 16 * k * ldq, ldq, n - 16 * k, pn, lane);
+        copy_out(sb + 1024, c + 16 * (k + 1) * ldq, ldq,
+                 k + 1 < nb ? n - 16 * (k + 1) : 0, pn, lane);
+        __syncwarp();  // the buffers are read before the next blocks are written
     }
 }
 

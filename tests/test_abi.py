@@ -410,6 +410,13 @@ def test_fp4_sizes():
     assert gk._fp4_sizes(129, 257, gk.FP4_NV, 1, False) == (129 * 144, 2 * 2 * 2048)
     assert gk._fp4_sizes(260, 256, gk.FP4_MX, 2, False) == (260 * 128, 4 * 1024)
     assert gk._fp4_sizes(260, 256, gk.FP4_MX, 2, True) == (260 * 128, 5 * 1024)
+    lib = _lib.load()
+    for rows, cols, groups in ((0, 5, 1), (1, 1, 1), (130, 0, 1), (384, 1000, 3), (255, 8193, 5)):
+        for fmt in (gk.FP4_MX, gk.FP4_NV):
+            for ragged in (False, True):
+                want = (lib.gk_fp4_data_bytes(rows, cols),
+                        lib.gk_fp4_scale_bytes(fmt, groups, int(ragged), rows, cols))
+                assert gk._fp4_sizes(rows, cols, fmt, groups, ragged) == want
 
 
 def test_fp4_validation_without_gpu():
