@@ -71,13 +71,13 @@ __device__ __forceinline__ float e4m3_to_float(uint32_t b) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFFu)));
 }
 
-// The value of an e2m1 code (0..15).
-__device__ __forceinline__ float e2m1_to_float(uint32_t c) {
-    const uint32_t m = c & 7u;
-    // 1 + m % 2 / 2 scaled by 2^(m / 2 - 1) from its exponent and mantissa bits; 0 and 0.5 apart
-    const uint32_t bits = m < 2 ? (m ? 0x3F000000u : 0u)
-                                : (((m >> 1) + 126u) << 23) | ((m & 1u) << 22);
-    return __uint_as_float(bits | ((c & 8u) << 28));
+// The values of two e2m1 codes (low nibble first).
+__device__ __forceinline__ float2 e2m1x2_to_float(uint32_t byte) {
+    uint32_t h2;
+    asm("{\n\t.reg .b8 lo, hi;\n\tmov.b16 {lo, hi}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, lo;\n\t}"
+        : "=r"(h2)
+        : "h"(static_cast<uint16_t>(byte)));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h2));
 }
 
 // 2^(b - 127), b = 255: NaN
@@ -92,20 +92,47 @@ struct NvScale {
 // The nv block scale, exactly: e4m3 of amax / (6 s). f32 gives the quotient within 2^-22; where
 // both ends of that interval round alike, so does the exact quotient. Otherwise it lies next to
 // the border between two codes, and amax is compared with border * 6 s, which f64 holds exactly
-// (the border has 5 significant bits, 6 s has 26).
+// (the border has 5 significant bits, 6 s has 26). The comparisons are rare and kept out of line:
+// inlined eight times over they drove the loop out of the instruction cache.
+__device__ __noinline__ uint32_t nv_scale_border(uint32_t lo, uint32_t hi, float amax, float s) {
+    const double mid = 0.5 * (static_cast<double>(e4m3_to_float(lo)) + e4m3_to_float(hi));
+    const double border = mid * (6.0 * static_cast<double>(s));
+    const double a = static_cast<double>(amax);
+    return a < border ? lo : a > border ? hi : (lo & 1u) ? hi : lo;
+}
 __device__ __forceinline__ uint32_t nv_block_scale(float amax, const NvScale& n) {
     const float q = amax * n.inv6;
     const uint32_t two = cvt_e4m3x2(q * (1.0f - 0x1p-21f), q * (1.0f + 0x1p-21f));
     const uint32_t lo = two & 0xFFu, hi = two >> 8;
-    if (lo == hi) return lo;
-    const double mid = 0.5 * (static_cast<double>(e4m3_to_float(lo)) + e4m3_to_float(hi));
-    const double border = mid * (6.0 * static_cast<double>(n.s));
-    const double a = static_cast<double>(amax);
-    return a < border ? lo : a > border ? hi : (lo & 1u) ? hi : lo;
+    return lo == hi ? lo : nv_scale_border(lo, hi, amax, n.s);
 }
 
-// Eight elements over d = sb * s, exactly as nv_block_scale: the quotient in f32 within 2^-21,
-// and next to a border the comparison |x| with border * sb * s in f64 (4 + 4 + 24 bits).
+// Eight elements over d = sb * s, decided exactly: the quotient in f32 within 2^-21 (r is 1 / d
+// within 2^-22), and next to a border the sign of |x| - border * d. There d = hi + lo without
+// error (sb has 4 significant bits), |x| - border * hi is a difference of near equals, exact in one
+// fused step, and border * lo is exact. 16-bit inputs over a matrix scale of few digits meet
+// borders often (a value in a hundred with s = 0.01), so only the elements concerned are looked
+// at; out of line, to keep the loop in the instruction cache.
+__device__ __noinline__ uint32_t nv_element_borders(uint32_t w, uint32_t w2, float x0, float x1,
+                                                    float x2, float x3, float x4, float x5,
+                                                    float x6, float x7, float sb, float s) {
+    const float hi = __fmul_rn(sb, s), lo = __fmaf_rn(sb, s, -hi);
+    uint32_t diff = w ^ w2;
+    while (diff) {
+        const int i = (__ffs(static_cast<int>(diff)) - 1) >> 2;
+        diff &= ~(15u << (4 * i));
+        const float a0 = i & 1 ? x1 : x0, a1 = i & 1 ? x3 : x2;
+        const float a2 = i & 1 ? x5 : x4, a3 = i & 1 ? x7 : x6;
+        const float b0 = i & 2 ? a1 : a0, b1 = i & 2 ? a3 : a2;
+        const float x = fabsf(i & 4 ? b1 : b0);
+        const uint32_t c = (w >> (4 * i)) & 15u, c2 = (w2 >> (4 * i)) & 15u;
+        const float2 v = e2m1x2_to_float((c & 7u) | ((c2 & 7u) << 4));
+        const float border = 0.5f * (v.x + v.y);
+        const float t = __fmaf_rn(-border, hi, x), u = border * lo;
+        if (t > u || (t == u && (c & 1u))) w = (w & ~(15u << (4 * i))) | (c2 << (4 * i));
+    }
+    return w;
+}
 __device__ __forceinline__ uint32_t nv_elements(const float (&x)[8], float r, float sb, float s) {
     const float rlo = r * (1.0f - 0x1p-20f), rhi = r * (1.0f + 0x1p-20f);
     float lo[8], hi[8];
@@ -114,22 +141,28 @@ __device__ __forceinline__ uint32_t nv_elements(const float (&x)[8], float r, fl
         lo[i] = x[i] * rlo;
         hi[i] = x[i] * rhi;
     }
-    uint32_t w = cvt_e2m1x8(lo);
-    const uint32_t w2 = cvt_e2m1x8(hi);
-    if (w != w2) {
-        const double d = static_cast<double>(sb) * static_cast<double>(s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t c = (w >> (4 * i)) & 15u, c2 = (w2 >> (4 * i)) & 15u;
-            if (c == c2) continue;
-            const double mid = 0.5 * (fabs(static_cast<double>(e2m1_to_float(c))) +
-                                      fabs(static_cast<double>(e2m1_to_float(c2))));
-            const double a = fabs(static_cast<double>(x[i])), border = mid * d;
-            const bool up = a > border || (a == border && (c & 1u));
-            if (up) w = (w & ~(15u << (4 * i))) | (c2 << (4 * i));
-        }
-    }
-    return w;
+    const uint32_t w = cvt_e2m1x8(lo), w2 = cvt_e2m1x8(hi);
+    if (w == w2) return w;
+    return nv_element_borders(w, w2, x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], sb, s);
+}
+
+// The largest magnitude of eight values, as bits (a NaN above every number).
+__device__ __forceinline__ uint32_t absmax_bits(const float (&x)[8]) {
+    float m;
+    asm("{\n\t.reg .f32 a, b;\n\t"
+        "max.NaN.abs.f32 a, %1, %2, %3;\n\t"
+        "max.NaN.abs.f32 b, %4, %5, %6;\n\t"
+        "max.NaN.abs.f32 a, a, %7, %8;\n\t"
+        "max.NaN.f32 %0, a, b;\n\t}"
+        : "=f"(m)
+        : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+    return __float_as_uint(m);
+}
+
+__device__ __forceinline__ float fast_rcp(float x) {  // within 1 ulp, normal results
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // ---- where a row lies ----------------------------------------------------------------------------
@@ -179,11 +212,13 @@ __device__ __forceinline__ bool find_row(const Fp4View& v, const RowMap& m, int 
     return true;
 }
 
+// Where the scales of row `in` of a 128-row block start; the scale sf lies sf / 4 * 512 + sf % 4 on.
 template <int FMT>
-__device__ __forceinline__ uint8_t* scale_ptr(const Fp4View& v, int block, int in, int sf) {
-    return v.scales + (static_cast<int64_t>(block) * v.stages * Fp4<FMT>::ATOMS + (sf >> 2)) * 512 +
-           (in & 31) * 16 + (in >> 5) * 4 + (sf & 3);
+__device__ __forceinline__ uint8_t* scale_row(const Fp4View& v, int block, int in) {
+    return v.scales + static_cast<int64_t>(block) * v.stages * Fp4<FMT>::SF_BYTES + (in & 31) * 16 +
+           (in >> 5) * 4;
 }
+__device__ __forceinline__ int scale_at(int sf) { return (sf >> 2) * 512 + (sf & 3); }
 
 // ---- quantisation --------------------------------------------------------------------------------
 
@@ -205,7 +240,7 @@ __device__ __forceinline__ uint32_t block_scale(uint32_t amax_bits, const NvScal
         }
         const uint32_t b = nv_block_scale(__uint_as_float(amax_bits), nv);
         sb = e4m3_to_float(b);
-        mul = b ? 1.0f / (sb * nv.s) : 0.0f;
+        mul = b ? fast_rcp(sb * nv.s) : 0.0f;
         return b;
     }
 }
@@ -281,7 +316,10 @@ __global__ void __launch_bounds__(256)
         if (!find_row(v, map, r, block, in, g, at)) continue;
         // a stack's groups lie gs apart; ragged groups and a single one lie row after row
         const T* src = x + (v.offsets ? static_cast<int64_t>(r) * rs : g * gs + at * rs);
-        uint8_t* dst = v.data + static_cast<int64_t>(r) * v.pitch + lane * 4;
+        uint8_t* dst = v.data + static_cast<int64_t>(r) * v.pitch +
+                       static_cast<int64_t>(st0) * (FBK / 2) + lane * 4;
+        uint8_t* sp = scale_row<FMT>(v, block, in) +
+                      static_cast<int64_t>(st0) * Fp4<FMT>::SF_BYTES + scale_at(lane / LPB);
         Raw8<T> raw[QU];
         if (vec && (st0 + QU) * FBK <= v.cols) {
 #pragma unroll
@@ -302,64 +340,79 @@ __global__ void __launch_bounds__(256)
             if (st >= v.stages) break;
             float e[8];
             raw[i].values(e);
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(e[j]) & 0x7FFFFFFFu);
+            uint32_t m = absmax_bits(e);
 #pragma unroll
             for (int d = 1; d < LPB; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
             float mul, sb;
             const uint32_t b = block_scale<FMT>(m, nv, mul, sb);
             const uint32_t w = block_codes<FMT>(e, m, mul, sb, nv);
-            const int byte = st * (FBK / 2);
-            if (byte + lane * 4 < v.pitch) *reinterpret_cast<uint32_t*>(dst + byte) = w;
+            if (st * (FBK / 2) + lane * 4 < v.pitch)
+                *reinterpret_cast<uint32_t*>(dst + i * (FBK / 2)) = w;
             if (lane % LPB == 0)
-                *scale_ptr<FMT>(v, block, in, st * (32 / LPB) + lane / LPB) =
+                sp[i * Fp4<FMT>::SF_BYTES] =
                     static_cast<uint8_t>(st * FBK + lane * 8 < v.cols ? b : 0u);
         }
     }
 }
 
-// The values back, in f32: code * block scale (exact) [* s, rounded once].
-template <int FMT>
+// The values back, in f32: code * block scale (exact) [* s, rounded once]. A warp takes up to QU
+// stages of a row; of each half stage a lane reads four codes and writes 16 bytes, so that a
+// warp's stores are contiguous.
+template <int FMT, int QU>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(Fp4View v, float s, float* __restrict__ out, int64_t rs, int64_t cs,
                           int vec) {
     __shared__ RowMap map;
     griddep_wait();
+    griddep_launch_dependents();
     if (!one_group(v))
         load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
                     blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
     const int lane = threadIdx.x & 31;
-    const uint32_t stages = static_cast<uint32_t>(v.stages);
-    const uint64_t units = static_cast<uint64_t>(v.rows) * stages;
+    const uint32_t chunks = static_cast<uint32_t>(v.stages + QU - 1) / QU;
+    const uint64_t units = static_cast<uint64_t>(v.rows) * chunks;
     const uint32_t step = gridDim.x * (blockDim.x >> 5);
     for (uint64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
-        const int r = units >> 32 ? static_cast<int>(u / stages)
-                                  : static_cast<int>(static_cast<uint32_t>(u) / stages);
-        const int st = static_cast<int>(u - static_cast<uint64_t>(r) * stages);
+        const int r = units >> 32 ? static_cast<int>(u / chunks)
+                                  : static_cast<int>(static_cast<uint32_t>(u) / chunks);
+        const int st0 = static_cast<int>(u - static_cast<uint64_t>(r) * chunks) * QU;
         int block, in, g, at;
         if (!find_row(v, map, r, block, in, g, at)) continue;
-        const int k = st * FBK + lane * 8;
-        if (k >= v.cols) continue;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(
-            v.data + static_cast<int64_t>(r) * v.pitch + static_cast<int64_t>(st) * (FBK / 2) +
-            lane * 4);
-        const uint32_t b = *scale_ptr<FMT>(v, block, in, k / Fp4<FMT>::BS);
-        const float sb = FMT == GK_FP4_MX ? e8m0_to_float(b) : e4m3_to_float(b);
-        float y[8];
+        const uint8_t* src = v.data + static_cast<int64_t>(r) * v.pitch +
+                             static_cast<int64_t>(st0) * (FBK / 2) + lane * 2;
+        const uint8_t* sp = scale_row<FMT>(v, block, in) +
+                            static_cast<int64_t>(st0) * Fp4<FMT>::SF_BYTES;
+        const int k0 = st0 * FBK + lane * 4;
+        uint32_t w[2 * QU], b[2 * QU];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            y[i] = e2m1_to_float(w >> (4 * i)) * sb;
-            if (FMT != GK_FP4_MX) y[i] *= s;
+        for (int i = 0; i < 2 * QU; ++i) {
+            w[i] = b[i] = 0;
+            if (k0 + i * 128 < v.cols) {
+                w[i] = *reinterpret_cast<const uint16_t*>(src + i * 64);
+                b[i] = sp[(i >> 1) * Fp4<FMT>::SF_BYTES +
+                          scale_at(((i & 1) * 128 + lane * 4) / Fp4<FMT>::BS)];
+            }
         }
-        float* dst = out + r * rs + k * cs;
-        if (vec && k + 8 <= v.cols) {
-            reinterpret_cast<float4*>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
-            reinterpret_cast<float4*>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
-        } else {
+        float* dst = out + r * rs + k0 * cs;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (k + i < v.cols) dst[i * cs] = y[i];
+        for (int i = 0; i < 2 * QU; ++i) {
+            const int left = v.cols - k0 - i * 128;  // columns from this lane's first on
+            if (left <= 0) break;
+            const float sb = FMT == GK_FP4_MX ? e8m0_to_float(b[i]) : e4m3_to_float(b[i]);
+            const float2 lo = e2m1x2_to_float(w[i] & 255u), hi = e2m1x2_to_float(w[i] >> 8);
+            float y[4] = {lo.x * sb, lo.y * sb, hi.x * sb, hi.y * sb};
+            if (FMT != GK_FP4_MX) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] *= s;
+            }
+            float* d = dst + static_cast<int64_t>(i) * 128 * cs;
+            if (vec && left >= 4) {
+                *reinterpret_cast<float4*>(d) = make_float4(y[0], y[1], y[2], y[3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < left) d[j * cs] = y[j];
+            }
         }
     }
 }
@@ -400,7 +453,8 @@ __global__ void __launch_bounds__(256)
         if (lane < NSF) {
             const int sf = st * NSF + lane;
             const bool in_row = sf * Fp4<FMT>::BS < v.cols;
-            *scale_ptr<FMT>(v, block, in, sf) = in_row ? scales[r * scales_ld + sf] : 0;
+            scale_row<FMT>(v, block, in)[static_cast<int64_t>(sf >> 2) * 512 + (sf & 3)] =
+                in_row ? scales[r * scales_ld + sf] : 0;
         }
     }
 }
@@ -1270,6 +1324,11 @@ int unit_grid(int64_t units) {
     return static_cast<int>(b < most ? b : most);
 }
 
+// Whether four stages per warp (QU) still give every SM 32 warps.
+bool large_view(const Fp4View& v) {
+    return static_cast<int64_t>(v.rows) * v.stages >= 4 * 32 * static_cast<int64_t>(sm_count());
+}
+
 template <int FMT, int BN>
 int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tq32,
                     const Fp4GemmParams& p, int grid, cudaStream_t st) {
@@ -1400,8 +1459,7 @@ int run_quantize(const void* x, int64_t rs, int64_t cs, int64_t gs, const Fp4Vie
             unit_grid(static_cast<int64_t>(v.rows) * ((v.stages + QU - 1) / QU)), 256, 0, st,
             static_cast<const T*>(x), rs, cs, gs, vec, v, nv);
     };
-    const bool large = static_cast<int64_t>(v.rows) * v.stages >= 4 * 32 * static_cast<int64_t>(sm_count());
-    return large ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 1>{});
+    return large_view(v) ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 1>{});
 }
 
 }  // namespace
@@ -1484,9 +1542,11 @@ int gk_dequantize_fp4(const gk_fp4_matrix* q, gk_matmut out, gk_stream_t stream)
     const Fp4View v = view_of(q);
     const int vec = out.cs == 1 && !(reinterpret_cast<uintptr_t>(out.data) & 15) &&
                     (v.rows <= 1 || out.rs % 4 == 0);
-    const int grid = unit_grid(static_cast<int64_t>(v.rows) * v.stages);
-    auto kern = q->fmt == GK_FP4_MX ? dequantize_fp4_kernel<GK_FP4_MX>
-                                    : dequantize_fp4_kernel<GK_FP4_NV>;
+    const int qu = large_view(v) ? 4 : 1;
+    const int grid = unit_grid(static_cast<int64_t>(v.rows) * ((v.stages + qu - 1) / qu));
+    auto kern = q->fmt == GK_FP4_MX
+                    ? (qu == 4 ? dequantize_fp4_kernel<GK_FP4_MX, 4> : dequantize_fp4_kernel<GK_FP4_MX, 1>)
+                    : (qu == 4 ? dequantize_fp4_kernel<GK_FP4_NV, 4> : dequantize_fp4_kernel<GK_FP4_NV, 1>);
     return launch_overlapped<Fp4View, float, float*, int64_t, int64_t, int>(
         1, kern, grid, 256, 0, static_cast<cudaStream_t>(stream), v, q->scale,
         static_cast<float*>(out.data), out.rs, out.cs, vec);
