@@ -95,6 +95,7 @@ struct GroupedParams {
     float alpha, beta;
     int32_t p_mn, q_mn;       // TMA: the operand is MN-major
     int32_t p_z;              // TMA: 1 = the P operand has a group dimension
+    int32_t p_4d, q_4d;       // TMA: MN-major boxes of a tile in one copy (see encode_mn4)
     int32_t f16;              // operands are f16 (else bf16)
     int32_t out_type;         // gk_dtype of C
     int32_t pieces;           // C leaves in 16-byte pieces (c_in_pieces)
@@ -132,10 +133,20 @@ struct GroupedCfg {
 // One tile of the schedule as every role sees it.
 struct GTile {
     int g, p0, q0;        // group, first row on the P and Q sides (inside the group)
-    int qn;               // rows of the Q side left from q0
+    int qn;               // its Q rows
     int64_t qbase;        // first row of the Q operand / of C along the Q side
     int k0, nk;           // first contraction row (weight gradient) and contraction length
 };
+
+// Q rows of a tile where `rows` of them are cut into tiles of at most BN: equal heights, rounded up
+// to STEP. (Whole tiles of BN and a short last one would cost more: the short tile loads as
+// much of P as a whole one, and is bound by that.)
+template <int BN, int STEP>
+__host__ __device__ __forceinline__ int tile_height(int rows) {
+    const int tiles = (rows + BN - 1) / BN;
+    const int h = (rows + tiles - 1) / tiles;
+    return (h + STEP - 1) & ~(STEP - 1);
+}
 
 template <int BN, int TM = BM>
 __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, GTile& t) {
@@ -143,15 +154,16 @@ __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, 
     if (!w.next(p.tiles_p, tp, tq)) return false;
     t.g = w.g;
     t.p0 = tp * TM;
-    t.q0 = tq * BN;
     const int o0 = w.off[t.g], m = w.off[t.g + 1] - o0;
+    const int qrows = p.wgrad ? static_cast<int>(p.nq) : m;
+    const int h = tile_height<BN, 32>(qrows);
+    t.q0 = tq * h;
+    t.qn = min(h, qrows - t.q0);
     if (p.wgrad) {
-        t.qn = static_cast<int>(p.nq) - t.q0;
         t.qbase = t.q0;
         t.k0 = o0;
         t.nk = p.zero ? 0 : m;
     } else {
-        t.qn = m - t.q0;
         t.qbase = static_cast<int64_t>(o0) + t.q0;
         t.k0 = 0;
         t.nk = p.zero ? 0 : p.kdim;
@@ -573,14 +585,18 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                     uint8_t* dq = sQ + stage * C::Q_BYTES;
                     if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
                     const int k = t.k0 + kb;
-                    if (p.p_mn) {
+                    if (p.p_4d) {
+                        tma_load_4d_pair(dp, &tmP, fb, 0, k, p0 >> 6, pz);
+                    } else if (p.p_mn) {
 #pragma unroll
                         for (int c = 0; c < BM / 64; ++c)
                             tma_load_3d_pair(dp + c * MN_BOX, &tmP, fb, p0 + 64 * c, k, pz);
                     } else {
                         tma_load_3d_pair(dp, &tmP, fb, k, p0, pz);
                     }
-                    if (p.q_mn) {
+                    if (p.q_4d) {
+                        tma_load_4d_pair(dq, &tmQ, fb, 0, k, qb >> 6, 0);
+                    } else if (p.q_mn) {
 #pragma unroll
                         for (int c = 0; c < BN / 128; ++c)
                             tma_load_3d_pair(dq + c * MN_BOX, &tmQ, fb, qb + 64 * c, k, 0);
@@ -915,8 +931,23 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
     memset(&tmq, 0, sizeof(tmq));
     if (tma) {
         const int qbox = pair ? bn / 2 : bn;
-        rc = encode_goperand(&tmp, p.P, p.p_mn, p.np, plen, gp, p.p_mn ? GBK : BM, err, sizeof(err));
-        if (!rc)
+        // Where the rows of an MN-major operand are whole 64-element chunks and every tile of
+        // the pair kernel starts on one, its two boxes come in one copy.
+        if (pair) {
+            const int h = p.wgrad ? tile_height<256, 32>(static_cast<int>(p.nq)) : 0;
+            p.p_4d = p.p_mn && p.np % 64 == 0;
+            p.q_4d = p.q_mn && p.nq % 64 == 0 && h % 128 == 0 && p.nq % h == 0;
+        }
+        const int64_t pld = plen > 1 ? p.P.ps : p.np, qld = plen > 1 ? p.Q.ps : p.nq;
+        if (p.p_4d)
+            rc = encode_tmap_mn4(&tmp, p.P.ptr, p.np, plen, gp, pld, gp > 1 ? p.P.gs : pld, err,
+                                 sizeof(err));
+        else
+            rc = encode_goperand(&tmp, p.P, p.p_mn, p.np, plen, gp, p.p_mn ? GBK : BM, err,
+                                 sizeof(err));
+        if (!rc && p.q_4d)
+            rc = encode_tmap_mn4(&tmq, p.Q.ptr, p.nq, plen, 1, qld, qld, err, sizeof(err));
+        else if (!rc)
             rc = encode_goperand(&tmq, p.Q, p.q_mn, qrows, plen, 1, p.q_mn ? GBK : qbox, err,
                                  sizeof(err));
         if (rc) return set_last_error(rc, err);

@@ -708,6 +708,28 @@ int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, i
     return 0;
 }
 
+int encode_tmap_mn4(CUtensorMap* map, const void* ptr, int64_t rows, int64_t len, int64_t groups,
+                    int64_t ld, int64_t gs, char* err, size_t errlen) {
+    PFN_tmapEncodeTiled enc = get_encode();
+    if (!enc) {
+        snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled is unavailable (driver too old?)");
+        return 5;
+    }
+    cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(len), static_cast<cuuint64_t>(rows / 64),
+                          static_cast<cuuint64_t>(groups)};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld) * 2, 128, static_cast<cuuint64_t>(gs) * 2};
+    cuuint32_t box[4] = {64, 64, 2, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(ptr), dims, strides,
+                     box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+        return 3;
+    }
+    return 0;
+}
+
 int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int box, char* err,
                       size_t errlen) {
     PFN_tmapEncodeTiled enc = get_encode();
