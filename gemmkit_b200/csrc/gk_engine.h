@@ -172,14 +172,15 @@ int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, i
                     int64_t ld1, int64_t ld2, int box0, int box1, char* err, size_t errlen);
 
 // A 4-D map of an MN-major operand of 16-bit elements (rows contiguous, a multiple of 64; `len`
-// contraction indices at pitch ld, groups at gs): boxes of 2 x (64 rows x 64 contraction indices),
-// one after the other in the 128-byte swizzle. Coordinates (0, contraction, row / 64, group).
+// contraction indices at pitch ld, groups at gs): boxes of `chunks` x (64 rows x 64 contraction
+// indices), one after the other in the 128-byte swizzle. Coordinates (0, contraction, row / 64, group).
 int encode_tmap_mn4(CUtensorMap* map, const void* ptr, int64_t rows, int64_t len, int64_t groups,
-                    int64_t ld, int64_t gs, char* err, size_t errlen);
+                    int64_t ld, int64_t gs, int chunks, char* err, size_t errlen);
 
-// A tensor map of `lines` contiguous lines of 1024 bytes, boxes of `box` lines, not swizzled.
-int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int box, char* err,
-                      size_t errlen);
+// A tensor map of `blocks` blocks of `lines` lines of 1024 bytes, all contiguous; boxes of `box`
+// lines of `box_blocks` blocks, not swizzled. Coordinates (0, line, block).
+int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int64_t blocks, int box,
+                      int box_blocks, char* err, size_t errlen);
 
 // Device status word for the current device (bounded-wait give-ups are or-ed into it).
 unsigned int* device_status_ptr();

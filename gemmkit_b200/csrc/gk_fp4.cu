@@ -972,11 +972,11 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                     2 * (C::STAGE_BYTES - (pieces ? C::Q_BYTES - pieces * 32 * BKB : 0));
                 const int prow = g * p.np + tp * 2 * BM + static_cast<int>(rank) * BM;
                 const int qrow = off[g] + q0 + static_cast<int>(rank) * half;
-                // lines of the scale maps: one stage of a 128-row block is SL lines (blocks that
-                // do not exist belong to rows that are not stored)
+                // one stage of a 128-row scale block is SL lines of the scale maps (blocks that do
+                // not exist belong to rows that are not stored)
                 constexpr int SL = C::SF / 1024;
-                const int pl = (g * p.npb + tp * 2 + static_cast<int>(rank)) * p.stages * SL;
-                const int ql = (qblk[g] + (q0 >> 7)) * p.stages * SL;
+                const int pb = g * p.npb + tp * 2 + static_cast<int>(rank);
+                const int qb = qblk[g] + (q0 >> 7);
                 for (int kb = 0; kb < p.stages; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
                                    GK_DEV_TIMEOUT_PRODUCER, tmo)) {
@@ -992,9 +992,8 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
                     for (int i = 0; i < pieces; ++i)
                         tma_load_3d_pair(dq + i * 32 * BKB, &tmQ32, fb, kb * (FBK / 4),
                                          qrow + 32 * i, 0);
-                    tma_load_3d_pair(sf, &tmPS, fb, 0, pl + kb * SL, 0);
-                    tma_load_3d_pair(sf + C::SF, &tmQS, fb, 0, ql + kb * SL, 0);
-                    tma_load_3d_pair(sf + 2 * C::SF, &tmQS, fb, 0, ql + (p.stages + kb) * SL, 0);
+                    tma_load_3d_pair(sf, &tmPS, fb, 0, kb * SL, pb);
+                    tma_load_3d_pair(sf + C::SF, &tmQS, fb, 0, kb * SL, qb);
                     issued |= 1u << stage;
                     last_par = (last_par & ~(1u << stage)) | (phase << stage);
                     if (++stage == STAGES) {
@@ -1419,14 +1418,17 @@ int run_fp4_gemm(Fp4GemmParams p, const gk_fp4_matrix* a, const gk_fp4_matrix* b
     }
     if (pair) {
         using C = Fp4PairCfg<FMT>;
-        // the scale buffers as lines of 1024 bytes (both sizes are whole lines)
+        // the scale buffers as blocks of lines of 1024 bytes; Q's two blocks come in one copy
         CUtensorMap tps, tqs;
-        rc = encode_tmap_lines(&tps, b->scales, bblocks * p.stages * lines, static_cast<int>(lines),
-                               err, sizeof(err));
-        const int64_t qb = static_cast<int64_t>(gk_fp4_scale_bytes(
-                               FMT, a->groups, a->offsets != nullptr, a->rows, a->cols)) / 1024;
+        const int64_t bl = p.stages * lines;  // lines of a block
+        rc = encode_tmap_lines(&tps, b->scales, bl, bblocks, static_cast<int>(lines), 1, err,
+                               sizeof(err));
+        const int64_t qblocks = static_cast<int64_t>(gk_fp4_scale_bytes(
+                                    FMT, a->groups, a->offsets != nullptr, a->rows, a->cols)) /
+                                (bl * 1024);
         if (!rc)
-            rc = encode_tmap_lines(&tqs, a->scales, qb, static_cast<int>(lines), err, sizeof(err));
+            rc = encode_tmap_lines(&tqs, a->scales, bl, qblocks, static_cast<int>(lines), 2, err,
+                                   sizeof(err));
         if (rc) return set_last_error(rc, err);
         const int grid = 2 * static_cast<int>(tiles < clusters ? tiles : clusters);
         return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap,

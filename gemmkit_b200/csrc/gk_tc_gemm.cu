@@ -709,7 +709,7 @@ int encode_tmap_u16(CUtensorMap* map, const void* ptr, int64_t d0, int64_t d1, i
 }
 
 int encode_tmap_mn4(CUtensorMap* map, const void* ptr, int64_t rows, int64_t len, int64_t groups,
-                    int64_t ld, int64_t gs, char* err, size_t errlen) {
+                    int64_t ld, int64_t gs, int chunks, char* err, size_t errlen) {
     PFN_tmapEncodeTiled enc = get_encode();
     if (!enc) {
         snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled is unavailable (driver too old?)");
@@ -718,7 +718,7 @@ int encode_tmap_mn4(CUtensorMap* map, const void* ptr, int64_t rows, int64_t len
     cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(len), static_cast<cuuint64_t>(rows / 64),
                           static_cast<cuuint64_t>(groups)};
     cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld) * 2, 128, static_cast<cuuint64_t>(gs) * 2};
-    cuuint32_t box[4] = {64, 64, 2, 1};
+    cuuint32_t box[4] = {64, 64, static_cast<cuuint32_t>(chunks), 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
     CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(ptr), dims, strides,
                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -730,16 +730,16 @@ int encode_tmap_mn4(CUtensorMap* map, const void* ptr, int64_t rows, int64_t len
     return 0;
 }
 
-int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int box, char* err,
-                      size_t errlen) {
+int encode_tmap_lines(CUtensorMap* map, const void* ptr, int64_t lines, int64_t blocks, int box,
+                      int box_blocks, char* err, size_t errlen) {
     PFN_tmapEncodeTiled enc = get_encode();
     if (!enc) {
         snprintf(err, errlen, "gemmkit: cuTensorMapEncodeTiled is unavailable (driver too old?)");
         return 5;
     }
-    cuuint64_t dims[3] = {256, static_cast<cuuint64_t>(lines), 1};
-    cuuint64_t strides[2] = {1024, 1024};
-    cuuint32_t boxd[3] = {256, static_cast<cuuint32_t>(box), 1};
+    cuuint64_t dims[3] = {256, static_cast<cuuint64_t>(lines), static_cast<cuuint64_t>(blocks)};
+    cuuint64_t strides[2] = {1024, static_cast<cuuint64_t>(lines) * 1024};
+    cuuint32_t boxd[3] = {256, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(box_blocks)};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), dims, strides,
                      boxd, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
