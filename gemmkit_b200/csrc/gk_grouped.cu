@@ -12,9 +12,13 @@
 // One persistent kernel: warp 1 issues tcgen05.mma kind::f16 (M = 128, N <= BN, f32
 // accumulators, two TMEM buffers), the epilogue warps drain one accumulator while the next tile
 // is computed, and a ring of shared-memory stages of 64 contraction elements in the 128-byte
-// swizzle is filled by TMA (one producer thread), or, for operands that TMA cannot address, by
-// eight loader warps that gather any strides. The tile schedule is computed on the device from
-// the offsets (gk_group.cuh), so the host never waits for them.
+// swizzle is filled by TMA (one producer thread). The tile schedule is computed on the device
+// from the offsets (gk_group.cuh), so the host never waits for them.
+//
+// Operands that TMA cannot address (no unit stride, a pitch that is no multiple of 16 bytes, a
+// base off a 16-byte boundary) are first copied to aligned scratch, line by line or transposed. (Loader warps
+// that gather such operands inside the product were tried: at most 170 TFLOP/s and 1.5 TB/s,
+// 143 us for 2000 x 2001 x 3001 against 46 us with the copies.)
 //
 // Operands lie K-major (the contraction contiguous: rows of A, weights stored n x k) or MN-major
 // (weights stored k x n, both operands of the weight gradient); the MMA reads either from the
@@ -28,6 +32,8 @@
 #include <cuda_runtime.h>
 #include <stdio.h>
 #include <string.h>
+
+#include <mutex>
 
 #include "gemmkit_cuda.h"
 #include "gk_engine.h"
@@ -74,7 +80,7 @@ struct OperandDesc {
     }
 };
 
-// An operand as the loaders read it: element (row r, contraction index p) of group g at
+// An operand: element (row r, contraction index p) of group g at
 // ptr + g * gs + r * rs + p * ps.
 struct GOperand {
     const uint16_t* ptr;
@@ -103,13 +109,11 @@ struct GroupedParams {
     unsigned int* status;
 };
 
-template <int BN, bool TMA>
+template <int BN>
 struct GroupedCfg {
     static constexpr int NEPI = BN >= 64 ? 8 : 4;
-    static constexpr int NLOAD = TMA ? 0 : 8;
     static constexpr int EPI_W0 = 4;
-    static constexpr int LOAD_W0 = EPI_W0 + NEPI;
-    static constexpr int THREADS = 32 * (LOAD_W0 + NLOAD);
+    static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
     static constexpr int WCOLS = BN / (NEPI / 4);
     static constexpr int P_BYTES = BM * BKB;
     static constexpr int Q_BYTES = BN * BKB;
@@ -171,36 +175,11 @@ __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, 
     return true;
 }
 
-// Gathers rows [r0, r0 + R) x contraction [k0, k0 + 64) of an operand with any strides into a
-// K-major 128-byte-swizzled stage (16-byte piece j of row r at piece j ^ (r mod 8)); rows at or
-// past `nr` and contraction indices at or past `nk` are zero. `t` of `nt` threads.
-template <int R>
-__device__ __forceinline__ void gather_stage(uint8_t* dst, const uint16_t* src, int64_t rs,
-                                             int64_t ps, int nr, int nk, int t, int nt) {
-    const bool kfast = ps == 1;  // neighbouring threads read neighbouring addresses
-    for (int i = t; i < R * 8; i += nt) {
-        const int r = kfast ? i >> 3 : i % R;
-        const int j = kfast ? i & 7 : i / R;
-        uint16_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int k = j * 8 + e;
-            v[e] = (r < nr && k < nk) ? __ldg(src + r * rs + k * ps) : static_cast<uint16_t>(0);
-        }
-        uint4 q;
-        q.x = v[0] | (static_cast<uint32_t>(v[1]) << 16);
-        q.y = v[2] | (static_cast<uint32_t>(v[3]) << 16);
-        q.z = v[4] | (static_cast<uint32_t>(v[5]) << 16);
-        q.w = v[6] | (static_cast<uint32_t>(v[7]) << 16);
-        *reinterpret_cast<uint4*>(dst + r * 128 + ((j ^ (r & 7)) << 4)) = q;
-    }
-}
-
-template <int BN, bool TMA>
-__global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
+template <int BN>
+__global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     grouped_half_kernel(const __grid_constant__ CUtensorMap tmP,
                         const __grid_constant__ CUtensorMap tmQ, const GroupedParams p) {
-    using C = GroupedCfg<BN, TMA>;
+    using C = GroupedCfg<BN>;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -222,7 +201,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
     const uint64_t tmo = p.timeout_ns;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], TMA ? 1 : C::NLOAD);
+            mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -235,7 +214,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (TMA && threadIdx.x == 0) {
+    if (threadIdx.x == 0 && !p.zero) {
         prefetch_tmap(&tmP);
         prefetch_tmap(&tmQ);
     }
@@ -255,7 +234,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
     GroupWalk walk(off, tile0, p.groups, blockIdx.x, gridDim.x);
     GTile t;
 
-    if (TMA && warp == 0) {
+    if (warp == 0) {
         if (lane == 0) {
             // ---------------- TMA producer ----------------
             int stage = 0;
@@ -309,7 +288,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                     mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
                               GK_DEV_TIMEOUT_DRAIN, tmo);
         }
-    } else if (TMA && warp == 2) {
+    } else if (warp == 2) {
         // ---------------- the contraction's ragged end (weight gradient) ----------------
         if (p.wgrad) {
             int blocks = 0;  // stages filled so far
@@ -332,40 +311,6 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(fixdone);
-            }
-        }
-    } else if (!TMA && warp >= C::LOAD_W0) {
-        // ---------------- loaders: any strides, one stage at a time ----------------
-        const int lt = threadIdx.x - 32 * C::LOAD_W0;
-        constexpr int NT = TMA ? 32 : 32 * C::NLOAD;
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        while (ok && next_tile<BN>(walk, p, t)) {
-            // the Q side's rows are absolute (ragged) in the forward product; the contraction
-            // starts at the group's first row in the weight gradient
-            const uint16_t* ps = p.P.ptr + t.g * p.P.gs + t.p0 * p.P.rs +
-                                 static_cast<int64_t>(t.k0) * p.P.ps;
-            const uint16_t* qs = p.Q.ptr + t.qbase * p.Q.rs + static_cast<int64_t>(t.k0) * p.Q.ps;
-            const int pn = static_cast<int>(min(static_cast<int64_t>(BM), p.np - t.p0));
-            const int qn = min(BN, t.qn);
-            for (int kb = 0; kb < t.nk; kb += GBK) {
-                if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
-                               GK_DEV_TIMEOUT_PRODUCER, tmo)) {
-                    ok = false;
-                    break;
-                }
-                gather_stage<BM>(sP + stage * C::P_BYTES, ps + kb * p.P.ps, p.P.rs, p.P.ps, pn,
-                                 t.nk - kb, lt, NT);
-                gather_stage<BN>(sQ + stage * C::Q_BYTES, qs + kb * p.Q.ps, p.Q.rs, p.Q.ps, qn,
-                                 t.nk - kb, lt, NT);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[stage]);
-                if (++stage == STAGES) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
             }
         }
     } else if (warp == 1) {
@@ -392,7 +337,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
                 tc_fence_after();
                 const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
                 // the group's end: the rows past it up to a multiple of 16 are zeroed
-                const bool cut = TMA && p.wgrad && t.nk - kb < GBK;
+                const bool cut = p.wgrad && t.nk - kb < GBK;
                 if (cut && (t.nk & 15)) {
                     if (lane == 0) mbar_arrive(fixreq);
                     if (!warp_wait(fixdone, fixpar, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
@@ -472,6 +417,120 @@ __global__ void __launch_bounds__(GroupedCfg<BN, TMA>::THREADS, 1)
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+}
+
+// ---- operands that TMA cannot address --------------------------------------------------------------
+
+// The 16 bytes at byte offset a (0, 2 .. 14) of the 32 in (lo, hi).
+__device__ __forceinline__ uint4 shift_bytes(const uint4& lo, const uint4& hi, uint32_t a) {
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (a & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (a & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const uint32_t b = (a & 2) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b),
+                      __funnelshift_r(w[2], w[3], b), __funnelshift_r(w[3], w[4], b));
+}
+
+constexpr int RU = 4;  // 16-byte pieces of a lane in flight
+
+// dst[g][l][e] = src[g * gs + l * pitch + e] for l < lines, e < len, zero for len <= e < dld (dld a
+// multiple of 8): lines that start at any 2-byte address, to 16-byte aligned ones. A warp takes
+// RU * 256 elements of a line; a piece is two aligned 16-byte loads shifted together (one where
+// the line is aligned), or single elements where those would leave the source's bytes [lo, hi).
+__global__ void __launch_bounds__(256)
+    realign_lines_kernel(uint16_t* __restrict__ dst, int64_t dld, const uint16_t* __restrict__ src,
+                         int64_t pitch, int64_t gs, int64_t lines, int64_t len, int64_t groups,
+                         const uint8_t* lo, const uint8_t* hi) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t chunks = (dld + RU * 256 - 1) / (RU * 256);
+    const int64_t units = groups * lines * chunks;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+         u < units; u += step) {
+        const int64_t gl = u / chunks, c = u - gl * chunks;
+        const int64_t g = gl / lines, l = gl - g * lines;
+        const uint16_t* s = src + g * gs + l * pitch;
+        uint16_t* d = dst + gl * dld;
+        const int64_t e0 = c * (RU * 256) + lane * 8;
+        const uint32_t a = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(s)) & 15u;
+        uint4 x[RU], y[RU];
+#pragma unroll
+        for (int i = 0; i < RU; ++i) {
+            const int64_t e = e0 + i * 256;
+            const int n = static_cast<int>(min(static_cast<int64_t>(8), len - e));
+            x[i] = y[i] = make_uint4(0, 0, 0, 0);
+            if (n <= 0) continue;
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(s + e) - a;
+            const bool two = a + 2 * n > 16;
+            if (p >= lo && p + (two ? 32 : 16) <= hi) {
+                x[i] = __ldg(reinterpret_cast<const uint4*>(p));
+                if (two) y[i] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+            } else {  // placed so that the shift below finds them
+                uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < n) {
+                        const uint32_t at = a / 2 + k;
+                        const uint32_t v = static_cast<uint32_t>(__ldg(s + e + k)) << (16 * (at & 1));
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; ++q)
+                            if ((at >> 1) == q) w[q] |= v;
+                    }
+                x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                y[i] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RU; ++i) {
+            const int64_t e = e0 + i * 256;
+            if (e >= dld) break;
+            uint4 q = shift_bytes(x[i], y[i], a);
+            const int64_t n = len - e;
+            q.x = n > 1 ? q.x : n > 0 ? q.x & 0xFFFFu : 0u;
+            q.y = n > 3 ? q.y : n > 2 ? q.y & 0xFFFFu : 0u;
+            q.z = n > 5 ? q.z : n > 4 ? q.z & 0xFFFFu : 0u;
+            q.w = n > 7 ? q.w : n > 6 ? q.w & 0xFFFFu : 0u;
+            *reinterpret_cast<uint4*>(d + e) = q;
+        }
+    }
+}
+
+// dst[g][l][e] = src[g * gs + l * sl + e * se], padded likewise, through a 32 x 32 tile: both sides
+// are coalesced whichever source stride is small.
+__global__ void __launch_bounds__(256)
+    realign_any_kernel(uint16_t* __restrict__ dst, int64_t dld, const uint16_t* __restrict__ src,
+                       int64_t sl, int64_t se, int64_t gs, int64_t lines, int64_t len,
+                       int64_t groups) {
+    __shared__ uint16_t tile[32][33];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t te = (dld + 31) / 32, tl = (lines + 31) / 32;
+    const bool e_fast = se <= sl;
+    for (int64_t t = blockIdx.x; t < groups * tl * te; t += gridDim.x) {
+        const int64_t g = t / (tl * te), r = t - g * tl * te;
+        const int64_t l0 = r / te * 32, e0 = (r - r / te * te) * 32;
+        for (int i = ty; i < 32; i += 8) {
+            const int64_t l = l0 + (e_fast ? i : tx), e = e0 + (e_fast ? tx : i);
+            const uint16_t v =
+                l < lines && e < len ? __ldg(src + g * gs + l * sl + e * se) : uint16_t{0};
+            tile[e_fast ? i : tx][e_fast ? tx : i] = v;
+        }
+        __syncthreads();
+        for (int i = ty; i < 32; i += 8) {
+            const int64_t l = l0 + i, e = e0 + tx;
+            if (l < lines && e < dld) dst[(g * lines + l) * dld + e] = tile[i][tx];
+        }
+        __syncthreads();
     }
 }
 
@@ -802,11 +861,11 @@ int launch_grouped_pair(const CUtensorMap& tp, const CUtensorMap& tq, const Grou
     return GK_OK;
 }
 
-template <int BN, bool TMA>
+template <int BN>
 int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p, int grid,
                    int pdl, cudaStream_t stream, char* err, size_t errlen) {
-    using C = GroupedCfg<BN, TMA>;
-    auto kern = grouped_half_kernel<BN, TMA>;
+    using C = GroupedCfg<BN>;
+    auto kern = grouped_half_kernel<BN>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kern, C::SMEM, done);
     if (e == cudaSuccess) {
@@ -858,6 +917,84 @@ int encode_goperand(CUtensorMap* map, const GOperand& o, int major, int64_t rows
 // are larger and fewer fit.
 int grouped_bn(int64_t q) { return q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256; }
 
+// Scratch for realigned operands: stream-ordered memory from a pool of the engine's own on the
+// current device, so that calls on several streams, and calls captured into several graphs, never
+// share any (a captured call allocates and frees inside its graph). The pool keeps what it has
+// grown to.
+cudaMemPool_t scratch_pool() {
+    static std::mutex m;
+    static cudaMemPool_t pools[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    std::lock_guard<std::mutex> lock(m);
+    if (!pools[dev]) {
+        cudaMemPoolProps props;
+        memset(&props, 0, sizeof(props));
+        props.allocType = cudaMemAllocationTypePinned;
+        props.handleTypes = cudaMemHandleTypeNone;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = dev;
+        uint64_t keep = UINT64_MAX;
+        if (cudaMemPoolCreate(&pools[dev], &props) != cudaSuccess ||
+            cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep) !=
+                cudaSuccess) {
+            cudaGetLastError();
+            pools[dev] = nullptr;
+        }
+    }
+    return pools[dev];
+}
+
+// A realigned copy of an operand (rows x len x groups) in scratch memory, K-major or, with `mn`,
+// MN-major; the operand is changed to describe it, and *scratch is what to free on the stream.
+int realign(GOperand* o, int64_t rows, int64_t len, int64_t groups, bool mn, int pdl,
+            cudaStream_t st, void** scratch) {
+    const int64_t lines = mn ? len : rows, run = mn ? rows : len;
+    const int64_t sl = mn ? o->ps : o->rs, se = mn ? o->rs : o->ps;
+    const int64_t dld = (run + 7) / 8 * 8;
+    cudaMemPool_t pool = scratch_pool();
+    cudaError_t e = pool ? cudaMallocFromPoolAsync(scratch, static_cast<size_t>(groups * lines * dld * 2),
+                                                   pool, st)
+                         : cudaErrorMemoryAllocation;
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        *scratch = nullptr;
+        return api_err(e == cudaErrorMemoryAllocation ? GK_ENOMEM : GK_ECUDA,
+                       "gemmkit: workspace allocation: %s", cudaGetErrorString(e));
+    }
+    uint16_t* dst = static_cast<uint16_t*>(*scratch);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    const int64_t most = static_cast<int64_t>(sm_count()) * 8;
+    if (se == 1 || run <= 1) {
+        const int64_t units = groups * lines * ((dld + RU * 256 - 1) / (RU * 256));
+        const int64_t blocks = (units + 7) / 8;
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks < most ? blocks : most));
+        const uint8_t* lo = reinterpret_cast<const uint8_t*>(o->ptr);
+        const uint8_t* hi = reinterpret_cast<const uint8_t*>(
+            o->ptr + (groups - 1) * o->gs + (lines - 1) * sl + run);
+        e = cudaLaunchKernelEx(&cfg, realign_lines_kernel, dst, dld, o->ptr, sl, o->gs, lines, run,
+                               groups, lo, hi);
+    } else {
+        const int64_t tiles = groups * ((lines + 31) / 32) * ((dld + 31) / 32);
+        cfg.gridDim = dim3(static_cast<unsigned>(tiles < most ? tiles : most));
+        e = cudaLaunchKernelEx(&cfg, realign_any_kernel, dst, dld, o->ptr, sl, se, o->gs, lines, run,
+                               groups);
+    }
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess)
+        return api_err(GK_ECUDA, "gemmkit: pack kernel launch failed: %s", cudaGetErrorString(e));
+    *o = mn ? GOperand{dst, 1, dld, lines * dld} : GOperand{dst, dld, 1, lines * dld};
+    return GK_OK;
+}
+
 // Clusters of the pair kernel that are resident at once on the current device.
 int pair_clusters() {
     static int cache[64] = {0};
@@ -889,6 +1026,8 @@ int pair_clusters() {
     return n;
 }
 
+int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaStream_t stream);
+
 int run_grouped(GroupedParams p, cudaStream_t stream) {
     int dev = 0;
     int rc = api_check_device(&dev);
@@ -899,12 +1038,34 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
     const int64_t gp = p.P.gs != 0 ? p.groups : 1;
     const int64_t plen = p.wgrad ? p.rows : p.kdim;
     const int64_t qrows = p.wgrad ? p.nq : p.rows;
-    p.p_mn = tma_major(p.P, p.np, plen, gp, true, !p.wgrad);
-    p.q_mn = tma_major(p.Q, qrows, plen, 1, p.wgrad != 0, !p.wgrad);
-    p.p_z = gp > 1;
-    const bool tma = !p.zero && p.p_mn >= 0 && p.q_mn >= 0;
-    if (!tma) p.p_mn = p.q_mn = 0;
+    void* scratch[2] = {nullptr, nullptr};
+    if (!p.zero) {
+        p.p_mn = tma_major(p.P, p.np, plen, gp, true, !p.wgrad);
+        p.q_mn = tma_major(p.Q, qrows, plen, 1, p.wgrad != 0, !p.wgrad);
+        const int pdl = api_pdl_enabled();
+        if (p.p_mn < 0) {  // the contiguous side stays so where the product can read it
+            p.p_mn = p.wgrad || (p.P.rs == 1 && p.P.ps != 1);
+            rc = realign(&p.P, p.np, plen, gp, p.p_mn != 0, pdl, stream, &scratch[0]);
+        }
+        if (!rc && p.q_mn < 0) {
+            p.q_mn = p.wgrad;
+            rc = realign(&p.Q, qrows, plen, 1, p.q_mn != 0, pdl, stream, &scratch[1]);
+        }
+    }
+    if (!rc) rc = run_planned(p, gp, plen, qrows, stream);
+    for (void* s : scratch)
+        if (s && cudaFreeAsync(s, stream) != cudaSuccess && !rc) {
+            cudaGetLastError();
+            rc = api_err(GK_ECUDA, "gemmkit: freeing the workspace failed");
+        }
+    return rc;
+}
 
+// Chooses the tiles and launches the product; both operands are ready for TMA.
+int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaStream_t stream) {
+    int rc = 0;
+    p.p_z = gp > 1;
+    const bool tma = !p.zero;
     const int64_t mean = (static_cast<int64_t>(p.rows) + p.groups - 1) / p.groups;
     const int64_t qside = p.wgrad ? p.nq : mean;
     // an upper bound of the tiles (the device computes the true number from the offsets)
@@ -966,8 +1127,7 @@ int run_grouped(GroupedParams p, cudaStream_t stream) {
     const int grid = static_cast<int>(tiles < sms ? tiles : sms);
     auto go = [&](auto bn_tag) {
         constexpr int BN = decltype(bn_tag)::value;
-        return tma ? launch_grouped<BN, true>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err))
-                   : launch_grouped<BN, false>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
+        return launch_grouped<BN>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
     };
     switch (bn) {
         case 32: rc = go(std::integral_constant<int, 32>{}); break;

@@ -325,10 +325,12 @@ typedef enum { GK_F32 = 0, GK_F16 = 1, GK_BF16 = 2 } gk_dtype;
  * A (rows x k) and B (k x n, group g at + g * b_gs elements; b_gs == 0: one B for every group)
  * are bf16, or f16 with is_f16; C is f32 or the operands' type (out_type), computed in f32 and
  * rounded once. beta == 0 never reads C; k == 0 or alpha == 0 is C <- beta * C on the groups'
- * rows and reads neither A nor B. Any non-negative strides; A with unit column stride and B with a
- * unit row or column stride, 16-byte aligned with every other stride a multiple of 16 bytes,
- * take the fast path. The gradient of A is the same call with C's gradient as A and B
- * viewed transposed. Needs no workspace, allocates nothing and may be captured. */
+ * rows and reads neither A nor B. Any non-negative strides. An A with unit column stride and a B
+ * with a unit row or column stride, 16-byte aligned and every other stride a multiple of 16 bytes,
+ * are read in place (in the weight gradient A and B with unit column strides); other operands
+ * are first copied to aligned scratch, stream-ordered memory from a pool that the engine keeps.
+ * The gradient of A is the same call with C's gradient as A and B viewed transposed. Calls may
+ * be captured and may run on several streams at once. */
 int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t *offsets, float alpha,
                          gk_matref a, gk_matref b, ptrdiff_t b_gs, float beta, gk_matmut c,
                          int out_type, gk_parallelism par, gk_stream_t stream);

@@ -75,6 +75,11 @@ def run_fwd(a, b, off, c, dtype, alpha=1.0, beta=0.0, stream=None, sync=True):
 
 
 def run_wgrad(a, b, off, c, dtype, alpha=1.0, beta=0.0):
+    run_wgrad_async(a, b, off, c, dtype, alpha, beta)
+    torch_cuda().cuda.synchronize()
+
+
+def run_wgrad_async(a, b, off, c, dtype, alpha=1.0, beta=0.0):
     import ctypes as C
     from gemmkit_b200 import _lib
     cv, gs = stack(c, gk.MatMut)
@@ -83,7 +88,6 @@ def run_wgrad(a, b, off, c, dtype, alpha=1.0, beta=0.0):
         int(dtype == "f16"), off.numel() - 1, C.c_void_p(off.data_ptr()), alpha, view(a).c(),
         view(b).c(), beta, cv.c(), gs, out, gk.SERIAL.c(), gk._stream(None))
     gk._check(rc)
-    torch_cuda().cuda.synchronize()
 
 
 def want_fwd(a, b, off, c0, alpha, beta):
@@ -496,3 +500,83 @@ def test_wgrad_exact_16_bit(dtype, sizes, m, n):
     want, _ = want_wgrad(a, b, off, c, 0.25, 0.0)
     assert torch.equal(c[:, :m, :n], want.to(tdt(dtype)))
     assert bool((c[:, m:] == 7).all()) and bool((c[:, :, n:] == 7).all())
+
+
+def test_realigned_operands_in_graphs_and_on_two_streams():
+    """Operands that are copied to aligned scratch first (odd pitches, no unit stride): captured calls
+    replayed on two streams at once, and eager calls on two streams, each with its own scratch."""
+    torch = torch_cuda()
+    rows, k, n, dtype = 300, 133, 259, "bf16"
+    off = offsets_of([100, 0, 150, 50])
+    a = data(1, (rows, k), dtype)
+    bs = [data(2 + i, (4, k, 2 * n), dtype)[:, :, ::2] for i in range(2)]  # no unit stride
+    cs = [torch.zeros((rows, n), device="cuda") for _ in range(2)]
+    ws = [torch.zeros((4, k, n), device="cuda") for _ in range(2)]
+    dy = data(9, (rows, n), dtype)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    wants = [want_fwd(a, b, off, torch.zeros_like(cs[0]), 1.0, 0.0)[0] for b in bs]
+    wgrad = want_wgrad(a, dy, off, ws[0], 1.0, 0.0)[0]
+    torch.cuda.synchronize()
+
+    def calls(i):
+        run_fwd(a, bs[i], off, cs[i], dtype, sync=False)
+        run_wgrad_async(a, dy, off, ws[i], dtype)
+
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                calls(i)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(cs[i].double(), wants[i]) and torch.equal(ws[i].double(), wgrad)
+    graphs = []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            calls(i)
+            calls(i)
+        graphs.append(g)
+        cs[i].zero_()
+        ws[i].zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(cs[i].double(), wants[i]) and torch.equal(ws[i].double(), wgrad)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_shapes_and_strides(seed):
+    """Small random problems with random pitches, offsets of the base and orders."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(seed)
+    for _ in range(12):
+        g = int(rng.integers(1, 6))
+        sizes = [int(x) for x in rng.integers(0, 90, g)]
+        lead, tail = int(rng.integers(0, 3)), int(rng.integers(0, 3))
+        rows, k, n = lead + sum(sizes) + tail, int(rng.integers(1, 300)), int(rng.integers(1, 300))
+        if rows == 0:
+            continue
+        off = offsets_of(sizes, lead)
+
+        def mat(r, c):
+            pad, at = int(rng.integers(0, 9)), int(rng.integers(0, 9))
+            if rng.random() < 0.5:
+                return data(int(rng.integers(1 << 30)), (r, c + pad + at), "bf16")[:, at:at + c]
+            return data(int(rng.integers(1 << 30)), (c, r + pad + at), "bf16")[:, at:at + r].t()
+
+        a = mat(rows, k)
+        b = mat(g * k, n) if rng.random() < 0.5 else mat(n, g * k).t()
+        b = torch.as_strided(b, (g, k, n), (k * b.stride(0), *b.stride()), b.storage_offset())
+        c = torch.full((rows, n), 7.0, device="cuda")
+        run_fwd(a, b, off, c, "bf16")
+        want, _ = want_fwd(a, b, off, torch.full_like(c, 7.0), 1.0, 0.0)
+        assert torch.equal(c.double(), want)
+        y = mat(rows, n)
+        w = torch.full((g, k, n), 7.0, device="cuda")
+        run_wgrad(a, y, off, w, "bf16")
+        want, _ = want_wgrad(a, y, off, w, 1.0, 0.0)
+        assert torch.equal(w.double(), want)
