@@ -1616,6 +1616,10 @@ int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, flo
             (api_overlaps(c.data, cb, o->data, o->data_len) ||
              api_overlaps(c.data, cb, o->scales, o->scales_len)))
             return api_err(GK_EINVAL, "gemmkit: C aliases A or B");
+    const double scaled = static_cast<double>(alpha) * a->scale * b->scale;
+    if (isfinite(alpha) && alpha != 0.0f &&
+        !(fabs(scaled) >= 1.17549435e-38 && fabs(scaled) <= 3.4028234e38))
+        return api_err(GK_EINVAL, "gemmkit: alpha times the matrix scales (%g) leaves f32", scaled);
     if (c.rows == 0 || c.cols == 0) return GK_OK;
     if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
     if ((rc = api_check_device(nullptr))) return rc;
@@ -1634,7 +1638,7 @@ int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, flo
     p.c = c.data;
     p.ldq = c.rs;
     p.ldp = c.cs;
-    p.alpha = static_cast<float>(static_cast<double>(alpha) * a->scale * b->scale);
+    p.alpha = static_cast<float>(scaled);
     p.beta = beta;
     p.out_type = out_type;
     p.pieces = c_in_pieces(c.data, out_type, c.rs, c.cs, 0, static_cast<int64_t>(n), beta);

@@ -952,10 +952,17 @@ int realign(GOperand* o, int64_t rows, int64_t len, int64_t groups, bool mn, int
     const int64_t lines = mn ? len : rows, run = mn ? rows : len;
     const int64_t sl = mn ? o->ps : o->rs, se = mn ? o->rs : o->ps;
     const int64_t dld = (run + 7) / 8 * 8;
-    cudaMemPool_t pool = scratch_pool();
-    cudaError_t e = pool ? cudaMallocFromPoolAsync(scratch, static_cast<size_t>(groups * lines * dld * 2),
-                                                   pool, st)
-                         : cudaErrorMemoryAllocation;
+    // a captured allocation belongs to its graph, whichever pool it names (and a pool cannot be
+    // created during a capture)
+    const size_t bytes = static_cast<size_t>(groups * lines * dld * 2);
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(st, &cap);
+    if (e == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
+        e = cudaMallocAsync(scratch, bytes, st);
+    } else if (e == cudaSuccess) {
+        cudaMemPool_t pool = scratch_pool();
+        e = pool ? cudaMallocFromPoolAsync(scratch, bytes, pool, st) : cudaErrorMemoryAllocation;
+    }
     if (e != cudaSuccess) {
         cudaGetLastError();
         *scratch = nullptr;
@@ -1233,8 +1240,8 @@ int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t* offsets
         size_t need = static_cast<size_t>((c.rows - 1) * c.rs + (c.cols - 1) * c.cs) + 1;
         if (static_cast<size_t>(c_gs) < need)
             return api_err(GK_EINVAL,
-                           "gemmkit: the groups of C overlap (group stride %td, a group spans %zu "
-                           "elements)",
+                           "gemmkit: the groups of C overlap or interleave (group stride %td, a group "
+                           "spans %zu elements)",
                            c_gs, need);
     }
     if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");

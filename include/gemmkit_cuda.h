@@ -337,8 +337,8 @@ int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t *offsets, floa
 /* The weight gradient: C[g] <- alpha * A_g^T * B_g + beta * C[g] with A (rows x m) and B (rows x
  * n) grouped as above, A_g the rows of group g, and C[g] (m x n) at + g * c_gs elements. The
  * contraction runs over the group's rows; an empty group's C[g] becomes beta * C[g] (zeros when
- * beta == 0). Rows of A and B outside the groups are never used, whatever they hold. The
- * groups of C must not overlap. */
+ * beta == 0). Rows of A and B outside the groups are never used, whatever they hold. Each
+ * group of C must end before the next begins. */
 int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t *offsets, float alpha,
                                gk_matref a, gk_matref b, float beta, gk_matmut c, ptrdiff_t c_gs,
                                int out_type, gk_parallelism par, gk_stream_t stream);
@@ -396,8 +396,9 @@ int gk_fp4_import(const uint8_t *codes, size_t codes_len, size_t codes_ld, const
  * (out_type, a gk_dtype), rounded once. With groups, row i of A's group g is multiplied by B's
  * g-th matrix: A's groups may be ragged (a device array, as in gk_gemm_half_grouped, with the same
  * rules for its contents and for rows outside the groups) or equal, B's are equal; both have the
- * same number. beta == 0 never reads C; k == 0 or alpha == 0 is C <- beta * C. Needs no
- * workspace, allocates nothing and may be captured. */
+ * same number. beta == 0 never reads C; k == 0 or alpha == 0 is C <- beta * C. The product of
+ * alpha and the two matrix scales must be a normal f32 number (or alpha 0, infinite or NaN).
+ * Needs no workspace, allocates nothing and may be captured. */
 int gk_gemm_fp4(float alpha, const gk_fp4_matrix *a, const gk_fp4_matrix *b, float beta,
                 gk_matmut c, int out_type, gk_parallelism par, gk_stream_t stream);
 

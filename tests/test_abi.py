@@ -462,6 +462,10 @@ def test_fp4_validation_without_gpu():
     expect_err(gemm(c=gk.MatMut.new((64, 24), 4, 6, 6, 0)), "aliases itself")
     expect_err(gemm(c=gk.MatMut.new((64, 23), 4, 6, 6, 1)), "C view of 4x6")
     expect_err(gemm(c=gk.MatMut.new((1 << 20, 24), 4, 6, 6, 1)), "C aliases A or B")
+    big = [fp4(r, 8, fmt=gk.FP4_NV, scale=2.0 ** 70, at=at) for r, at in ((4, 1 << 20), (6, 1 << 22))]
+    expect_err(gemm(a=big[0], b=big[1]), "leaves f32")
+    small = [fp4(r, 8, fmt=gk.FP4_NV, scale=2.0 ** -70, at=at) for r, at in ((4, 1 << 20), (6, 1 << 22))]
+    expect_err(gemm(a=small[0], b=small[1]), "leaves f32")
     lib = _lib.load()
     assert lib.gk_gemm_fp4(1.0, None, C.byref(b.c), 0.0, c.c(), 0, gk.SERIAL.c(), None) == gk.GK_EINVAL
     assert b"null 4-bit matrix A" in lib.gk_last_error()

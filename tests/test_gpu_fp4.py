@@ -524,3 +524,54 @@ def test_product_exact_16_bit(fmt, out, sizes, lead, tail, k, n):
         assert torch.equal(c, want.to(tdt(out)))
         at = c.storage_offset()
         assert bool((buf[:, :at] == 7).all()) and bool((buf[:, at + n:] == 7).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_empty_contractions_and_inputs(fmt):
+    """k == 0: C <- beta * C on the groups' rows; no rows: nothing."""
+    torch = torch_cuda()
+    off = torch.tensor([1, 4, 4, 8], dtype=torch.int32, device="cuda")
+    a = gk.Fp4Matrix.empty(9, 0, fmt, offsets=off)
+    b = gk.Fp4Matrix.empty(3 * 24, 0, fmt, groups=3)
+    for beta in (0.0, 0.5):
+        for out in (torch.float32, torch.bfloat16):
+            c = torch.full((9, 24), 8.0, device="cuda", dtype=out)
+            product(a, b, c, beta=beta)
+            want = torch.full_like(c, 8.0)
+            want[1:8] *= beta
+            assert torch.equal(c, want)
+    x = torch.zeros(0, 64, device="cuda")
+    q = gk.quantize_fp4(gk.MatRef(x, 0, 64, 64, 1), fmt)
+    w = gk.quantize_fp4(mat(torch.zeros(24, 64, device="cuda")), fmt)
+    product(q, w, torch.zeros(0, 24, device="cuda"))
+    assert q.rows == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_most_groups(fmt):
+    torch = torch_cuda()
+    sizes = [(i * 7) % 5 if i % 3 == 0 else 0 for i in range(1024)]
+    rows = sum(sizes)
+    off = torch.tensor(np.cumsum([0] + sizes), dtype=torch.int32, device="cuda")
+    a, av = grid_operand(1, rows, 96, fmt, offsets=off)
+    b, bv = grid_operand(2, 1024 * 24, 96, fmt, groups=1024)
+    c = torch.full((rows, 24), 7.0, device="cuda")
+    product(a, b, c)
+    o = off.tolist()
+    want = torch.cat([av[o[e]:o[e + 1]] @ bv[e * 24:(e + 1) * 24].T for e in range(1024)])
+    assert torch.equal(c.double(), want)
+
+
+def test_extreme_matrix_scales():
+    """Matrix scales at the ends of their range whose product is 1."""
+    torch = torch_cuda()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(40, 96, generator=gen, device="cuda")
+    w = torch.randn(56, 96, generator=gen, device="cuda")
+    one = [gk.quantize_fp4(mat(t), gk.FP4_NV) for t in (x, w)]
+    far = [gk.quantize_fp4(mat(t * s), gk.FP4_NV, scale=s)
+           for t, s in ((x, 2.0 ** 100), (w, 2.0 ** -100))]
+    c = [torch.zeros(40, 56, device="cuda") for _ in range(2)]
+    product(*one, c[0])
+    product(*far, c[1])
+    assert torch.equal(c[0], c[1])

@@ -580,3 +580,66 @@ def test_random_shapes_and_strides(seed):
         run_wgrad(a, y, off, w, "bf16")
         want, _ = want_wgrad(a, y, off, w, 1.0, 0.0)
         assert torch.equal(w.double(), want)
+
+
+def test_empty_contractions_and_inputs():
+    """k == 0 and no rows at all: C <- beta * C on the groups' rows, on every group of a weight
+    gradient."""
+    torch = torch_cuda()
+    off = offsets_of([3, 0, 4], 1)
+    for beta in (0.0, 0.5):
+        c = torch.full((9, 24), 8.0, device="cuda")
+        run_fwd(torch.zeros((9, 0), device="cuda", dtype=torch.bfloat16),
+                torch.zeros((3, 0, 24), device="cuda", dtype=torch.bfloat16), off, c, "bf16", beta=beta)
+        want = torch.full_like(c, 8.0)
+        want[1:8] *= beta
+        assert torch.equal(c, want)
+        for out in (torch.float32, torch.bfloat16):
+            w = torch.full((3, 40, 24), 8.0, device="cuda", dtype=out)
+            run_wgrad(torch.zeros((0, 40), device="cuda", dtype=torch.bfloat16),
+                      torch.zeros((0, 24), device="cuda", dtype=torch.bfloat16), offsets_of([0, 0, 0]),
+                      w, "bf16", beta=beta)
+            assert torch.equal(w, torch.full_like(w, 8.0 * beta))
+
+
+def test_most_groups():
+    """1024 groups, most of them empty."""
+    torch = torch_cuda()
+    sizes = [(i * 7) % 5 if i % 3 == 0 else 0 for i in range(1024)]
+    off, rows = offsets_of(sizes), sum(sizes)
+    a, b = data(1, (rows, 40), "bf16"), data(2, (1024, 40, 24), "bf16")
+    c = torch.full((rows, 24), 7.0, device="cuda")
+    run_fwd(a, b, off, c, "bf16")
+    assert torch.equal(c.double(), want_fwd(a, b, off, c, 1.0, 0.0)[0])
+    y = data(3, (rows, 24), "bf16")
+    w = torch.full((1024, 40, 24), 7.0, device="cuda")
+    run_wgrad(a, y, off, w, "bf16")
+    assert torch.equal(w.double(), want_wgrad(a, y, off, w, 1.0, 0.0)[0])
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first calls are captured (aligned operands, then operands that need scratch)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, gemmkit_b200 as gk
+off = torch.tensor([0, 30, 50], dtype=torch.int32, device="cuda")
+for k, n in ((64, 72), (33, 71)):
+    a = torch.randint(-4, 5, (50, k), device="cuda").bfloat16()
+    b = torch.randint(-4, 5, (2, k, n), device="cuda").bfloat16()
+    c = torch.zeros(50, n, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        gk.gemm_half_grouped(1.0, gk.MatRef.from_row_major(a, 50, k), gk.MatRef.from_row_major(b, k, n),
+                             k * n, off, 0.0, gk.MatMut.from_row_major(c, 50, n), sync=False)
+    g.replay()
+    torch.cuda.synchronize()
+    want = torch.cat([a[:30].double() @ b[0].double(), a[30:].double() @ b[1].double()])
+    assert torch.equal(c.double(), want), (k, n)
+print("ok")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0 and "ok" in out.stdout, out.stderr[-2000:]
