@@ -562,7 +562,7 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
 template <int FMT, int BN>
 __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
-                    const __grid_constant__ CUtensorMap tmQ32, const Fp4GemmParams p) {
+                    const Fp4GemmParams p) {
     using C = Fp4Cfg<FMT, BN>;
     constexpr int STAGES = C::STAGES;
     constexpr int ATOMS = Fp4<FMT>::ATOMS;
@@ -602,7 +602,6 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
         if (!p.zero) {
             prefetch_tmap(&tmP);
             prefetch_tmap(&tmQ);
-            prefetch_tmap(&tmQ32);
         }
     }
     if (warp == 1) {
@@ -622,52 +621,48 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
     int tp, tq;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- producer ----------------
-            int stage = 0;
-            uint32_t phase = 0, issued = 0, last_par = 0;
-            bool ok = true;
-            while (ok && walk.next(p.tiles_p, tp, tq)) {
-                const int g = walk.g, q0 = tq * BN;
-                const int64_t pb = static_cast<int64_t>(g) * p.npb + tp;
-                const int64_t qb = static_cast<int64_t>(qblk[g]) + (q0 >> 7);
-                const int prow = g * p.np + tp * BM, qrow = off[g] + q0;
-                const int ns = p.zero ? 0 : p.stages;
-                // a short tile loads its rows in pieces of 32 (the same bytes in shared memory)
-                const int qn = off[g + 1] - off[g] - q0;
-                const int pieces = qn > BN - 32 ? 0 : (qn + 31) >> 5;
-                const uint32_t bytes = C::STAGE_BYTES - (pieces ? C::Q_BYTES - pieces * 32 * BKB : 0);
-                for (int kb = 0; kb < ns; ++kb) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
-                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
-                        ok = false;
-                        break;
-                    }
+        // ---------------- producer (the whole warp, one lane issues) ----------------
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last_par = 0;
+        bool ok = true;
+        while (ok && walk.next(p.tiles_p, tp, tq)) {
+            const int g = walk.g, q0 = tq * BN;
+            const int64_t pb = static_cast<int64_t>(g) * p.npb + tp;
+            const int64_t qb = static_cast<int64_t>(qblk[g]) + (q0 >> 7);
+            const int prow = g * p.np + tp * BM, qrow = off[g] + q0;
+            const int ns = p.zero ? 0 : p.stages;
+            const uint8_t* ps = p.psf + pb * p.stages * C::SF;
+            const uint8_t* qs = p.qsf + qb * p.stages * C::SF;
+            for (int kb = 0; kb < ns; ++kb) {
+                if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
                     uint64_t* fb = &full[stage];
-                    mbar_arrive_expect_tx(fb, bytes);
+                    mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
                     tma_load_3d(sP + stage * C::P_BYTES, &tmP, fb, kb * (FBK / 4), prow, 0);
-                    uint8_t* dq = sQ + stage * C::Q_BYTES;
-                    if (pieces == 0) tma_load_3d(dq, &tmQ, fb, kb * (FBK / 4), qrow, 0);
-                    for (int i = 0; i < pieces; ++i)
-                        tma_load_3d(dq + i * 32 * BKB, &tmQ32, fb, kb * (FBK / 4), qrow + 32 * i, 0);
+                    tma_load_3d(sQ + stage * C::Q_BYTES, &tmQ, fb, kb * (FBK / 4), qrow, 0);
                     uint8_t* sf = sSF + stage * 2 * C::SF;
-                    bulk_load(sf, p.psf + (pb * p.stages + kb) * C::SF, C::SF, fb);
-                    bulk_load(sf + C::SF, p.qsf + (qb * p.stages + kb) * C::SF, C::SF, fb);
-                    issued |= 1u << stage;
-                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    bulk_load(sf, ps + static_cast<int64_t>(kb) * C::SF, C::SF, fb);
+                    bulk_load(sf + C::SF, qs + static_cast<int64_t>(kb) * C::SF, C::SF, fb);
+                }
+                __syncwarp();
+                issued |= 1u << stage;
+                last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            griddep_launch_dependents();
-            int dummy = 0;
-            for (int s = 0; s < STAGES; ++s)
-                if (issued & (1u << s))
-                    mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
-                              GK_DEV_TIMEOUT_DRAIN, tmo);
         }
+        griddep_launch_dependents();
+        int dummy = 0;
+        for (int s = 0; s < STAGES; ++s)
+            if (issued & (1u << s))
+                mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN,
+                          tmo);
     } else if (warp == 1) {
         // ---------------- MMA issuer (the whole warp, one lane issues) ----------------
         const uint64_t dP = sdesc_kmajor_sw128(smem_u32(sP));
@@ -888,7 +883,6 @@ __device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) 
 template <int FMT>
 __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
     fp4_pair_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
-                    const __grid_constant__ CUtensorMap tmQ32,
                     const __grid_constant__ CUtensorMap tmPS,
                     const __grid_constant__ CUtensorMap tmQS, const Fp4GemmParams p) {
     using C = Fp4PairCfg<FMT>;
@@ -933,7 +927,6 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
         fence_mbar_init();
         prefetch_tmap(&tmP);
         prefetch_tmap(&tmQ);
-        prefetch_tmap(&tmQ32);
         prefetch_tmap(&tmPS);
         prefetch_tmap(&tmQS);
     }
@@ -958,58 +951,52 @@ __global__ void __launch_bounds__(Fp4PairCfg<FMT>::THREADS, 1)
     int tp, tq;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- producer (both CTAs) ----------------
-            int stage = 0;
-            uint32_t phase = 0, issued = 0, last_par = 0;
-            bool ok = true;
-            while (ok && walk.next(p.tiles_p, tp, tq)) {
-                const int g = walk.g, q0 = tq * BN;
-                const int qn = off[g + 1] - off[g] - q0;
-                const int half = min(BN, (qn + 31) & ~31) >> 1;  // Q rows of each CTA
-                const int pieces = half > 96 ? 0 : (half + 31) >> 5;
-                const uint32_t bytes =
-                    2 * (C::STAGE_BYTES - (pieces ? C::Q_BYTES - pieces * 32 * BKB : 0));
-                const int prow = g * p.np + tp * 2 * BM + static_cast<int>(rank) * BM;
-                const int qrow = off[g] + q0 + static_cast<int>(rank) * half;
-                // one stage of a 128-row scale block is SL lines of the scale maps (blocks that do
-                // not exist belong to rows that are not stored)
-                constexpr int SL = C::SF / 1024;
-                const int pb = g * p.npb + tp * 2 + static_cast<int>(rank);
-                const int qb = qblk[g] + (q0 >> 7);
-                for (int kb = 0; kb < p.stages; ++kb) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
-                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
-                        ok = false;
-                        break;
-                    }
+        // ---------------- producer (both CTAs; the whole warp, one lane issues) ----------------
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last_par = 0;
+        bool ok = true;
+        while (ok && walk.next(p.tiles_p, tp, tq)) {
+            const int g = walk.g, q0 = tq * BN;
+            const int qn = off[g + 1] - off[g] - q0;
+            const int half = min(BN, (qn + 31) & ~31) >> 1;  // Q rows of each CTA
+            const int prow = g * p.np + tp * 2 * BM + static_cast<int>(rank) * BM;
+            const int qrow = off[g] + q0 + static_cast<int>(rank) * half;
+            // one stage of a 128-row scale block is SL lines of the scale maps (blocks that do
+            // not exist belong to rows that are not stored)
+            constexpr int SL = C::SF / 1024;
+            const int pb = g * p.npb + tp * 2 + static_cast<int>(rank);
+            const int qb = qblk[g] + (q0 >> 7);
+            for (int kb = 0; kb < p.stages; ++kb) {
+                if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
                     const uint32_t fb = full_l + 8u * stage;
-                    if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
-                    uint8_t* dq = sQ + stage * C::Q_BYTES;
+                    if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
                     uint8_t* sf = sSF + stage * C::SF_STAGE;
                     tma_load_3d_pair(sP + stage * C::P_BYTES, &tmP, fb, kb * (FBK / 4), prow, 0);
-                    if (pieces == 0) tma_load_3d_pair(dq, &tmQ, fb, kb * (FBK / 4), qrow, 0);
-                    for (int i = 0; i < pieces; ++i)
-                        tma_load_3d_pair(dq + i * 32 * BKB, &tmQ32, fb, kb * (FBK / 4),
-                                         qrow + 32 * i, 0);
+                    tma_load_3d_pair(sQ + stage * C::Q_BYTES, &tmQ, fb, kb * (FBK / 4), qrow, 0);
                     tma_load_3d_pair(sf, &tmPS, fb, 0, kb * SL, pb);
                     tma_load_3d_pair(sf + C::SF, &tmQS, fb, 0, kb * SL, qb);
-                    issued |= 1u << stage;
-                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                }
+                __syncwarp();
+                issued |= 1u << stage;
+                last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            griddep_launch_dependents();
-            if (leader) {
-                int dummy = 0;
-                for (int s = 0; s < STAGES; ++s)
-                    if (issued & (1u << s))
-                        mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
-                                  GK_DEV_TIMEOUT_DRAIN, tmo);
-            }
+        }
+        griddep_launch_dependents();
+        if (leader) {
+            int dummy = 0;
+            for (int s = 0; s < STAGES; ++s)
+                if (issued & (1u << s))
+                    mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
+                              GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp == 1) {
         if (leader) {
@@ -1329,16 +1316,16 @@ bool large_view(const Fp4View& v) {
 }
 
 template <int FMT, int BN>
-int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const CUtensorMap& tq32,
-                    const Fp4GemmParams& p, int grid, cudaStream_t st) {
+int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const Fp4GemmParams& p, int grid,
+                    cudaStream_t st) {
     using C = Fp4Cfg<FMT, BN>;
     auto kern = fp4_gemm_kernel<FMT, BN>;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(kern, C::SMEM, done);
     if (e != cudaSuccess)
         return api_err(GK_ECUDA, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, Fp4GemmParams>(
-        1, kern, grid, C::THREADS, C::SMEM, st, tp, tq, tq32, p);
+    return launch_overlapped<CUtensorMap, CUtensorMap, Fp4GemmParams>(
+        1, kern, grid, C::THREADS, C::SMEM, st, tp, tq, p);
 }
 
 // Clusters of the pair kernel that are resident at once on the current device (0 on failure).
@@ -1397,10 +1384,9 @@ int run_fp4_gemm(Fp4GemmParams p, const gk_fp4_matrix* a, const gk_fp4_matrix* b
         static_cast<int64_t>(p.groups) * p.np > INT32_MAX / 2)
         return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
     p.tiles_p = static_cast<int>((p.np + tm - 1) / tm);
-    CUtensorMap tmp, tmq, tmq32;
+    CUtensorMap tmp, tmq;
     memset(&tmp, 0, sizeof(tmp));
     memset(&tmq, 0, sizeof(tmq));
-    memset(&tmq32, 0, sizeof(tmq32));
     char err[256] = "";
     int rc = 0;
     if (!p.zero) {
@@ -1411,10 +1397,7 @@ int run_fp4_gemm(Fp4GemmParams p, const gk_fp4_matrix* a, const gk_fp4_matrix* b
         if (!rc)
             rc = encode_tmap_u16(&tmq, a->data, pe, p.rows, 1, pe, pe, 64, pair ? 128 : bn, err,
                                  sizeof(err));
-        if (!rc && bn > 32)
-            rc = encode_tmap_u16(&tmq32, a->data, pe, p.rows, 1, pe, pe, 64, 32, err, sizeof(err));
         if (rc) return set_last_error(rc, err);
-        if (bn == 32) tmq32 = tmq;
     }
     if (pair) {
         using C = Fp4PairCfg<FMT>;
@@ -1431,16 +1414,15 @@ int run_fp4_gemm(Fp4GemmParams p, const gk_fp4_matrix* a, const gk_fp4_matrix* b
                                    sizeof(err));
         if (rc) return set_last_error(rc, err);
         const int grid = 2 * static_cast<int>(tiles < clusters ? tiles : clusters);
-        return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap,
-                                 Fp4GemmParams>(2, fp4_pair_kernel<FMT>, grid, C::THREADS, C::SMEM,
-                                                st, tmp, tmq, tmq32, tps, tqs, p);
+        return launch_overlapped<CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Fp4GemmParams>(
+            2, fp4_pair_kernel<FMT>, grid, C::THREADS, C::SMEM, st, tmp, tmq, tps, tqs, p);
     }
     const int sms = sm_count();
     const int grid = static_cast<int>(tiles < sms ? tiles : sms);
     switch (bn) {
-        case 32: return launch_fp4_gemm<FMT, 32>(tmp, tmq, tmq32, p, grid, st);
-        case 64: return launch_fp4_gemm<FMT, 64>(tmp, tmq, tmq32, p, grid, st);
-        default: return launch_fp4_gemm<FMT, 128>(tmp, tmq, tmq32, p, grid, st);
+        case 32: return launch_fp4_gemm<FMT, 32>(tmp, tmq, p, grid, st);
+        case 64: return launch_fp4_gemm<FMT, 64>(tmp, tmq, p, grid, st);
+        default: return launch_fp4_gemm<FMT, 128>(tmp, tmq, p, grid, st);
     }
 }
 

@@ -235,20 +235,20 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     GTile t;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- TMA producer ----------------
-            int stage = 0;
-            uint32_t phase = 0, issued = 0, last_par = 0;
-            bool ok = true;
-            while (ok && next_tile<BN>(walk, p, t)) {
-                const int pz = p.p_z ? t.g : 0;
-                const int qb = static_cast<int>(t.qbase);
-                for (int kb = 0; kb < t.nk; kb += GBK) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
-                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
-                        ok = false;
-                        break;
-                    }
+        // ---------------- TMA producer (the whole warp, one lane issues) ----------------
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last_par = 0;
+        bool ok = true;
+        while (ok && next_tile<BN>(walk, p, t)) {
+            const int pz = p.p_z ? t.g : 0;
+            const int qb = static_cast<int>(t.qbase);
+            for (int kb = 0; kb < t.nk; kb += GBK) {
+                if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
                     uint64_t* fb = &full[stage];
                     uint8_t* dp = sP + stage * C::P_BYTES;
                     uint8_t* dq = sQ + stage * C::Q_BYTES;
@@ -272,22 +272,23 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                     } else {
                         tma_load_3d(dq, &tmQ, fb, k, qb, 0);
                     }
-                    issued |= 1u << stage;
-                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                }
+                __syncwarp();
+                issued |= 1u << stage;
+                last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            griddep_launch_dependents();
-            // every issued copy has landed before the CTA may exit
-            int dummy = 0;
-            for (int s = 0; s < STAGES; ++s)
-                if (issued & (1u << s))
-                    mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
-                              GK_DEV_TIMEOUT_DRAIN, tmo);
         }
+        griddep_launch_dependents();
+        // every issued copy has landed before the CTA may exit
+        int dummy = 0;
+        for (int s = 0; s < STAGES; ++s)
+            if (issued & (1u << s))
+                mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN,
+                          tmo);
     } else if (warp == 2) {
         // ---------------- the contraction's ragged end (weight gradient) ----------------
         if (p.wgrad) {
@@ -626,23 +627,23 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
     GTile t;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- TMA producer (both CTAs) ----------------
-            int stage = 0;
-            uint32_t phase = 0, issued = 0, last_par = 0;
-            bool ok = true;
-            while (ok && next_tile<BN, TM>(walk, p, t)) {
-                const int pz = p.p_z ? t.g : 0;
-                const int p0 = t.p0 + static_cast<int>(rank) * BM;
-                // the MMA's N, and this CTA's half of its rows
-                const int n = min(BN, (t.qn + 31) & ~31);
-                const int qb = static_cast<int>(t.qbase) + static_cast<int>(rank) * (n >> 1);
-                for (int kb = 0; kb < t.nk; kb += GBK) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
-                                   GK_DEV_TIMEOUT_PRODUCER, tmo)) {
-                        ok = false;
-                        break;
-                    }
+        // ---------------- TMA producer (both CTAs; the whole warp, one lane issues) ------------
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last_par = 0;
+        bool ok = true;
+        while (ok && next_tile<BN, TM>(walk, p, t)) {
+            const int pz = p.p_z ? t.g : 0;
+            const int p0 = t.p0 + static_cast<int>(rank) * BM;
+            // the MMA's N, and this CTA's half of its rows
+            const int n = min(BN, (t.qn + 31) & ~31);
+            const int qb = static_cast<int>(t.qbase) + static_cast<int>(rank) * (n >> 1);
+            for (int kb = 0; kb < t.nk; kb += GBK) {
+                if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_PRODUCER, tmo)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
                     const uint32_t fb = full_l + 8u * stage;
                     uint8_t* dp = sP + stage * C::P_BYTES;
                     uint8_t* dq = sQ + stage * C::Q_BYTES;
@@ -666,22 +667,23 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                     } else {
                         tma_load_3d_pair(dq, &tmQ, fb, k, qb, 0);
                     }
-                    issued |= 1u << stage;
-                    last_par = (last_par & ~(1u << stage)) | (phase << stage);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                }
+                __syncwarp();
+                issued |= 1u << stage;
+                last_par = (last_par & ~(1u << stage)) | (phase << stage);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            griddep_launch_dependents();
-            if (leader) {  // its full barriers count both CTAs' copies
-                int dummy = 0;
-                for (int s = 0; s < STAGES; ++s)
-                    if (issued & (1u << s))
-                        mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
-                                  GK_DEV_TIMEOUT_DRAIN, tmo);
-            }
+        }
+        griddep_launch_dependents();
+        if (leader) {  // its full barriers count both CTAs' copies
+            int dummy = 0;
+            for (int s = 0; s < STAGES; ++s)
+                if (issued & (1u << s))
+                    mbar_wait(&full[s], (last_par >> s) & 1u, &dummy, p.status,
+                              GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp == 1) {
         if (leader) {
