@@ -25,7 +25,10 @@
 // boxes as they land. In the weight gradient the contraction ends where the group ends, in the
 // middle of a stage: the stage's later MMAs are skipped, and warp 2 zeroes the rows between the
 // end and the next multiple of 16 in both operands (they belong to other groups and may hold
-// anything) before the MMA thread may read them.
+// anything). The copies of such a stage complete on a barrier of warp 2's (rfull), and warp 2
+// completes the stage's full[] when it is done, so the zeroing passes while earlier stages are
+// multiplied. (Asked for by the MMA warp when it got there it cost 2 us a tile: 39 against 26
+// us for 64 experts' gradients of 1024 x 512 over 65 rows.)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -119,7 +122,7 @@ struct GroupedCfg {
     static constexpr int Q_BYTES = BN * BKB;
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
-    static constexpr int BAR_BYTES = 256;
+    static constexpr int BAR_BYTES = 512;
     static constexpr int EPI_BYTES = NEPI * EPI_BUF;
     static constexpr int RAW_STAGES =
         (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
@@ -131,7 +134,7 @@ struct GroupedCfg {
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
     static_assert(BN == 32 || BN == 64 || BN == 128 || BN == 256, "tile width");
     static_assert(STAGES >= 2 && SMEM <= SMEM_LIMIT, "shared memory budget");
-    static_assert((2 * STAGES + 8) * 8 <= BAR_BYTES, "barrier area");
+    static_assert((3 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
 };
 
 // One tile of the schedule as every role sees it.
@@ -175,6 +178,19 @@ __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, 
     return true;
 }
 
+// Whether the stage of contraction block kb holds the end of its group inside 16 indices.
+__device__ __forceinline__ bool ragged_stage(const GroupedParams& p, const GTile& t, int kb) {
+    return p.wgrad && t.nk - kb < GBK && (t.nk & 15) != 0;
+}
+
+// Zeroes contraction indices [v, next multiple of 16) of `boxes` MN-major boxes (lines of 128 bytes).
+__device__ __forceinline__ void zero_rows(uint8_t* box, int boxes, int v, int lane) {
+    const int n = (16 - (v & 15)) * 8;  // 16-byte pieces per box
+    for (int c = 0; c < boxes; ++c)
+        for (int i = lane; i < n; i += 32)
+            *reinterpret_cast<uint4*>(box + c * MN_BOX + v * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
 template <int BN>
 __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     grouped_half_kernel(const __grid_constant__ CUtensorMap tmP,
@@ -187,12 +203,11 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     uint8_t* sQ = smem + STAGES * C::P_BYTES;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
     uint64_t* empty = full + STAGES;
-    uint64_t* tfull = empty + STAGES;
+    uint64_t* rfull = empty + STAGES;  // a stage that holds a group's ragged end has landed
+    uint64_t* tfull = rfull + STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint64_t* fixreq = drain + 1;  // the stage holding a group's ragged end has landed
-    uint64_t* fixdone = drain + 2; // ... and its rows past the end are zero
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 3);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
     int* tile0 = off + GROUP_TABLE_INTS;
@@ -203,14 +218,13 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+            mbar_init(&rfull[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
             mbar_init(&tempty[a], C::NEPI);
         }
         mbar_init(drain, 1);
-        mbar_init(fixreq, 1);
-        mbar_init(fixdone, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -249,7 +263,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                     break;
                 }
                 if (elect_one()) {
-                    uint64_t* fb = &full[stage];
+                    uint64_t* fb = ragged_stage(p, t, kb) ? &rfull[stage] : &full[stage];
                     uint8_t* dp = sP + stage * C::P_BYTES;
                     uint8_t* dq = sQ + stage * C::Q_BYTES;
                     mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
@@ -292,32 +306,28 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     } else if (warp == 2) {
         // ---------------- the contraction's ragged end (weight gradient) ----------------
         if (p.wgrad) {
-            int blocks = 0;  // stages filled so far
-            uint32_t par = 0;
+            int blocks = 0;        // stages filled so far
+            uint32_t parity = 0;   // rfull's, a bit per stage
             while (next_tile<BN>(walk, p, t)) {
                 blocks += (t.nk + GBK - 1) / GBK;
                 if ((t.nk & 15) == 0) continue;
                 const int stage = (blocks - 1) % STAGES;
-                if (!warp_wait(fixreq, par, abort_flag, p.status, GK_DEV_TIMEOUT_PRODUCER, tmo))
+                if (!warp_wait(&rfull[stage], (parity >> stage) & 1u, abort_flag, p.status,
+                               GK_DEV_TIMEOUT_PRODUCER, tmo))
                     break;
-                par ^= 1u;
-                const int v = t.nk & (GBK - 1), zrows = 16 - (t.nk & 15);  // rows [v, v + zrows)
-                constexpr int CH = (BM + BN) / 64;
-                for (int i = lane; i < CH * zrows * 8; i += 32) {
-                    const int c = i / (zrows * 8), r = i % (zrows * 8);
-                    uint8_t* box = c < BM / 64 ? sP + stage * C::P_BYTES + c * MN_BOX
-                                               : sQ + stage * C::Q_BYTES + (c - BM / 64) * MN_BOX;
-                    *reinterpret_cast<uint4*>(box + v * 128 + r * 16) = make_uint4(0, 0, 0, 0);
-                }
+                parity ^= 1u << stage;
+                const int v = t.nk & (GBK - 1);
+                zero_rows(sP + stage * C::P_BYTES, BM / 64, v, lane);
+                zero_rows(sQ + stage * C::Q_BYTES, BN / 64, v, lane);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(fixdone);
+                if (lane == 0) mbar_arrive(&full[stage]);
             }
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (the whole warp, one lane issues) ----------------
         int stage = 0;
-        uint32_t phase = 0, fixpar = 0;
+        uint32_t phase = 0;
         const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
         bool ok = true;
         for (int local = 0; ok && next_tile<BN>(walk, p, t); ++local) {
@@ -337,17 +347,8 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                 }
                 tc_fence_after();
                 const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
-                // the group's end: the rows past it up to a multiple of 16 are zeroed
+                // the group's end: only the MMAs up to it (rounded up to 16) are issued
                 const bool cut = p.wgrad && t.nk - kb < GBK;
-                if (cut && (t.nk & 15)) {
-                    if (lane == 0) mbar_arrive(fixreq);
-                    if (!warp_wait(fixdone, fixpar, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
-                        ok = false;
-                        break;
-                    }
-                    fixpar ^= 1u;
-                    tc_fence_after();
-                }
                 if (elect_one()) {
                     if (cut) {
                         const int steps = (t.nk - kb + 15) >> 4;
@@ -562,7 +563,7 @@ struct GPairCfg {
     static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
-    static_assert(STAGES >= 4 && (2 * STAGES + 8) * 8 <= BAR_BYTES, "barrier area");
+    static_assert(STAGES >= 4 && (4 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
 };
 
 __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
@@ -576,12 +577,12 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
     uint8_t* sQ = smem + STAGES * C::P_BYTES;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
     uint64_t* empty = full + STAGES;
-    uint64_t* tfull = empty + STAGES;
+    uint64_t* rfull = empty + STAGES;  // own half of a stage with a ragged end has landed
+    uint64_t* peerz = rfull + STAGES;  // leader's: the peer has zeroed its half
+    uint64_t* tfull = peerz + STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint64_t* fixreq = drain + 1;
-    uint64_t* fixdone = drain + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 3);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(smem + C::OFF_TAB);
     int* tile0 = off + GROUP_TABLE_INTS;
@@ -594,14 +595,14 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);  // the leader's producer; the peer's copies only add bytes
             mbar_init(&empty[s], 1);
+            mbar_init(&rfull[s], 1);
+            mbar_init(&peerz[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
             mbar_init(&tempty[a], 2 * C::NEPI);  // every epilogue warp of both CTAs
         }
         mbar_init(drain, 1);
-        mbar_init(fixreq, 1);
-        mbar_init(fixdone, 2);  // both CTAs' warps
         *abort_flag = 0;
         fence_mbar_init();
         prefetch_tmap(&tmP);
@@ -623,6 +624,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t full_l = mapa_shared(smem_u32(&full[0]), 0);
     const uint32_t tempty_l = mapa_shared(smem_u32(&tempty[0]), 0);
+    const uint32_t rfull_own = mapa_shared(smem_u32(&rfull[0]), rank);
     GroupWalk walk(off, tile0, p.groups, blockIdx.x >> 1, gridDim.x >> 1);
     GTile t;
 
@@ -644,10 +646,15 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                     break;
                 }
                 if (elect_one()) {
-                    const uint32_t fb = full_l + 8u * stage;
+                    // a ragged stage's halves complete on each CTA's own rfull
+                    const bool ragged = ragged_stage(p, t, kb);
+                    const uint32_t fb = (ragged ? rfull_own : full_l) + 8u * stage;
                     uint8_t* dp = sP + stage * C::P_BYTES;
                     uint8_t* dq = sQ + stage * C::Q_BYTES;
-                    if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
+                    if (ragged)
+                        mbar_arrive_expect_tx(&rfull[stage], C::STAGE_BYTES);
+                    else if (leader)
+                        mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
                     const int k = t.k0 + kb;
                     if (p.p_4d) {
                         tma_load_4d_pair(dp, &tmP, fb, 0, k, p0 >> 6, pz);
@@ -688,10 +695,8 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
     } else if (warp == 1) {
         if (leader) {
             // ---------------- MMA issuer (leader; the whole warp, one lane issues) ----------------
-            const uint32_t fixreq0 = mapa_shared(smem_u32(fixreq), 0);
-            const uint32_t fixreq1 = mapa_shared(smem_u32(fixreq), 1);
             int stage = 0;
-            uint32_t phase = 0, fixpar = 0;
+            uint32_t phase = 0;
             const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
             bool ok = true;
             for (int local = 0; ok && next_tile<BN, TM>(walk, p, t); ++local) {
@@ -714,20 +719,6 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                     tc_fence_after();
                     const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
                     const bool cut = p.wgrad && t.nk - kb < GBK;
-                    if (cut && (t.nk & 15)) {
-                        if (lane == 0) {
-                            mbar_arrive_cluster(fixreq0);
-                            mbar_arrive_cluster(fixreq1);
-                        }
-                        const bool fixed = mbar_wait_cluster(fixdone, fixpar, abort_flag, p.status,
-                                                             GK_DEV_TIMEOUT_MMA, tmo);
-                        if (__any_sync(0xffffffffu, !fixed)) {
-                            ok = false;
-                            break;
-                        }
-                        fixpar ^= 1u;
-                        tc_fence_after();
-                    }
                     if (elect_one()) {
                         if (cut) {
                             const int steps = (t.nk - kb + 15) >> 4;
@@ -759,29 +750,32 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
         }
     } else if (warp == 2) {
         // ---------------- the contraction's ragged end (both CTAs) ----------------
+        // Each CTA's warp zeroes its own half; the leader's completes full[] once both have.
         if (p.wgrad) {
-            const uint32_t done = mapa_shared(smem_u32(fixdone), 0);
-            int blocks = 0;
-            uint32_t par = 0;
+            const uint32_t peerz_l = mapa_shared(smem_u32(peerz), 0);
+            int blocks = 0;        // stages filled so far
+            uint32_t parity = 0;   // rfull's and peerz's, a bit per stage
             while (next_tile<BN, TM>(walk, p, t)) {
                 blocks += (t.nk + GBK - 1) / GBK;
                 if ((t.nk & 15) == 0) continue;
                 const int stage = (blocks - 1) % STAGES;
-                const bool ok = mbar_wait_cluster(fixreq, par, abort_flag, p.status,
-                                                  GK_DEV_TIMEOUT_PRODUCER, tmo);
-                if (__any_sync(0xffffffffu, !ok)) break;
-                par ^= 1u;
-                const int v = t.nk & (GBK - 1), zrows = 16 - (t.nk & 15);
-                constexpr int CH = (BM + BN / 2) / 64;
-                for (int i = lane; i < CH * zrows * 8; i += 32) {
-                    const int c = i / (zrows * 8), r = i % (zrows * 8);
-                    uint8_t* box = c < BM / 64 ? sP + stage * C::P_BYTES + c * MN_BOX
-                                               : sQ + stage * C::Q_BYTES + (c - BM / 64) * MN_BOX;
-                    *reinterpret_cast<uint4*>(box + v * 128 + r * 16) = make_uint4(0, 0, 0, 0);
-                }
+                const uint32_t par = (parity >> stage) & 1u;
+                if (!warp_wait(&rfull[stage], par, abort_flag, p.status, GK_DEV_TIMEOUT_PRODUCER, tmo))
+                    break;
+                parity ^= 1u << stage;
+                const int v = t.nk & (GBK - 1);
+                zero_rows(sP + stage * C::P_BYTES, BM / 64, v, lane);
+                zero_rows(sQ + stage * C::Q_BYTES, BN / 128, v, lane);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(done);
+                if (!leader) {
+                    if (lane == 0) mbar_arrive_cluster(peerz_l + 8u * stage);
+                    continue;
+                }
+                const bool ok = mbar_wait_cluster(&peerz[stage], par, abort_flag, p.status,
+                                                  GK_DEV_TIMEOUT_PRODUCER, tmo);
+                if (__any_sync(0xffffffffu, !ok)) break;
+                if (lane == 0) mbar_arrive(&full[stage]);
             }
         }
     } else if (warp >= C::EPI_W0) {
