@@ -222,6 +222,10 @@ __device__ __forceinline__ int scale_at(int sf) { return (sf >> 2) * 512 + (sf &
 
 // ---- quantisation --------------------------------------------------------------------------------
 
+// The kernels below start while the kernel that writes their input may still be running (they wait
+// for it before they read), so the input is not read-only for their lifetime: plain loads, no
+// read-only path and no __restrict__.
+
 // One block's scale from the largest magnitude's bits (as f32): the scale byte, and what the
 // elements are multiplied with.
 template <int FMT>
@@ -266,7 +270,7 @@ struct Raw8 {
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-            q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            q[i] = reinterpret_cast<const uint4*>(p)[i];
     }
     // element by element: any stride, zero at or past column `cols`
     __device__ __forceinline__ void load(const T* src, int64_t cs, int k, int cols) {
@@ -294,7 +298,7 @@ struct Raw8 {
 // in flight, else 1: for one row of 4096 the four would only follow each other.
 template <int FMT, typename T, int QU>
 __global__ void __launch_bounds__(256)
-    quantize_fp4_kernel(const T* __restrict__ x, int64_t rs, int64_t cs, int64_t gs, int vec,
+    quantize_fp4_kernel(const T* x, int64_t rs, int64_t cs, int64_t gs, int vec,
                         Fp4View v, NvScale nv) {
     __shared__ RowMap map;
     griddep_wait();
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(256)
 // warp's stores are contiguous.
 template <int FMT, int QU>
 __global__ void __launch_bounds__(256)
-    dequantize_fp4_kernel(Fp4View v, float s, float* __restrict__ out, int64_t rs, int64_t cs,
+    dequantize_fp4_kernel(Fp4View v, float s, float* out, int64_t rs, int64_t cs,
                           int vec) {
     __shared__ RowMap map;
     griddep_wait();
@@ -420,8 +424,8 @@ __global__ void __launch_bounds__(256)
 // Row-major codes (two a byte) and scales (one byte a block) into the layout above.
 template <int FMT>
 __global__ void __launch_bounds__(256)
-    import_fp4_kernel(const uint8_t* __restrict__ codes, int64_t codes_ld,
-                      const uint8_t* __restrict__ scales, int64_t scales_ld, Fp4View v) {
+    import_fp4_kernel(const uint8_t* codes, int64_t codes_ld,
+                      const uint8_t* scales, int64_t scales_ld, Fp4View v) {
     __shared__ RowMap map;
     griddep_wait();
     if (!one_group(v))

@@ -423,6 +423,8 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
 }
 
 // ---- operands that TMA cannot address --------------------------------------------------------------
+// (Plain loads: these kernels may start before the kernel that writes their source has ended, and
+// only wait for it, so the source is not read-only for their lifetime.)
 
 // The 16 bytes at byte offset a (0, 2 .. 14) of the 32 in (lo, hi).
 __device__ __forceinline__ uint4 shift_bytes(const uint4& lo, const uint4& hi, uint32_t a) {
@@ -447,7 +449,7 @@ constexpr int RU = 4;  // 16-byte pieces of a lane in flight
 // RU * 256 elements of a line; a piece is two aligned 16-byte loads shifted together (one where
 // the line is aligned), or single elements where those would leave the source's bytes [lo, hi).
 __global__ void __launch_bounds__(256)
-    realign_lines_kernel(uint16_t* __restrict__ dst, int64_t dld, const uint16_t* __restrict__ src,
+    realign_lines_kernel(uint16_t* dst, int64_t dld, const uint16_t* src,
                          int64_t pitch, int64_t gs, int64_t lines, int64_t len, int64_t groups,
                          const uint8_t* lo, const uint8_t* hi) {
     griddep_wait();
@@ -474,15 +476,15 @@ __global__ void __launch_bounds__(256)
             const uint8_t* p = reinterpret_cast<const uint8_t*>(s + e) - a;
             const bool two = a + 2 * n > 16;
             if (p >= lo && p + (two ? 32 : 16) <= hi) {
-                x[i] = __ldg(reinterpret_cast<const uint4*>(p));
-                if (two) y[i] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+                x[i] = *reinterpret_cast<const uint4*>(p);
+                if (two) y[i] = reinterpret_cast<const uint4*>(p)[1];
             } else {  // placed so that the shift below finds them
                 uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     if (k < n) {
                         const uint32_t at = a / 2 + k;
-                        const uint32_t v = static_cast<uint32_t>(__ldg(s + e + k)) << (16 * (at & 1));
+                        const uint32_t v = static_cast<uint32_t>(s[e + k]) << (16 * (at & 1));
 #pragma unroll
                         for (uint32_t q = 0; q < 8; ++q)
                             if ((at >> 1) == q) w[q] |= v;
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(256)
 // dst[g][l][e] = src[g * gs + l * sl + e * se], padded likewise, through a 32 x 32 tile: both sides
 // are coalesced whichever source stride is small.
 __global__ void __launch_bounds__(256)
-    realign_any_kernel(uint16_t* __restrict__ dst, int64_t dld, const uint16_t* __restrict__ src,
+    realign_any_kernel(uint16_t* dst, int64_t dld, const uint16_t* src,
                        int64_t sl, int64_t se, int64_t gs, int64_t lines, int64_t len,
                        int64_t groups) {
     __shared__ uint16_t tile[32][33];
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(256)
         for (int i = ty; i < 32; i += 8) {
             const int64_t l = l0 + (e_fast ? i : tx), e = e0 + (e_fast ? tx : i);
             const uint16_t v =
-                l < lines && e < len ? __ldg(src + g * gs + l * sl + e * se) : uint16_t{0};
+                l < lines && e < len ? src[g * gs + l * sl + e * se] : uint16_t{0};
             tile[e_fast ? i : tx][e_fast ? tx : i] = v;
         }
         __syncthreads();

@@ -575,3 +575,37 @@ def test_extreme_matrix_scales():
     product(*one, c[0])
     product(*far, c[1])
     assert torch.equal(c[0], c[1])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_chain_without_synchronisation(fmt):
+    """A chain of quantise, product by expert, 16-bit grouped product and back, every call reading
+    what the one before wrote and writing buffers that earlier calls read, with nothing waited for:
+    the same bits as with a synchronisation after every call."""
+    torch = torch_cuda()
+    rows, d, h, g = 700, 512, 384, 3
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    off = torch.tensor([0, 300, 301, 700], dtype=torch.int32, device="cuda")
+    s = 1.0 if fmt == gk.FP4_MX else 0.002
+    w4 = gk.quantize_fp4(gk.MatRef.from_row_major(
+        torch.randn(g * h, d, generator=gen, device="cuda") * d ** -0.5, h, d), fmt, scale=s, groups=g,
+        x_gs=h * d)
+    w2 = (torch.randn(g, h, d, generator=gen, device="cuda") * h ** -0.5).bfloat16()
+    x0 = torch.randn(rows, d, generator=gen, device="cuda").bfloat16()
+
+    def chain(sync):
+        x, y = x0.clone(), torch.zeros(rows, h, device="cuda", dtype=torch.bfloat16)
+        q = gk.Fp4Matrix.empty(rows, d, fmt, s, offsets=off)
+        for _ in range(30):
+            gk.quantize_fp4(gk.MatRef.from_row_major(x, rows, d), fmt, out=q, sync=sync)
+            gk.gemm_fp4(1.0, q, w4, 0.0, gk.MatMut.from_row_major(y, rows, h), sync=sync)
+            gk.gemm_half_grouped(1.0, gk.MatRef.from_row_major(y, rows, h),
+                                 gk.MatRef.from_row_major(w2, h, d), h * d, off, 0.0,
+                                 gk.MatMut.from_row_major(x, rows, d), sync=sync)
+        torch.cuda.synchronize()
+        return x
+
+    want = chain(True)
+    assert bool(want.isfinite().all()) and float(want.abs().max()) > 0
+    for _ in range(5):
+        assert torch.equal(chain(False), want)
