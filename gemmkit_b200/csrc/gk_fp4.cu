@@ -58,6 +58,18 @@ __device__ __forceinline__ uint32_t cvt_e2m1x8(const float (&x)[8]) {
     return w;
 }
 
+// y = x * m, two products an instruction.
+__device__ __forceinline__ void scale8(const float (&x)[8], float m, float (&y)[8]) {
+    uint64_t mm;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(mm) : "f"(m));
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tmul.rn.f32x2 t, t, %4;\n\t"
+            "mov.b64 {%0, %1}, t;\n\t}"
+            : "=f"(y[i]), "=f"(y[i + 1])
+            : "f"(x[i]), "f"(x[i + 1]), "l"(mm));
+}
+
 // Two f32 to e4m3 (round to nearest even, saturating): lo in the low byte.
 __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     uint16_t h;
@@ -134,13 +146,9 @@ __device__ __noinline__ uint32_t nv_element_borders(uint32_t w, uint32_t w2, flo
     return w;
 }
 __device__ __forceinline__ uint32_t nv_elements(const float (&x)[8], float r, float sb, float s) {
-    const float rlo = r * (1.0f - 0x1p-20f), rhi = r * (1.0f + 0x1p-20f);
     float lo[8], hi[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo[i] = x[i] * rlo;
-        hi[i] = x[i] * rhi;
-    }
+    scale8(x, r * (1.0f - 0x1p-20f), lo);
+    scale8(x, r * (1.0f + 0x1p-20f), hi);
     const uint32_t w = cvt_e2m1x8(lo), w2 = cvt_e2m1x8(hi);
     if (w == w2) return w;
     return nv_element_borders(w, w2, x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], sb, s);
@@ -255,34 +263,34 @@ __device__ __forceinline__ uint32_t block_codes(const float (&x)[8], uint32_t am
     if (amax_bits >= 0x7F800000u) return 0u;
     if constexpr (FMT == GK_FP4_MX) {
         float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i] * mul;  // a power of two: exact
+        scale8(x, mul, y);  // a power of two: exact
         return cvt_e2m1x8(y);
     } else {
         return nv_elements(x, mul, sb, nv.s);
     }
 }
 
-// Eight elements of a row as loaded: 16 bytes of 16-bit floats, or 32 of f32.
-template <typename T>
-struct Raw8 {
-    uint4 q[sizeof(T) / 2];
+// E (8 or 16) elements of a row as loaded.
+template <typename T, int E>
+struct RawRow {
+    static constexpr int N = static_cast<int>(sizeof(T)) * 8 / 16;  // pieces of 16 bytes in eight
+    uint4 q[N * E / 8];
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-            q[i] = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < N * E / 8; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
     }
     // element by element: any stride, zero at or past column `cols`
     __device__ __forceinline__ void load(const T* src, int64_t cs, int k, int cols) {
-        T v[8];
+        T v[E];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < E; ++i)
             v[i] = k + i < cols ? src[static_cast<int64_t>(k + i) * cs] : T(0.0f);
         memcpy(q, v, sizeof(v));
     }
-    __device__ __forceinline__ void values(float (&x)[8]) const {
+    // elements 8 h .. 8 h + 7
+    __device__ __forceinline__ void values(int h, float (&x)[8]) const {
         T v[8];
-        memcpy(v, q, sizeof(v));
+        memcpy(v, q + h * N, sizeof(v));
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = to_f(v[i]);
     }
@@ -291,48 +299,61 @@ struct Raw8 {
     static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 };
 
-// A warp takes up to QU stages (256 elements each) of a row, a lane eight elements of each: loads
-// of 16 bytes (two for f32), the block's maximum by shuffles, four bytes of codes stored.
-// Elements past the row are zero, and so are the scales of blocks past it (the product reads
-// whole stages). QU is 4 where that still gives every SM's warps a unit, so that enough loads are
-// in flight, else 1: for one row of 4096 the four would only follow each other.
-template <int FMT, typename T, int QU>
+// A warp takes QU steps of a row, a lane E elements of each: E / 8 stages of 256 elements a step,
+// loads of 16 bytes, the block's maximum by shuffles, E / 2 bytes of codes stored. Elements past
+// the row are zero, and so are the scales of blocks past it (the product reads whole stages).
+//   E is 16 for many 16-bit rows read in whole pieces: the scale's arithmetic, a large part of the
+// work in nv, is then done by one lane of a block (nv) or two (mx) instead of two or four.
+// 8192 x 8192 of bf16: 31.9 us with 8, 28.3 with 16 (mx), 48.9 and 40.0 (nv). It is 8 for f32,
+// where 16 would put a lane's loads 64 bytes from its neighbour's (4096 x 4096 in mx: 8.4 against
+// 10.8 us), for rows read element by element (333 x 4099 of f32: 3.7 against 6.7 us), and for a
+// few rows, where the longer chain of a lane shows (1 x 4096 in nv: 1.7 against 1.9 us).
+//   A unit is 4 stages where that still gives every SM's warps one, so that enough loads are in
+// flight, else one: for one row of 4096 more would only follow each other.
+template <int FMT, typename T, int E, int QU>
 __global__ void __launch_bounds__(256)
-    quantize_fp4_kernel(const T* x, int64_t rs, int64_t cs, int64_t gs, int vec,
-                        Fp4View v, NvScale nv) {
+    quantize_fp4_kernel(const T* x, int64_t rs, int64_t cs, int64_t gs, int vec, Fp4View v,
+                        NvScale nv) {
     __shared__ RowMap map;
     griddep_wait();
     griddep_launch_dependents();
     if (!one_group(v))
         load_groups(v.offsets, v.groups, v.rows, map.off, map.blk,
                     blockIdx.x == 0 ? v.status : nullptr, [](int m) { return (m + 127) >> 7; });
-    const int lane = threadIdx.x & 31;
-    constexpr int LPB = Fp4<FMT>::BS / 8;  // lanes per block
-    const uint32_t chunks = static_cast<uint32_t>(v.stages + QU - 1) / QU;  // of a row
+    constexpr int SPW = E / 8;               // stages a step
+    constexpr int UNIT = QU * SPW;           // stages of a unit
+    constexpr int LPS = 32 / SPW;            // lanes of a stage
+    constexpr int LPB = Fp4<FMT>::BS / E;    // lanes of a block
+    const int lane = threadIdx.x & 31, in_stage = lane % LPS;
+    const uint32_t chunks = static_cast<uint32_t>(v.stages + UNIT - 1) / UNIT;  // of a row
     // units (row, chunk), counted in 64 bits only where 32 do not hold them
     const uint64_t units = static_cast<uint64_t>(v.rows) * chunks;
     const uint32_t step = gridDim.x * (blockDim.x >> 5);
     for (uint64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
         const int r = units >> 32 ? static_cast<int>(u / chunks)
                                   : static_cast<int>(static_cast<uint32_t>(u) / chunks);
-        const int st0 = static_cast<int>(u - static_cast<uint64_t>(r) * chunks) * QU;
+        // this lane's first stage; its next ones lie SPW on
+        const int st0 =
+            static_cast<int>(u - static_cast<uint64_t>(r) * chunks) * UNIT + lane / LPS;
         int block, in, g, at;
         if (!find_row(v, map, r, block, in, g, at)) continue;
         // a stack's groups lie gs apart; ragged groups and a single one lie row after row
         const T* src = x + (v.offsets ? static_cast<int64_t>(r) * rs : g * gs + at * rs);
         uint8_t* dst = v.data + static_cast<int64_t>(r) * v.pitch +
-                       static_cast<int64_t>(st0) * (FBK / 2) + lane * 4;
+                       static_cast<int64_t>(st0) * (FBK / 2) + in_stage * (E / 2);
         uint8_t* sp = scale_row<FMT>(v, block, in) +
-                      static_cast<int64_t>(st0) * Fp4<FMT>::SF_BYTES + scale_at(lane / LPB);
-        Raw8<T> raw[QU];
-        if (vec && (st0 + QU) * FBK <= v.cols) {
+                      static_cast<int64_t>(st0) * Fp4<FMT>::SF_BYTES + scale_at(in_stage / LPB);
+        const int k0 = st0 * FBK + in_stage * E;
+        RawRow<T, E> raw[QU];
+        // a whole unit without a branch between its loads, so that they go out together
+        if (vec && (st0 - lane / LPS + UNIT) * FBK <= v.cols) {
 #pragma unroll
-            for (int i = 0; i < QU; ++i) raw[i].load(src + (st0 + i) * FBK + lane * 8);
+            for (int i = 0; i < QU; ++i) raw[i].load(src + k0 + i * SPW * FBK);
         } else {
 #pragma unroll
             for (int i = 0; i < QU; ++i) {
-                const int k = (st0 + i) * FBK + lane * 8;
-                if (vec && k + 8 <= v.cols)
+                const int k = k0 + i * SPW * FBK;
+                if (vec && k + E <= v.cols)
                     raw[i].load(src + k);
                 else
                     raw[i].load(src, cs, k, v.cols);
@@ -340,21 +361,28 @@ __global__ void __launch_bounds__(256)
         }
 #pragma unroll
         for (int i = 0; i < QU; ++i) {
-            const int st = st0 + i;
-            if (st >= v.stages) break;
-            float e[8];
-            raw[i].values(e);
-            uint32_t m = absmax_bits(e);
+            const int st = st0 + i * SPW;
+            if (st - lane / LPS >= v.stages) break;
+            float e[SPW][8];
+            uint32_t m = 0;
+#pragma unroll
+            for (int h = 0; h < SPW; ++h) {
+                raw[i].values(h, e[h]);
+                m = max(m, absmax_bits(e[h]));
+            }
 #pragma unroll
             for (int d = 1; d < LPB; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
             float mul, sb;
             const uint32_t b = block_scale<FMT>(m, nv, mul, sb);
-            const uint32_t w = block_codes<FMT>(e, m, mul, sb, nv);
-            if (st * (FBK / 2) + lane * 4 < v.pitch)
-                *reinterpret_cast<uint32_t*>(dst + i * (FBK / 2)) = w;
-            if (lane % LPB == 0)
-                sp[i * Fp4<FMT>::SF_BYTES] =
-                    static_cast<uint8_t>(st * FBK + lane * 8 < v.cols ? b : 0u);
+            uint32_t w[SPW];
+#pragma unroll
+            for (int h = 0; h < SPW; ++h) w[h] = block_codes<FMT>(e[h], m, mul, sb, nv);
+            if (st >= v.stages) break;  // the second half's stage may lie past the row
+            if (st * (FBK / 2) + in_stage * (E / 2) < v.pitch)
+                memcpy(__builtin_assume_aligned(dst + i * SPW * (FBK / 2), sizeof(w)), w, sizeof(w));
+            if (in_stage % LPB == 0)
+                sp[i * SPW * Fp4<FMT>::SF_BYTES] =
+                    static_cast<uint8_t>(st * FBK + in_stage * E < v.cols ? b : 0u);
         }
     }
 }
@@ -1314,7 +1342,7 @@ int unit_grid(int64_t units) {
     return static_cast<int>(b < most ? b : most);
 }
 
-// Whether four stages per warp (QU) still give every SM 32 warps.
+// Whether four stages per warp still give every SM 32 warps.
 bool large_view(const Fp4View& v) {
     return static_cast<int64_t>(v.rows) * v.stages >= 4 * 32 * static_cast<int64_t>(sm_count());
 }
@@ -1440,14 +1468,19 @@ int run_quantize(const void* x, int64_t rs, int64_t cs, int64_t gs, const Fp4Vie
                     (rows1 || (rs * es) % 16 == 0) &&
                     (v.offsets || v.groups == 1 || (gs * es) % 16 == 0);
     const NvScale nv{scale, 1.0f / (6.0f * scale)};
-    auto go = [&](auto qu_tag) {
-        constexpr int QU = decltype(qu_tag)::value;
+    auto go = [&](auto e_tag, auto unit_tag) {
+        constexpr int E = decltype(e_tag)::value, UNIT = decltype(unit_tag)::value;
         return launch_overlapped<const T*, int64_t, int64_t, int64_t, int, Fp4View, NvScale>(
-            1, quantize_fp4_kernel<FMT, T, QU>,
-            unit_grid(static_cast<int64_t>(v.rows) * ((v.stages + QU - 1) / QU)), 256, 0, st,
+            1, quantize_fp4_kernel<FMT, T, E, UNIT * 8 / E>,
+            unit_grid(static_cast<int64_t>(v.rows) * ((v.stages + UNIT - 1) / UNIT)), 256, 0, st,
             static_cast<const T*>(x), rs, cs, gs, vec, v, nv);
     };
-    return large_view(v) ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 1>{});
+    using std::integral_constant;
+    const bool large = large_view(v);
+    if constexpr (sizeof(T) == 2)
+        if (vec && large) return go(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    return large ? go(integral_constant<int, 8>{}, integral_constant<int, 4>{})
+                 : go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
 }
 
 }  // namespace
