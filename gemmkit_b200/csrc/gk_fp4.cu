@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(Fp4Cfg<FMT, BN>::THREADS, 1)
 // OVER), the scales lie in the last OVER columns. The epilogue reads the shared columns first and
 // hands them over (thead) before it stores anything; the next tile's MMAs wait for that, not for
 // the rest. The scales have SLOTS slots; a slot is refilled once the MMAs of the stage that used it
-// last have finished (their commit on empty[]). Warp 3 issues the copies of scales to TMEM ahead of
+// last have finished (their commit on empty[]). Warps 2 and 3 copy the scales to TMEM ahead of
 // the MMA warp: issued between the MMAs by the same thread, the 12 (nv) or 6 (mx) copies of a
 // stage took MMA issue time.
 

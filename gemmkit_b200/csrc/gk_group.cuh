@@ -107,15 +107,20 @@ struct GroupWalk {
     __device__ __forceinline__ bool next(int tiles_p, int& tp, int& tq) {
         t += step;
         if (t >= total) return false;
-        while (t >= tile0[g + 1]) ++g;
-        const int r = t - tile0[g];
+        locate(t, tiles_p, tp, tq);
+        return true;
+    }
+
+    // The group and the indices of tile i; i does not fall from call to call.
+    __device__ __forceinline__ void locate(int i, int tiles_p, int& tp, int& tq) {
+        while (i >= tile0[g + 1]) ++g;
+        const int r = i - tile0[g];
         const int nq = (tile0[g + 1] - tile0[g]) / tiles_p;
         const int band = r / (BAND * tiles_p);
         const int rr = r - band * BAND * tiles_p;
         const int h = min(BAND, nq - band * BAND);
         tp = rr / h;
         tq = band * BAND + rr - tp * h;
-        return true;
     }
 };
 

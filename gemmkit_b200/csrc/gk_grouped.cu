@@ -143,6 +143,7 @@ struct GTile {
     int qn;               // its Q rows
     int64_t qbase;        // first row of the Q operand / of C along the Q side
     int k0, nk;           // first contraction row (weight gradient) and contraction length
+    int pb;               // its blocks of 256 P rows (tall pair tiles: 1 or 2)
 };
 
 // Q rows of a tile where `rows` of them are cut into tiles of at most BN: equal heights, rounded up
@@ -155,12 +156,38 @@ __host__ __device__ __forceinline__ int tile_height(int rows) {
     return (h + STEP - 1) & ~(STEP - 1);
 }
 
-template <int BN, int TM = BM>
+// The walk over tall tiles (2 TM P rows, p.tiles_p of them on the P side): where what is left after
+// the last full wave of clusters would fill at most half of them, its tiles are walked in halves of
+// TM rows, so that the last wave takes half the time.
+template <int TM>
+__device__ __forceinline__ bool next_tall(GroupWalk& w, const GroupedParams& p, GTile& t, int& tq) {
+    const int rest = w.total % w.step;
+    const int split = 2 * rest <= w.step ? w.total - rest : w.total;
+    for (;;) {
+        w.t += w.step;
+        const int over = w.t - split;
+        if (over >= 2 * (w.total - split)) return false;
+        int tp;
+        w.locate(over < 0 ? w.t : split + (over >> 1), p.tiles_p, tp, tq);
+        t.p0 = tp * 2 * TM + (over >= 0 ? (over & 1) * TM : 0);
+        if (t.p0 >= p.np) continue;  // the second half of a tile that has one
+        t.pb = over < 0 && p.np - t.p0 > TM ? 2 : 1;
+        return true;
+    }
+}
+
+// PB: blocks of TM P rows in a tile.
+template <int BN, int TM = BM, int PB = 1>
 __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, GTile& t) {
     int tp, tq;
-    if (!w.next(p.tiles_p, tp, tq)) return false;
+    if constexpr (PB == 1) {
+        if (!w.next(p.tiles_p, tp, tq)) return false;
+        t.p0 = tp * TM;
+        t.pb = 1;
+    } else {
+        if (!next_tall<TM>(w, p, t, tq)) return false;
+    }
     t.g = w.g;
-    t.p0 = tp * TM;
     const int o0 = w.off[t.g], m = w.off[t.g + 1] - o0;
     const int qrows = p.wgrad ? static_cast<int>(p.nq) : m;
     const int h = tile_height<BN, 32>(qrows);
@@ -547,13 +574,14 @@ __global__ void __launch_bounds__(256)
 // (even CTA) issues every MMA; barriers as in the engine's other pair kernel: full[] and tempty[]
 // live in the leader, empty[] and tfull[] in both (one multicast commit each).
 
+template <int PB>
 struct GPairCfg {
     static constexpr int BN = 256;
     static constexpr int NEPI = 8;
     static constexpr int EPI_W0 = 4;
     static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
     static constexpr int WCOLS = BN / 2;
-    static constexpr int P_BYTES = BM * BKB;
+    static constexpr int P_BYTES = PB * BM * BKB;
     static constexpr int Q_BYTES = BN / 2 * BKB;
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
@@ -565,13 +593,15 @@ struct GPairCfg {
     static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
+    static constexpr int LATE = STAGES - 1, TAIL = 3;  // tall tiles: see the MMA warp
     static_assert(STAGES >= 4 && (4 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
 };
 
-__global__ void __launch_bounds__(GPairCfg::THREADS, 1)
+template <int PB>
+__global__ void __launch_bounds__(GPairCfg<PB>::THREADS, 1)
     grouped_pair_kernel(const __grid_constant__ CUtensorMap tmP,
                         const __grid_constant__ CUtensorMap tmQ, const GroupedParams p) {
-    using C = GPairCfg;
+    using C = GPairCfg<PB>;
     constexpr int STAGES = C::STAGES, BN = C::BN, TM = 2 * BM;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -635,7 +665,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
         int stage = 0;
         uint32_t phase = 0, issued = 0, last_par = 0;
         bool ok = true;
-        while (ok && next_tile<BN, TM>(walk, p, t)) {
+        while (ok && next_tile<BN, TM, PB>(walk, p, t)) {
             const int pz = p.p_z ? t.g : 0;
             const int p0 = t.p0 + static_cast<int>(rank) * BM;
             // the MMA's N, and this CTA's half of its rows
@@ -651,21 +681,27 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                     // a ragged stage's halves complete on each CTA's own rfull
                     const bool ragged = ragged_stage(p, t, kb);
                     const uint32_t fb = (ragged ? rfull_own : full_l) + 8u * stage;
-                    uint8_t* dp = sP + stage * C::P_BYTES;
                     uint8_t* dq = sQ + stage * C::Q_BYTES;
+                    const uint32_t bytes = t.pb * BM * BKB + C::Q_BYTES;
                     if (ragged)
-                        mbar_arrive_expect_tx(&rfull[stage], C::STAGE_BYTES);
+                        mbar_arrive_expect_tx(&rfull[stage], bytes);
                     else if (leader)
-                        mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
+                        mbar_arrive_expect_tx(&full[stage], 2 * bytes);
                     const int k = t.k0 + kb;
-                    if (p.p_4d) {
-                        tma_load_4d_pair(dp, &tmP, fb, 0, k, p0 >> 6, pz);
-                    } else if (p.p_mn) {
 #pragma unroll
-                        for (int c = 0; c < BM / 64; ++c)
-                            tma_load_3d_pair(dp + c * MN_BOX, &tmP, fb, p0 + 64 * c, k, pz);
-                    } else {
-                        tma_load_3d_pair(dp, &tmP, fb, k, p0, pz);
+                    for (int b = 0; b < PB; ++b) {
+                        if (b >= t.pb) break;
+                        uint8_t* dp = sP + stage * C::P_BYTES + b * BM * BKB;
+                        const int pr = p0 + b * TM;
+                        if (p.p_4d) {
+                            tma_load_4d_pair(dp, &tmP, fb, 0, k, pr >> 6, pz);
+                        } else if (p.p_mn) {
+#pragma unroll
+                            for (int c = 0; c < BM / 64; ++c)
+                                tma_load_3d_pair(dp + c * MN_BOX, &tmP, fb, pr + 64 * c, k, pz);
+                        } else {
+                            tma_load_3d_pair(dp, &tmP, fb, k, pr, pz);
+                        }
                     }
                     if (p.q_4d) {
                         tma_load_4d_pair(dq, &tmQ, fb, 0, k, qb >> 6, 0);
@@ -701,17 +737,36 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
             uint32_t phase = 0;
             const OperandDesc dP(smem_u32(sP), p.p_mn), dQ(smem_u32(sQ), p.q_mn);
             bool ok = true;
-            for (int local = 0; ok && next_tile<BN, TM>(walk, p, t); ++local) {
-                const int acc = local & 1;
-                const uint32_t aph = (local >> 1) & 1;
+            uint32_t idesc = 0;
+            // the MMAs of a stage for the accumulator at d and the P block at `po`
+            auto issue = [&](uint32_t d, uint32_t po, uint32_t qo, int kb, int nk) {
+                if (p.wgrad && nk - kb < GBK) {
+                    const int steps = (nk - kb + 15) >> 4;
+                    for (int ks = 0; ks < steps; ++ks)
+                        mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
+                                     (kb | ks) != 0 ? 1u : 0u);
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < GBK / 16; ++ks)
+                        mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
+                                     (kb | ks) != 0 ? 1u : 0u);
+                }
+            };
+            int used1 = 0;  // tall tiles: those so far that used accumulator 1
+            for (int local = 0; ok && next_tile<BN, TM, PB>(walk, p, t); ++local) {
+                const int acc = PB == 1 ? local & 1 : 0;
+                const uint32_t aph = (PB == 1 ? local >> 1 : local) & 1;
                 if (!warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
                                tmo))
                     break;
                 tc_fence_after();
-                const uint32_t idesc = idesc_f16(TM, min(BN, (t.qn + 31) & ~31), p.f16 == 0) |
-                                       (static_cast<uint32_t>(p.p_mn) << 15) |
-                                       (static_cast<uint32_t>(p.q_mn) << 16);
+                idesc = idesc_f16(TM, min(BN, (t.qn + 31) & ~31), p.f16 == 0) |
+                        (static_cast<uint32_t>(p.p_mn) << 15) |
+                        (static_cast<uint32_t>(p.q_mn) << 16);
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                const bool two = PB == 2 && t.pb == 2;
+                bool free1 = false;            // accumulator 1 is drained
+                int late = 0, late0 = stage;   // stages that wait for block 1's MMAs, the first
                 for (int kb = 0; kb < t.nk; kb += GBK) {
                     if (!warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA,
                                    tmo)) {
@@ -719,31 +774,59 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t po = stage * C::P_BYTES, qo = stage * C::Q_BYTES;
-                    const bool cut = p.wgrad && t.nk - kb < GBK;
+                    const bool last = kb + GBK >= t.nk;
                     if (elect_one()) {
-                        if (cut) {
-                            const int steps = (t.nk - kb + 15) >> 4;
-                            for (int ks = 0; ks < steps; ++ks)
-                                mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
-                                             (kb | ks) != 0 ? 1u : 0u);
-                        } else {
-#pragma unroll
-                            for (int ks = 0; ks < GBK / 16; ++ks)
-                                mma_f16_pair(d, dP.at(po, ks), dQ.at(qo, ks), idesc,
-                                             (kb | ks) != 0 ? 1u : 0u);
-                        }
-                        mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                        issue(d, stage * C::P_BYTES, stage * C::Q_BYTES, kb, t.nk);
+                        if (!two) mma_commit_pair_both(smem_u32(&empty[stage]), 0x3);
+                        if (last) mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
                     }
                     __syncwarp();
+                    if (two) {
+                        const bool must = ++late == C::LATE || last;
+                        if (!free1) {
+                            const uint32_t par = (used1 & 1) ^ 1u;
+                            if (must) {
+                                if (!warp_wait(&tempty[1], par, abort_flag, p.status,
+                                               GK_DEV_TIMEOUT_MMA, tmo)) {
+                                    ok = false;
+                                    break;
+                                }
+                                free1 = true;
+                            } else {
+                                free1 = __all_sync(0xffffffffu, mbar_test(&tempty[1], par));
+                            }
+                            tc_fence_after();
+                        }
+                        if (must || (free1 && kb + C::TAIL * GBK < t.nk)) {
+                            for (; late > 0; --late) {
+                                if (elect_one()) {
+                                    issue(d + BN, late0 * C::P_BYTES + BM * BKB,
+                                          late0 * C::Q_BYTES, kb - (late - 1) * GBK, t.nk);
+                                    mma_commit_pair_both(smem_u32(&empty[late0]), 0x3);
+                                }
+                                __syncwarp();
+                                if (++late0 == STAGES) late0 = 0;
+                            }
+                        }
+                    }
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                if (elect_one()) mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
-                __syncwarp();
+                if (t.nk == 0) {  // an empty group's tile: its zeros are the epilogue's
+                    if (two && !warp_wait(&tempty[1], (used1 & 1) ^ 1u, abort_flag, p.status,
+                                          GK_DEV_TIMEOUT_MMA, tmo))
+                        break;
+                    if (elect_one()) mma_commit_pair_both(smem_u32(&tfull[acc]), 0x3);
+                    __syncwarp();
+                }
+                if (two) {
+                    if (elect_one()) mma_commit_pair_both(smem_u32(&tfull[1]), 0x3);
+                    __syncwarp();
+                    ++used1;
+                }
             }
             if (elect_one()) mma_commit_pair(mapa_shared(smem_u32(drain), rank));
             __syncwarp();
@@ -757,7 +840,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
             const uint32_t peerz_l = mapa_shared(smem_u32(peerz), 0);
             int blocks = 0;        // stages filled so far
             uint32_t parity = 0;   // rfull's and peerz's, a bit per stage
-            while (next_tile<BN, TM>(walk, p, t)) {
+            while (next_tile<BN, TM, PB>(walk, p, t)) {
                 blocks += (t.nk + GBK - 1) / GBK;
                 if ((t.nk & 15) == 0) continue;
                 const int stage = (blocks - 1) % STAGES;
@@ -766,7 +849,7 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
                     break;
                 parity ^= 1u << stage;
                 const int v = t.nk & (GBK - 1);
-                zero_rows(sP + stage * C::P_BYTES, BM / 64, v, lane);
+                zero_rows(sP + stage * C::P_BYTES, t.pb * (BM / 64), v, lane);
                 zero_rows(sQ + stage * C::Q_BYTES, BN / 128, v, lane);
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -785,37 +868,98 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
         uint8_t* ebuf = smem + C::OFF_EPI + (warp - C::EPI_W0) * EPI_BUF;
-        for (int local = 0; next_tile<BN, TM>(walk, p, t); ++local) {
-            const int acc = local & 1;
-            const uint32_t aph = (local >> 1) & 1;
-            if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
-                break;
-            tc_fence_after();
-            const int i0 = t.p0 + static_cast<int>(rank) * BM + q * 32;  // the warp's first P row
-            const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i0 * p.ldp;
-            const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
-                                static_cast<uint32_t>(acc * BN + cbase);
-            const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
-            if (p.pieces) {
-                store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
-                             t.qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, t.nk > 0);
-            } else {
-                for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
-                    uint32_t v[32];
+        if constexpr (PB == 2) {
+            // Each accumulator goes to registers, rounded, before anything of it is stored: the
+            // next tile's MMAs wait for that only.
+            constexpr int NB = C::WCOLS / 16;  // blocks of 16 Q rows
+            int used1 = 0;
+            for (int local = 0; next_tile<BN, TM, PB>(walk, p, t); ++local) {
+                bool ok = true;
+                for (int b = 0; b < t.pb && ok; ++b) {
+                    const uint32_t par = (b == 0 ? local : used1++) & 1;
+                    if (!(ok = warp_wait(&tfull[b], par, abort_flag, p.status,
+                                         GK_DEV_TIMEOUT_EPILOGUE, tmo)))
+                        break;
+                    tc_fence_after();
+                    const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                        static_cast<uint32_t>(b * BN + cbase);
+                    Block16 x[NB];
                     if (t.nk > 0) {
-                        tmem_ld_x32(tb + c, v);
+#pragma unroll
+                        for (int k = 0; k < NB; k += 4) {
+                            uint32_t v[4][16];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) tmem_ld_frag16(tb + 16 * (k + i), v[i]);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                frag_fence(v[i]);
+                                x[k + i].round(v[i], p.alpha, p.out_type);
+                            }
+                        }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = 0u;
+                        for (int k = 0; k < NB; ++k)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) x[k].w[i] = 0u;
                     }
-                    if (lane < pn)
-                        store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
-                                  t.qn - cbase - c, p.alpha, p.beta);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster_relaxed(tempty_l + 8u * b);
+                    const int i0 = t.p0 + b * TM + static_cast<int>(rank) * BM + q * 32;
+                    const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+                    uint16_t* c = static_cast<uint16_t*>(p.c) + (p.wgrad ? t.g * p.gsc : 0) +
+                                  (t.qbase + cbase) * p.ldq + i0;
+                    const uint32_t sb = smem_u32(ebuf);
+#pragma unroll
+                    for (int k = 0; k < NB; k += 2) {
+                        if (cbase + 16 * k < t.qn) {
+                            x[k].stage(sb, lane);
+                            x[k + 1].stage(sb + 1024, lane);
+                            __syncwarp();
+                            copy_out(sb, c + 16 * k * p.ldq, p.ldq, t.qn - cbase - 16 * k, pn,
+                                     lane);
+                            copy_out(sb + 1024, c + 16 * (k + 1) * p.ldq, p.ldq,
+                                     t.qn - cbase - 16 * (k + 1), pn, lane);
+                            __syncwarp();
+                        }
+                    }
                 }
+                if (!ok) break;
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(tempty_l + 8u * acc);
+        } else {
+            for (int local = 0; next_tile<BN, TM, PB>(walk, p, t); ++local) {
+                const int acc = local & 1;
+                const uint32_t aph = (local >> 1) & 1;
+                if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
+                    break;
+                tc_fence_after();
+                const int i0 = t.p0 + static_cast<int>(rank) * BM + q * 32;  // the warp's first P row
+                const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i0 * p.ldp;
+                const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                    static_cast<uint32_t>(acc * BN + cbase);
+                const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+                if (p.pieces) {
+                    store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
+                                 t.qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, t.nk > 0);
+                } else {
+                    for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
+                        uint32_t v[32];
+                        if (t.nk > 0) {
+                            tmem_ld_x32(tb + c, v);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = 0u;
+                        }
+                        if (lane < pn)
+                            store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
+                                      t.qn - cbase - c, p.alpha, p.beta);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(tempty_l + 8u * acc);
+            }
         }
     }
 
@@ -828,11 +972,12 @@ __global__ void __launch_bounds__(GPairCfg::THREADS, 1)
     }
 }
 
+template <int PB>
 int launch_grouped_pair(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p,
                         int grid, int pdl, cudaStream_t stream, char* err, size_t errlen) {
-    using C = GPairCfg;
+    using C = GPairCfg<PB>;
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_smem(grouped_pair_kernel, C::SMEM, done);
+    cudaError_t e = allow_smem(grouped_pair_kernel<PB>, C::SMEM, done);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
@@ -849,7 +994,7 @@ int launch_grouped_pair(const CUtensorMap& tp, const CUtensorMap& tq, const Grou
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = pdl ? 2 : 1;
-        e = cudaLaunchKernelEx(&cfg, grouped_pair_kernel, tp, tq, p);
+        e = cudaLaunchKernelEx(&cfg, grouped_pair_kernel<PB>, tp, tq, p);
     }
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) {
@@ -1010,8 +1155,8 @@ int pair_clusters() {
         cudaLaunchConfig_t q;
         memset(&q, 0, sizeof(q));
         q.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
-        q.blockDim = dim3(GPairCfg::THREADS);
-        q.dynamicSmemBytes = GPairCfg::SMEM;
+        q.blockDim = dim3(GPairCfg<1>::THREADS);
+        q.dynamicSmemBytes = GPairCfg<1>::SMEM;
         cudaLaunchAttribute a[1];
         a[0].id = cudaLaunchAttributeClusterDimension;
         a[0].val.clusterDim.x = 2;
@@ -1020,9 +1165,9 @@ int pair_clusters() {
         q.attrs = a;
         q.numAttrs = 1;
         int c = 0;
-        if (cudaFuncSetAttribute(grouped_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 GPairCfg::SMEM) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&c, grouped_pair_kernel, &q) != cudaSuccess || c <= 0) {
+        if (cudaFuncSetAttribute(grouped_pair_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 GPairCfg<1>::SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&c, grouped_pair_kernel<1>, &q) != cudaSuccess || c <= 0) {
             cudaGetLastError();
             c = sm_count() / 2;
         }
@@ -1085,13 +1230,14 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
     const int64_t pair_tiles = tiles_bound(2 * BM, 256) - (p.wgrad ? 0 : p.groups);
     const bool pair = tma && p.np > BM && qside > BM && pair_tiles >= clusters;
     const int bn = pair ? 256 : grouped_bn(p.wgrad && qside < 64 ? 64 : qside);
-    const int tm = pair ? 2 * BM : BM;
+    p.pieces = c_in_pieces(p.c, p.out_type, p.ldq, p.ldp, p.gsc, p.np, p.beta);
+    const bool tall = pair && p.pieces && p.np > 2 * BM && pair_tiles >= 2 * clusters;
+    const int tm = tall ? 4 * BM : pair ? 2 * BM : BM;
     const int64_t tiles = tiles_bound(tm, bn);
     if (tiles > INT32_MAX / 2)
         return set_last_error(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
     p.tiles_p = static_cast<int>((p.np + tm - 1) / tm);
     p.tiles_q = static_cast<int>((p.nq + bn - 1) / bn);
-    p.pieces = c_in_pieces(p.c, p.out_type, p.ldq, p.ldp, p.gsc, p.np, p.beta);
     p.timeout_ns = 4000000000ull;
     p.status = device_status_ptr();
     const int pdl = api_pdl_enabled();
@@ -1125,7 +1271,8 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
     }
     if (pair) {
         const int grid = 2 * static_cast<int>(tiles < clusters ? tiles : clusters);
-        rc = launch_grouped_pair(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
+        rc = tall ? launch_grouped_pair<2>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err))
+                  : launch_grouped_pair<1>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
         return rc ? set_last_error(rc, err) : GK_OK;
     }
     const int sms = sm_count();

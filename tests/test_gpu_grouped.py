@@ -502,6 +502,47 @@ def test_wgrad_exact_16_bit(dtype, sizes, m, n):
     assert bool((c[:, m:] == 7).all()) and bool((c[:, :, n:] == 7).all())
 
 
+# Many full tiles and 16-bit C in whole pieces: tiles of 512 columns of C. Odd numbers of
+# 256-column blocks, a last block of 8, contractions of one stage, of a few and of many.
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("major", ["k", "n"])
+@pytest.mark.parametrize("sizes,lead,tail,n", [([1301, 0, 2, 2150], 3, 4, 4360),
+                                               ([8192], 0, 0, 1288), ([2000, 3000, 257], 0, 1, 2304),
+                                               ([1024] * 9, 0, 0, 1032)])
+@pytest.mark.parametrize("k", [8, 72, 200, 1000])
+def test_forward_exact_tall_tiles(dtype, major, sizes, lead, tail, n, k):
+    torch = torch_cuda()
+    rows, off = lead + sum(sizes) + tail, offsets_of(sizes, lead)
+    a = data(1, (rows, k), dtype)
+    b = data(2, (len(sizes), n, k), dtype).transpose(1, 2) if major == "k" else \
+        data(2, (len(sizes), k, n), dtype)
+    a[:lead] = float("nan")
+    a[rows - tail:] = float("inf")
+    c = torch.full((rows, n + 8), 7.0, device="cuda", dtype=tdt(dtype))
+    run_fwd(a, b, off, c[:, :n], dtype)
+    want, _ = want_fwd(a, b, off, torch.full((rows, n), 7.0, device="cuda"), 1.0, 0.0)
+    assert torch.equal(c[:, :n], want.to(tdt(dtype)))
+    assert bool((c[:, n:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes,lead,tail", [([1000, 0, 705, 17, 64, 1], 2, 5), ([2049, 190], 0, 1),
+                                             ([0, 0, 130], 0, 0), ([3, 5, 0, 200, 257, 31], 1, 0)])
+@pytest.mark.parametrize("m,n", [(2048, 2304), (1032, 4360), (4100, 2056)])
+def test_wgrad_exact_tall_tiles(dtype, sizes, lead, tail, m, n):
+    torch = torch_cuda()
+    rows, off = lead + sum(sizes) + tail, offsets_of(sizes, lead)
+    a, b = data(1, (rows, m), dtype), data(2, (rows, n), dtype)
+    for t in (a, b):
+        t[:lead] = float("nan")
+        t[rows - tail:] = float("inf")
+    c = torch.full((len(sizes), m + 1, n), 7.0, device="cuda", dtype=tdt(dtype))
+    run_wgrad(a, b, off, c[:, :m], dtype)
+    want, _ = want_wgrad(a, b, off, c, 1.0, 0.0)
+    assert torch.equal(c[:, :m], want.to(tdt(dtype)))
+    assert bool((c[:, m:] == 7).all())
+
+
 def test_realigned_operands_in_graphs_and_on_two_streams():
     """Operands that are copied to aligned scratch first (odd pitches, no unit stride): captured calls
     replayed on two streams at once, and eager calls on two streams, each with its own scratch."""
