@@ -871,7 +871,6 @@ __global__ void __launch_bounds__(GPairCfg<PB>::THREADS, 1)
         if constexpr (PB == 2) {
             // Each accumulator goes to registers, rounded, before anything of it is stored: the
             // next tile's MMAs wait for that only.
-            constexpr int NB = C::WCOLS / 16;  // blocks of 16 Q rows
             int used1 = 0;
             for (int local = 0; next_tile<BN, TM, PB>(walk, p, t); ++local) {
                 bool ok = true;
@@ -883,25 +882,19 @@ __global__ void __launch_bounds__(GPairCfg<PB>::THREADS, 1)
                     tc_fence_after();
                     const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                         static_cast<uint32_t>(b * BN + cbase);
-                    Block16 x[NB];
+                    uint32_t w[C::WCOLS / 2];
                     if (t.nk > 0) {
 #pragma unroll
-                        for (int k = 0; k < NB; k += 4) {
-                            uint32_t v[4][16];
+                        for (int k = 0; k < C::WCOLS; k += 32) {
+                            uint32_t v[32];
+                            tmem_ld_x32(tb + k, v);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) tmem_ld_frag16(tb + 16 * (k + i), v[i]);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                frag_fence(v[i]);
-                                x[k + i].round(v[i], p.alpha, p.out_type);
-                            }
+                            for (int i = 0; i < 16; ++i)
+                                w[k / 2 + i] = round_pair(v[2 * i], v[2 * i + 1], p.alpha, p.out_type);
                         }
                     } else {
 #pragma unroll
-                        for (int k = 0; k < NB; ++k)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) x[k].w[i] = 0u;
+                        for (int k = 0; k < C::WCOLS / 2; ++k) w[k] = 0u;
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -910,20 +903,7 @@ __global__ void __launch_bounds__(GPairCfg<PB>::THREADS, 1)
                     const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
                     uint16_t* c = static_cast<uint16_t*>(p.c) + (p.wgrad ? t.g * p.gsc : 0) +
                                   (t.qbase + cbase) * p.ldq + i0;
-                    const uint32_t sb = smem_u32(ebuf);
-#pragma unroll
-                    for (int k = 0; k < NB; k += 2) {
-                        if (cbase + 16 * k < t.qn) {
-                            x[k].stage(sb, lane);
-                            x[k + 1].stage(sb + 1024, lane);
-                            __syncwarp();
-                            copy_out(sb, c + 16 * k * p.ldq, p.ldq, t.qn - cbase - 16 * k, pn,
-                                     lane);
-                            copy_out(sb + 1024, c + 16 * (k + 1) * p.ldq, p.ldq,
-                                     t.qn - cbase - 16 * (k + 1), pn, lane);
-                            __syncwarp();
-                        }
-                    }
+                    store_pairs(w, c, p.ldq, t.qn - cbase, pn, lane);
                 }
                 if (!ok) break;
             }

@@ -136,6 +136,31 @@ __device__ __forceinline__ void copy_out(uint32_t sb, uint16_t* c, int64_t ldq, 
     }
 }
 
+// ---- 16-bit rows of C without shared memory ----------------------------------------------------
+//
+// Two accumulator columns of one TMEM lane (P row) are rounded into a word; neighbouring lanes
+// exchange halves, so that the even lane holds rows l, l + 1 of the even column and the odd lane
+// those of the odd one, four bytes each: a store of the warp writes two Q rows of 64 bytes.
+//   w[j]: columns 2 j and 2 j + 1 of this lane's P row (N words); n of the columns exist in C.
+template <int N>
+__device__ __forceinline__ void store_pairs(const uint32_t (&w)[N], uint16_t* c, int64_t ldq, int n,
+                                            int pn, int lane) {
+    const int odd = lane & 1;
+    const uint32_t give = odd ? 0x5410u : 0x7632u;
+    const uint32_t sel0 = odd ? 0x3254u : 0x5410u, sel1 = odd ? 0x3276u : 0x7610u;
+    uint16_t* q = c + (lane & 30) + odd * ldq;
+    const int left = (lane & 30) < pn ? n - odd : 0;  // columns of this lane: 0, 2, 4, ... < left
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const uint32_t got =
+            __shfl_xor_sync(0xffffffffu, __byte_perm(w[j], w[j + 1], give), 1);
+        const uint32_t x = __byte_perm(w[j], got, sel0), y = __byte_perm(w[j + 1], got, sel1);
+        if (2 * j < left) *reinterpret_cast<uint32_t*>(q) = x;
+        if (2 * j + 2 < left) *reinterpret_cast<uint32_t*>(q + 2 * ldq) = y;
+        q += 4 * ldq;
+    }
+}
+
 constexpr int EPI_BUF = 2048;  // shared memory per epilogue warp: two staged blocks
 
 // `cols` accumulator columns (a multiple of 16) from TMEM address tb, of which the first n exist in
