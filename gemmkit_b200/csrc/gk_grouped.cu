@@ -16,9 +16,9 @@
 // from the offsets (gk_group.cuh), so the host never waits for them.
 //
 // Operands that TMA cannot address (no unit stride, a pitch that is no multiple of 16 bytes, a
-// base off a 16-byte boundary) are first copied to aligned scratch, line by line or transposed. (Loader warps
-// that gather such operands inside the product were tried: at most 170 TFLOP/s and 1.5 TB/s,
-// 143 us for 2000 x 2001 x 3001 against 46 us with the copies.)
+// base off a 16-byte boundary) are first copied to aligned scratch, line by line or transposed.
+// (Loader warps that gather such operands inside the product were tried: at most 170 TFLOP/s and
+// 1.5 TB/s, 143 us for 2000 x 2001 x 3001 against 46 us with the copies.)
 //
 // Operands lie K-major (the contraction contiguous: rows of A, weights stored n x k) or MN-major
 // (weights stored k x n, both operands of the weight gradient); the MMA reads either from the
@@ -567,12 +567,23 @@ __global__ void __launch_bounds__(256)
 
 // ---- the CTA-pair form ----------------------------------------------------------------------------
 //
-// Two CTAs of a cluster compute a tile of 256 P rows x up to 256 Q rows with tcgen05 cta_group::2:
-// each loads its 128 rows of P and half of the Q rows (the peer's half is read from its shared
-// memory by the MMA), so an SM moves a third less operand data per MAC than the one-CTA kernel's
-// 128 x 256 tile, whose rate the shared-memory traffic holds at about 55 % of the peak. The leader
-// (even CTA) issues every MMA; barriers as in the engine's other pair kernel: full[] and tempty[]
-// live in the leader, empty[] and tfull[] in both (one multicast commit each).
+// Two CTAs of a cluster compute a tile of PB x 256 P rows x up to 256 Q rows with tcgen05
+// cta_group::2: each loads its 128 rows of every P block and half of the Q rows (the peer's half is
+// read from its shared memory by the MMA). The leader (even CTA) issues every MMA; barriers as in
+// the engine's other pair kernel: full[] and tempty[] live in the leader, empty[] and tfull[] in
+// both (one multicast commit each).
+//   What bounds it is shared memory. A 256 x 256 tile needs 64 bytes of operands per SM and
+// cycle of MMA from L2, and moves them through shared memory twice: all that it gives. Counted
+// at 8192^3, a stage took 604 cycles for 512 of MMA, and shorter Q tiles took as long. PB = 2 loads
+// 48 bytes per cycle instead (949k active cycles instead of 1070k for 907k of MMA; 746 -> 659
+// us; 8 experts of 4096 -> 14336 over 8192 rows, skewed: 727 -> 659 us).
+//   PB = 2 fills TMEM with one tile: accumulator b is P block b's. So that the MMAs need not wait for
+// the epilogue, the two blocks run shifted at a tile's ends. The last TAIL stages run for block 0
+// first, whose accumulator is then read while block 1's MMAs run; the next tile starts with block 0
+// alone (up to LATE stages) until accumulator 1 is read. The epilogue takes an accumulator to
+// registers, rounds and releases it before it stores, and stores without shared memory, which the
+// MMAs need (28.6 instead of 29.8 us for 4096 x 1024 x 4096). TAIL 1 or 2 instead of 3 cost 1 to 2 %
+// at contractions of 512, nothing at long ones. C of another layout or type, and beta, take PB = 1.
 
 template <int PB>
 struct GPairCfg {
@@ -586,14 +597,14 @@ struct GPairCfg {
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
     static constexpr int TAB_BYTES = (2 * GROUP_TABLE_INTS * 4 + 15) / 16 * 16;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int EPI_BYTES = NEPI * EPI_BUF;
+    static constexpr int EPI_BYTES = PB == 1 ? NEPI * EPI_BUF : 0;
     static constexpr int STAGES =
         (SMEM_LIMIT - 1024 - BAR_BYTES - TAB_BYTES - EPI_BYTES) / STAGE_BYTES;
     static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
     static constexpr int OFF_BARS = OFF_EPI + EPI_BYTES;
     static constexpr int OFF_TAB = OFF_BARS + BAR_BYTES;
     static constexpr int SMEM = 1024 + OFF_TAB + TAB_BYTES;
-    static constexpr int LATE = STAGES - 1, TAIL = 3;  // tall tiles: see the MMA warp
+    static constexpr int LATE = STAGES - 1, TAIL = 3;  // PB = 2: see above
     static_assert(STAGES >= 4 && (4 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
 };
 
@@ -1211,7 +1222,16 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
     const bool pair = tma && p.np > BM && qside > BM && pair_tiles >= clusters;
     const int bn = pair ? 256 : grouped_bn(p.wgrad && qside < 64 ? 64 : qside);
     p.pieces = c_in_pieces(p.c, p.out_type, p.ldq, p.ldp, p.gsc, p.np, p.beta);
-    const bool tall = pair && p.pieces && p.np > 2 * BM && pair_tiles >= 2 * clusters;
+    // 512-column tiles where C allows their epilogue and they do not leave more clusters idle: a
+    // wave of halves takes about 11/12 of a wave of 256 x 256 tiles (46 against 50 us for
+    // 4096 -> 4096 over 2048 rows, two each), but 4096 -> 9472 over 512 rows is one wave of 74 square
+    // tiles and two of halves (30 against 44 us).
+    const int64_t q_tiles = p.wgrad ? (p.nq + 255) / 256 * p.groups  // forward: about half a tile
+                                    : (p.rows + 255) / 256 + (p.groups - 1) / 2;  // over per group
+    const int64_t waves = ((p.np + 2 * BM - 1) / (2 * BM) * q_tiles + clusters - 1) / clusters;
+    const int64_t tall_tiles = (p.np + 4 * BM - 1) / (4 * BM) * q_tiles, rest = tall_tiles % clusters;
+    const int64_t half_waves = tall_tiles / clusters * 2 + (rest == 0 ? 0 : 2 * rest <= clusters ? 1 : 2);
+    const bool tall = pair && p.pieces && p.np > 2 * BM && 11 * half_waves <= 12 * waves;
     const int tm = tall ? 4 * BM : pair ? 2 * BM : BM;
     const int64_t tiles = tiles_bound(tm, bn);
     if (tiles > INT32_MAX / 2)
@@ -1250,7 +1270,9 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
         if (rc) return set_last_error(rc, err);
     }
     if (pair) {
-        const int grid = 2 * static_cast<int>(tiles < clusters ? tiles : clusters);
+        // (tall tiles may be walked in halves)
+        const int64_t units = tall ? 2 * tiles : tiles;
+        const int grid = 2 * static_cast<int>(units < clusters ? units : clusters);
         rc = tall ? launch_grouped_pair<2>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err))
                   : launch_grouped_pair<1>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
         return rc ? set_last_error(rc, err) : GK_OK;
