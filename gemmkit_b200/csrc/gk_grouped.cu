@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(256)
 //   What bounds it is shared memory. A 256 x 256 tile needs 64 bytes of operands per SM and
 // cycle of MMA from L2, and moves them through shared memory twice: all that it gives. Counted
 // at 8192^3, a stage took 604 cycles for 512 of MMA, and shorter Q tiles took as long. PB = 2 loads
-// 48 bytes per cycle instead (949k active cycles instead of 1070k for 907k of MMA; 746 -> 659
+// 48 bytes per cycle instead (943k active cycles instead of 1070k for 907k of MMA; 746 -> 659
 // us; 8 experts of 4096 -> 14336 over 8192 rows, skewed: 727 -> 659 us).
 //   PB = 2 fills TMEM with one tile: accumulator b is P block b's. So that the MMAs need not wait for
 // the epilogue, the two blocks run shifted at a tile's ends. The last TAIL stages run for block 0
