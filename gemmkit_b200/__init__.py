@@ -655,8 +655,9 @@ class Fp4Matrix:
 
     @staticmethod
     def empty(rows: int, cols: int, fmt: int, scale: float = 1.0, groups: int = 1, offsets=None,
-              device=None) -> "Fp4Matrix":
-        """An unwritten matrix on the current device (a destination for quantize_fp4)."""
+              device=None, stream=None) -> "Fp4Matrix":
+        """An unwritten matrix on the current device (a destination for quantize_fp4), its memory
+        allocated for torch's current stream or for `stream`."""
         calls = _cuda or _cuda_calls()
         if calls is None:
             raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
@@ -669,7 +670,12 @@ class Fp4Matrix:
                                           f"{groups} groups")
         # one allocation: codes, then scales (both parts whole 16-byte pieces)
         nd, ns = _fp4_sizes(rows, cols, fmt, groups, offsets is not None)
-        buf = torch.empty(nd + ns, dtype=torch.uint8, device=device or torch.device("cuda", calls[1]()))
+        device = device or torch.device("cuda", calls[1]())
+        if stream is None:
+            buf = torch.empty(nd + ns, dtype=torch.uint8, device=device)
+        else:  # not what the current stream may still be writing
+            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
+                buf = torch.empty(nd + ns, dtype=torch.uint8, device=device)
         q = Fp4Matrix.__new__(Fp4Matrix)
         q.rows, q.cols, q.fmt, q.scale = rows, cols, fmt, float(scale)
         q.groups, q.offsets, q._data, q._scales = groups, offsets, buf, None
@@ -689,7 +695,7 @@ class Fp4Matrix:
                     (t.shape[1] > 1 and t.stride(1) != 1):
                 raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold {rows} contiguous rows of "
                                               "bytes")
-        q = Fp4Matrix.empty(rows, cols, fmt, scale, groups, offsets, codes.device)
+        q = Fp4Matrix.empty(rows, cols, fmt, scale, groups, offsets, codes.device, stream)
 
         def part(t):
             ld = t.stride(0) if rows > 1 else t.shape[1]
@@ -717,12 +723,13 @@ def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: 
     they are; weights with a column per output as the transposed view (n x k). With `offsets` the
     rows form ragged groups; with groups > 1 `x` views the first of `groups` matrices that lie
     x_gs elements apart. `out` reuses a matrix of the same shape, format and groups (its scale and
-    groups then hold); x_type names the element type of a (pointer, length) pair."""
+    groups then hold), otherwise the result's memory is allocated for the call's stream; x_type names
+    the element type of a (pointer, length) pair."""
     _same_device("X", x.data, "offsets", offsets, "out", None if out is None else out._data)
     if out is None:
         stacked = offsets is None and groups > 1
         out = Fp4Matrix.empty(x.rows * groups if stacked else x.rows, x.cols, fmt, scale, groups,
-                              offsets)
+                              offsets, stream=stream)
     elif out.fmt != fmt:
         raise GemmkitError(GK_EINVAL, "gemmkit: the output is held in another 4-bit format")
     if x_type is None:

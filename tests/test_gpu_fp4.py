@@ -609,3 +609,24 @@ def test_chain_without_synchronisation(fmt):
     assert bool(want.isfinite().all()) and float(want.abs().max()) > 0
     for _ in range(5):
         assert torch.equal(chain(False), want)
+
+
+def test_result_memory_belongs_to_the_call_s_stream():
+    """A matrix that quantize_fp4 makes for another stream does not lie where the current stream may
+    still be writing: a buffer freed behind a delayed fill."""
+    torch = torch_cuda()
+    rows, k = 4096, 4096
+    x = torch.randn(rows, k, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    X = gk.MatRef.from_row_major(x, rows, k)
+    want = gk.quantize_fp4(X, gk.FP4_MX)
+    size = want._data.numel()
+    other = torch.cuda.Stream()
+    torch.zeros(8, dtype=torch.uint8, device="cuda").fill_(1)  # a kernel's first use waits
+    torch.cuda.synchronize()
+    held = torch.empty(size, dtype=torch.uint8, device="cuda")
+    torch.cuda._sleep(40_000_000)  # some 20 milliseconds on the current stream
+    held.fill_(0x55)
+    del held
+    q = gk.quantize_fp4(X, gk.FP4_MX, stream=other.cuda_stream, sync=False)
+    torch.cuda.synchronize()
+    assert torch.equal(q._data, want._data)
