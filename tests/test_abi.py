@@ -471,3 +471,49 @@ def test_fp4_validation_without_gpu():
     assert b"null 4-bit matrix A" in lib.gk_last_error()
     assert lib.gk_fp4_import(64, 15, 4, 128, 4, 1, C.byref(a.c), None) == gk.GK_EINVAL
     assert b"takes rows of 4 code bytes and 1 scales" in lib.gk_last_error()
+
+
+def test_fp4_matrix_parts_must_lie_in_device_memory():
+    """A 4-bit matrix's offsets and scales are read on the device as its codes are: a tensor in host
+    memory is refused where the matrix is made, and where a matrix that got one is used."""
+    import torch
+    host = torch.tensor([0, 4], dtype=torch.int32)
+    byte = torch.zeros(4096, dtype=torch.uint8)
+    expect_err(lambda: fp4(4, 8, offsets=host), "offsets is not in device memory")
+    expect_err(lambda: gk.Fp4Matrix.empty(4, 8, gk.FP4_MX, offsets=host),
+               "offsets is not in device memory")
+    at = (1 << 20, 4096)
+    expect_err(lambda: gk.Fp4Matrix(4, 8, gk.FP4_MX, 1.0, 1, None, at, byte),
+               "scales is not in device memory")
+    expect_err(lambda: gk.Fp4Matrix(4, 8, gk.FP4_MX, 1.0, 1, None, byte, at),
+               "data is not in device memory")
+
+    x, c = gk.MatRef.new((64, 32), 4, 8, 8, 1), gk.MatMut.new((64, 24), 4, 6, 6, 1)
+    y = gk.MatMut.new((64, 32), 4, 8, 8, 1)
+    b = fp4(6, 8, at=1 << 22)
+    for part, name in (("offsets", "offsets"), ("_scales", "scales")):
+        q = fp4(4, 8)
+        setattr(q, part, host if part == "offsets" else byte)
+        expect_err(lambda: gk.quantize_fp4(x, gk.FP4_MX, out=q, x_type=0, sync=False),
+                   f"out's {name} is not in device memory")
+        expect_err(lambda: gk.dequantize_fp4(q, y, sync=False), f"Q's {name} is not in device memory")
+        expect_err(lambda: gk.gemm_fp4(1.0, q, b, 0.0, c, c_type=0, sync=False),
+                   f"A's {name} is not in device memory")
+        w = fp4(6, 8, at=1 << 22)
+        setattr(w, part, host if part == "offsets" else byte)
+        expect_err(lambda: gk.gemm_fp4(1.0, fp4(4, 8), w, 0.0, c, c_type=0, sync=False),
+                   f"B's {name} is not in device memory")
+
+
+def test_fp4_matrix_parts_must_lie_on_one_device():
+    """Parts on two devices (stand-ins that answer as tensors there do)."""
+    class On:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def get_device(self):
+            return self.dev
+
+    gk._one_device("data", On(1), "scales", (64, 4), "offsets", On(1))
+    expect_err(lambda: gk._one_device("data", On(0), "scales", None, "offsets", On(1)),
+               "offsets is on cuda:1, data is on cuda:0")
