@@ -1657,7 +1657,8 @@ int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, flo
     p.c = c.data;
     p.ldq = c.rs;
     p.ldp = c.cs;
-    p.alpha = static_cast<float>(scaled);
+    // (an empty product is zero whatever alpha is, an infinity or a NaN too)
+    p.alpha = p.zero ? 0.0f : static_cast<float>(scaled);
     p.beta = beta;
     p.out_type = out_type;
     p.pieces = c_in_pieces(c.data, out_type, c.rs, c.cs, 0, static_cast<int64_t>(n), beta);

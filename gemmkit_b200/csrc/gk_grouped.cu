@@ -205,6 +205,12 @@ __device__ __forceinline__ bool next_tile(GroupWalk& w, const GroupedParams& p, 
     return true;
 }
 
+// The factor of a tile's accumulators. An empty contraction is zero whatever alpha is (an infinity or
+// a NaN too): C <- beta C.
+__device__ __forceinline__ float tile_alpha(const GroupedParams& p, const GTile& t) {
+    return t.nk > 0 ? p.alpha : 0.0f;
+}
+
 // Whether the stage of contraction block kb holds the end of its group inside 16 indices.
 __device__ __forceinline__ bool ragged_stage(const GroupedParams& p, const GTile& t, int kb) {
     return p.wgrad && t.nk - kb < GBK && (t.nk & 15) != 0;
@@ -418,9 +424,10 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
             const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                 static_cast<uint32_t>(acc * BN + cbase);
             const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+            const float alpha = tile_alpha(p, t);
             if (p.pieces) {
                 store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
-                             t.qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, t.nk > 0);
+                             t.qn - cbase, pn, alpha, p.out_type, ebuf, lane, t.nk > 0);
             } else {
                 for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
                     uint32_t v[32];
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                     }
                     if (lane < pn)
                         store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
-                                  t.qn - cbase - c, p.alpha, p.beta);
+                                  t.qn - cbase - c, alpha, p.beta);
                 }
             }
             tc_fence_before();
@@ -930,9 +937,10 @@ __global__ void __launch_bounds__(GPairCfg<PB>::THREADS, 1)
                 const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                     static_cast<uint32_t>(acc * BN + cbase);
                 const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+                const float alpha = tile_alpha(p, t);
                 if (p.pieces) {
                     store_cols16(tb, C::WCOLS, static_cast<uint16_t*>(p.c) + at + cbase * p.ldq, p.ldq,
-                                 t.qn - cbase, pn, p.alpha, p.out_type, ebuf, lane, t.nk > 0);
+                                 t.qn - cbase, pn, alpha, p.out_type, ebuf, lane, t.nk > 0);
                 } else {
                     for (int c = 0; c < C::WCOLS && cbase + c < t.qn; c += 32) {
                         uint32_t v[32];
@@ -944,7 +952,7 @@ __global__ void __launch_bounds__(GPairCfg<PB>::THREADS, 1)
                         }
                         if (lane < pn)
                             store_any(p.c, p.out_type, at + lane * p.ldp + (cbase + c) * p.ldq, p.ldq, v,
-                                      t.qn - cbase - c, p.alpha, p.beta);
+                                      t.qn - cbase - c, alpha, p.beta);
                     }
                 }
                 tc_fence_before();

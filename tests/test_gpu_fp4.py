@@ -630,3 +630,21 @@ def test_result_memory_belongs_to_the_call_s_stream():
     q = gk.quantize_fp4(X, gk.FP4_MX, stream=other.cuda_stream, sync=False)
     torch.cuda.synchronize()
     assert torch.equal(q._data, want._data)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows", [9, 50, 2048])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("alpha", [float("inf"), float("nan")])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_product_without_contraction_ignores_alpha(fmt, rows, out, alpha, beta):
+    """k == 0: C <- beta * C on the groups' rows whatever alpha is."""
+    torch = torch_cuda()
+    off = torch.tensor([1, 4, 4, rows - 1], dtype=torch.int32, device="cuda")
+    a = gk.Fp4Matrix.empty(rows, 0, fmt, offsets=off)
+    b = gk.Fp4Matrix.empty(3 * 24, 0, fmt, groups=3)
+    c = torch.full((rows, 24), 8.0, device="cuda", dtype=tdt(out))
+    product(a, b, c, alpha, beta)
+    want = torch.full_like(c, 8.0)
+    want[1:rows - 1] = 8.0 * beta
+    assert torch.equal(c, want)

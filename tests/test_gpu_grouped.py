@@ -684,3 +684,42 @@ print("ok")
     out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
                          timeout=300)
     assert out.returncode == 0 and "ok" in out.stdout, out.stderr[-2000:]
+
+
+# Sizes for each tile plan of the weight gradient: one CTA with 64, 128 and 256 rows of the Q side,
+# CTA pairs with 256 columns (f32 C) and with 512 (16-bit C).
+@pytest.mark.parametrize("sizes,m,n,out", [([3, 0, 20], 40, 24, "f32"), ([3, 0, 20], 40, 24, "bf16"),
+                                           ([70, 0, 1], 100, 72, "f32"),
+                                           ([70, 0, 1], 200, 136, "bf16"),
+                                           ([5, 0, 100], 1032, 2304, "f32"),
+                                           ([5, 0, 100], 1032, 2304, "bf16")])
+@pytest.mark.parametrize("alpha", [float("inf"), -float("inf"), float("nan"), -3.0])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_empty_group_gradient_ignores_alpha(sizes, m, n, out, alpha, beta):
+    """An empty group's C[g] becomes beta * C[g], with an infinite or NaN alpha too; the other groups
+    get alpha times their product (integers: exact before that product)."""
+    torch = torch_cuda()
+    off = offsets_of(sizes)
+    a, b = data(1, (sum(sizes), m), "bf16"), data(2, (sum(sizes), n), "bf16")
+    c = torch.full((len(sizes), m, n), 8.0, device="cuda", dtype=tdt(out))
+    run_wgrad(a, b, off, c, "bf16", alpha, beta)
+    acc, _ = want_wgrad(a, b, off, c, 1.0, 0.0)
+    want = (alpha * acc + beta * 8.0).to(tdt(out))
+    want[1] = beta * 8.0
+    assert bool(((c == want) | (c.isnan() & want.isnan())).all())
+
+
+@pytest.mark.parametrize("rows,n", [(9, 24), (200, 136), (2048, 2304)])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("alpha", [float("inf"), float("nan")])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_forward_without_contraction_ignores_alpha(rows, n, out, alpha, beta):
+    """k == 0: C <- beta * C on the groups' rows whatever alpha is."""
+    torch = torch_cuda()
+    off = offsets_of([rows - 4, 0, 2], 1)
+    c = torch.full((rows, n), 8.0, device="cuda", dtype=tdt(out))
+    run_fwd(torch.zeros((rows, 0), device="cuda", dtype=torch.bfloat16),
+            torch.zeros((3, 0, n), device="cuda", dtype=torch.bfloat16), off, c, "bf16", alpha, beta)
+    want = torch.full_like(c, 8.0)
+    want[1:rows - 1] = 8.0 * beta
+    assert torch.equal(c, want)
