@@ -61,15 +61,15 @@ int check_device(int* dev_out) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_err(e, "no CUDA device");
-    static int ok[64] = {0};
+    static gk::PerDevice<int> known;  // 1: an sm_100 device, 2: another
     if (dev < 0 || dev >= 64) return set_err(GK_ENODEV, "gemmkit: device index out of range");
-    if (ok[dev] == 0) {
+    const int is = known.get(dev, [dev] {
         int major = 0, minor = 0;
         cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
         cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-        ok[dev] = (major == 10 && minor == 0) ? 1 : 2;
-    }
-    if (ok[dev] != 1)
+        return (major == 10 && minor == 0) ? 1 : 2;
+    });
+    if (is != 1)
         return set_err(GK_ENODEV, "gemmkit: the CUDA engine needs an sm_100 (B200) device");
     if (dev_out) *dev_out = dev;
     return GK_OK;

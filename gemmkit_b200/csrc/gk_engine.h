@@ -16,6 +16,7 @@
 #include <atomic>
 
 #include "gemmkit_cuda.h"
+#include "gk_once.h"
 
 namespace gk {
 
@@ -225,10 +226,10 @@ inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
     int dev = 0;
     cudaGetDevice(&dev);
     const uint64_t bit = uint64_t{1} << (dev & 63);
-    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     return e;
 }
 

@@ -1364,11 +1364,10 @@ int launch_fp4_gemm(const CUtensorMap& tp, const CUtensorMap& tq, const Fp4GemmP
 template <int FMT>
 int fp4_pair_clusters() {
     using C = Fp4PairCfg<FMT>;
-    static int cache[64] = {0};
+    static PerDevice<int> cache;
     int dev = 0;
     cudaGetDevice(&dev);
-    int& n = cache[dev & 63];
-    if (n == 0) {
+    return cache.get(dev, [] {
         cudaLaunchConfig_t q;
         memset(&q, 0, sizeof(q));
         q.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
@@ -1388,9 +1387,8 @@ int fp4_pair_clusters() {
             cudaGetLastError();
             c = sm_count() / 2;
         }
-        n = c;
-    }
-    return n;
+        return c;
+    });
 }
 
 template <int FMT>

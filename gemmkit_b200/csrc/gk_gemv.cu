@@ -851,17 +851,11 @@ static int launch_gemv_nb(const TcProblem& pr, const TcPlan& plan, GemvParams gp
     gp.x_row_bytes = pr.K * ES;
 
     auto kern = gemv_kernel<KIND, OUT, NB>;
-    static int attr_done[64] = {0};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!attr_done[dev & 63]) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             C::SMEM);
-        if (e != cudaSuccess) {
-            snprintf(err, errlen, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-            return e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? 5 : 3;
-        }
-        attr_done[dev & 63] = 1;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t se = allow_smem(kern, C::SMEM, done);
+    if (se != cudaSuccess) {
+        snprintf(err, errlen, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(se));
+        return se == cudaErrorNoDevice || se == cudaErrorInsufficientDriver ? 5 : 3;
     }
     // The K split: bounded by the partial slots the leader's ring holds, and lowered until
     // every tile's cluster can be resident at once.

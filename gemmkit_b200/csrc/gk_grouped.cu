@@ -1146,11 +1146,10 @@ int realign(GOperand* o, int64_t rows, int64_t len, int64_t groups, bool mn, int
 
 // Clusters of the pair kernel that are resident at once on the current device.
 int pair_clusters() {
-    static int cache[64] = {0};
+    static PerDevice<int> cache;
     int dev = 0;
     cudaGetDevice(&dev);
-    int& n = cache[dev & 63];
-    if (n == 0) {
+    return cache.get(dev, [] {
         cudaLaunchConfig_t q;
         memset(&q, 0, sizeof(q));
         q.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
@@ -1170,9 +1169,8 @@ int pair_clusters() {
             cudaGetLastError();
             c = sm_count() / 2;
         }
-        n = c;
-    }
-    return n;
+        return c;
+    });
 }
 
 int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaStream_t stream);

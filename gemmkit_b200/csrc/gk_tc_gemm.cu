@@ -497,28 +497,26 @@ void set_tile_divs(GemmParams* gp) {
 static __device__ unsigned int g_status[64];
 
 unsigned int* device_status_ptr() {
-    static unsigned int* cache[64] = {nullptr};
+    static PerDevice<unsigned int*> cache;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (!cache[dev & 63]) {
+    return cache.get(dev, [dev]() -> unsigned int* {
         void* p = nullptr;
         if (cudaGetSymbolAddress(&p, g_status) != cudaSuccess) return nullptr;
-        cache[dev & 63] = static_cast<unsigned int*>(p) + (dev & 63);
-    }
-    return cache[dev & 63];
+        return static_cast<unsigned int*>(p) + (dev & 63);
+    });
 }
 
 int sm_count() {
-    static int cache[64] = {0};
+    static PerDevice<int> cache;
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return 148;
-    if (cache[dev] == 0) {
+    return cache.get(dev, [dev] {
         int n = 0;
         cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-        cache[dev] = n > 0 ? n : 148;
-    }
-    return cache[dev];
+        return n > 0 ? n : 148;
+    });
 }
 
 // A small per-thread cache of encoded tensor maps: serving loops call the same shapes over
@@ -815,16 +813,11 @@ static int launch_one(const TcProblem& pr, const TcPlan& plan, GemmParams gp, ch
     gp.a_slab = pr.a.slab;
     gp.b_slab = pr.b.slab;
     auto kern = tc_gemm_kernel<KIND, OUT, BN>;
-    static int attr_done[64] = {0};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!attr_done[dev & 63]) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-        if (e != cudaSuccess) {
-            snprintf(err, errlen, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-            return e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? 5 : 3;
-        }
-        attr_done[dev & 63] = 1;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t se = allow_smem(kern, C::SMEM, done);
+    if (se != cudaSuccess) {
+        snprintf(err, errlen, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(se));
+        return se == cudaErrorNoDevice || se == cudaErrorInsufficientDriver ? 5 : 3;
     }
     gp.tiles_n = plan.tiles_n;
     gp.tiles_per_batch = gp.tiles_m * gp.tiles_n;

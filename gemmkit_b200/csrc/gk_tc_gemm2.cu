@@ -895,17 +895,13 @@ static int launch_pair_one(const TcProblem& pr, const TcPlan& plan, GemmParams g
         if (rc) return rc;
     }
     auto kern = tc_gemm_pair_kernel<KIND, OUT, BN, EPI16>;
-    static int attr_done[64] = {0};
+    static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaGetDevice(&dev);
-    if (!attr_done[dev & 63]) {
-        cudaError_t e =
-            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-        if (e != cudaSuccess) {
-            snprintf(err, errlen, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-            return 3;
-        }
-        attr_done[dev & 63] = 1;
+    const cudaError_t se = allow_smem(kern, C::SMEM, done);
+    if (se != cudaSuccess) {
+        snprintf(err, errlen, "gemmkit: cudaFuncSetAttribute: %s", cudaGetErrorString(se));
+        return 3;
     }
     gp.tiles_n = plan.tiles_n;
     gp.tiles_per_batch = gp.tiles_m * gp.tiles_n;
@@ -917,7 +913,7 @@ static int launch_pair_one(const TcProblem& pr, const TcPlan& plan, GemmParams g
     memset(&cfg, 0, sizeof(cfg));
     // A persistent grid must be co-resident: GPC boundaries can leave fewer two-SM clusters
     // than SMs / 2, so ask the runtime how many clusters of this kernel fit at once.
-    static int max_clusters[64] = {0};
+    static PerDevice<int> max_clusters;
     int grid = plan.grid;
     {
         cudaLaunchConfig_t q;
@@ -932,16 +928,16 @@ static int launch_pair_one(const TcProblem& pr, const TcPlan& plan, GemmParams g
         qa[0].val.clusterDim.z = 1;
         q.attrs = qa;
         q.numAttrs = 1;
-        if (!max_clusters[dev & 63]) {
+        const int most = max_clusters.get(dev, [&] {
             int n = 0;
             if (cudaOccupancyMaxActiveClusters(&n, kern, &q) != cudaSuccess || n <= 0) {
                 cudaGetLastError();
                 n = 1;
             }
-            max_clusters[dev & 63] = n;
-        }
+            return n;
+        });
         const int tiles = plan.num_tiles;
-        const int pairs = tiles < max_clusters[dev & 63] ? tiles : max_clusters[dev & 63];
+        const int pairs = tiles < most ? tiles : most;
         grid = 2 * pairs;
         // Tail split: a last wave that would occupy at most half the pairs runs as half tiles.
         const int rem = tiles % pairs;
