@@ -27,7 +27,7 @@ __all__ = [
     "gemm_i8_packed_b_requant", "gemm_i8_requant_batched", "gemm_i8_requant_batched_ptr",
     "gemm_half_f32", "gemm_bf16_f32_unchecked", "gemm_f16_f32_unchecked",
     "gemm_half_f32_batched", "gemm_half_f32_fused", "gemm_i8_fused", "gemm_i8_fused_unchecked", "Activation", "quantize_f32_i8", "gemm_i8_noalloc_unchecked", "set_tile_n", "knob_names", "knob_get",
-    "gemm_half_grouped", "gemm_half_grouped_wgrad", "Fp4Matrix", "quantize_fp4", "dequantize_fp4",
+    "gemm_half_grouped", "gemm_half_grouped_wgrad", "scratch_release", "Fp4Matrix", "quantize_fp4", "dequantize_fp4",
     "gemm_fp4", "FP4_MX", "FP4_NV", "knob_set", "device_status", "selftest_wait_timeout",
 ]
 
@@ -638,6 +638,12 @@ def gemm_half_grouped_wgrad(alpha: float, a: MatRef, b: MatRef, offsets, beta: f
                                                   par.c(), _stream(stream)))
     if sync:
         _sync(stream)
+
+
+def scratch_release(device: int = 0) -> None:
+    """Give the scratch that the grouped products keep for operands that they had to realign back
+    to the device (at most 1/64 of its memory stays with the engine otherwise); synchronises it."""
+    _check(_lib.load().gk_scratch_release(device))
 
 
 # ---- microscaled 4-bit floating point --------------------------------------------------------

@@ -126,6 +126,7 @@ SIGNATURES = {
                                    C.c_int, Parallelism, vp]),
     "gk_gemm_half_grouped_wgrad": (i32, [C.c_int, sz, vp, f32, MatRefC, MatRefC, f32, MatMutC, pd,
                                          C.c_int, Parallelism, vp]),
+    "gk_scratch_release": (i32, [C.c_int]),
     "gk_fp4_data_bytes": (sz, [sz, sz]),
     "gk_fp4_scale_bytes": (sz, [C.c_int, sz, C.c_int, sz, sz]),
     "gk_quantize_fp4": (i32, [MatRefC, C.c_int, pd, C.POINTER(Fp4MatrixC), vp]),

@@ -1061,28 +1061,38 @@ int grouped_bn(int64_t q) { return q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 
 
 // Scratch for realigned operands: stream-ordered memory from a pool of the engine's own on the
 // current device, so that calls on several streams, and calls captured into several graphs, never
-// share any (a captured call allocates and frees inside its graph). The pool keeps what it has
-// grown to.
-cudaMemPool_t scratch_pool() {
+// share any (a captured call allocates and frees inside its graph). At every synchronisation the
+// pool gives back what it holds beyond 1 / SCRATCH_SHARE of the device's memory (2.8 of 179 GiB), and
+// gk_scratch_release the rest. (Held without a bound, one call with a large stack of odd weights
+// kept its size from the process's other allocations for good. Mapping memory anew is not cheap:
+// with a bound below its 0.94 GB a synchronised call with 8 weights of 4096 x 14336 took 2.3
+// instead of 0.49 ms.)
+constexpr size_t SCRATCH_SHARE = 64;
+
+// The pool of device `dev`; with `make`, made at the first call (nullptr on failure).
+cudaMemPool_t scratch_pool(int dev, bool make) {
     static std::mutex m;
     static cudaMemPool_t pools[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(m);
-    if (!pools[dev]) {
+    if (!pools[dev] && make) {
         cudaMemPoolProps props;
         memset(&props, 0, sizeof(props));
         props.allocType = cudaMemAllocationTypePinned;
         props.handleTypes = cudaMemHandleTypeNone;
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = dev;
-        uint64_t keep = UINT64_MAX;
-        if (cudaMemPoolCreate(&pools[dev], &props) != cudaSuccess ||
-            cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep) !=
-                cudaSuccess) {
+        size_t unused = 0, total = 0;
+        cudaMemPool_t pool = nullptr;
+        if (cudaMemGetInfo(&unused, &total) != cudaSuccess ||
+            cudaMemPoolCreate(&pool, &props) != cudaSuccess) {
             cudaGetLastError();
-            pools[dev] = nullptr;
+            return nullptr;
         }
+        uint64_t keep = total / SCRATCH_SHARE;
+        if (cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess)
+            cudaGetLastError();  // it then keeps nothing
+        pools[dev] = pool;
     }
     return pools[dev];
 }
@@ -1102,8 +1112,15 @@ int realign(GOperand* o, int64_t rows, int64_t len, int64_t groups, bool mn, int
     if (e == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
         e = cudaMallocAsync(scratch, bytes, st);
     } else if (e == cudaSuccess) {
-        cudaMemPool_t pool = scratch_pool();
+        int dev = -1;
+        cudaGetDevice(&dev);
+        cudaMemPool_t pool = scratch_pool(dev, true);
         e = pool ? cudaMallocFromPoolAsync(scratch, bytes, pool, st) : cudaErrorMemoryAllocation;
+        if (e == cudaErrorMemoryAllocation && pool) {  // once more, without what the pool holds unused
+            cudaGetLastError();
+            cudaMemPoolTrimTo(pool, 0);
+            e = cudaMallocFromPoolAsync(scratch, bytes, pool, st);
+        }
     }
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -1338,6 +1355,25 @@ int check_stack(size_t len, size_t groups, size_t rows, size_t cols, ptrdiff_t r
 using namespace gk;
 
 extern "C" {
+
+int gk_scratch_release(int device) {
+    int prev = 0;
+    cudaGetDevice(&prev);
+    if (cudaSetDevice(device) != cudaSuccess) {
+        cudaGetLastError();
+        return api_err(GK_ENODEV, "gemmkit: bad device");
+    }
+    cudaMemPool_t pool = scratch_pool(device, false);
+    cudaError_t e = cudaSuccess;
+    if (pool) {  // what was freed is unused once the calls that used it have ended
+        e = cudaDeviceSynchronize();
+        if (e == cudaSuccess) e = cudaMemPoolTrimTo(pool, 0);
+    }
+    cudaSetDevice(prev);
+    if (e != cudaSuccess)
+        return api_err(GK_ECUDA, "gemmkit: releasing the scratch: %s", cudaGetErrorString(e));
+    return GK_OK;
+}
 
 int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t* offsets, float alpha,
                          gk_matref a, gk_matref b, ptrdiff_t b_gs, float beta, gk_matmut c,

@@ -328,7 +328,9 @@ typedef enum { GK_F32 = 0, GK_F16 = 1, GK_BF16 = 2 } gk_dtype;
  * rows and reads neither A nor B. Any non-negative strides. An A with unit column stride and a B
  * with a unit row or column stride, 16-byte aligned and every other stride a multiple of 16 bytes,
  * are read in place (in the weight gradient A and B with unit column strides); other operands
- * are first copied to aligned scratch, stream-ordered memory from a pool that the engine keeps.
+ * are first copied to aligned scratch, stream-ordered memory of the operand's size (all groups of
+ * B) from a pool of the engine's, which keeps at most 1/64 of the device's memory past the next
+ * synchronisation (see gk_scratch_release). In a capture the scratch is the graph's own.
  * The gradient of A is the same call with C's gradient as A and B viewed transposed. Calls may
  * be captured and may run on several streams at once. */
 int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t *offsets, float alpha,
@@ -342,6 +344,9 @@ int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t *offsets, floa
 int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t *offsets, float alpha,
                                gk_matref a, gk_matref b, float beta, gk_matmut c, ptrdiff_t c_gs,
                                int out_type, gk_parallelism par, gk_stream_t stream);
+/* Gives the scratch that the two entries above keep on `device` back to it; synchronizes the
+ * device when there is any. Not during a capture. */
+int gk_scratch_release(int device);
 
 /* ---- microscaled 4-bit floating point (no counterpart in gemmkit) ----------------------- */
 

@@ -517,3 +517,10 @@ def test_fp4_matrix_parts_must_lie_on_one_device():
     gk._one_device("data", On(1), "scales", (64, 4), "offsets", On(1))
     expect_err(lambda: gk._one_device("data", On(0), "scales", None, "offsets", On(1)),
                "offsets is on cuda:1, data is on cuda:0")
+
+
+def test_scratch_release_without_gpu():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("for machines without a GPU")
+    expect_err(lambda: gk.scratch_release(0), "bad device", code=gk.GK_ENODEV)

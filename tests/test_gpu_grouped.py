@@ -723,3 +723,31 @@ def test_forward_without_contraction_ignores_alpha(rows, n, out, alpha, beta):
     want = torch.full_like(c, 8.0)
     want[1:rows - 1] = 8.0 * beta
     assert torch.equal(c, want)
+
+
+def test_scratch_is_given_back():
+    """Operands that are copied to scratch: past a synchronisation the engine keeps at most 1/64 of
+    the device's memory, and nothing after scratch_release; calls go on working."""
+    torch = torch_cuda()
+    rows, k, n, g = 16, 8192, 8192, 27
+    off = torch.tensor([0, 4] + [8] * (g - 2) + [rows], dtype=torch.int32, device="cuda")
+    b = torch.zeros((g, n, k + 1), device="cuda", dtype=torch.bfloat16)
+    b[0], b[1], b[-1] = data(2, (3, n, k + 1), "bf16")
+    b = b[:, :, :k].transpose(1, 2)  # an odd pitch: 3.6 GB of scratch
+    a = data(1, (rows, k), "bf16")
+    c = torch.zeros((rows, n), device="cuda")
+    small = data(3, (1, 72, 65), "bf16")  # the process's first use of the pool and the kernels
+    run_fwd(data(4, (3, 72), "bf16"), small, offsets_of([3]), torch.zeros((3, 65), device="cuda"), "bf16")
+    want, _ = want_fwd(a, b, off, c, 1.0, 0.0)
+    gk.scratch_release()
+    for release in (False, True, False, True):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        free, total = torch.cuda.mem_get_info()
+        c.fill_(7.0)
+        run_fwd(a, b, off, c, "bf16")
+        torch.cuda.synchronize()
+        assert torch.equal(c.double(), want)
+        if release:
+            gk.scratch_release()
+        assert free - torch.cuda.mem_get_info()[0] <= (0 if release else total // 64)
