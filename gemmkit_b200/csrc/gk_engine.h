@@ -233,6 +233,13 @@ inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
     return e;
 }
 
+// The limit of a grouped or 4-bit kernel's bounded waits, for tiles of up to `stages` stages: a role
+// may wait for a whole tile's contraction, and one CTA takes 0.26 to 0.39 us a stage (8 x 8 over 2^30
+// rows: 16.8 million stages, 5.2 s).
+inline uint64_t wait_limit_ns(int64_t stages) {
+    return 4000000000ull + 2000ull * static_cast<uint64_t>(stages);
+}
+
 // Sets this thread's gk_last_error() text (gk_api.cu); returns `code`.
 int set_last_error(int code, const char* text);
 

@@ -1660,7 +1660,7 @@ int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, flo
     p.beta = beta;
     p.out_type = out_type;
     p.pieces = c_in_pieces(c.data, out_type, c.rs, c.cs, 0, static_cast<int64_t>(n), beta);
-    p.timeout_ns = 4000000000ull;
+    p.timeout_ns = wait_limit_ns(p.stages);
     p.status = device_status_ptr();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return a->fmt == GK_FP4_MX ? run_fp4_gemm<GK_FP4_MX>(p, a, b, st)

@@ -1261,7 +1261,7 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
         return set_last_error(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
     p.tiles_p = static_cast<int>((p.np + tm - 1) / tm);
     p.tiles_q = static_cast<int>((p.nq + bn - 1) / bn);
-    p.timeout_ns = 4000000000ull;
+    p.timeout_ns = wait_limit_ns((plen + GBK - 1) / GBK);
     p.status = device_status_ptr();
     const int pdl = api_pdl_enabled();
     char err[256] = "";

@@ -159,3 +159,29 @@ def test_fp4_wide_c(memory, fmt, sizes, n, out, odd, last, beta):
     want = torch.cat([av[o[e]:o[e + 1]] @ bv[e * n:(e + 1) * n].T for e in range(g)]) + \
         beta * c0.double()
     assert torch.equal(c, want.to(tdt(out)))
+
+
+@pytest.mark.parametrize("entry", ["forward", "wgrad"])
+def test_longest_contraction(entry):
+    """A contraction at the engine's limit (2^30 - 1) in one tile takes about 5 seconds: none of the
+    kernel's bounded waits may give up meanwhile. Zeros but for integers at the two ends, in the middle
+    and at random places: every sum is exact."""
+    torch = torch_cuda()
+    k, m, n = (2 ** 30 - 8 if entry == "forward" else 2 ** 30 - 1), 8, 8
+    rng = np.random.default_rng(3)
+    at = np.unique(np.concatenate([rng.integers(0, k, 3000), [0, 1, k // 2, k - 17, k - 2, k - 1]]))
+    x, y = data(1, (len(at), m), "bf16"), data(2, (len(at), n), "bf16")
+    at = torch.from_numpy(at).cuda()
+    want = x.double().T @ y.double()
+    shape = (lambda w: (w, k)) if entry == "forward" else (lambda w: (k, w))
+    a, b = (torch.zeros(shape(w), dtype=torch.bfloat16, device="cuda") for w in (m, n))
+    c = torch.full((m, n), 7.0, device="cuda")
+    if entry == "forward":
+        a[:, at], b[:, at] = x.T, y.T
+        run_fwd(a, b.t()[None], offsets_of([m]), c, "bf16")
+    else:
+        a[at], b[at] = x, y
+        run_wgrad(a, b, offsets_of([k]), c[None], "bf16")
+    assert torch.equal(c.double(), want)
+    del a, b
+    torch.cuda.empty_cache()
