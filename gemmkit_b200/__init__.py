@@ -567,10 +567,10 @@ def _same_device(*named) -> None:
                                       f"current device is cuda:{cur}")
 
 
-def _one_device(*named) -> None:
+def _one_device(*named):
     """The parts of one matrix lie in the memory of one device (names and tensors in turn, as in
-    _same_device; which device that is matters when the matrix is used)."""
-    at = None
+    _same_device): the first tensor among them, which stands for all when the matrix is used."""
+    at = first = None
     for i in range(1, len(named), 2):
         t = named[i]
         if t is None or isinstance(t, tuple):
@@ -578,11 +578,12 @@ def _one_device(*named) -> None:
         dev = t.get_device()
         if dev < 0:
             raise GemmkitError(GK_EINVAL, f"gemmkit: {named[i - 1]} is not in device memory")
-        if at is None:
-            at = named[i - 1], dev
+        if first is None:
+            at, first = (named[i - 1], dev), t
         elif dev != at[1]:
             raise GemmkitError(GK_EINVAL, f"gemmkit: {named[i - 1]} is on cuda:{dev}, {at[0]} is on "
                                           f"cuda:{at[1]}")
+    return first
 
 
 def _offsets(offsets):
@@ -662,14 +663,10 @@ class Fp4Matrix:
         self.rows, self.cols, self.fmt, self.scale = int(rows), int(cols), fmt, float(scale)
         self.groups, self.offsets = groups, offsets
         self._data, self._scales = data, scales
-        _one_device("data", data, "scales", scales, "offsets", offsets)
+        self._where = _one_device("data", data, "scales", scales, "offsets", offsets)
         off = None if offsets is None else _offsets(offsets)[0]
         self.c = _lib.Fp4MatrixC(fmt, self.scale, groups, off, self.rows, self.cols, *_flat(data),
                                  *_flat(scales))
-
-    def _parts(self, name: str):
-        """The names and tensors that a call with this matrix reads through, for _same_device."""
-        return name, self._data, name + "'s scales", self._scales, name + "'s offsets", self.offsets
 
     @property
     def data(self):
@@ -706,8 +703,8 @@ class Fp4Matrix:
         else:  # not what the current stream may still be writing
             with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
                 buf = torch.empty(nd + ns, dtype=torch.uint8, device=device)
-        _one_device("the matrix", buf, "offsets", offsets)
         q = Fp4Matrix.__new__(Fp4Matrix)
+        q._where = _one_device("the matrix", buf, "offsets", offsets)
         q.rows, q.cols, q.fmt, q.scale = rows, cols, fmt, float(scale)
         q.groups, q.offsets, q._data, q._scales = groups, offsets, buf, None
         at = buf.data_ptr()
@@ -756,9 +753,7 @@ def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: 
     x_gs elements apart. `out` reuses a matrix of the same shape, format and groups (its scale and
     groups then hold), otherwise the result's memory is allocated for the call's stream; x_type names
     the element type of a (pointer, length) pair."""
-    _same_device("X", x.data, "offsets", offsets)
-    if out is not None:
-        _same_device(*out._parts("out"))
+    _same_device("X", x.data, "offsets", offsets, "out", None if out is None else out._where)
     if out is None:
         stacked = offsets is None and groups > 1
         out = Fp4Matrix.empty(x.rows * groups if stacked else x.rows, x.cols, fmt, scale, groups,
@@ -775,7 +770,7 @@ def quantize_fp4(x: MatRef, fmt: int, scale: float = 1.0, offsets=None, groups: 
 
 def dequantize_fp4(q: Fp4Matrix, out: MatMut, stream=None, sync: bool = True) -> None:
     """The f32 values that a 4-bit matrix stands for (extension)."""
-    _same_device(*q._parts("Q"), "C", out.data)
+    _same_device("Q", q._where, "C", out.data)
     if _elem_type(out.data, _lib.DT_F32) != _lib.DT_F32:
         raise GemmkitError(GK_EINVAL, "gemmkit: C must hold f32 elements")
     _check(_lib.load().gk_dequantize_fp4(C.byref(q.c), out.c(), _stream(stream)))
@@ -790,7 +785,7 @@ def gemm_fp4(alpha: float, a: Fp4Matrix, b: Fp4Matrix, beta: float, c: MatMut,
     C f32, f16 or bf16 by its tensor's dtype (c_type for a (pointer, length) pair). With groups,
     row i of A's group g is multiplied by B's g-th matrix: A ragged (offsets) or equal groups, B a
     stack of as many."""
-    _same_device(*a._parts("A"), *b._parts("B"), "C", c.data)
+    _same_device("A", a._where, "B", b._where, "C", c.data)
     if c_type is None:
         c_type = _elem_type(c.data, -1)
     _check(_lib.load().gk_gemm_fp4(float(alpha), C.byref(a.c), C.byref(b.c), float(beta), c.c(),

@@ -475,7 +475,7 @@ def test_fp4_validation_without_gpu():
 
 def test_fp4_matrix_parts_must_lie_in_device_memory():
     """A 4-bit matrix's offsets and scales are read on the device as its codes are: a tensor in host
-    memory is refused where the matrix is made, and where a matrix that got one is used."""
+    memory is refused where the matrix is made, which is when their addresses are taken."""
     import torch
     host = torch.tensor([0, 4], dtype=torch.int32)
     byte = torch.zeros(4096, dtype=torch.uint8)
@@ -488,35 +488,55 @@ def test_fp4_matrix_parts_must_lie_in_device_memory():
     expect_err(lambda: gk.Fp4Matrix(4, 8, gk.FP4_MX, 1.0, 1, None, byte, at),
                "data is not in device memory")
 
-    x, c = gk.MatRef.new((64, 32), 4, 8, 8, 1), gk.MatMut.new((64, 24), 4, 6, 6, 1)
-    y = gk.MatMut.new((64, 32), 4, 8, 8, 1)
-    b = fp4(6, 8, at=1 << 22)
-    for part, name in (("offsets", "offsets"), ("_scales", "scales")):
-        q = fp4(4, 8)
-        setattr(q, part, host if part == "offsets" else byte)
-        expect_err(lambda: gk.quantize_fp4(x, gk.FP4_MX, out=q, x_type=0, sync=False),
-                   f"out's {name} is not in device memory")
-        expect_err(lambda: gk.dequantize_fp4(q, y, sync=False), f"Q's {name} is not in device memory")
-        expect_err(lambda: gk.gemm_fp4(1.0, q, b, 0.0, c, c_type=0, sync=False),
-                   f"A's {name} is not in device memory")
-        w = fp4(6, 8, at=1 << 22)
-        setattr(w, part, host if part == "offsets" else byte)
-        expect_err(lambda: gk.gemm_fp4(1.0, fp4(4, 8), w, 0.0, c, c_type=0, sync=False),
-                   f"B's {name} is not in device memory")
+
+class On:
+    """Stands for an int32 tensor of two entries in the memory of device `dev`."""
+    dtype = "torch.int32"
+
+    def __init__(self, dev):
+        self.dev = dev
+
+    def get_device(self):
+        return self.dev
+
+    def dim(self):
+        return 1
+
+    def is_contiguous(self):
+        return True
+
+    def numel(self):
+        return 2
+
+    def data_ptr(self):
+        return 4096
 
 
 def test_fp4_matrix_parts_must_lie_on_one_device():
-    """Parts on two devices (stand-ins that answer as tensors there do)."""
-    class On:
-        def __init__(self, dev):
-            self.dev = dev
-
-        def get_device(self):
-            return self.dev
-
-    gk._one_device("data", On(1), "scales", (64, 4), "offsets", On(1))
-    expect_err(lambda: gk._one_device("data", On(0), "scales", None, "offsets", On(1)),
+    at = (1 << 20, 4096)
+    gk.Fp4Matrix(4, 8, gk.FP4_MX, 1.0, 1, On(1), On(1), at)
+    expect_err(lambda: gk.Fp4Matrix(4, 8, gk.FP4_MX, 1.0, 1, On(1), On(0), at),
                "offsets is on cuda:1, data is on cuda:0")
+    expect_err(lambda: gk.Fp4Matrix(4, 8, gk.FP4_MX, 1.0, 1, None, On(0), On(1)),
+               "scales is on cuda:1, data is on cuda:0")
+
+
+@pytest.mark.parametrize("part", ["offsets", "data", "scales"])
+def test_fp4_matrix_on_another_device_is_refused(part):
+    """Whichever of a matrix's parts is the tensor that tells where it lies."""
+    def there(rows, at):
+        parts = {"offsets": None, "data": (at, 4096), "scales": (at + (1 << 16), 4096)}
+        parts[part] = On(63)
+        return gk.Fp4Matrix(rows, 8, gk.FP4_MX, 1.0, 1, *parts.values())
+
+    x, c = gk.MatRef.new((64, 32), 4, 8, 8, 1), gk.MatMut.new((64, 24), 4, 6, 6, 1)
+    y = gk.MatMut.new((64, 32), 4, 8, 8, 1)
+    q, w = there(4, 1 << 20), there(6, 1 << 22)
+    expect_err(lambda: gk.quantize_fp4(x, gk.FP4_MX, out=q, x_type=0, sync=False), "out is on cuda:63")
+    expect_err(lambda: gk.dequantize_fp4(q, y, sync=False), "Q is on cuda:63")
+    expect_err(lambda: gk.gemm_fp4(1.0, q, fp4(6, 8, at=1 << 22), 0.0, c, c_type=0, sync=False),
+               "A is on cuda:63")
+    expect_err(lambda: gk.gemm_fp4(1.0, fp4(4, 8), w, 0.0, c, c_type=0, sync=False), "B is on cuda:63")
 
 
 def test_scratch_release_without_gpu():
