@@ -664,7 +664,12 @@ class Fp4Matrix:
         self.groups, self.offsets = groups, offsets
         self._data, self._scales = data, scales
         self._where = _one_device("data", data, "scales", scales, "offsets", offsets)
-        off = None if offsets is None else _offsets(offsets)[0]
+        off = None
+        if offsets is not None:
+            off, n = _offsets(offsets)
+            if n != groups:  # the kernels read groups + 1 offsets
+                raise GemmkitError(GK_EINVAL, f"gemmkit: {groups} groups take {groups + 1} offsets "
+                                              f"(has {n + 1})")
         self.c = _lib.Fp4MatrixC(fmt, self.scale, groups, off, self.rows, self.cols, *_flat(data),
                                  *_flat(scales))
 

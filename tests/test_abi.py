@@ -539,6 +539,14 @@ def test_fp4_matrix_on_another_device_is_refused(part):
     expect_err(lambda: gk.gemm_fp4(1.0, fp4(4, 8), w, 0.0, c, c_type=0, sync=False), "B is on cuda:63")
 
 
+def test_fp4_matrix_offsets_must_match_its_groups():
+    """The kernels read groups + 1 offsets: a matrix over fewer (or more) is refused."""
+    for groups, n in ((2, 2), (1, 3), (0, 2), (1000, 2)):
+        expect_err(lambda: fp4(4, 8, groups=groups, offsets=(4096, n)),
+                   f"{groups} groups take {groups + 1} offsets (has {n})")
+    fp4(4, 8, groups=2, offsets=(4096, 3))
+
+
 def test_scratch_release_without_gpu():
     import torch
     if torch.cuda.is_available():
