@@ -682,6 +682,11 @@ bool api_overlaps(const void* pa, size_t bytes_a, const void* pb, size_t bytes_b
     return overlaps_bytes(pa, bytes_a, 1, pb, bytes_b, 1);
 }
 int api_pdl_enabled() { return pdl_enabled() ? 1 : 0; }
+int api_check_aligned(const void* p, size_t size, const char* name) {
+    if (reinterpret_cast<uintptr_t>(p) % size)
+        return set_err(GK_EINVAL, "gemmkit: %s is not aligned to its elements of %zu bytes", name, size);
+    return GK_OK;
+}
 }  // namespace gk
 
 // ==========================================================================================

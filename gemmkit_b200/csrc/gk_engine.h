@@ -253,5 +253,7 @@ int api_validate_gemm_views(const gk_matref& a, const gk_matref& b, const gk_mat
 bool api_self_aliases(size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs);
 bool api_overlaps(const void* pa, size_t bytes_a, const void* pb, size_t bytes_b);
 int api_pdl_enabled();
+// Refuses an address that is no multiple of its elements' size.
+int api_check_aligned(const void* p, size_t size, const char* name);
 
 }  // namespace gk

@@ -1273,6 +1273,7 @@ int check_fp4(const gk_fp4_matrix* q, const char* name) {
                                       ? "gemmkit: %s: the mx format has no matrix scale (must be 1)"
                                       : "gemmkit: %s: the matrix scale must lie in [2^-100, 2^100]",
                        name);
+    if (int rc = api_check_aligned(q->offsets, 4, "offsets")) return rc;
     if (q->rows == 0 || q->cols == 0) return GK_OK;
     if (!q->data || !q->scales) return api_err(GK_EINVAL, "gemmkit: %s: null data or scales", name);
     if ((reinterpret_cast<uintptr_t>(q->data) | reinterpret_cast<uintptr_t>(q->scales)) & 15)
@@ -1514,6 +1515,7 @@ int gk_quantize_fp4(gk_matref x, int x_type, ptrdiff_t x_gs, const gk_fp4_matrix
     if ((rc = api_check_view(x.len, x.rows, x.cols, x.rs, x.cs, "X"))) return rc;
     if (x.rows == 0 || x.cols == 0) return GK_OK;
     if (!x.data) return api_err(GK_EINVAL, "gemmkit: null X");
+    if ((rc = api_check_aligned(x.data, x_type == GK_F32 ? 4 : 2, "X"))) return rc;
     if (stacked) {
         const __int128 last = static_cast<__int128>(dst->groups - 1) * x_gs + 1 +
                               static_cast<__int128>(x.rows - 1) * x.rs +
@@ -1554,6 +1556,7 @@ int gk_dequantize_fp4(const gk_fp4_matrix* q, gk_matmut out, gk_stream_t stream)
         return api_err(GK_EINVAL, "gemmkit: C view aliases itself");
     if (out.rows == 0 || out.cols == 0) return GK_OK;
     if (!out.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    if ((rc = api_check_aligned(out.data, 4, "C"))) return rc;
     if (api_overlaps(out.data, out.len * 4, q->data, q->data_len) ||
         api_overlaps(out.data, out.len * 4, q->scales, q->scales_len))
         return api_err(GK_EINVAL, "gemmkit: C aliases the 4-bit matrix");
@@ -1639,6 +1642,7 @@ int gk_gemm_fp4(float alpha, const gk_fp4_matrix* a, const gk_fp4_matrix* b, flo
         return api_err(GK_EINVAL, "gemmkit: alpha times the matrix scales (%g) leaves f32", scaled);
     if (c.rows == 0 || c.cols == 0) return GK_OK;
     if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    if ((rc = api_check_aligned(c.data, out_type == GK_F32 ? 4 : 2, "C"))) return rc;
     if ((rc = api_check_device(nullptr))) return rc;
     Fp4GemmParams p;
     memset(&p, 0, sizeof(p));

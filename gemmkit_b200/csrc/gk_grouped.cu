@@ -1321,6 +1321,7 @@ int check_groups(size_t groups, const int32_t* offsets, size_t rows, int is_f16,
         return api_err(GK_EINVAL, "gemmkit: grouped products take 1 to %d groups (groups = %zu)",
                        MAX_GROUPS, groups);
     if (!offsets) return api_err(GK_EINVAL, "gemmkit: null offsets");
+    if (int rc = api_check_aligned(offsets, 4, "offsets")) return rc;
     if (rows > INT32_MAX / 2)
         return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
     if (out_type != GK_F32 && out_type != (is_f16 ? GK_F16 : GK_BF16))
@@ -1390,6 +1391,9 @@ int gk_gemm_half_grouped(int is_f16, size_t groups, const int32_t* offsets, floa
     if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
     const bool zero = a.cols == 0 || alpha == 0.0f;
     if (!zero && (!a.data || !b.data)) return api_err(GK_EINVAL, "gemmkit: null A or B");
+    if ((rc = api_check_aligned(a.data, 2, "A")) || (rc = api_check_aligned(b.data, 2, "B")) ||
+        (rc = api_check_aligned(c.data, so, "C")))
+        return rc;
     GroupedParams p;
     memset(&p, 0, sizeof(p));
     p.P = GOperand{static_cast<const uint16_t*>(b.data), b.cs, b.rs, b_gs};
@@ -1436,6 +1440,9 @@ int gk_gemm_half_grouped_wgrad(int is_f16, size_t groups, const int32_t* offsets
     if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
     const bool zero = a.rows == 0 || alpha == 0.0f;
     if (!zero && (!a.data || !b.data)) return api_err(GK_EINVAL, "gemmkit: null A or B");
+    if ((rc = api_check_aligned(a.data, 2, "A")) || (rc = api_check_aligned(b.data, 2, "B")) ||
+        (rc = api_check_aligned(c.data, so, "C")))
+        return rc;
     GroupedParams p;
     memset(&p, 0, sizeof(p));
     p.P = GOperand{static_cast<const uint16_t*>(b.data), b.cs, b.rs, 0};

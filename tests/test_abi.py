@@ -547,6 +547,49 @@ def test_fp4_matrix_offsets_must_match_its_groups():
     fp4(4, 8, groups=2, offsets=(4096, 3))
 
 
+def test_grouped_and_fp4_addresses_must_be_aligned():
+    """An address (of a (pointer, length) pair) that is no multiple of its elements' size would fault
+    on the device."""
+    lib = _lib.load()
+    off, par = 4096, gk.SERIAL.c()
+
+    def fwd(a=1 << 12, b=1 << 14, c=1 << 16, offsets=off, out=0):
+        return lib.gk_gemm_half_grouped(
+            0, 2, C.c_void_p(offsets), 1.0, gk.MatRef.new((a, 12), 4, 3, 3, 1).c(),
+            gk.MatRef.new((b, 30), 3, 5, 5, 1).c(), 15, 0.0, gk.MatMut.new((c, 20), 4, 5, 5, 1).c(), out,
+            par, None)
+
+    def wgrad(a=1 << 12, b=1 << 14, c=1 << 16, offsets=off, out=0):
+        return lib.gk_gemm_half_grouped_wgrad(
+            0, 2, C.c_void_p(offsets), 1.0, gk.MatRef.new((a, 12), 4, 3, 3, 1).c(),
+            gk.MatRef.new((b, 20), 4, 5, 5, 1).c(), 0.0, gk.MatMut.new((c, 30), 3, 5, 5, 1).c(), 15, out,
+            par, None)
+
+    def refused(rc, text):
+        assert rc == gk.GK_EINVAL and text in lib.gk_last_error().decode(), (rc, lib.gk_last_error())
+
+    for call in (fwd, wgrad):
+        refused(call(a=(1 << 12) + 1), "A is not aligned to its elements of 2 bytes")
+        refused(call(b=(1 << 14) + 3), "B is not aligned to its elements of 2 bytes")
+        refused(call(c=(1 << 16) + 2), "C is not aligned to its elements of 4 bytes")
+        refused(call(c=(1 << 16) + 1, out=2), "C is not aligned to its elements of 2 bytes")
+        refused(call(offsets=off + 2), "offsets is not aligned to its elements of 4 bytes")
+
+    q = fp4(4, 8)
+    for t, at, size in ((0, 66, 4), (1, 65, 2), (2, 67, 2)):
+        expect_err(lambda: gk.quantize_fp4(gk.MatRef.new((at, 32), 4, 8, 8, 1), gk.FP4_MX, out=q, x_type=t),
+                   f"X is not aligned to its elements of {size} bytes")
+    expect_err(lambda: gk.dequantize_fp4(q, gk.MatMut.new((66, 32), 4, 8, 8, 1)),
+               "C is not aligned to its elements of 4 bytes")
+    b = fp4(6, 8, at=1 << 22)
+    for t, at, size in ((0, 66, 4), (1, 65, 2), (2, 67, 2)):
+        expect_err(lambda: gk.gemm_fp4(1.0, q, b, 0.0, gk.MatMut.new((at, 24), 4, 6, 6, 1), c_type=t),
+                   f"C is not aligned to its elements of {size} bytes")
+    r = fp4(4, 8, groups=2, offsets=(4098, 3))
+    expect_err(lambda: gk.dequantize_fp4(r, gk.MatMut.new((64, 32), 4, 8, 8, 1)),
+               "offsets is not aligned to its elements of 4 bytes")
+
+
 def test_scratch_release_without_gpu():
     import torch
     if torch.cuda.is_available():
