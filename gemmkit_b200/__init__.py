@@ -691,10 +691,10 @@ class Fp4Matrix:
         allocated for torch's current stream or for `stream`."""
         off = None
         if offsets is not None:
-            _one_device("offsets", offsets)
             off, groups = _offsets(offsets)
         calls = _cuda or _cuda_calls()
         if calls is None:
+            _one_device("offsets", offsets)
             raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
         torch = calls[0]
         if fmt not in (FP4_MX, FP4_NV) or groups < 1 or rows < 0 or cols < 0:
@@ -708,8 +708,10 @@ class Fp4Matrix:
         else:  # not what the current stream may still be writing
             with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
                 buf = torch.empty(nd + ns, dtype=torch.uint8, device=device)
+        if offsets is not None:
+            _one_device("the matrix", buf, "offsets", offsets)
         q = Fp4Matrix.__new__(Fp4Matrix)
-        q._where = _one_device("the matrix", buf, "offsets", offsets)
+        q._where = buf
         q.rows, q.cols, q.fmt, q.scale = rows, cols, fmt, float(scale)
         q.groups, q.offsets, q._data, q._scales = groups, offsets, buf, None
         at = buf.data_ptr()
