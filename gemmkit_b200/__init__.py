@@ -28,7 +28,9 @@ __all__ = [
     "gemm_half_f32", "gemm_bf16_f32_unchecked", "gemm_f16_f32_unchecked",
     "gemm_half_f32_batched", "gemm_half_f32_fused", "gemm_i8_fused", "gemm_i8_fused_unchecked", "Activation", "quantize_f32_i8", "gemm_i8_noalloc_unchecked", "set_tile_n", "knob_names", "knob_get",
     "gemm_half_grouped", "gemm_half_grouped_wgrad", "scratch_release", "Fp4Matrix", "quantize_fp4", "dequantize_fp4",
-    "gemm_fp4", "FP4_MX", "FP4_NV", "knob_set", "device_status", "selftest_wait_timeout",
+    "gemm_fp4", "gemm_half_epilogue", "gemm_half_dact", "act_backward", "Act8Matrix",
+    "quantize_act8", "dequantize_act8", "gemm_act8_wgrad", "MoeBalance", "moe_balance",
+    "moe_balance_backward", "FP4_MX", "FP4_NV", "knob_set", "device_status", "selftest_wait_timeout",
 ]
 
 
@@ -445,7 +447,9 @@ def gemm_half_f32(alpha: float, a: MatRef, b: MatRef, beta: float, c: MatMut, is
 
 
 class Activation:
-    """gemmkit::Activation (gemmkit/src/api.rs:63): ReLU or LeakyReLU(slope)."""
+    """gemmkit::Activation (gemmkit/src/api.rs:63): ReLU or LeakyReLU(slope); and, for the
+    feed-forward layers' entries (gemm_half_epilogue and the like) only, GELU, its tanh form and
+    SiLU."""
 
     def __init__(self, kind: int, slope: float = 0.0):
         self.kind, self.slope = kind, slope
@@ -457,6 +461,18 @@ class Activation:
     @staticmethod
     def LeakyRelu(slope: float) -> "Activation":
         return Activation(_lib.ACT_LEAKY_RELU, float(slope))
+
+    @staticmethod
+    def Gelu() -> "Activation":
+        return Activation(_lib.ACT_GELU)
+
+    @staticmethod
+    def GeluTanh() -> "Activation":
+        return Activation(_lib.ACT_GELU_TANH)
+
+    @staticmethod
+    def Silu() -> "Activation":
+        return Activation(_lib.ACT_SILU)
 
 
 def gemm_half_f32_fused(alpha: float, a: MatRef, b: MatRef, beta: float, c: MatMut, bias=None,
@@ -797,6 +813,337 @@ def gemm_fp4(alpha: float, a: Fp4Matrix, b: Fp4Matrix, beta: float, c: MatMut,
         c_type = _elem_type(c.data, -1)
     _check(_lib.load().gk_gemm_fp4(float(alpha), C.byref(a.c), C.byref(b.c), float(beta), c.c(),
                                    c_type, par.c(), _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+# ---- feed-forward layers, dense or by expert ---------------------------------------------------
+
+_NO_REF, _NO_MUT = MatRefC(), MatMutC()
+
+
+def _half_type(name: str, data, half: int, f32_too: bool = False) -> int:
+    t = _elem_type(data, half)
+    if t != half and not (f32_too and t == _lib.DT_F32):
+        raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold "
+                                      f"{'f16' if half == _lib.DT_F16 else 'bf16'} elements"
+                                      f"{' or f32' if f32_too else ''}")
+    return t
+
+
+def _groups_of(offsets):
+    """(pointer, groups) of optional offsets."""
+    if offsets is None:
+        return None, 1
+    ptr, groups = _offsets(offsets)
+    return ptr, max(groups, 0)
+
+
+def _vector(name, t, half, groups, n, gs):
+    """(pointer, length, group stride, type) of a bias or its gradient."""
+    if t is None:
+        return None, 0, 0, half
+    if not isinstance(t, tuple) and not t.is_contiguous():
+        raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must be contiguous")
+    return (*_flat(t), n if gs is None else int(gs), _half_type(name, t, half, True))
+
+
+def gemm_half_epilogue(alpha: float, a: MatRef, b: MatRef, c: MatMut, bias=None,
+                       act: Optional[Activation] = None, residual: Optional[MatRef] = None,
+                       z: Optional[MatMut] = None, offsets=None, b_gs: int = 0,
+                       bias_gs: Optional[int] = None, is_f16=False, par: Parallelism = SERIAL,
+                       stream=None, sync: bool = True) -> None:
+    """A feed-forward layer's product (extension): z = alpha*A*B + bias, C <- act(z) + residual, in
+    f32 on the accumulators and rounded once. A (rows x k) and B (k x n) hold bf16 (f16 with is_f16),
+    C f32 or their type; `residual` has C's type and may be C itself; `z`, where the activation's
+    input is kept for the backward pass, and `bias` (n elements; f32 allowed) the operands' type.
+    With `offsets` the rows form groups as in gemm_half_grouped, `b` views group 0's matrix in a
+    stack at stride b_gs, and group g's bias lies g * bias_gs (default n) elements on. Rows outside
+    the groups are left as they are."""
+    half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
+    rd, zd = residual and residual.data, z and z.data
+    _same_device("A", a.data, "B", b.data, "C", c.data, "offsets", offsets, "bias", bias,
+                 "residual", rd, "z", zd)
+    for name, d in (("A", a.data), ("B", b.data), ("z", zd)):
+        if d is not None:
+            _half_type(name, d, half)
+    out = _elem_type(c.data, half)
+    if rd is not None and _elem_type(rd, out) != out:
+        raise GemmkitError(GK_EINVAL, "gemmkit: the residual must have C's type")
+    ptr, groups = _groups_of(offsets)
+    epi = _lib.EpilogueC(act.kind if act else _lib.ACT_NONE, act.slope if act else 0.0,
+                         *_vector("bias", bias, half, groups, c.cols, bias_gs),
+                         residual.c() if residual else _NO_REF, z.c() if z else _NO_MUT)
+    _check(_lib.load().gk_gemm_half_epilogue(int(is_f16), groups, ptr, float(alpha), a.c(), b.c(),
+                                             int(b_gs), C.byref(epi), c.c(), out, par.c(),
+                                             _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+def _epilogue_bwd(z, act, dbias, dbias_gs, half, groups, n):
+    kind, slope = (act.kind, act.slope) if act else (_lib.ACT_NONE, 0.0)
+    z16, z8 = _NO_REF, None
+    if isinstance(z, Act8Matrix):
+        z8 = C.pointer(z.c)
+    elif z is not None:
+        _half_type("z", z.data, half)
+        z16 = z.c()
+    return _lib.EpilogueBwdC(kind, slope, z16, z8,
+                             *_vector("dbias", dbias, half, groups, n, dbias_gs))
+
+
+def _z_data(z):
+    return None if z is None else z._where if isinstance(z, Act8Matrix) else z.data
+
+
+def gemm_half_dact(alpha: float, a: MatRef, b: MatRef, z, act: Optional[Activation], c: MatMut,
+                   dbias=None, offsets=None, b_gs: int = 0, dbias_gs: Optional[int] = None,
+                   is_f16=False, par: Parallelism = SERIAL, stream=None, sync: bool = True) -> None:
+    """The gradient through such a layer's activation (extension): C <- alpha*A*B * act'(z), A the
+    gradient of the next layer's output, B its weights viewed transposed (k x n), `z` the activation's
+    input as a MatRef in the operands' type or an Act8Matrix (None with act None). `dbias` (n
+    elements a group, f32 or the operands' type) gets the sums of C over each group's rows. C may be
+    z itself. Offsets, groups and types as in gemm_half_epilogue."""
+    half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
+    _same_device("A", a.data, "B", b.data, "C", c.data, "offsets", offsets, "z", _z_data(z),
+                 "dbias", dbias)
+    for name, d in (("A", a.data), ("B", b.data)):
+        _half_type(name, d, half)
+    ptr, groups = _groups_of(offsets)
+    epi = _epilogue_bwd(z, act, dbias, dbias_gs, half, groups, c.cols)
+    _check(_lib.load().gk_gemm_half_dact(int(is_f16), groups, ptr, float(alpha), a.c(), b.c(),
+                                         int(b_gs), C.byref(epi), c.c(), _elem_type(c.data, half),
+                                         par.c(), _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+def act_backward(dy: MatRef, z, act: Optional[Activation], dz: Optional[MatMut], dbias=None,
+                 offsets=None, dbias_gs: Optional[int] = None, is_f16=False, stream=None,
+                 sync: bool = True) -> None:
+    """The same without a product (extension): dz <- dy * act'(z) and the sums of dz over each
+    group's rows in `dbias`; either may be None. dy holds bf16 (f16 with is_f16), dz f32 or that
+    type; dz may be dy or z itself."""
+    half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
+    dzd = dz and dz.data
+    _same_device("dY", dy.data, "dZ", dzd, "offsets", offsets, "z", _z_data(z), "dbias", dbias)
+    _half_type("dY", dy.data, half)
+    out = half if dzd is None else _elem_type(dzd, half)
+    ptr, groups = _groups_of(offsets)
+    epi = _epilogue_bwd(z, act, dbias, dbias_gs, half, groups, dy.cols)
+    _check(_lib.load().gk_act_backward(int(is_f16), groups, ptr, dy.c(), C.byref(epi),
+                                       dz.c() if dz else _NO_MUT, out, _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+class Act8Matrix:
+    """A rows x cols matrix of activations kept in 8 bits for the backward pass (extension; see
+    gk_act8_matrix in the C header): int8 codes with a power of two per 32 elements of a row. Made by
+    quantize_act8 or empty, or from tensors: `codes` int8, rows at a pitch that is a multiple of 32,
+    and `exponents` uint8, ceil(cols / 32) a row. A run of rows of a matrix is one too (`rows_of`)."""
+
+    def __init__(self, rows: int, cols: int, codes, exponents):
+        self.rows, self.cols = int(rows), int(cols)
+        nb = (self.cols + 31) // 32
+        for name, t, types, n in (("codes", codes, ("torch.int8",), self.cols),
+                                  ("exponents", exponents, ("torch.uint8",), nb)):
+            if str(t.dtype) not in types or t.dim() != 2 or tuple(t.shape) != (self.rows, n) or \
+                    (n > 1 and self.rows and t.stride(1) != 1):
+                raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must be {self.rows}x{n} "
+                                              f"{types[0][6:]} with contiguous rows")
+        self._where = _one_device("codes", codes, "exponents", exponents)
+        self._codes, self._exps = codes, exponents
+        lds = [t.stride(0) if self.rows > 1 else up
+               for t, up in ((codes, (self.cols + 31) // 32 * 32), (exponents, nb))]
+        # what lies behind the first element in its storage: the codes' last block may pass the row
+        ends = [t.untyped_storage().nbytes() - t.storage_offset() for t in (codes, exponents)]
+        self.c = _lib.Act8MatrixC(self.rows, self.cols, codes.data_ptr(),
+                                  min(ends[0], self.rows * lds[0]), lds[0], exponents.data_ptr(),
+                                  min(ends[1], self.rows * lds[1]), lds[1])
+
+    @property
+    def codes(self):
+        """The codes (rows x cols, int8)."""
+        return self._codes
+
+    @property
+    def exponents(self):
+        """The exponent bytes (rows x ceil(cols / 32), uint8): 127 is a largest magnitude in [1, 2)."""
+        return self._exps
+
+    @staticmethod
+    def empty(rows: int, cols: int, stream=None) -> "Act8Matrix":
+        """An unwritten matrix on the current device, its memory allocated for torch's current stream
+        or for `stream`."""
+        calls = _cuda or _cuda_calls()
+        if calls is None:
+            raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
+        if rows < 0 or cols < 0:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: no 8-bit matrix of {rows}x{cols}")
+        torch = calls[0]
+        device = torch.device("cuda", calls[1]())
+        nb = (cols + 31) // 32
+        pitch = (nb + 15) // 16 * 16  # of the exponents: whole 16-byte pieces, as the codes' rows
+        n = rows * nb * 32
+        if stream is None:
+            buf = torch.empty(n + rows * pitch, dtype=torch.uint8, device=device)
+        else:  # not what the current stream may still be writing
+            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
+                buf = torch.empty(n + rows * pitch, dtype=torch.uint8, device=device)
+        q = Act8Matrix.__new__(Act8Matrix)
+        q.rows, q.cols, q._where = rows, cols, buf
+        q._codes = buf[:n].view(torch.int8).view(rows, nb * 32)[:, :cols]
+        q._exps = buf[n:].view(rows, pitch)[:, :nb]
+        at = buf.data_ptr()
+        q.c = _lib.Act8MatrixC(rows, cols, at, n, nb * 32, at + n, rows * pitch, pitch)
+        return q
+
+    def rows_of(self, first: int, last: int) -> "Act8Matrix":
+        """Rows first .. last - 1, the same memory."""
+        if not 0 <= first <= last <= self.rows:
+            raise GemmkitError(GK_EINVAL, f"gemmkit: no rows {first} to {last} of {self.rows}")
+        q = Act8Matrix.__new__(Act8Matrix)
+        q.rows, q.cols, q._where = last - first, self.cols, self._where
+        q._codes, q._exps = self._codes[first:last], self._exps[first:last]
+        c = self.c
+        a, b = first * c.codes_ld, first * c.exps_ld
+        q.c = _lib.Act8MatrixC(q.rows, q.cols, (c.codes or 0) + a, max(0, c.codes_len - a), c.codes_ld,
+                               (c.exps or 0) + b, max(0, c.exps_len - b), c.exps_ld)
+        return q
+
+
+def quantize_act8(x: MatRef, out: Optional[Act8Matrix] = None, x_type: Optional[int] = None,
+                  stream=None, sync: bool = True) -> Act8Matrix:
+    """x (f32, f16 or bf16) in 8 bits (extension): per 32 consecutive elements of a row a power of two,
+    codes rounded half to even in [-127, 127]. `out` reuses a matrix of the same shape, otherwise the
+    result's memory is allocated for the call's stream; x_type names the element type of a (pointer,
+    length) pair."""
+    _same_device("X", x.data, "out", None if out is None else out._where)
+    if out is None:
+        out = Act8Matrix.empty(x.rows, x.cols, stream=stream)
+    if x_type is None:
+        x_type = _elem_type(x.data, -1)
+    _check(_lib.load().gk_quantize_act8(x.c(), x_type, C.byref(out.c), _stream(stream)))
+    if sync:
+        _sync(stream)
+    return out
+
+
+def dequantize_act8(q: Act8Matrix, out: MatMut, out_type: Optional[int] = None, stream=None,
+                    sync: bool = True) -> None:
+    """The values that an 8-bit matrix stands for, in f32, bf16 (both exact) or f16 (exact where the
+    source was f16)."""
+    _same_device("Q", q._where, "C", out.data)
+    if out_type is None:
+        out_type = _elem_type(out.data, -1)
+    _check(_lib.load().gk_dequantize_act8(C.byref(q.c), out.c(), out_type, _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+def gemm_act8_wgrad(alpha: float, a: Act8Matrix, b: MatRef, beta: float, c: MatMut, offsets=None,
+                    c_gs: int = 0, is_f16=False, par: Parallelism = SERIAL, stream=None,
+                    sync: bool = True) -> None:
+    """The weight gradient from a layer's input kept in 8 bits (extension): C[g] <- alpha*A_g^T*B_g +
+    beta*C[g], A (rows x m) an Act8Matrix, B (rows x n) in bf16 (f16 with is_f16), C f32 or B's
+    type; groups, offsets (None: all rows) and the stack of C as in gemm_half_grouped_wgrad."""
+    half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
+    _same_device("A", a._where, "B", b.data, "C", c.data, "offsets", offsets)
+    _half_type("B", b.data, half)
+    ptr, groups = _groups_of(offsets)
+    _check(_lib.load().gk_gemm_act8_wgrad(int(is_f16), groups, ptr, float(alpha), C.byref(a.c), b.c(),
+                                          float(beta), c.c(), int(c_gs), _elem_type(c.data, half),
+                                          par.c(), _stream(stream)))
+    if sync:
+        _sync(stream)
+
+
+# ---- the router's balance loss ------------------------------------------------------------------
+
+class MoeBalance:
+    """What moe_balance gives, device tensors: `loss` (f32, one), `counts` (int32, a router's experts),
+    `offsets` (int32, one more: the offsets of the products by expert), `rates` (f32, for
+    moe_balance_backward)."""
+
+    def __init__(self, loss, counts, offsets, rates):
+        self.loss, self.counts, self.offsets, self.rates = loss, counts, offsets, rates
+
+    @staticmethod
+    def empty(experts: int, stream=None) -> "MoeBalance":
+        """Unwritten results on the current device, allocated for torch's current stream or `stream`."""
+        calls = _cuda or _cuda_calls()
+        if calls is None:
+            raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
+        torch = calls[0]
+        device = torch.device("cuda", calls[1]())
+
+        def make():
+            return torch.empty(3 * experts + 2, dtype=torch.int32, device=device)
+        if stream is None:
+            buf = make()
+        else:
+            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
+                buf = make()
+        e = experts
+        return MoeBalance(buf[:1].view(torch.float32), buf[1:1 + e], buf[1 + e:2 + 2 * e],
+                          buf[2 + 2 * e:].view(torch.float32))
+
+
+def _ids(ids, tokens):
+    """(pointer, length, ids a token, 64-bit) of a tokens x top tensor."""
+    kinds = {"torch.int32": 0, "torch.int64": 1}
+    if str(ids.dtype) not in kinds or ids.dim() != 2 or ids.shape[0] != tokens or \
+            not ids.is_contiguous():
+        raise GemmkitError(GK_EINVAL, f"gemmkit: ids must be a contiguous {tokens} x top tensor of int32 "
+                                      "or int64")
+    return ids.data_ptr(), ids.numel(), ids.shape[1], kinds[str(ids.dtype)]
+
+
+def moe_balance(logits: MatRef, ids, coef: float = 1.0, out: Optional[MoeBalance] = None,
+                x_type: Optional[int] = None, stream=None, sync: bool = True) -> MoeBalance:
+    """A router's balance loss and the experts' counts and offsets (extension): `logits` (tokens x
+    experts, f32, f16 or bf16), `ids` (tokens x top, int32 or int64, contiguous) the experts that each
+    token goes to, a negative id for none; a token without any is padding. loss = coef * experts *
+    sum_e (counts_e / routed) * (mean of softmax(logits)_e over the live tokens)."""
+    o = out
+    _same_device("logits", logits.data, "ids", ids,
+                 *(() if o is None else ("loss", o.loss, "counts", o.counts, "offsets", o.offsets,
+                                         "rates", o.rates)))
+    i = _ids(ids, logits.rows)
+    if o is None:
+        o = MoeBalance.empty(logits.cols, stream=stream)
+    elif o.counts.numel() != logits.cols or o.offsets.numel() != logits.cols + 1 or \
+            o.rates.numel() != logits.cols:
+        raise GemmkitError(GK_EINVAL, f"gemmkit: the results are not of {logits.cols} experts")
+    if x_type is None:
+        x_type = _elem_type(logits.data, -1)
+    _check(_lib.load().gk_moe_balance(logits.c(), x_type, *i, float(coef), o.loss.data_ptr(),
+                                      o.counts.data_ptr(), o.offsets.data_ptr(), o.rates.data_ptr(),
+                                      _stream(stream)))
+    if sync:
+        _sync(stream)
+    return o
+
+
+def moe_balance_backward(logits: MatRef, ids, balance: MoeBalance, dloss, dlogits: MatMut,
+                         x_type: Optional[int] = None, stream=None, sync: bool = True) -> None:
+    """The loss's gradient by the logits (extension), times `dloss` (one f32 on the device); padding
+    gets zeros. dlogits has the logits' type and may be the logits themselves."""
+    _same_device("logits", logits.data, "ids", ids, "rates", balance.rates, "dloss", dloss, "dlogits",
+                 dlogits.data)
+    i = _ids(ids, logits.rows)
+    if balance.rates.numel() != logits.cols:
+        raise GemmkitError(GK_EINVAL, f"gemmkit: the results are not of {logits.cols} experts")
+    if str(dloss.dtype) != "torch.float32" or dloss.numel() != 1:
+        raise GemmkitError(GK_EINVAL, "gemmkit: dloss must be one f32")
+    if x_type is None:
+        x_type = _elem_type(logits.data, -1)
+    if _elem_type(dlogits.data, x_type) != x_type:
+        raise GemmkitError(GK_EINVAL, "gemmkit: dlogits must have the logits' type")
+    _check(_lib.load().gk_moe_balance_backward(logits.c(), x_type, *i, balance.rates.data_ptr(),
+                                               dloss.data_ptr(), dlogits.c(), _stream(stream)))
     if sync:
         _sync(stream)
 

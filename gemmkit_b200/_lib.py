@@ -12,7 +12,7 @@ from . import _build
 
 GK_OK, GK_EINVAL, GK_ENOMEM, GK_ECUDA, GK_ETIMEOUT, GK_ENODEV = range(6)
 AXIS_NONE, AXIS_ROW, AXIS_COL = 0, 1, 2
-ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_LEAKY_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(6)
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 FP4_MX, FP4_NV = 0, 1
 
@@ -50,6 +50,21 @@ class ProblemC(C.Structure):
 class Fp4MatrixC(C.Structure):
     _fields_ = [("fmt", i32), ("scale", f32), ("groups", sz), ("offsets", vp), ("rows", sz),
                 ("cols", sz), ("data", vp), ("data_len", sz), ("scales", vp), ("scales_len", sz)]
+
+
+class Act8MatrixC(C.Structure):
+    _fields_ = [("rows", sz), ("cols", sz), ("codes", vp), ("codes_len", sz), ("codes_ld", sz),
+                ("exps", vp), ("exps_len", sz), ("exps_ld", sz)]
+
+
+class EpilogueC(C.Structure):
+    _fields_ = [("act", i32), ("slope", f32), ("bias", vp), ("bias_len", sz), ("bias_gs", pd),
+                ("bias_type", i32), ("residual", MatRefC), ("z", MatMutC)]
+
+
+class EpilogueBwdC(C.Structure):
+    _fields_ = [("act", i32), ("slope", f32), ("z", MatRefC), ("z8", C.POINTER(Act8MatrixC)),
+                ("dbias", vp), ("dbias_len", sz), ("dbias_gs", pd), ("dbias_type", i32)]
 
 
 SIGNATURES = {
@@ -134,6 +149,18 @@ SIGNATURES = {
     "gk_fp4_import": (i32, [vp, sz, sz, vp, sz, sz, C.POINTER(Fp4MatrixC), vp]),
     "gk_gemm_fp4": (i32, [f32, C.POINTER(Fp4MatrixC), C.POINTER(Fp4MatrixC), f32, MatMutC, C.c_int,
                           Parallelism, vp]),
+    "gk_gemm_half_epilogue": (i32, [C.c_int, sz, vp, f32, MatRefC, MatRefC, pd,
+                                    C.POINTER(EpilogueC), MatMutC, C.c_int, Parallelism, vp]),
+    "gk_gemm_half_dact": (i32, [C.c_int, sz, vp, f32, MatRefC, MatRefC, pd,
+                                C.POINTER(EpilogueBwdC), MatMutC, C.c_int, Parallelism, vp]),
+    "gk_act_backward": (i32, [C.c_int, sz, vp, MatRefC, C.POINTER(EpilogueBwdC), MatMutC, C.c_int,
+                              vp]),
+    "gk_quantize_act8": (i32, [MatRefC, C.c_int, C.POINTER(Act8MatrixC), vp]),
+    "gk_dequantize_act8": (i32, [C.POINTER(Act8MatrixC), MatMutC, C.c_int, vp]),
+    "gk_gemm_act8_wgrad": (i32, [C.c_int, sz, vp, f32, C.POINTER(Act8MatrixC), MatRefC, f32,
+                                 MatMutC, pd, C.c_int, Parallelism, vp]),
+    "gk_moe_balance": (i32, [MatRefC, C.c_int, vp, sz, sz, C.c_int, f32, vp, vp, vp, vp, vp]),
+    "gk_moe_balance_backward": (i32, [MatRefC, C.c_int, vp, sz, sz, C.c_int, vp, vp, MatMutC, vp]),
     "gk_set_tile_n": (i32, [C.c_int]),
     "gk_knob_names": (C.c_char_p, []),
     "gk_knob_get": (i32, [C.c_char_p, C.POINTER(C.c_int64)]),

@@ -1,0 +1,360 @@
+// gk_act8.cu -- activations kept in 8 bits for the backward pass (gk_act8.cuh): quantisation, the values
+// back, and the weight gradient from them.
+//
+// A block of 32 elements of a row shares a power of two:
+//   e = floor(log2 max |x|), at least -127;  code = x 2^(6 - e), half to even, clamped to +-127
+// Powers of two keep both directions exact: x 2^(6 - e) has the digits of x, and a code times 2^(e - 6)
+// has at most 7, so bf16 and f32 hold every value, and f16 where the source was f16 (a block whose
+// unit lies below f16's 2^-24 holds multiples of that already). The backward pass therefore
+// multiplies what the checkpoint stands for, with no second rounding.
+//
+// Both kernels move each byte once and are bound by memory. A warp takes AU steps of 256 elements of a
+// row, eight consecutive ones a lane: 16-byte loads, the block's maximum over four lanes by two
+// shuffles, 8-byte stores.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "gemmkit_cuda.h"
+#include "gk_act8.cuh"
+#include "gk_engine.h"
+#include "gk_launch.h"
+#include "gk_sm100.cuh"
+#include "gk_store.cuh"
+
+namespace gk {
+
+namespace {
+
+constexpr int AU = 4;  // steps of a unit, all of their loads issued together
+
+template <typename T>
+struct Eight {  // eight elements as they lie in memory
+    uint32_t w[sizeof(T) * 2];
+    __device__ __forceinline__ void load(const T* x) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+            const uint4 v = ld_global_v4(reinterpret_cast<const uint8_t*>(x) + 16 * i);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    }
+    // element by element, zeros from n on
+    __device__ __forceinline__ void load(const T* x, int64_t cs, int n) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) w[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4)
+                    w[i] = __float_as_uint(x[i * cs]);
+                else
+                    w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(x)[i * cs])
+                                << (16 * (i & 1));
+            }
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (std::is_same_v<T, float>) {
+            return __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, __half>) {
+            return __half2float(__ushort_as_half(static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)))));
+        } else {
+            return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        }
+    }
+};
+
+struct Act8Out {
+    int8_t* codes;
+    uint8_t* exps;
+    int64_t codes_ld, exps_ld;
+    int64_t rows;
+    int32_t cols;
+};
+
+// vec: rows of x are contiguous and start on 16-byte boundaries.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    quantize_act8_kernel(const T* x, int64_t rs, int64_t cs, int vec, Act8Out q) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t chunks = (q.cols + AU * 256 - 1) / (AU * 256);
+    const int64_t units = q.rows * chunks, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+         u < units; u += step) {
+        const int64_t r = u / chunks;
+        const int c0 = static_cast<int>(u - r * chunks) * AU * 256 + lane * 8;
+        const T* src = x + r * rs;
+        Eight<T> raw[AU];
+#pragma unroll
+        for (int i = 0; i < AU; ++i) {
+            const int c = c0 + i * 256;
+            if (vec && c + 8 <= q.cols)
+                raw[i].load(src + c);
+            else
+                raw[i].load(src + c * cs, cs, q.cols - c);
+        }
+#pragma unroll
+        for (int i = 0; i < AU; ++i) {
+            const int c = c0 + i * 256;
+            if (c - lane * 8 >= q.cols) break;  // the whole warp
+            float v[8];
+            uint32_t m = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = raw[i].value(k);
+                m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+            }
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const uint32_t b = m >> 23;  // the biased exponent is e + 127; 255: an infinity or a NaN
+            // x 2^(6 - e), in two exact steps where 2^(6 - e) would not be a normal number
+            const float first = b < 64 ? 0x1p64f : 1.0f;
+            const float mul = __uint_as_float((b < 64 ? 196u - b : 260u - b) << 23);
+            uint32_t y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float s = fminf(fmaxf(v[k] * first * mul, -127.0f), 127.0f);
+                // 1.5 2^23 + s: rounded to an integer, half to even, its low byte the code
+                y[k] = b == 255 ? 0u : __float_as_uint(s + 12582912.0f);
+            }
+            uint32_t w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                w[h] = __byte_perm(__byte_perm(y[4 * h], y[4 * h + 1], 0x0040),
+                                   __byte_perm(y[4 * h + 2], y[4 * h + 3], 0x0040), 0x5410);
+            if (c < (q.cols + 31) / 32 * 32) {
+                *reinterpret_cast<uint2*>(q.codes + r * q.codes_ld + c) = make_uint2(w[0], w[1]);
+                if ((lane & 3) == 0) q.exps[r * q.exps_ld + (c >> 5)] = static_cast<uint8_t>(b);
+            }
+        }
+    }
+}
+
+// vec: rows of out are contiguous and start on 16-byte boundaries.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    dequantize_act8_kernel(Act8View q, int64_t rows, int32_t cols, T* out, int64_t rs, int64_t cs,
+                           int vec) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t chunks = (cols + AU * 256 - 1) / (AU * 256);
+    const int64_t units = rows * chunks, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+         u < units; u += step) {
+        const int64_t r = u / chunks;
+        const int c0 = static_cast<int>(u - r * chunks) * AU * 256 + lane * 8;
+        uint2 w[AU];
+        uint32_t b[AU];
+#pragma unroll
+        for (int i = 0; i < AU; ++i) {
+            const int c = c0 + i * 256;
+            w[i] = make_uint2(0u, 0u);
+            b[i] = 0u;
+            if (c < cols) {
+                w[i] = *reinterpret_cast<const uint2*>(q.codes + r * q.codes_ld + c);
+                b[i] = q.exps[r * q.exps_ld + (c >> 5)];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AU; ++i) {
+            const int c = c0 + i * 256, n = cols - c;
+            if (n <= 0) break;
+            const float unit = act8_unit(b[i]);
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = act8_code((k < 4 ? w[i].x : w[i].y) ^ 0x80808080u, k & 3) * unit;
+            T* o = out + r * rs + c * cs;
+            if (vec && n >= 8) {
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int h = 0; h < 8; h += 4)
+                        st_global_v4(o + h, __float_as_uint(v[h]), __float_as_uint(v[h + 1]),
+                                     __float_as_uint(v[h + 2]), __float_as_uint(v[h + 3]));
+                } else {
+                    constexpr int TYPE = std::is_same_v<T, __half> ? GK_F16 : GK_BF16;
+                    uint32_t p[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        p[h] = round_pair(__float_as_uint(v[2 * h]), __float_as_uint(v[2 * h + 1]), 1.0f,
+                                          TYPE);
+                    st_global_v4(o, p[0], p[1], p[2], p[3]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < n) to_out(o + k * cs, v[k]);
+            }
+        }
+    }
+}
+
+dim3 unit_grid(int64_t rows, int64_t cols) {
+    const int64_t blocks = (rows * ((cols + AU * 256 - 1) / (AU * 256)) + 7) / 8;
+    const int64_t most = static_cast<int64_t>(sm_count()) * 32;
+    return dim3(static_cast<unsigned>(blocks < most ? blocks : most));
+}
+
+bool whole_rows(const void* p, int64_t rows, int64_t rs, int64_t cs, size_t es) {
+    return cs == 1 && (rows <= 1 || rs * static_cast<int64_t>(es) % 16 == 0) &&
+           (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+template <typename T>
+int quantize(const gk_matref& x, const Act8Out& q, cudaStream_t st) {
+    return launch_overlapped(quantize_act8_kernel<T>, unit_grid(q.rows, q.cols), 256, st,
+                             static_cast<const T*>(x.data), static_cast<int64_t>(x.rs),
+                             static_cast<int64_t>(x.cs),
+                             whole_rows(x.data, q.rows, x.rs, x.cs, sizeof(T)) ? 1 : 0, q);
+}
+
+template <typename T>
+int dequantize(const gk_act8_matrix& q, void* out, int64_t rs, int64_t cs, cudaStream_t st) {
+    const Act8View v{q.codes, q.exps, static_cast<int64_t>(q.codes_ld), static_cast<int64_t>(q.exps_ld)};
+    const int64_t rows = static_cast<int64_t>(q.rows);
+    return launch_overlapped(dequantize_act8_kernel<T>, unit_grid(rows, static_cast<int64_t>(q.cols)), 256,
+                             st, v, rows, static_cast<int32_t>(q.cols), static_cast<T*>(out), rs, cs,
+                             whole_rows(out, rows, rs, cs, sizeof(T)) ? 1 : 0);
+}
+
+int check_type(int type) {
+    if (type != GK_F32 && type != GK_F16 && type != GK_BF16)
+        return api_err(GK_EINVAL, "gemmkit: unknown element type %d", type);
+    return GK_OK;
+}
+
+size_t view_bytes(size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs, size_t es) {
+    return rows && cols ? ((rows - 1) * rs + (cols - 1) * cs + 1) * es : 0;
+}
+
+}  // namespace
+
+int check_act8(const gk_act8_matrix* q, const char* name) {
+    if (!q) return api_err(GK_EINVAL, "gemmkit: null %s", name);
+    if (q->rows > INT32_MAX / 2 || q->cols > INT32_MAX / 2 || q->codes_ld > INT64_MAX / 4 ||
+        q->exps_ld > INT64_MAX / 4)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    if (q->rows == 0 || q->cols == 0) return GK_OK;
+    if (!q->codes || !q->exps) return api_err(GK_EINVAL, "gemmkit: null codes or exponents of %s", name);
+    const size_t blocks = (q->cols + ACT8_BLOCK - 1) / ACT8_BLOCK;
+    if (q->codes_ld % ACT8_BLOCK || q->codes_ld < q->cols)
+        return api_err(GK_EINVAL,
+                       "gemmkit: the pitch of %s's codes (%zu) must be a multiple of 32 that holds its "
+                       "%zu columns",
+                       name, q->codes_ld, q->cols);
+    if (q->rows > 1 && q->exps_ld < blocks)
+        return api_err(GK_EINVAL, "gemmkit: the pitch of %s's exponents (%zu) must hold %zu blocks", name,
+                       q->exps_ld, blocks);
+    if (reinterpret_cast<uintptr_t>(q->codes) & 15)
+        return api_err(GK_EINVAL, "gemmkit: the codes of %s must be 16-byte aligned", name);
+    const unsigned __int128 codes = static_cast<unsigned __int128>(q->rows - 1) * q->codes_ld + blocks * 32;
+    const unsigned __int128 exps = static_cast<unsigned __int128>(q->rows - 1) * q->exps_ld + blocks;
+    if (codes > q->codes_len || exps > q->exps_len)
+        return api_err(GK_EINVAL, "gemmkit: %s of %zux%zu needs %zu bytes of codes (has %zu) and %zu of "
+                       "exponents (has %zu)",
+                       name, q->rows, q->cols, static_cast<size_t>(codes), q->codes_len,
+                       static_cast<size_t>(exps), q->exps_len);
+    return GK_OK;
+}
+
+}  // namespace gk
+
+using namespace gk;
+
+extern "C" {
+
+int gk_quantize_act8(gk_matref x, int x_type, const gk_act8_matrix* dst, gk_stream_t stream) {
+    int rc = check_act8(dst, "the destination");
+    if (rc || (rc = check_type(x_type)) ||
+        (rc = api_check_view(x.len, x.rows, x.cols, x.rs, x.cs, "X")))
+        return rc;
+    if (x.rows != dst->rows || x.cols != dst->cols)
+        return api_err(GK_EINVAL, "gemmkit: the source is %zux%zu, the 8-bit matrix holds %zux%zu", x.rows,
+                       x.cols, dst->rows, dst->cols);
+    if (x.rows == 0 || x.cols == 0) return GK_OK;
+    if (!x.data) return api_err(GK_EINVAL, "gemmkit: null X");
+    const size_t es = x_type == GK_F32 ? 4 : 2;
+    if ((rc = api_check_aligned(x.data, es, "X"))) return rc;
+    const size_t bytes = view_bytes(x.rows, x.cols, x.rs, x.cs, es);
+    if (api_overlaps(x.data, bytes, dst->codes, dst->codes_len) ||
+        api_overlaps(x.data, bytes, dst->exps, dst->exps_len) ||
+        api_overlaps(dst->codes, dst->codes_len, dst->exps, dst->exps_len))
+        return api_err(GK_EINVAL, "gemmkit: the 8-bit matrix aliases its source or itself");
+    int dev = 0;
+    if ((rc = api_check_device(&dev))) return rc;
+    const Act8Out q{dst->codes, dst->exps, static_cast<int64_t>(dst->codes_ld),
+                    static_cast<int64_t>(dst->exps_ld), static_cast<int64_t>(dst->rows),
+                    static_cast<int32_t>(dst->cols)};
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return x_type == GK_F32   ? quantize<float>(x, q, st)
+           : x_type == GK_F16 ? quantize<__half>(x, q, st)
+                              : quantize<__nv_bfloat16>(x, q, st);
+}
+
+int gk_dequantize_act8(const gk_act8_matrix* q, gk_matmut out, int out_type, gk_stream_t stream) {
+    int rc = check_act8(q, "the source");
+    if (rc || (rc = check_type(out_type)) ||
+        (rc = api_check_view(out.len, out.rows, out.cols, out.rs, out.cs, "C")))
+        return rc;
+    if (out.rows != q->rows || out.cols != q->cols)
+        return api_err(GK_EINVAL, "gemmkit: the 8-bit matrix holds %zux%zu, the output is %zux%zu", q->rows,
+                       q->cols, out.rows, out.cols);
+    if (api_self_aliases(out.rows, out.cols, out.rs, out.cs))
+        return api_err(GK_EINVAL, "gemmkit: C view aliases itself");
+    if (out.rows == 0 || out.cols == 0) return GK_OK;
+    if (!out.data) return api_err(GK_EINVAL, "gemmkit: null C");
+    const size_t es = out_type == GK_F32 ? 4 : 2;
+    if ((rc = api_check_aligned(out.data, es, "C"))) return rc;
+    const size_t bytes = view_bytes(out.rows, out.cols, out.rs, out.cs, es);
+    if (api_overlaps(out.data, bytes, q->codes, q->codes_len) ||
+        api_overlaps(out.data, bytes, q->exps, q->exps_len))
+        return api_err(GK_EINVAL, "gemmkit: C aliases the 8-bit matrix");
+    int dev = 0;
+    if ((rc = api_check_device(&dev))) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return out_type == GK_F32   ? dequantize<float>(*q, out.data, out.rs, out.cs, st)
+           : out_type == GK_F16 ? dequantize<__half>(*q, out.data, out.rs, out.cs, st)
+                                : dequantize<__nv_bfloat16>(*q, out.data, out.rs, out.cs, st);
+}
+
+int gk_gemm_act8_wgrad(int is_f16, size_t groups, const int32_t* offsets, float alpha,
+                       const gk_act8_matrix* a, gk_matref b, float beta, gk_matmut c,
+                       ptrdiff_t c_gs, int out_type, gk_parallelism par, gk_stream_t stream) {
+    (void)par;
+    int rc = check_act8(a, "A");
+    if (rc) return rc;
+    // A's values, in memory that the call takes and gives back
+    const size_t ld = (a->cols + 7) / 8 * 8;
+    gk_matref av{nullptr, a->rows * ld, a->rows, a->cols, static_cast<ptrdiff_t>(ld), 1};
+    if ((rc = check_wgrad(is_f16, groups, offsets, true, alpha, av, b, c, c_gs, out_type))) return rc;
+    const size_t cb = view_bytes(c.rows, c.cols, c.rs, c.cs, out_type == GK_F32 ? 4 : 2) +
+                      (groups - 1) * c_gs * (out_type == GK_F32 ? 4 : 2);
+    if (c.data && (api_overlaps(c.data, cb, a->codes, a->codes_len) ||
+                   api_overlaps(c.data, cb, a->exps, a->exps_len)))
+        return api_err(GK_EINVAL, "gemmkit: C aliases A or B");
+    if (c.rows == 0 || c.cols == 0) return GK_OK;
+    int dev = 0;
+    if ((rc = api_check_device(&dev))) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    void* scratch = nullptr;
+    if (a->rows && alpha != 0.0f) {
+        if ((rc = scratch_alloc(&scratch, a->rows * ld * 2, st))) return rc;
+        rc = is_f16 ? dequantize<__half>(*a, scratch, static_cast<int64_t>(ld), 1, st)
+                    : dequantize<__nv_bfloat16>(*a, scratch, static_cast<int64_t>(ld), 1, st);
+        av.data = scratch;
+    }
+    // The product's lanes lie along C's columns; where C's rows are the contiguous side it is
+    // computed transposed.
+    if (!rc && c.rs == 1 && c.cs != 1) {
+        const gk_matmut ct{c.data, c.len, c.cols, c.rows, c.cs, c.rs};
+        rc = run_wgrad(is_f16, groups, offsets, alpha, b, av, beta, ct, c_gs, out_type, st);
+    } else if (!rc) {
+        rc = run_wgrad(is_f16, groups, offsets, alpha, av, b, beta, c, c_gs, out_type, st);
+    }
+    const int fr = scratch_free(scratch, st);
+    return rc ? rc : fr;
+}
+
+}  // extern "C"

@@ -1,0 +1,476 @@
+// gk_balance.cu -- a router's balance loss, the experts' counts and offsets, and the loss's gradient.
+//
+//   p_te = softmax of token t's logits;  P_e = mean of p_te over the live tokens;  f_e = counts_e / routed
+//   loss = coef E sum_e f_e P_e;   dloss/dlogit_te = rates_e-weighted:  p_te (rates_e - sum_j p_tj rates_j),
+//   rates_e = coef E f_e / live
+//
+// Bound by memory: the logits are read once in each direction. A warp takes a token, its logits in
+// registers (V consecutive ones a lane, J times), and in the forward pass adds its p to sums that stay
+// in registers over all of its tokens; counts are integers in shared memory. Each block leaves its sums
+// and counts, a last block adds them (one block does all of it where there are few tokens). No
+// floating atomics: which token a warp takes depends on the sizes alone, and so does every sum.
+// Differences of logits go through expf, sums over blocks through f64.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "gemmkit_cuda.h"
+#include "gk_engine.h"
+#include "gk_launch.h"
+#include "gk_sm100.cuh"
+#include "gk_store.cuh"
+
+namespace gk {
+
+namespace {
+
+constexpr int MAX_EXPERTS = 1024;
+constexpr int BW = 16;           // warps of a block
+constexpr int TOKENS_A_WARP = 4; // at least, before another block is added
+
+struct Router {
+    const void* x;
+    int64_t rs, cs;
+    int32_t type, ids64;
+    const void* ids;
+    int32_t top, tokens, experts;
+    unsigned int* status;
+};
+
+// A token's logits as they lie: lane l holds elements (32 j + l) V .. + V - 1.
+template <int V, int J>
+struct Logits {
+    uint32_t w[J * V];  // f32 bits, or 16-bit values two a word (V == 4), or one a word (V == 1)
+    __device__ __forceinline__ void load(const Router& p, int t, int lane) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int e = (32 * j + lane) * V;
+            if (e >= p.experts) continue;
+            const int64_t at = t * p.rs + e * p.cs;
+            if constexpr (V == 1) {
+                w[j] = p.type == GK_F32 ? static_cast<const uint32_t*>(p.x)[at]
+                                        : static_cast<const uint16_t*>(p.x)[at];
+            } else if (p.type == GK_F32) {
+                const uint4 v = ld_global_v4(static_cast<const float*>(p.x) + at);
+                w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.x) + at);
+                w[4 * j] = v.x, w[4 * j + 1] = v.y;
+            }
+        }
+    }
+    __device__ __forceinline__ float value(const Router& p, int j, int v) const {
+        if (p.type == GK_F32) return __uint_as_float(w[V * j + v]);
+        const uint32_t h = V == 1 ? w[j] : w[V * j + v / 2] >> (16 * (v & 1));
+        return p.type == GK_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xFFFFu)))
+                                : __uint_as_float(h << 16);
+    }
+    // The softmax; 0 everywhere where every logit is minus infinity.
+    __device__ __forceinline__ void softmax(const Router& p, int lane, float (&y)[J * V]) const {
+        float m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                y[V * j + v] = (32 * j + lane) * V < p.experts ? value(p, j, v) : -INFINITY;
+                m = fmaxf(m, y[V * j + v]);
+            }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const bool none = m == -INFINITY;
+        const float base = none ? 0.0f : m;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < J * V; ++i) {
+            y[i] = expf(y[i] - base);
+            s += y[i];
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        // (a row of NaN also has no maximum: its sum is NaN, and stays so)
+        const float inv = none && s == 0.0f ? 0.0f : 1.0f / s;
+#pragma unroll
+        for (int i = 0; i < J * V; ++i) y[i] *= inv;
+    }
+};
+
+// The warp's token's ids into `hist` (when there is one); whether it has any.
+__device__ __forceinline__ bool token_ids(const Router& p, int t, int* hist, int lane) {
+    bool any = false, bad = false;
+    for (int i = lane; i < p.top; i += 32) {
+        const int64_t at = static_cast<int64_t>(t) * p.top + i;
+        const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at]
+                                   : static_cast<const int32_t*>(p.ids)[at];
+        if (id >= 0 && id < p.experts) {
+            any = true;
+            if (hist) atomicAdd(&hist[id], 1);
+        } else if (id >= 0) {
+            bad = true;
+        }
+    }
+    if (hist && bad) atomicOr(p.status, GK_DEV_BAD_OFFSETS);
+    return __any_sync(0xffffffffu, any);
+}
+
+// What a block leaves: experts sums (f32), experts counts and the live tokens, at a pitch of `pitch` words.
+__host__ __device__ inline int part_pitch(int experts) { return 2 * experts + 1; }
+
+// The blocks' parts into the results. All threads of one block.
+__device__ __forceinline__ void finish(const uint32_t* part, int blocks, int experts, float coef,
+                                       float* loss, int32_t* counts, int32_t* offsets, float* rates) {
+    __shared__ double red[BW];
+    __shared__ int scan[BW];
+    __shared__ int live_all, routed_all;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int pitch = part_pitch(experts);
+    if (tid == 0) live_all = 0;
+    __syncthreads();
+    int live = 0;
+    for (int b = tid; b < blocks; b += blockDim.x)
+        live += static_cast<int>(part[static_cast<int64_t>(b) * pitch + 2 * experts]);
+    if (live) atomicAdd(&live_all, live);
+    // thread e and, where there are more experts than threads, e + blockDim.x
+    constexpr int PER = MAX_EXPERTS / (32 * BW);
+    double sum[PER];
+    int cnt[PER], carry = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = k * blockDim.x + tid;
+        double s = 0.0;
+        int c = 0;
+        if (e < experts) {
+#pragma unroll 8
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t* at = part + static_cast<int64_t>(b) * pitch;
+                s += static_cast<double>(__uint_as_float(at[e]));
+                c += static_cast<int>(at[experts + e]);
+            }
+        }
+        sum[k] = s;
+        cnt[k] = c;
+        // running sums of the counts
+        int inc = c;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += u;
+        }
+        if (lane == 31) scan[w] = inc;
+        __syncthreads();
+        int before = carry;
+        for (int i = 0; i < w; ++i) before += scan[i];
+        if (e < experts) {
+            counts[e] = c;
+            offsets[e + 1] = before + inc;
+        }
+        for (int i = 0; i < BW; ++i) carry += scan[i];
+        __syncthreads();
+    }
+    if (tid == 0) {
+        offsets[0] = 0;
+        routed_all = carry;
+    }
+    __syncthreads();
+    const int tokens = live_all, routed = routed_all;
+    double a = 0.0;
+    const double unit = routed > 0 ? static_cast<double>(coef) * experts / routed / tokens : 0.0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = k * blockDim.x + tid;
+        if (e < experts) {
+            rates[e] = static_cast<float>(unit * cnt[k]);
+            if (routed > 0) a += unit * cnt[k] * sum[k];
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+    if (lane == 0) red[w] = a;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < BW; ++i) a += red[i];
+        *loss = static_cast<float>(a);
+    }
+}
+
+struct BalanceOut {
+    float coef;
+    float* loss;
+    int32_t* counts;
+    int32_t* offsets;
+    float* rates;
+};
+
+template <int V, int J>
+__global__ void __launch_bounds__(32 * BW)
+    balance_kernel(const Router p, uint32_t* part, const BalanceOut o) {
+    extern __shared__ float smem[];  // BW x experts sums, then the block's part
+    uint32_t* own = reinterpret_cast<uint32_t*>(smem + BW * p.experts);
+    int* hist = reinterpret_cast<int*>(own + p.experts);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i <= p.experts; i += blockDim.x) hist[i] = 0;  // counts, live tokens
+    griddep_wait();
+    griddep_launch_dependents();
+    __syncthreads();
+    float sum[J * V];
+#pragma unroll
+    for (int i = 0; i < J * V; ++i) sum[i] = 0.0f;
+    int live = 0;
+    const int step = gridDim.x * BW;
+    for (int64_t t0 = blockIdx.x * BW + w; t0 < p.tokens; t0 += 2 * step) {
+        Logits<V, J> x[2];
+        x[0].load(p, static_cast<int>(t0), lane);
+        const bool two = t0 + step < p.tokens;
+        if (two) x[1].load(p, static_cast<int>(t0 + step), lane);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (k == 1 && !two) break;
+            if (!token_ids(p, static_cast<int>(t0 + k * step), hist, lane)) continue;
+            ++live;
+            float y[J * V];
+            x[k].softmax(p, lane, y);
+#pragma unroll
+            for (int i = 0; i < J * V; ++i) sum[i] += y[i];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = (32 * j + lane) * V + v;
+            if (e < p.experts) smem[w * p.experts + e] = sum[V * j + v];
+        }
+    if (lane == 0 && live) atomicAdd(&hist[p.experts], live);
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
+        float a = smem[e];
+#pragma unroll
+        for (int i = 1; i < BW; ++i) a += smem[i * p.experts + e];
+        own[e] = __float_as_uint(a);
+    }
+    __syncthreads();
+    if (gridDim.x == 1) {
+        finish(own, 1, p.experts, o.coef, o.loss, o.counts, o.offsets, o.rates);
+    } else {
+        const int pitch = part_pitch(p.experts);
+        for (int i = threadIdx.x; i < pitch; i += blockDim.x)
+            part[static_cast<int64_t>(blockIdx.x) * pitch + i] = own[i];
+    }
+}
+
+__global__ void __launch_bounds__(32 * BW)
+    balance_finish_kernel(const uint32_t* part, int blocks, int experts, const BalanceOut o) {
+    griddep_wait();
+    griddep_launch_dependents();
+    finish(part, blocks, experts, o.coef, o.loss, o.counts, o.offsets, o.rates);
+}
+
+template <int V, int J>
+__global__ void __launch_bounds__(256)
+    balance_backward_kernel(const Router p, const float* rates, const float* dloss, void* dx,
+                            int64_t ds, int64_t dc) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    float rate[J * V];
+    const float scale = *dloss;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = (32 * j + lane) * V + v;
+            rate[V * j + v] = e < p.experts ? rates[e] : 0.0f;
+        }
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * warps + w; t < p.tokens; t += step) {
+        Logits<V, J> x;
+        x.load(p, static_cast<int>(t), lane);
+        float y[J * V];
+        if (token_ids(p, static_cast<int>(t), nullptr, lane)) {
+            x.softmax(p, lane, y);
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < J * V; ++i) dot = fmaf(y[i], rate[i], dot);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+#pragma unroll
+            for (int i = 0; i < J * V; ++i) y[i] = scale * y[i] * (rate[i] - dot);
+        } else {
+#pragma unroll
+            for (int i = 0; i < J * V; ++i) y[i] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int e = (32 * j + lane) * V;
+            if (e >= p.experts) continue;
+            const int64_t at = t * ds + e * dc;
+            if constexpr (V == 1) {
+                if (p.type == GK_F32)
+                    to_out(static_cast<float*>(dx) + at, y[j]);
+                else if (p.type == GK_F16)
+                    to_out(static_cast<__half*>(dx) + at, y[j]);
+                else
+                    to_out(static_cast<__nv_bfloat16*>(dx) + at, y[j]);
+            } else {
+                uint32_t b[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) b[v] = __float_as_uint(y[4 * j + v]);
+                if (p.type == GK_F32)
+                    st_global_v4(static_cast<float*>(dx) + at, b[0], b[1], b[2], b[3]);
+                else
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dx) + at) =
+                        make_uint2(round_pair(b[0], b[1], 1.0f, p.type),
+                                   round_pair(b[2], b[3], 1.0f, p.type));
+            }
+        }
+    }
+}
+
+// f(V, J) as constants: V = 4 where a row's logits are whole 4-element pieces, J the smallest of those
+// compiled that holds the experts (up to 8 in pieces, 32 otherwise).
+template <typename F>
+int with_layout(bool vec, int experts, F f) {
+    auto c = [](auto v) { return v; };
+    using std::integral_constant;
+    if (vec) {
+        if (experts <= 128) return f(c(integral_constant<int, 4>{}), c(integral_constant<int, 1>{}));
+        if (experts <= 256) return f(c(integral_constant<int, 4>{}), c(integral_constant<int, 2>{}));
+        return f(c(integral_constant<int, 4>{}), c(integral_constant<int, 8>{}));
+    }
+    if (experts <= 32) return f(c(integral_constant<int, 1>{}), c(integral_constant<int, 1>{}));
+    if (experts <= 256) return f(c(integral_constant<int, 1>{}), c(integral_constant<int, 8>{}));
+    return f(c(integral_constant<int, 1>{}), c(integral_constant<int, 32>{}));
+}
+
+bool in_fours(const void* p, int64_t rows, int64_t cols, int64_t rs, int64_t cs, size_t es) {
+    return cs == 1 && cols % 4 == 0 && (rows <= 1 || rs % 4 == 0) &&
+           reinterpret_cast<uintptr_t>(p) % (4 * es) == 0;
+}
+
+size_t view_bytes(size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs, size_t es) {
+    return rows && cols ? ((rows - 1) * rs + (cols - 1) * cs + 1) * es : 0;
+}
+
+int check_router(const gk_matref& x, int x_type, const void* ids, size_t ids_len, size_t top, int ids64,
+                 Router* p) {
+    if (x_type != GK_F32 && x_type != GK_F16 && x_type != GK_BF16)
+        return api_err(GK_EINVAL, "gemmkit: unknown element type %d", x_type);
+    int rc = api_check_view(x.len, x.rows, x.cols, x.rs, x.cs, "logits");
+    if (rc) return rc;
+    if (x.cols < 1 || x.cols > MAX_EXPERTS)
+        return api_err(GK_EINVAL, "gemmkit: a router has 1 to %d experts (has %zu)", MAX_EXPERTS, x.cols);
+    if (top < 1 || top > INT32_MAX / 2 || x.rows > INT32_MAX / 2 || x.rows * top > INT32_MAX)
+        return api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
+    if (ids_len < x.rows * top)
+        return api_err(GK_EINVAL, "gemmkit: %zu tokens with %zu experts each need as many ids (has %zu)",
+                       x.rows, top, ids_len);
+    if (x.rows && (!x.data || !ids)) return api_err(GK_EINVAL, "gemmkit: null logits or ids");
+    if ((rc = api_check_aligned(x.data, x_type == GK_F32 ? 4 : 2, "logits")) ||
+        (rc = api_check_aligned(ids, ids64 ? 8 : 4, "ids")))
+        return rc;
+    *p = Router{x.data, x.rs, x.cs, x_type, ids64 != 0, ids, static_cast<int32_t>(top),
+                static_cast<int32_t>(x.rows), static_cast<int32_t>(x.cols), nullptr};
+    return GK_OK;
+}
+
+}  // namespace
+
+}  // namespace gk
+
+using namespace gk;
+
+extern "C" {
+
+int gk_moe_balance(gk_matref logits, int x_type, const void* ids, size_t ids_len, size_t top, int ids64,
+                   float coef, float* loss, int32_t* counts, int32_t* offsets, float* rates,
+                   gk_stream_t stream) {
+    Router p;
+    int rc = check_router(logits, x_type, ids, ids_len, top, ids64, &p);
+    if (rc) return rc;
+    if (!loss || !counts || !offsets || !rates) return api_err(GK_EINVAL, "gemmkit: null output");
+    if ((rc = api_check_aligned(loss, 4, "loss")) || (rc = api_check_aligned(counts, 4, "counts")) ||
+        (rc = api_check_aligned(offsets, 4, "offsets")) || (rc = api_check_aligned(rates, 4, "rates")))
+        return rc;
+    const size_t es = x_type == GK_F32 ? 4 : 2, n = logits.cols;
+    const struct {
+        const void* p;
+        size_t bytes;
+    } all[6] = {{loss, 4},  {counts, 4 * n}, {offsets, 4 * (n + 1)},
+                {rates, 4 * n},
+                {logits.data, view_bytes(logits.rows, n, logits.rs, logits.cs, es)},
+                {ids, logits.rows * top * (ids64 ? 8 : 4)}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < 6; ++j)
+            if (all[j].p && all[j].bytes && api_overlaps(all[i].p, all[i].bytes, all[j].p, all[j].bytes))
+                return api_err(GK_EINVAL, "gemmkit: the outputs alias each other or the inputs");
+    int dev = 0;
+    if ((rc = api_check_device(&dev))) return rc;
+    p.status = device_status_ptr();
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t want = (static_cast<int64_t>(p.tokens) + BW * TOKENS_A_WARP - 1) / (BW * TOKENS_A_WARP);
+    const int blocks = static_cast<int>(want < 1 ? 1 : want < sm_count() ? want : sm_count());
+    const BalanceOut o{coef, loss, counts, offsets, rates};
+    void* part = nullptr;
+    if (blocks > 1 &&
+        (rc = scratch_alloc(&part, static_cast<size_t>(blocks) * part_pitch(p.experts) * 4, st)))
+        return rc;
+    const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es);
+    rc = with_layout(vec, p.experts, [&](auto v, auto j) {
+        auto kern = balance_kernel<decltype(v)::value, decltype(j)::value>;
+        const int smem = ((BW + 2) * p.experts + 1) * 4;
+        static std::atomic<uint64_t> done{0};
+        const cudaError_t e = allow_smem(kern, ((BW + 2) * MAX_EXPERTS + 1) * 4, done);
+        if (e != cudaSuccess)
+            return api_err(GK_ECUDA, "gemmkit: kernel launch failed: %s", cudaGetErrorString(e));
+        return launch_overlapped_smem(kern, dim3(static_cast<unsigned>(blocks)), 32 * BW, smem, st, p,
+                                      static_cast<uint32_t*>(part), o);
+    });
+    if (!rc && blocks > 1)
+        rc = launch_overlapped(balance_finish_kernel, dim3(1), 32 * BW, st,
+                               static_cast<const uint32_t*>(part), blocks, p.experts, o);
+    const int fr = scratch_free(part, st);
+    return rc ? rc : fr;
+}
+
+int gk_moe_balance_backward(gk_matref logits, int x_type, const void* ids, size_t ids_len, size_t top,
+                            int ids64, const float* rates, const float* dloss, gk_matmut dlogits,
+                            gk_stream_t stream) {
+    Router p;
+    int rc = check_router(logits, x_type, ids, ids_len, top, ids64, &p);
+    if (rc) return rc;
+    if (dlogits.rows != logits.rows || dlogits.cols != logits.cols)
+        return api_err(GK_EINVAL, "gemmkit: the gradient is %zux%zu, the logits are %zux%zu", dlogits.rows,
+                       dlogits.cols, logits.rows, logits.cols);
+    if ((rc = api_check_view(dlogits.len, dlogits.rows, dlogits.cols, dlogits.rs, dlogits.cs, "dlogits")))
+        return rc;
+    if (api_self_aliases(dlogits.rows, dlogits.cols, dlogits.rs, dlogits.cs))
+        return api_err(GK_EINVAL, "gemmkit: dlogits view aliases itself");
+    if (!rates || !dloss) return api_err(GK_EINVAL, "gemmkit: null rates or dloss");
+    if (p.tokens == 0) return GK_OK;
+    if (!dlogits.data) return api_err(GK_EINVAL, "gemmkit: null dlogits");
+    const size_t es = x_type == GK_F32 ? 4 : 2, n = logits.cols;
+    if ((rc = api_check_aligned(dlogits.data, es, "dlogits")) ||
+        (rc = api_check_aligned(rates, 4, "rates")) || (rc = api_check_aligned(dloss, 4, "dloss")))
+        return rc;
+    const size_t db = view_bytes(dlogits.rows, n, dlogits.rs, dlogits.cs, es);
+    const bool same = dlogits.data == logits.data && (p.tokens <= 1 || dlogits.rs == logits.rs) &&
+                      (n <= 1 || dlogits.cs == logits.cs);
+    if ((!same && api_overlaps(dlogits.data, db, logits.data,
+                               view_bytes(logits.rows, n, logits.rs, logits.cs, es))) ||
+        api_overlaps(dlogits.data, db, ids, logits.rows * top * (ids64 ? 8 : 4)) ||
+        api_overlaps(dlogits.data, db, rates, 4 * n) || api_overlaps(dlogits.data, db, dloss, 4))
+        return api_err(GK_EINVAL, "gemmkit: dlogits alias another operand");
+    int dev = 0;
+    if ((rc = api_check_device(&dev))) return rc;
+    p.status = device_status_ptr();
+    const int64_t want = (static_cast<int64_t>(p.tokens) + 7) / 8, most = 8ll * sm_count();
+    const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es) &&
+                     in_fours(dlogits.data, p.tokens, p.experts, dlogits.rs, dlogits.cs, es);
+    return with_layout(vec, p.experts, [&](auto v, auto j) {
+        return launch_overlapped(balance_backward_kernel<decltype(v)::value, decltype(j)::value>,
+                                 dim3(static_cast<unsigned>(want < most ? want : most)), 256,
+                                 static_cast<cudaStream_t>(stream), p, rates, dloss, dlogits.data,
+                                 static_cast<int64_t>(dlogits.rs), static_cast<int64_t>(dlogits.cs));
+    });
+}
+
+}  // extern "C"

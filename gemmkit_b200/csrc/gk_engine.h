@@ -219,6 +219,19 @@ int launch_quantize_rows(const float* x, int64_t rsx, int64_t csx, int64_t rows,
                          int8_t* q, int64_t rsq, int64_t csq, float scale, int32_t zp,
                          float* scales, cudaStream_t s);
 
+// Stream-ordered scratch from the engine's pool on the current device (gk_grouped.cu); in a capture it
+// is the graph's own. A freed nullptr is nothing.
+int scratch_alloc(void** scratch, size_t bytes, cudaStream_t st);
+int scratch_free(void* scratch, cudaStream_t st);
+
+// The weight gradient of rows grouped by expert (gk_grouped.cu), for entries that have one of its
+// operands in another form.
+int check_wgrad(int is_f16, size_t groups, const int32_t* offsets, bool held, float alpha,
+                const gk_matref& a, const gk_matref& b, const gk_matmut& c, ptrdiff_t c_gs, int out_type);
+int run_wgrad(int is_f16, size_t groups, const int32_t* offsets, float alpha, const gk_matref& a,
+              const gk_matref& b, float beta, const gk_matmut& c, ptrdiff_t c_gs, int out_type,
+              cudaStream_t stream);
+
 // Allows `kern` its dynamic shared memory on the current device, once per device (`done` holds a
 // bit per device and belongs to the kernel).
 template <typename K>
@@ -253,6 +266,8 @@ int api_validate_gemm_views(const gk_matref& a, const gk_matref& b, const gk_mat
 bool api_self_aliases(size_t rows, size_t cols, ptrdiff_t rs, ptrdiff_t cs);
 bool api_overlaps(const void* pa, size_t bytes_a, const void* pb, size_t bytes_b);
 int api_pdl_enabled();
+// A matrix in 8 bits: its shape, lengths and alignment (gk_act8.cu).
+int check_act8(const gk_act8_matrix* q, const char* name);
 // Refuses an address that is no multiple of its elements' size.
 int api_check_aligned(const void* p, size_t size, const char* name);
 

@@ -1,0 +1,329 @@
+// gk_epilogue.cuh -- the epilogues of a feed-forward layer's products, on the accumulators of the
+// grouped kernels (gk_grouped.cuh).
+//
+//   forward    z = alpha acc + bias;  C = act(z) + R, and z itself on demand
+//   backward   C = alpha acc * act'(z);  the sums of C over a group's rows on demand
+//
+// All of it in f32 on the accumulators as they are, rounded once where it is stored. The backward
+// pass takes z from a 16-bit matrix or from a checkpoint in 8 bits (gk_act8.cuh).
+//
+// A lane holds one P row (a column of C) and consecutive Q rows (rows of C), so a bias is one value
+// a lane and a column sum one register. 16-bit matrices with unit column stride move in pairs: of
+// two neighbouring lanes the even one reads and writes four bytes of the even Q rows, the odd one of
+// the odd ones (store_pairs), half as many instructions as element by element; the halves are
+// exchanged by one shuffle for four elements. The same lane reads an element of R (or z) and
+// later stores that of C, so C may be R (or z) itself.
+#pragma once
+
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "gemmkit_cuda.h"
+#include "gk_act8.cuh"
+#include "gk_sm100.cuh"
+#include "gk_store.cuh"
+
+namespace gk {
+
+enum : int { EPI_STORE = 0, EPI_FWD = 1, EPI_BWD = 2 };
+
+struct EpiArgs {
+    int32_t act;              // gk_act
+    float slope;              // LeakyReLU's
+    const void* bias;         // forward; nullptr: none
+    int64_t bias_gs;          // elements from one group's bias to the next's
+    int32_t bias_type;        // gk_dtype of the bias (forward) or of the sums (backward)
+    int32_t pairs;            // every 16-bit matrix of the epilogue moves in pairs (see above)
+    const void* side;         // forward: R, of C's type; backward: z, of the operands' type
+    int64_t sq, sp;           // its strides along the Q side (rows) and the P side (columns)
+    uint16_t* z;              // forward: where z is kept, of the operands' type; nullptr: nowhere
+    int64_t zq, zp;
+    Act8View z8;              // backward: z as a checkpoint (codes != nullptr)
+    void* dbias;              // backward: sums over the rows of each group; nullptr: none
+    int64_t dbias_gs;
+    float* part;              // backward: the tiles' sums
+};
+
+// ---- activations ------------------------------------------------------------------------------------
+//
+// ReLU and LeakyReLU as in the engine's other epilogues (fused_apply: a NaN becomes 0). GELU and SiLU
+// keep a NaN; an argument below -100 counts as -100 (the value is -0 from far above that on in f32),
+// so that minus infinity gives the limit 0 instead of inf * 0.
+//   GELU is z Phi(z), Phi(z) = (1 + erf(z / sqrt 2)) / 2; its tanh form is z sigma(2 u), u = sqrt(2 / pi)
+// (z + 0.044715 z^3), since (1 + tanh u) / 2 = sigma(2 u); SiLU is z sigma(z). sigma(t) = 1 / (1 +
+// exp(-t)) by the fast exponential and division: about 2^-21 + |t| 2^-24 off relative to it, at most a
+// thousandth of a 16-bit rounding wherever the result is not below 2^-100.
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float sigmoid(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
+
+constexpr float SQRT_HALF = 0.70710678f, SQRT_2_PI = 0.79788456f, RSQRT_2PI = 0.39894228f;
+constexpr float GELU_C = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z, float slope) {
+    if constexpr (ACT == GK_ACT_RELU) {
+        return z > 0.0f ? z : 0.0f;
+    } else if constexpr (ACT == GK_ACT_LEAKY_RELU) {
+        return fmaf(slope, z < 0.0f ? z : 0.0f, z > 0.0f ? z : 0.0f);
+    } else if constexpr (ACT == GK_ACT_GELU) {
+        z = max_nan(z, -100.0f);
+        const float h = 0.5f * z;
+        return fmaf(h, erff(z * SQRT_HALF), h);
+    } else if constexpr (ACT == GK_ACT_GELU_TANH) {
+        z = max_nan(z, -100.0f);
+        return z * sigmoid(2.0f * SQRT_2_PI * fmaf(GELU_C * z * z, z, z));
+    } else if constexpr (ACT == GK_ACT_SILU) {
+        z = max_nan(z, -100.0f);
+        return z * sigmoid(z);
+    } else {
+        return z;
+    }
+}
+
+// The derivative. GELU and SiLU take arguments beyond +-100 as +-100 (the limits 0 and 1).
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z, float slope) {
+    if constexpr (ACT == GK_ACT_RELU) {
+        return z > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == GK_ACT_LEAKY_RELU) {
+        return z > 0.0f ? 1.0f : slope;
+    } else if constexpr (ACT == GK_ACT_GELU) {
+        z = min_nan(max_nan(z, -100.0f), 100.0f);
+        return fmaf(z * RSQRT_2PI, __expf(-0.5f * z * z), fmaf(0.5f, erff(z * SQRT_HALF), 0.5f));
+    } else if constexpr (ACT == GK_ACT_GELU_TANH) {
+        z = min_nan(max_nan(z, -100.0f), 100.0f);
+        const float z2 = z * z;
+        const float s = sigmoid(2.0f * SQRT_2_PI * fmaf(GELU_C * z2, z, z));
+        return fmaf(z * s * (1.0f - s), 2.0f * SQRT_2_PI * fmaf(3.0f * GELU_C, z2, 1.0f), s);
+    } else if constexpr (ACT == GK_ACT_SILU) {
+        z = min_nan(max_nan(z, -100.0f), 100.0f);
+        const float s = sigmoid(z);
+        return fmaf(z * s, 1.0f - s, s);
+    } else {
+        return 1.0f;
+    }
+}
+
+// f(the activation as a constant), compiled for each of them.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+    switch (act) {
+        case GK_ACT_RELU: f(std::integral_constant<int, GK_ACT_RELU>{}); break;
+        case GK_ACT_LEAKY_RELU: f(std::integral_constant<int, GK_ACT_LEAKY_RELU>{}); break;
+        case GK_ACT_GELU: f(std::integral_constant<int, GK_ACT_GELU>{}); break;
+        case GK_ACT_GELU_TANH: f(std::integral_constant<int, GK_ACT_GELU_TANH>{}); break;
+        case GK_ACT_SILU: f(std::integral_constant<int, GK_ACT_SILU>{}); break;
+        default: f(std::integral_constant<int, GK_ACT_NONE>{}); break;
+    }
+}
+
+// ---- 16-bit pairs ------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi, int f16) {
+    uint32_t w;
+    if (f16)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+
+__device__ __forceinline__ float half_lo(uint32_t w, int f16) {
+    return f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xFFFFu)))
+               : __uint_as_float(w << 16);
+}
+__device__ __forceinline__ float half_hi(uint32_t w, int f16) {
+    return f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)))
+               : __uint_as_float(w & 0xFFFF0000u);
+}
+
+// The loads of store_pairs' layout, not yet exchanged: N words hold the 2 N columns of this lane pair.
+template <int N>
+__device__ __forceinline__ void load_pairs(uint32_t (&w)[N], const uint16_t* c, int64_t ldq, int n,
+                                           int pn, int lane) {
+    const int odd = lane & 1;
+    const uint16_t* q = c + (lane & 30) + odd * ldq;
+    const int left = (lane & 30) < pn ? n - odd : 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        w[j] = 2 * j < left ? *reinterpret_cast<const uint32_t*>(q + 2 * j * ldq) : 0u;
+}
+
+// The exchange: w[j] becomes columns 2 j and 2 j + 1 of this lane's own P row (store_pairs' exchange
+// undone, which is the same one).
+template <int N>
+__device__ __forceinline__ void own_pairs(uint32_t (&w)[N], int lane) {
+    const int odd = lane & 1;
+    const uint32_t give = odd ? 0x5410u : 0x7632u;
+    const uint32_t sel0 = odd ? 0x3254u : 0x5410u, sel1 = odd ? 0x3276u : 0x7610u;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(w[j], w[j + 1], give), 1);
+        w[j] = __byte_perm(w[j], got, sel0);
+        w[j + 1] = __byte_perm(w[j + 1], got, sel1);
+    }
+}
+
+// ---- a warp's accumulators ----------------------------------------------------------------------------
+
+// Where a warp's columns lie: P rows i0 .. i0 + pn - 1 of C exist (a lane each), Q rows r .. r + n - 1.
+struct EpiAt {
+    int i0, pn;
+    int64_t r;
+    int n;
+    __device__ __forceinline__ EpiAt plus(int c) const { return EpiAt{i0, pn, r + c, n - c}; }
+};
+
+// N columns of the matrix that the epilogue reads beside the accumulators, all loads issued together:
+// R, or z in 16 bits (pairs, or element by element), or z in 8 bits.
+template <int EPI, int N>
+struct EpiSide {
+    uint32_t w[N / 2];
+    uint32_t sb;  // z in 8 bits: lane e holds the exponent byte of column e
+    // PAIRS: see EpiArgs; f32 sides are read where they are used.
+    template <bool PAIRS>
+    __device__ __forceinline__ void load(const EpiArgs& e, const EpiAt& at, bool f32, int lane) {
+        if (EPI == EPI_BWD && e.z8.codes) {
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j) {
+                const int c = 4 * j + (lane >> 3);
+                w[j] = at.pn > 0 && c < at.n
+                           ? *reinterpret_cast<const uint32_t*>(
+                                 e.z8.codes + (at.r + c) * e.z8.codes_ld + at.i0 + (lane & 7) * 4)
+                           : 0u;
+            }
+            sb = at.pn > 0 && lane < N && lane < at.n
+                     ? e.z8.exps[(at.r + lane) * e.z8.exps_ld + (at.i0 >> 5)]
+                     : 0u;
+        } else if (e.side) {
+            if constexpr (PAIRS) {
+                load_pairs(w, static_cast<const uint16_t*>(e.side) + at.r * e.sq + at.i0, e.sq, at.n,
+                           at.pn, lane);
+            } else if (!f32) {
+                const uint16_t* s = static_cast<const uint16_t*>(e.side) + at.r * e.sq +
+                                    (at.i0 + lane) * e.sp;
+                const int n = lane < at.pn ? at.n : 0;
+                uint16_t v[N];
+#pragma unroll
+                for (int c = 0; c < N; ++c) v[c] = c < n ? s[c * e.sq] : uint16_t{0};
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j)
+                    w[j] = v[2 * j] | (static_cast<uint32_t>(v[2 * j + 1]) << 16);
+            }
+        }
+    }
+    // After load(): the pairs' exchange, or this lane's byte positions.
+    template <bool PAIRS>
+    __device__ __forceinline__ void own(const EpiArgs& e, int lane) {
+        if (EPI == EPI_BWD && e.z8.codes) {
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j) w[j] ^= 0x80808080u;
+            sb = __float_as_uint(act8_unit(sb));
+        } else if (PAIRS && e.side) {
+            own_pairs(w, lane);
+        }
+    }
+    // Column c of this lane's P row.
+    __device__ __forceinline__ float z8(int c, int lane) const {
+        const uint32_t x = __shfl_sync(0xffffffffu, w[c / 4], (c % 4) * 8 + (lane >> 2));
+        const float unit = __uint_as_float(__shfl_sync(0xffffffffu, sb, c));
+        return act8_code(x, lane & 3) * unit;
+    }
+    __device__ __forceinline__ float half(int c, int f16) const {
+        return c & 1 ? half_hi(w[c / 2], f16) : half_lo(w[c / 2], f16);
+    }
+};
+
+// N accumulators of each lane (f32 bits), their side loaded and owned, through the activation and into
+// C: a row of C is 32 P rows of the warp. `sum` gains the stored columns (backward).
+template <int EPI, int ACT, int N, bool PAIRS>
+__device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_type, int f16,
+                                            int64_t ldq, int64_t ldp, const EpiAt& at,
+                                            const uint32_t (&v)[N], const EpiSide<EPI, N>& s,
+                                            float alpha, float bias, float& sum, int lane) {
+    float y[N];
+    const bool live = lane < at.pn;
+    const int64_t own = (at.i0 + lane) * ldp + at.r * ldq;  // element by element
+    if constexpr (EPI == EPI_FWD) {
+        uint32_t zw[N / 2];
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float a = fmaf(alpha, __uint_as_float(v[j]), bias);
+            const float b = fmaf(alpha, __uint_as_float(v[j + 1]), bias);
+            zw[j / 2] = pack_half2(a, b, f16);
+            y[j] = act_value<ACT>(a, e.slope);
+            y[j + 1] = act_value<ACT>(b, e.slope);
+        }
+        if (e.side) {
+            if (PAIRS || out_type != GK_F32) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) y[j] += s.half(j, f16);
+            } else {
+                const float* r = static_cast<const float*>(e.side) + (at.i0 + lane) * e.sp +
+                                 at.r * e.sq;
+                const int n = live ? at.n : 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) y[j] += j < n ? r[j * e.sq] : 0.0f;
+            }
+        }
+        if (e.z) {
+            if constexpr (PAIRS) {
+                store_pairs(zw, e.z + at.r * e.zq + at.i0, e.zq, at.n, at.pn, lane);
+            } else {
+                uint16_t* z = e.z + (at.i0 + lane) * e.zp + at.r * e.zq;
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (live && j < at.n)
+                        z[j * e.zq] = static_cast<uint16_t>(zw[j / 2] >> (16 * (j & 1)));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float z = e.z8.codes ? s.z8(j, lane) : s.half(j, f16);
+            y[j] = alpha * __uint_as_float(v[j]) * act_slope<ACT>(z, e.slope);
+            if (j < at.n) sum += y[j];
+        }
+    }
+    if constexpr (PAIRS) {
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) w[j] = pack_half2(y[2 * j], y[2 * j + 1], f16);
+        store_pairs(w, static_cast<uint16_t*>(c) + at.r * ldq + at.i0, ldq, at.n, at.pn, lane);
+    } else if (out_type == GK_F32) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (live && j < at.n) static_cast<float*>(c)[own + j * ldq] = y[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const uint32_t w = pack_half2(y[j], y[j + 1], f16);
+            uint16_t* o = static_cast<uint16_t*>(c) + own + j * ldq;
+            if (live && j < at.n) *o = static_cast<uint16_t>(w);
+            if (live && j + 1 < at.n) o[ldq] = static_cast<uint16_t>(w >> 16);
+        }
+    }
+}
+
+// The bias of this lane's P row.
+__device__ __forceinline__ float epi_bias(const EpiArgs& e, int g, int i0, int pn, int lane) {
+    if (!e.bias || lane >= pn) return 0.0f;
+    const int64_t i = g * e.bias_gs + i0 + lane;
+    if (e.bias_type == GK_F32) return static_cast<const float*>(e.bias)[i];
+    const uint32_t w = static_cast<const uint16_t*>(e.bias)[i];
+    return half_lo(w, e.bias_type == GK_F16);
+}
+
+}  // namespace gk

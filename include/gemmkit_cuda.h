@@ -276,7 +276,15 @@ int gk_gemm_half_f32_batched_unchecked(gk_workspace *ws, int is_f16, size_t batc
  * tier takes gemm_fused_unchecked's (bias, bias_dim, has_bias, act) selectors, the checked
  * tier validates the views like gk_gemm_half_f32 and the bias length like gemmkit. With k == 0
  * or alpha == 0, C <- act(beta*C + bias) (gemmkit/src/dispatch/float.rs:671-676). */
-enum gk_act { GK_ACT_NONE = 0, GK_ACT_RELU = 1, GK_ACT_LEAKY_RELU = 2 };
+enum gk_act {
+    GK_ACT_NONE = 0,
+    GK_ACT_RELU = 1,
+    GK_ACT_LEAKY_RELU = 2,
+    /* for the feed-forward layer's entries only (gk_gemm_half_epilogue and the like) */
+    GK_ACT_GELU = 3,      /* z (1 + erf(z / sqrt 2)) / 2 */
+    GK_ACT_GELU_TANH = 4, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+    GK_ACT_SILU = 5,      /* z / (1 + exp(-z)) */
+};
 int gk_gemm_half_f32_fused_unchecked(gk_workspace *ws, int is_f16, size_t m, size_t k, size_t n,
                                      float alpha, const uint16_t *a, ptrdiff_t rsa,
                                      ptrdiff_t csa, const uint16_t *b, ptrdiff_t rsb,
@@ -406,6 +414,123 @@ int gk_fp4_import(const uint8_t *codes, size_t codes_len, size_t codes_ld, const
  * Needs no workspace, allocates nothing and may be captured. */
 int gk_gemm_fp4(float alpha, const gk_fp4_matrix *a, const gk_fp4_matrix *b, float beta,
                 gk_matmut c, int out_type, gk_parallelism par, gk_stream_t stream);
+
+/* ---- feed-forward layers, dense or by expert (no counterpart in gemmkit) ------------------ */
+
+/* What follows the product in a feed-forward layer, in f32 on its accumulators:
+ *     z = alpha * A * B[g] + bias[g];   C = act(z) + residual.
+ * bias: n elements a group, bias_gs apart, f32 or the operands' type (bias_type, a gk_dtype); NULL for
+ * none. residual (rows x n, C's type; data NULL for none) may be C itself, the same view. z (rows x n,
+ * the operands' type, rounded once; data NULL when it is not kept) is what the backward pass needs.
+ * GELU and SiLU keep a NaN and give 0 at minus infinity; ReLU and LeakyReLU take a NaN to 0, as the
+ * engine's other epilogues do. */
+typedef struct {
+    int32_t act;  /* enum gk_act */
+    float slope;  /* LeakyReLU's */
+    const void *bias;
+    size_t bias_len;
+    ptrdiff_t bias_gs;
+    int32_t bias_type;
+    gk_matref residual;
+    gk_matmut z;
+} gk_epilogue;
+
+/* C[i, :] <- act(alpha * A[i, :] * B[g] + bias[g]) + residual[i, :], the product as in
+ * gk_gemm_half_grouped: A (rows x k) and B (k x n a group, groups b_gs elements apart) in bf16 or f16, C
+ * in f32 or their type, rows grouped by a device array of offsets; offsets == NULL (groups must be 1)
+ * is a plain product of all rows. k == 0 or alpha == 0 is a product of zeros: C <- act(bias) +
+ * residual. Rows outside the groups are neither read nor written, in any matrix. Operands that
+ * cannot be read in place take scratch as there. Calls may be captured and may run on several
+ * streams at once. */
+int gk_gemm_half_epilogue(int is_f16, size_t groups, const int32_t *offsets, float alpha,
+                          gk_matref a, gk_matref b, ptrdiff_t b_gs, const gk_epilogue *epi,
+                          gk_matmut c, int out_type, gk_parallelism par, gk_stream_t stream);
+
+/* A rows x cols matrix in 8 bits with a power of two per 32 consecutive elements of a row (MXINT8 of the
+ * OCP Microscaling Formats specification v1.0), for activations that are kept for a backward pass:
+ * element (r, c) stands for codes[r * codes_ld + c] * 2^(exps[r * exps_ld + c / 32] - 133). Codes
+ * lie in [-127, 127]; an exponent byte of 255 makes its block NaN. In device memory that the caller
+ * owns: codes 16-byte aligned with rows at a pitch that is a multiple of 32 bytes and holds all
+ * columns, one exponent byte per block (ceil(cols / 32) a row). Lengths in bytes. Rows follow each
+ * other plainly, so a run of rows is a matrix too. */
+typedef struct {
+    size_t rows, cols;
+    int8_t *codes;
+    size_t codes_len, codes_ld;
+    uint8_t *exps;
+    size_t exps_len, exps_ld;
+} gk_act8_matrix;
+
+/* x (f32, f16 or bf16 by x_type; any non-negative strides) into dst: per block e = floor(log2
+ * max |x|) (at least -127), code = x / 2^(e - 6) rounded half to even and clamped to +-127, exponent
+ * byte e + 127 (exact, as if in infinite precision). A block that holds an infinity or a NaN gets the
+ * byte 255. Bytes of a row's pitch past its columns are not written past the row's last block. */
+int gk_quantize_act8(gk_matref x, int x_type, const gk_act8_matrix *dst, gk_stream_t stream);
+/* The values that q stands for, in f32, f16 or bf16 (out_type): exact in f32 and bf16, and in f16 where
+ * the source was f16 (otherwise rounded). */
+int gk_dequantize_act8(const gk_act8_matrix *q, gk_matmut out, int out_type, gk_stream_t stream);
+
+/* What the backward pass of such a layer needs besides the products: act'(z), with z in 16 bits (rows x n,
+ * the operands' type), or in 8 bits (z8 != NULL; z is then not looked at), or nothing for
+ * GK_ACT_NONE (z.data NULL); and the bias's gradient, the sums over each group's rows, n elements
+ * a group, dbias_gs apart, f32 or the operands' type (NULL: not wanted). The sums are of the f32
+ * values, in f32 over a tile's rows and in f64 over the tiles, in an order that only the sizes set:
+ * they repeat bit for bit. An empty group's are 0. act' is the limit at infinities; ReLU's is 0 and
+ * LeakyReLU's the slope at 0. */
+typedef struct {
+    int32_t act;
+    float slope;
+    gk_matref z;
+    const gk_act8_matrix *z8;
+    void *dbias;
+    size_t dbias_len;
+    ptrdiff_t dbias_gs;
+    int32_t dbias_type;
+} gk_epilogue_bwd;
+
+/* C[i, :] <- alpha * A[i, :] * B[g] * act'(z[i, :]): the gradient by z of the layer before, A the
+ * gradient that reaches this layer's output and B its weights viewed transposed; dbias[g] the sums
+ * of C (before its rounding) over the group's rows. C may be z itself, the same view. Everything
+ * else as in gk_gemm_half_epilogue; the sums take scratch of 4 bytes for each 64 or more elements
+ * of C. */
+int gk_gemm_half_dact(int is_f16, size_t groups, const int32_t *offsets, float alpha, gk_matref a,
+                      gk_matref b, ptrdiff_t b_gs, const gk_epilogue_bwd *epi, gk_matmut c,
+                      int out_type, gk_parallelism par, gk_stream_t stream);
+/* The same without a product: dz <- dy * act'(z) and the sums of dz (before its rounding). dy (rows x n)
+ * is bf16 or f16, dz f32 or that type; dz.data NULL: only the sums. dz may be dy or z itself, the same
+ * view. */
+int gk_act_backward(int is_f16, size_t groups, const int32_t *offsets, gk_matref dy,
+                    const gk_epilogue_bwd *epi, gk_matmut dz, int out_type, gk_stream_t stream);
+
+/* The weight gradient from a checkpoint in 8 bits: C[g] <- alpha * A_g^T * B_g + beta * C[g] as in
+ * gk_gemm_half_grouped_wgrad, with A (rows x m) held in 8 bits and its values taken as they are
+ * (rounded to f16 with is_f16, see gk_dequantize_act8); offsets == NULL (groups 1): all rows. */
+int gk_gemm_act8_wgrad(int is_f16, size_t groups, const int32_t *offsets, float alpha,
+                       const gk_act8_matrix *a, gk_matref b, float beta, gk_matmut c,
+                       ptrdiff_t c_gs, int out_type, gk_parallelism par, gk_stream_t stream);
+
+/* ---- the router's balance loss (no counterpart in gemmkit) --------------------------------- */
+
+/* Of T x experts router logits (f32, f16 or bf16 by x_type; any non-negative strides; 1 to 1024 experts) and
+ * the `top` experts that each token goes to (ids: T x top, contiguous, int32, or int64 with ids64;
+ * a negative id is no expert, and a token without any is padding):
+ *     counts[e]   how often e is among the ids            offsets[e]  counts[0] + .. + counts[e - 1]
+ *     loss = coef * experts * sum_e (counts[e] / routed) * mean over live tokens of softmax(logits)[e]
+ * with routed the sum of all counts, live tokens those with an id. coef is 1 for a plain balance
+ * loss. counts (experts), offsets (experts + 1, as gk_gemm_half_grouped takes them), loss (one) are
+ * device arrays; rates (experts f32, device) is kept for the backward pass: coef * experts * counts[e] /
+ * routed / live tokens. Nothing live: loss and rates 0. A token whose logits are all minus infinity
+ * adds probability 0; one with a NaN or plus infinity makes the loss NaN. An id of `experts` or
+ * more counts as negative and sets GK_STATUS_OFFSETS in the device status. Sums run in an order
+ * that only the sizes set. Needs scratch of 8 * experts bytes a block of tokens. */
+int gk_moe_balance(gk_matref logits, int x_type, const void *ids, size_t ids_len, size_t top,
+                   int ids64, float coef, float *loss, int32_t *counts, int32_t *offsets,
+                   float *rates, gk_stream_t stream);
+/* dlogits[t, e] <- dloss * p_te * (rates[e] - sum_j p_tj rates[j]), zeros for padding; dlogits has the
+ * logits' type and may be the logits themselves, the same view. dloss is one f32 on the device. */
+int gk_moe_balance_backward(gk_matref logits, int x_type, const void *ids, size_t ids_len, size_t top,
+                            int ids64, const float *rates, const float *dloss, gk_matmut dlogits,
+                            gk_stream_t stream);
 
 /* ---- producer step: f32 activations -> i8 (no counterpart in gemmkit) ---------------- */
 
