@@ -8,9 +8,11 @@
 // unit lies below f16's 2^-24 holds multiples of that already). The backward pass therefore
 // multiplies what the checkpoint stands for, with no second rounding.
 //
-// Both kernels move each byte once and are bound by memory. A warp takes AU steps of 256 elements of a
-// row, eight consecutive ones a lane: 16-byte loads, the block's maximum over four lanes by two
-// shuffles, 8-byte stores.
+// Both kernels move each byte once and are bound by memory. The matrix is a run of pieces of E elements,
+// row after row; a lane takes AU of them, 32 pieces apart, all of their loads issued together (so short
+// rows fill warps too). E is 16 where the elements have 16 bits, 8 in f32: 16-byte loads and stores
+// either way, and a block's maximum over two or four lanes. (With E = 8 for 16 bits, and pieces that ended
+// with a row's 1024 elements, 8192 x 8192 of bf16 took 44 and 47 us; now 45 and 34.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,24 +28,30 @@ namespace gk {
 
 namespace {
 
-constexpr int AU = 4;  // steps of a unit, all of their loads issued together
+constexpr int AU = 4;  // pieces of a lane
 
 template <typename T>
-struct Eight {  // eight elements as they lie in memory
-    uint32_t w[sizeof(T) * 2];
+constexpr int piece() {
+    return sizeof(T) == 2 ? 16 : 8;
+}
+
+template <typename T>
+struct Piece {  // its elements as they lie in memory
+    static constexpr int E = piece<T>(), W = E * sizeof(T) / 4;
+    uint32_t w[W];
     __device__ __forceinline__ void load(const T* x) {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
-            const uint4 v = ld_global_v4(reinterpret_cast<const uint8_t*>(x) + 16 * i);
-            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        for (int i = 0; i < W; i += 4) {
+            const uint4 v = ld_global_v4(reinterpret_cast<const uint32_t*>(x) + i);
+            w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
         }
     }
     // element by element, zeros from n on
     __device__ __forceinline__ void load(const T* x, int64_t cs, int n) {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) w[i] = 0u;
+        for (int i = 0; i < W; ++i) w[i] = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < E; ++i)
             if (i < n) {
                 if constexpr (sizeof(T) == 4)
                     w[i] = __float_as_uint(x[i * cs]);
@@ -63,6 +71,24 @@ struct Eight {  // eight elements as they lie in memory
     }
 };
 
+// x clamped to +-127 (one instruction: the smaller magnitude with the product's sign).
+__device__ __forceinline__ float clamp_127(float x) {
+    float r;
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(127.0f));
+    return r;
+}
+
+// Where piece i lies: `per` of them make the whole blocks of a row. (Divided in 64 bits only where 32 do not
+// hold the pieces.)
+struct At {
+    int64_t r;
+    int c;
+    __device__ __forceinline__ At(uint64_t i, uint32_t per, bool wide, int e) {
+        r = wide ? i / per : static_cast<uint32_t>(i) / per;
+        c = static_cast<int>(i - r * per) * e;
+    }
+};
+
 struct Act8Out {
     int8_t* codes;
     uint8_t* exps;
@@ -77,56 +103,66 @@ __global__ void __launch_bounds__(256)
     quantize_act8_kernel(const T* x, int64_t rs, int64_t cs, int vec, Act8Out q) {
     griddep_wait();
     griddep_launch_dependents();
+    constexpr int E = piece<T>(), LANES = ACT8_BLOCK / E;  // lanes of a block
     const int lane = threadIdx.x & 31;
-    const int64_t chunks = (q.cols + AU * 256 - 1) / (AU * 256);
-    const int64_t units = q.rows * chunks, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-         u < units; u += step) {
-        const int64_t r = u / chunks;
-        const int c0 = static_cast<int>(u - r * chunks) * AU * 256 + lane * 8;
-        const T* src = x + r * rs;
-        Eight<T> raw[AU];
+    const uint32_t per = static_cast<uint32_t>((q.cols + 31) / 32 * LANES);
+    const uint64_t pieces = static_cast<uint64_t>(q.rows) * per;
+    const bool wide = pieces + 32 * AU > 0xFFFFFFFFull;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * (blockDim.x >> 5) * (32 * AU);
+    for (uint64_t u = static_cast<uint64_t>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (32 * AU);
+         u < pieces; u += step) {
+        Piece<T> raw[AU];
 #pragma unroll
         for (int i = 0; i < AU; ++i) {
-            const int c = c0 + i * 256;
-            if (vec && c + 8 <= q.cols)
-                raw[i].load(src + c);
-            else
-                raw[i].load(src + c * cs, cs, q.cols - c);
+            const At at(u + 32 * i + lane, per, wide, E);
+            const T* src = x + at.r * rs;
+            if (at.r < q.rows) {
+                if (vec && at.c + E <= q.cols)
+                    raw[i].load(src + at.c);
+                else
+                    raw[i].load(src + at.c * cs, cs, q.cols - at.c);
+            } else {
+                raw[i].load(src, cs, 0);
+            }
         }
 #pragma unroll
         for (int i = 0; i < AU; ++i) {
-            const int c = c0 + i * 256;
-            if (c - lane * 8 >= q.cols) break;  // the whole warp
-            float v[8];
+            if (u + 32 * i >= pieces) break;  // the whole warp
+            float v[E];
             uint32_t m = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < E; ++k) {
                 v[k] = raw[i].value(k);
                 m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
             }
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+#pragma unroll
+            for (int d = 1; d < LANES; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
             const uint32_t b = m >> 23;  // the biased exponent is e + 127; 255: an infinity or a NaN
             // x 2^(6 - e), in two exact steps where 2^(6 - e) would not be a normal number
-            const float first = b < 64 ? 0x1p64f : 1.0f;
+            if (__any_sync(0xffffffffu, b < 64)) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) v[k] = b < 64 ? v[k] * 0x1p64f : v[k];
+            }
             const float mul = __uint_as_float((b < 64 ? 196u - b : 260u - b) << 23);
-            uint32_t y[8];
+            uint32_t y[E], w[E / 4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float s = fminf(fmaxf(v[k] * first * mul, -127.0f), 127.0f);
-                // 1.5 2^23 + s: rounded to an integer, half to even, its low byte the code
-                y[k] = b == 255 ? 0u : __float_as_uint(s + 12582912.0f);
-            }
-            uint32_t w[2];
+            for (int k = 0; k < E; ++k)
+                // below 128 in magnitude; 1.5 2^23 + s: rounded to an integer, half to even, its low
+                // byte the code
+                y[k] = __float_as_uint(clamp_127(v[k] * mul) + 12582912.0f);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                w[h] = __byte_perm(__byte_perm(y[4 * h], y[4 * h + 1], 0x0040),
-                                   __byte_perm(y[4 * h + 2], y[4 * h + 3], 0x0040), 0x5410);
-            if (c < (q.cols + 31) / 32 * 32) {
-                *reinterpret_cast<uint2*>(q.codes + r * q.codes_ld + c) = make_uint2(w[0], w[1]);
-                if ((lane & 3) == 0) q.exps[r * q.exps_ld + (c >> 5)] = static_cast<uint8_t>(b);
-            }
+            for (int h = 0; h < E / 4; ++h)
+                w[h] = b == 255 ? 0u
+                                : __byte_perm(__byte_perm(y[4 * h], y[4 * h + 1], 0x0040),
+                                              __byte_perm(y[4 * h + 2], y[4 * h + 3], 0x0040), 0x5410);
+            const At at(u + 32 * i + lane, per, wide, E);
+            if (at.r >= q.rows) continue;
+            int8_t* dst = q.codes + at.r * q.codes_ld + at.c;
+            if constexpr (E == 16)
+                st_global_v4(dst, w[0], w[1], w[2], w[3]);
+            else
+                *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+            if (lane % LANES == 0) q.exps[at.r * q.exps_ld + (at.c >> 5)] = static_cast<uint8_t>(b);
         }
     }
 }
@@ -138,62 +174,64 @@ __global__ void __launch_bounds__(256)
                            int vec) {
     griddep_wait();
     griddep_launch_dependents();
+    constexpr int E = piece<T>();
     const int lane = threadIdx.x & 31;
-    const int64_t chunks = (cols + AU * 256 - 1) / (AU * 256);
-    const int64_t units = rows * chunks, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-         u < units; u += step) {
-        const int64_t r = u / chunks;
-        const int c0 = static_cast<int>(u - r * chunks) * AU * 256 + lane * 8;
-        uint2 w[AU];
-        uint32_t b[AU];
+    const uint32_t per = static_cast<uint32_t>((cols + E - 1) / E);
+    const uint64_t pieces = static_cast<uint64_t>(rows) * per;
+    const bool wide = pieces + 32 * AU > 0xFFFFFFFFull;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * (blockDim.x >> 5) * (32 * AU);
+    for (uint64_t u = static_cast<uint64_t>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (32 * AU);
+         u < pieces; u += step) {
+        uint32_t w[AU][E / 4], b[AU];
 #pragma unroll
         for (int i = 0; i < AU; ++i) {
-            const int c = c0 + i * 256;
-            w[i] = make_uint2(0u, 0u);
-            b[i] = 0u;
-            if (c < cols) {
-                w[i] = *reinterpret_cast<const uint2*>(q.codes + r * q.codes_ld + c);
-                b[i] = q.exps[r * q.exps_ld + (c >> 5)];
+            const At at(u + 32 * i + lane, per, wide, E);
+            if (at.r >= rows) continue;
+            const int8_t* src = q.codes + at.r * q.codes_ld + at.c;
+            if constexpr (E == 16) {
+                const uint4 v = ld_global_v4(src);
+                w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(src);
+                w[i][0] = v.x, w[i][1] = v.y;
             }
+            b[i] = q.exps[at.r * q.exps_ld + (at.c >> 5)];
         }
 #pragma unroll
         for (int i = 0; i < AU; ++i) {
-            const int c = c0 + i * 256, n = cols - c;
-            if (n <= 0) break;
+            const At at(u + 32 * i + lane, per, wide, E);
+            if (at.r >= rows) break;
+            const int n = cols - at.c;
             const float unit = act8_unit(b[i]);
-            float v[8];
+            float v[E];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                v[k] = act8_code((k < 4 ? w[i].x : w[i].y) ^ 0x80808080u, k & 3) * unit;
-            T* o = out + r * rs + c * cs;
-            if (vec && n >= 8) {
-                if constexpr (sizeof(T) == 4) {
+            for (int k = 0; k < E; ++k) v[k] = act8_code(w[i][k / 4] ^ 0x80808080u, k & 3) * unit;
+            T* o = out + at.r * rs + at.c * cs;
+            if (vec && n >= E) {
+                uint32_t p[E * sizeof(T) / 4];
 #pragma unroll
-                    for (int h = 0; h < 8; h += 4)
-                        st_global_v4(o + h, __float_as_uint(v[h]), __float_as_uint(v[h + 1]),
-                                     __float_as_uint(v[h + 2]), __float_as_uint(v[h + 3]));
-                } else {
-                    constexpr int TYPE = std::is_same_v<T, __half> ? GK_F16 : GK_BF16;
-                    uint32_t p[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
+                for (int h = 0; h < static_cast<int>(E * sizeof(T) / 4); ++h) {
+                    if constexpr (sizeof(T) == 4)
+                        p[h] = __float_as_uint(v[h]);
+                    else
                         p[h] = round_pair(__float_as_uint(v[2 * h]), __float_as_uint(v[2 * h + 1]), 1.0f,
-                                          TYPE);
-                    st_global_v4(o, p[0], p[1], p[2], p[3]);
+                                          std::is_same_v<T, __half> ? GK_F16 : GK_BF16);
                 }
+#pragma unroll
+                for (int h = 0; h < static_cast<int>(E * sizeof(T) / 4); h += 4)
+                    st_global_v4(reinterpret_cast<uint32_t*>(o) + h, p[h], p[h + 1], p[h + 2], p[h + 3]);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < E; ++k)
                     if (k < n) to_out(o + k * cs, v[k]);
             }
         }
     }
 }
 
-dim3 unit_grid(int64_t rows, int64_t cols) {
-    const int64_t blocks = (rows * ((cols + AU * 256 - 1) / (AU * 256)) + 7) / 8;
-    const int64_t most = static_cast<int64_t>(sm_count()) * 32;
+dim3 piece_grid(int64_t rows, int64_t cols, int e) {
+    const int64_t blocks = (rows * ((cols + 31) / 32 * (32 / e)) + 256 * AU - 1) / (256 * AU);
+    const int64_t most = static_cast<int64_t>(sm_count()) * 4;  // what is resident
     return dim3(static_cast<unsigned>(blocks < most ? blocks : most));
 }
 
@@ -204,7 +242,7 @@ bool whole_rows(const void* p, int64_t rows, int64_t rs, int64_t cs, size_t es) 
 
 template <typename T>
 int quantize(const gk_matref& x, const Act8Out& q, cudaStream_t st) {
-    return launch_overlapped(quantize_act8_kernel<T>, unit_grid(q.rows, q.cols), 256, st,
+    return launch_overlapped(quantize_act8_kernel<T>, piece_grid(q.rows, q.cols, piece<T>()), 256, st,
                              static_cast<const T*>(x.data), static_cast<int64_t>(x.rs),
                              static_cast<int64_t>(x.cs),
                              whole_rows(x.data, q.rows, x.rs, x.cs, sizeof(T)) ? 1 : 0, q);
@@ -214,8 +252,8 @@ template <typename T>
 int dequantize(const gk_act8_matrix& q, void* out, int64_t rs, int64_t cs, cudaStream_t st) {
     const Act8View v{q.codes, q.exps, static_cast<int64_t>(q.codes_ld), static_cast<int64_t>(q.exps_ld)};
     const int64_t rows = static_cast<int64_t>(q.rows);
-    return launch_overlapped(dequantize_act8_kernel<T>, unit_grid(rows, static_cast<int64_t>(q.cols)), 256,
-                             st, v, rows, static_cast<int32_t>(q.cols), static_cast<T*>(out), rs, cs,
+    return launch_overlapped(dequantize_act8_kernel<T>, piece_grid(rows, static_cast<int64_t>(q.cols), piece<T>()),
+                             256, st, v, rows, static_cast<int32_t>(q.cols), static_cast<T*>(out), rs, cs,
                              whole_rows(out, rows, rs, cs, sizeof(T)) ? 1 : 0);
 }
 

@@ -9,7 +9,8 @@
 // in registers over all of its tokens; counts are integers in shared memory. Each block leaves its sums
 // and counts, a last block adds them (one block does all of it where there are few tokens). No
 // floating atomics: which token a warp takes depends on the sizes alone, and so does every sum.
-// Differences of logits go through expf, sums over blocks through f64.
+// Differences of logits go through the fast exponential (2^-22, and 2^-24 of the difference: the large p
+// come from small differences), sums over blocks through f64.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,31 +27,31 @@ namespace {
 
 constexpr int MAX_EXPERTS = 1024;
 constexpr int BW = 16;           // warps of a block
-constexpr int TOKENS_A_WARP = 4; // at least, before another block is added
+constexpr int TOKENS_A_WARP = 4; // before another block is added
 
 struct Router {
     const void* x;
     int64_t rs, cs;
-    int32_t type, ids64;
+    int32_t ids64;
     const void* ids;
     int32_t top, tokens, experts;
     unsigned int* status;
 };
 
 // A token's logits as they lie: lane l holds elements (32 j + l) V .. + V - 1.
-template <int V, int J>
+template <int T, int V, int J>
 struct Logits {
     uint32_t w[J * V];  // f32 bits, or 16-bit values two a word (V == 4), or one a word (V == 1)
-    __device__ __forceinline__ void load(const Router& p, int t, int lane) {
+    __device__ __forceinline__ void load(const Router& p, int64_t t, int lane) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int e = (32 * j + lane) * V;
             if (e >= p.experts) continue;
             const int64_t at = t * p.rs + e * p.cs;
             if constexpr (V == 1) {
-                w[j] = p.type == GK_F32 ? static_cast<const uint32_t*>(p.x)[at]
+                w[j] = T == GK_F32 ? static_cast<const uint32_t*>(p.x)[at]
                                         : static_cast<const uint16_t*>(p.x)[at];
-            } else if (p.type == GK_F32) {
+            } else if (T == GK_F32) {
                 const uint4 v = ld_global_v4(static_cast<const float*>(p.x) + at);
                 w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
             } else {
@@ -59,11 +60,11 @@ struct Logits {
             }
         }
     }
-    __device__ __forceinline__ float value(const Router& p, int j, int v) const {
-        if (p.type == GK_F32) return __uint_as_float(w[V * j + v]);
+    __device__ __forceinline__ float value(int j, int v) const {
+        if (T == GK_F32) return __uint_as_float(w[V * j + v]);
         const uint32_t h = V == 1 ? w[j] : w[V * j + v / 2] >> (16 * (v & 1));
-        return p.type == GK_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xFFFFu)))
-                                : __uint_as_float(h << 16);
+        return T == GK_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xFFFFu)))
+                           : __uint_as_float(h << 16);
     }
     // The softmax; 0 everywhere where every logit is minus infinity.
     __device__ __forceinline__ void softmax(const Router& p, int lane, float (&y)[J * V]) const {
@@ -72,7 +73,7 @@ struct Logits {
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                y[V * j + v] = (32 * j + lane) * V < p.experts ? value(p, j, v) : -INFINITY;
+                y[V * j + v] = (32 * j + lane) * V < p.experts ? value(j, v) : -INFINITY;
                 m = fmaxf(m, y[V * j + v]);
             }
 #pragma unroll
@@ -82,7 +83,7 @@ struct Logits {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < J * V; ++i) {
-            y[i] = expf(y[i] - base);
+            y[i] = __expf(y[i] - base);
             s += y[i];
         }
 #pragma unroll
@@ -94,102 +95,42 @@ struct Logits {
     }
 };
 
-// The warp's token's ids into `hist` (when there is one); whether it has any.
-__device__ __forceinline__ bool token_ids(const Router& p, int t, int* hist, int lane) {
-    bool any = false, bad = false;
-    for (int i = lane; i < p.top; i += 32) {
-        const int64_t at = static_cast<int64_t>(t) * p.top + i;
+// Tokens that a warp takes at a time: as many as keep its loads in flight.
+template <int V, int J>
+constexpr int together() {
+    return V * J <= 8 ? 4 : 1;
+}
+
+// The ids of n tokens from t0 on (they lie one after the other) into `hist`, when there is one; a bit for
+// each token that has any.
+__device__ __forceinline__ uint32_t token_ids(const Router& p, int64_t t0, int n, int* hist, int lane) {
+    uint32_t live = 0;
+    bool bad = false;
+    for (int i = lane; i < n * p.top; i += 32) {
+        const int64_t at = t0 * p.top + i;
         const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at]
                                    : static_cast<const int32_t*>(p.ids)[at];
         if (id >= 0 && id < p.experts) {
-            any = true;
+            const int k = (i >= p.top) + (i >= 2 * p.top) + (i >= 3 * p.top);
+            live |= 1u << k;
             if (hist) atomicAdd(&hist[id], 1);
         } else if (id >= 0) {
             bad = true;
         }
     }
     if (hist && bad) atomicOr(p.status, GK_DEV_BAD_OFFSETS);
-    return __any_sync(0xffffffffu, any);
+    return __reduce_or_sync(0xffffffffu, live);
 }
 
-// What a block leaves: experts sums (f32), experts counts and the live tokens, at a pitch of `pitch` words.
+// What a block leaves, in words: experts sums (f32), experts counts and the live tokens. Behind all
+// blocks' parts, in whole 16-byte pieces, lie their totals: experts sums (f64), experts counts, the live
+// tokens and the blocks of the second kernel that are done.
 __host__ __device__ inline int part_pitch(int experts) { return 2 * experts + 1; }
-
-// The blocks' parts into the results. All threads of one block.
-__device__ __forceinline__ void finish(const uint32_t* part, int blocks, int experts, float coef,
-                                       float* loss, int32_t* counts, int32_t* offsets, float* rates) {
-    __shared__ double red[BW];
-    __shared__ int scan[BW];
-    __shared__ int live_all, routed_all;
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    const int pitch = part_pitch(experts);
-    if (tid == 0) live_all = 0;
-    __syncthreads();
-    int live = 0;
-    for (int b = tid; b < blocks; b += blockDim.x)
-        live += static_cast<int>(part[static_cast<int64_t>(b) * pitch + 2 * experts]);
-    if (live) atomicAdd(&live_all, live);
-    // thread e and, where there are more experts than threads, e + blockDim.x
-    constexpr int PER = MAX_EXPERTS / (32 * BW);
-    double sum[PER];
-    int cnt[PER], carry = 0;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int e = k * blockDim.x + tid;
-        double s = 0.0;
-        int c = 0;
-        if (e < experts) {
-#pragma unroll 8
-            for (int b = 0; b < blocks; ++b) {
-                const uint32_t* at = part + static_cast<int64_t>(b) * pitch;
-                s += static_cast<double>(__uint_as_float(at[e]));
-                c += static_cast<int>(at[experts + e]);
-            }
-        }
-        sum[k] = s;
-        cnt[k] = c;
-        // running sums of the counts
-        int inc = c;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, d);
-            if (lane >= d) inc += u;
-        }
-        if (lane == 31) scan[w] = inc;
-        __syncthreads();
-        int before = carry;
-        for (int i = 0; i < w; ++i) before += scan[i];
-        if (e < experts) {
-            counts[e] = c;
-            offsets[e + 1] = before + inc;
-        }
-        for (int i = 0; i < BW; ++i) carry += scan[i];
-        __syncthreads();
-    }
-    if (tid == 0) {
-        offsets[0] = 0;
-        routed_all = carry;
-    }
-    __syncthreads();
-    const int tokens = live_all, routed = routed_all;
-    double a = 0.0;
-    const double unit = routed > 0 ? static_cast<double>(coef) * experts / routed / tokens : 0.0;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int e = k * blockDim.x + tid;
-        if (e < experts) {
-            rates[e] = static_cast<float>(unit * cnt[k]);
-            if (routed > 0) a += unit * cnt[k] * sum[k];
-        }
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
-    if (lane == 0) red[w] = a;
-    __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < BW; ++i) a += red[i];
-        *loss = static_cast<float>(a);
-    }
+__host__ __device__ inline int64_t totals_at(int blocks, int experts) {
+    return (static_cast<int64_t>(blocks) * part_pitch(experts) + 3) / 4 * 4;
+}
+__host__ __device__ inline int64_t part_words(int blocks, int experts) {
+    return totals_at(blocks, experts) + 3 * experts + 2;
 }
 
 struct BalanceOut {
@@ -200,9 +141,62 @@ struct BalanceOut {
     float* rates;
 };
 
-template <int V, int J>
+// The results from the totals; sum(e) and count(e) give an expert's. All threads of a block of W warps.
+template <int W, typename S, typename N>
+__device__ __forceinline__ void finish(S sum, N count, int tokens, int experts, const BalanceOut& o) {
+    __shared__ double red[W];
+    __shared__ int scan[W];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    constexpr int PER = MAX_EXPERTS / (32 * W);  // thread e, and e + 32 W
+    int cnt[PER], routed = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = k * 32 * W + tid;
+        const int c = e < experts ? count(e) : 0;
+        cnt[k] = c;
+        int inc = c;  // running sums of the counts
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += u;
+        }
+        if (lane == 31) scan[w] = inc;
+        __syncthreads();
+        int before = routed;
+        for (int i = 0; i < w; ++i) before += scan[i];
+        if (e < experts) {
+            o.counts[e] = c;
+            o.offsets[e + 1] = before + inc;
+        }
+        for (int i = 0; i < W; ++i) routed += scan[i];
+        __syncthreads();
+    }
+    if (tid == 0) o.offsets[0] = 0;
+    double a = 0.0;
+    const double unit =
+        routed > 0 ? static_cast<double>(o.coef) * experts / routed / tokens : 0.0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = k * 32 * W + tid;
+        if (e < experts) {
+            o.rates[e] = static_cast<float>(unit * cnt[k]);
+            if (routed > 0) a += unit * cnt[k] * sum(e);
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+    if (lane == 0) red[w] = a;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < W; ++i) a += red[i];
+        *o.loss = static_cast<float>(a);
+    }
+}
+
+template <int T, int V, int J>
 __global__ void __launch_bounds__(32 * BW)
     balance_kernel(const Router p, uint32_t* part, const BalanceOut o) {
+    constexpr int U = together<V, J>();
     extern __shared__ float smem[];  // BW x experts sums, then the block's part
     uint32_t* own = reinterpret_cast<uint32_t*>(smem + BW * p.experts);
     int* hist = reinterpret_cast<int*>(own + p.experts);
@@ -215,17 +209,18 @@ __global__ void __launch_bounds__(32 * BW)
 #pragma unroll
     for (int i = 0; i < J * V; ++i) sum[i] = 0.0f;
     int live = 0;
-    const int step = gridDim.x * BW;
-    for (int64_t t0 = blockIdx.x * BW + w; t0 < p.tokens; t0 += 2 * step) {
-        Logits<V, J> x[2];
-        x[0].load(p, static_cast<int>(t0), lane);
-        const bool two = t0 + step < p.tokens;
-        if (two) x[1].load(p, static_cast<int>(t0 + step), lane);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * BW * U;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * BW + w) * U; t0 < p.tokens; t0 += step) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(U), p.tokens - t0));
+        Logits<T, V, J> x[U];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (k == 1 && !two) break;
-            if (!token_ids(p, static_cast<int>(t0 + k * step), hist, lane)) continue;
-            ++live;
+        for (int k = 0; k < U; ++k)
+            if (k < n) x[k].load(p, t0 + k, lane);
+        const uint32_t has = token_ids(p, t0, n, hist, lane);
+        live += __popc(has);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (!(has >> k & 1)) continue;
             float y[J * V];
             x[k].softmax(p, lane, y);
 #pragma unroll
@@ -249,25 +244,81 @@ __global__ void __launch_bounds__(32 * BW)
     }
     __syncthreads();
     if (gridDim.x == 1) {
-        finish(own, 1, p.experts, o.coef, o.loss, o.counts, o.offsets, o.rates);
-    } else {
-        const int pitch = part_pitch(p.experts);
-        for (int i = threadIdx.x; i < pitch; i += blockDim.x)
-            part[static_cast<int64_t>(blockIdx.x) * pitch + i] = own[i];
+        finish<BW>([&](int e) { return static_cast<double>(__uint_as_float(own[e])); },
+               [&](int e) { return hist[e]; }, hist[p.experts], p.experts, o);
+        return;
     }
+    const int pitch = part_pitch(p.experts);
+    for (int i = threadIdx.x; i < pitch; i += blockDim.x)
+        part[static_cast<int64_t>(blockIdx.x) * pitch + i] = own[i];
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        part[totals_at(gridDim.x, p.experts) + 3 * p.experts + 1] = 0;
 }
 
-__global__ void __launch_bounds__(32 * BW)
-    balance_finish_kernel(const uint32_t* part, int blocks, int experts, const BalanceOut o) {
+// The parts of `blocks` blocks: a block adds 32 experts', a thread every FW-th part's, in f64; the block
+// that is done last turns the totals into the results. (One block for all parts took 34 us for
+// 148 x 256, a chain of 148 additions in f64.)
+constexpr int FW = 32;
+
+__global__ void __launch_bounds__(32 * FW)
+    balance_finish_kernel(uint32_t* part, int blocks, int experts, const BalanceOut o) {
+    __shared__ double s[FW][32];
+    __shared__ int c[FW][32];
+    __shared__ int last;
     griddep_wait();
     griddep_launch_dependents();
-    finish(part, blocks, experts, o.coef, o.loss, o.counts, o.offsets, o.rates);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int pitch = part_pitch(experts), e = blockIdx.x * 32 + lane;
+    uint32_t* totals = part + totals_at(blocks, experts);
+    double* sums = reinterpret_cast<double*>(totals);
+    int* counts = reinterpret_cast<int*>(totals + 2 * experts);
+    double a = 0.0;
+    int n = 0, live = 0;
+#pragma unroll 10
+    for (int b = w; b < blocks; b += FW) {
+        const uint32_t* at = part + static_cast<int64_t>(b) * pitch;
+        if (e < experts) {
+            a += static_cast<double>(__uint_as_float(at[e]));
+            n += static_cast<int>(at[experts + e]);
+        }
+        if (blockIdx.x == 0) live += static_cast<int>(at[2 * experts]);
+    }
+    s[w][lane] = a;
+    c[w][lane] = n;
+    __syncthreads();
+    if (w == 0 && e < experts) {
+        for (int i = 1; i < FW; ++i) {
+            a += s[i][lane];
+            n += c[i][lane];
+        }
+        sums[e] = a;
+        counts[e] = n;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        if (lane == 0) c[w][0] = live;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int i = 1; i < FW; ++i) live += c[i][0];
+            counts[experts] = live;
+        }
+    }
+    if (w == 0) __threadfence();  // what this warp wrote, before the count
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = atomicAdd(reinterpret_cast<unsigned*>(counts + experts + 1), 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    finish<FW>([&](int i) { return __ldcg(sums + i); }, [&](int i) { return __ldcg(counts + i); },
+           __ldcg(counts + experts), experts, o);
 }
 
-template <int V, int J>
+template <int T, int V, int J>
 __global__ void __launch_bounds__(256)
     balance_backward_kernel(const Router p, const float* rates, const float* dloss, void* dx,
                             int64_t ds, int64_t dc) {
+    constexpr int U = together<V, J>();
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -280,65 +331,80 @@ __global__ void __launch_bounds__(256)
             const int e = (32 * j + lane) * V + v;
             rate[V * j + v] = e < p.experts ? rates[e] : 0.0f;
         }
-    const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * warps + w; t < p.tokens; t += step) {
-        Logits<V, J> x;
-        x.load(p, static_cast<int>(t), lane);
-        float y[J * V];
-        if (token_ids(p, static_cast<int>(t), nullptr, lane)) {
-            x.softmax(p, lane, y);
-            float dot = 0.0f;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps * U;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + w) * U; t0 < p.tokens; t0 += step) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(U), p.tokens - t0));
+        Logits<T, V, J> x[U];
 #pragma unroll
-            for (int i = 0; i < J * V; ++i) dot = fmaf(y[i], rate[i], dot);
+        for (int k = 0; k < U; ++k)
+            if (k < n) x[k].load(p, t0 + k, lane);
+        const uint32_t has = token_ids(p, t0, n, nullptr, lane);
 #pragma unroll
-            for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        for (int k = 0; k < U; ++k) {
+            if (k >= n) break;
+            float y[J * V];
+            if (has >> k & 1) {
+                x[k].softmax(p, lane, y);
+                float dot = 0.0f;
 #pragma unroll
-            for (int i = 0; i < J * V; ++i) y[i] = scale * y[i] * (rate[i] - dot);
-        } else {
+                for (int i = 0; i < J * V; ++i) dot = fmaf(y[i], rate[i], dot);
 #pragma unroll
-            for (int i = 0; i < J * V; ++i) y[i] = 0.0f;
-        }
+                for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e = (32 * j + lane) * V;
-            if (e >= p.experts) continue;
-            const int64_t at = t * ds + e * dc;
-            if constexpr (V == 1) {
-                if (p.type == GK_F32)
-                    to_out(static_cast<float*>(dx) + at, y[j]);
-                else if (p.type == GK_F16)
-                    to_out(static_cast<__half*>(dx) + at, y[j]);
-                else
-                    to_out(static_cast<__nv_bfloat16*>(dx) + at, y[j]);
+                for (int i = 0; i < J * V; ++i) y[i] = scale * y[i] * (rate[i] - dot);
             } else {
-                uint32_t b[4];
 #pragma unroll
-                for (int v = 0; v < 4; ++v) b[v] = __float_as_uint(y[4 * j + v]);
-                if (p.type == GK_F32)
-                    st_global_v4(static_cast<float*>(dx) + at, b[0], b[1], b[2], b[3]);
-                else
-                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dx) + at) =
-                        make_uint2(round_pair(b[0], b[1], 1.0f, p.type),
-                                   round_pair(b[2], b[3], 1.0f, p.type));
+                for (int i = 0; i < J * V; ++i) y[i] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = (32 * j + lane) * V;
+                if (e >= p.experts) continue;
+                const int64_t at = (t0 + k) * ds + e * dc;
+                if constexpr (V == 1) {
+                    if (T == GK_F32)
+                        to_out(static_cast<float*>(dx) + at, y[j]);
+                    else if (T == GK_F16)
+                        to_out(static_cast<__half*>(dx) + at, y[j]);
+                    else
+                        to_out(static_cast<__nv_bfloat16*>(dx) + at, y[j]);
+                } else {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) b[v] = __float_as_uint(y[4 * j + v]);
+                    if (T == GK_F32)
+                        st_global_v4(static_cast<float*>(dx) + at, b[0], b[1], b[2], b[3]);
+                    else
+                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dx) + at) =
+                            make_uint2(round_pair(b[0], b[1], 1.0f, T),
+                                       round_pair(b[2], b[3], 1.0f, T));
+                }
             }
         }
     }
 }
 
-// f(V, J) as constants: V = 4 where a row's logits are whole 4-element pieces, J the smallest of those
-// compiled that holds the experts (up to 8 in pieces, 32 otherwise).
+// f(type, V, J) as constants: V = 4 where a row's logits are whole 4-element pieces, J the smallest of
+// those compiled that holds the experts (up to 8 in pieces, 32 otherwise).
 template <typename F>
-int with_layout(bool vec, int experts, F f) {
-    auto c = [](auto v) { return v; };
-    using std::integral_constant;
-    if (vec) {
-        if (experts <= 128) return f(c(integral_constant<int, 4>{}), c(integral_constant<int, 1>{}));
-        if (experts <= 256) return f(c(integral_constant<int, 4>{}), c(integral_constant<int, 2>{}));
-        return f(c(integral_constant<int, 4>{}), c(integral_constant<int, 8>{}));
-    }
-    if (experts <= 32) return f(c(integral_constant<int, 1>{}), c(integral_constant<int, 1>{}));
-    if (experts <= 256) return f(c(integral_constant<int, 1>{}), c(integral_constant<int, 8>{}));
-    return f(c(integral_constant<int, 1>{}), c(integral_constant<int, 32>{}));
+int with_layout(int type, bool vec, int experts, F f) {
+    auto pick = [&](auto t) {
+        auto go = [&](auto v, auto j) { return f(t, v, j); };
+        using std::integral_constant;
+        if (vec) {
+            integral_constant<int, 4> v;
+            if (experts <= 128) return go(v, integral_constant<int, 1>{});
+            if (experts <= 256) return go(v, integral_constant<int, 2>{});
+            return go(v, integral_constant<int, 8>{});
+        }
+        integral_constant<int, 1> v;
+        if (experts <= 32) return go(v, integral_constant<int, 1>{});
+        if (experts <= 256) return go(v, integral_constant<int, 8>{});
+        return go(v, integral_constant<int, 32>{});
+    };
+    if (type == GK_F32) return pick(std::integral_constant<int, GK_F32>{});
+    if (type == GK_F16) return pick(std::integral_constant<int, GK_F16>{});
+    return pick(std::integral_constant<int, GK_BF16>{});
 }
 
 bool in_fours(const void* p, int64_t rows, int64_t cols, int64_t rs, int64_t cs, size_t es) {
@@ -367,7 +433,7 @@ int check_router(const gk_matref& x, int x_type, const void* ids, size_t ids_len
     if ((rc = api_check_aligned(x.data, x_type == GK_F32 ? 4 : 2, "logits")) ||
         (rc = api_check_aligned(ids, ids64 ? 8 : 4, "ids")))
         return rc;
-    *p = Router{x.data, x.rs, x.cs, x_type, ids64 != 0, ids, static_cast<int32_t>(top),
+    *p = Router{x.data, x.rs, x.cs, ids64 != 0, ids, static_cast<int32_t>(top),
                 static_cast<int32_t>(x.rows), static_cast<int32_t>(x.cols), nullptr};
     return GK_OK;
 }
@@ -407,15 +473,16 @@ int gk_moe_balance(gk_matref logits, int x_type, const void* ids, size_t ids_len
     p.status = device_status_ptr();
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t want = (static_cast<int64_t>(p.tokens) + BW * TOKENS_A_WARP - 1) / (BW * TOKENS_A_WARP);
-    const int blocks = static_cast<int>(want < 1 ? 1 : want < sm_count() ? want : sm_count());
+    const int64_t most = 2ll * sm_count();  // resident with up to 256 experts
+    const int blocks = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
     const BalanceOut o{coef, loss, counts, offsets, rates};
     void* part = nullptr;
     if (blocks > 1 &&
-        (rc = scratch_alloc(&part, static_cast<size_t>(blocks) * part_pitch(p.experts) * 4, st)))
+        (rc = scratch_alloc(&part, static_cast<size_t>(part_words(blocks, p.experts)) * 4, st)))
         return rc;
     const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es);
-    rc = with_layout(vec, p.experts, [&](auto v, auto j) {
-        auto kern = balance_kernel<decltype(v)::value, decltype(j)::value>;
+    rc = with_layout(x_type, vec, p.experts, [&](auto t, auto v, auto j) {
+        auto kern = balance_kernel<decltype(t)::value, decltype(v)::value, decltype(j)::value>;
         const int smem = ((BW + 2) * p.experts + 1) * 4;
         static std::atomic<uint64_t> done{0};
         const cudaError_t e = allow_smem(kern, ((BW + 2) * MAX_EXPERTS + 1) * 4, done);
@@ -425,8 +492,8 @@ int gk_moe_balance(gk_matref logits, int x_type, const void* ids, size_t ids_len
                                       static_cast<uint32_t*>(part), o);
     });
     if (!rc && blocks > 1)
-        rc = launch_overlapped(balance_finish_kernel, dim3(1), 32 * BW, st,
-                               static_cast<const uint32_t*>(part), blocks, p.experts, o);
+        rc = launch_overlapped(balance_finish_kernel, dim3(static_cast<unsigned>((p.experts + 31) / 32)),
+                               32 * FW, st, static_cast<uint32_t*>(part), blocks, p.experts, o);
     const int fr = scratch_free(part, st);
     return rc ? rc : fr;
 }
@@ -462,11 +529,11 @@ int gk_moe_balance_backward(gk_matref logits, int x_type, const void* ids, size_
     int dev = 0;
     if ((rc = api_check_device(&dev))) return rc;
     p.status = device_status_ptr();
-    const int64_t want = (static_cast<int64_t>(p.tokens) + 7) / 8, most = 8ll * sm_count();
+    const int64_t want = (static_cast<int64_t>(p.tokens) + 31) / 32, most = 4ll * sm_count();
     const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es) &&
                      in_fours(dlogits.data, p.tokens, p.experts, dlogits.rs, dlogits.cs, es);
-    return with_layout(vec, p.experts, [&](auto v, auto j) {
-        return launch_overlapped(balance_backward_kernel<decltype(v)::value, decltype(j)::value>,
+    return with_layout(x_type, vec, p.experts, [&](auto t, auto v, auto j) {
+        return launch_overlapped(balance_backward_kernel<decltype(t)::value, decltype(v)::value, decltype(j)::value>,
                                  dim3(static_cast<unsigned>(want < most ? want : most)), 256,
                                  static_cast<cudaStream_t>(stream), p, rates, dloss, dlogits.data,
                                  static_cast<int64_t>(dlogits.rs), static_cast<int64_t>(dlogits.cs));

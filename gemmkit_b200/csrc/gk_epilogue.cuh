@@ -10,7 +10,7 @@
 // A lane holds one P row (a column of C) and consecutive Q rows (rows of C), so a bias is one value
 // a lane and a column sum one register. 16-bit matrices with unit column stride move in pairs: of
 // two neighbouring lanes the even one reads and writes four bytes of the even Q rows, the odd one of
-// the odd ones (store_pairs), half as many instructions as element by element; the halves are
+// the odd ones, half as many instructions as element by element; the halves are
 // exchanged by one shuffle for four elements. The same lane reads an element of R (or z) and
 // later stores that of C, so C may be R (or z) itself.
 #pragma once
@@ -26,7 +26,11 @@
 
 namespace gk {
 
-enum : int { EPI_STORE = 0, EPI_FWD = 1, EPI_BWD = 2 };
+// What a kernel does with its accumulators; EPI_F16 is added where 16-bit matrices hold f16 (else bf16).
+enum : int { EPI_STORE = 0, EPI_FWD = 1, EPI_BWD = 2, EPI_F16 = 4 };
+constexpr bool epi_fwd(int epi) { return (epi & 3) == EPI_FWD; }
+constexpr bool epi_bwd(int epi) { return (epi & 3) == EPI_BWD; }
+constexpr bool epi_f16(int epi) { return (epi & EPI_F16) != 0; }
 
 struct EpiArgs {
     int32_t act;              // gk_act
@@ -48,28 +52,55 @@ struct EpiArgs {
 // ---- activations ------------------------------------------------------------------------------------
 //
 // ReLU and LeakyReLU as in the engine's other epilogues (fused_apply: a NaN becomes 0). GELU and SiLU
-// keep a NaN; an argument below -100 counts as -100 (the value is -0 from far above that on in f32),
-// so that minus infinity gives the limit 0 instead of inf * 0.
-//   GELU is z Phi(z), Phi(z) = (1 + erf(z / sqrt 2)) / 2; its tanh form is z sigma(2 u), u = sqrt(2 / pi)
-// (z + 0.044715 z^3), since (1 + tanh u) / 2 = sigma(2 u); SiLU is z sigma(z). sigma(t) = 1 / (1 +
-// exp(-t)) by the fast exponential and division: about 2^-21 + |t| 2^-24 off relative to it, at most a
-// thousandth of a 16-bit rounding wherever the result is not below 2^-100.
+// keep a NaN; magnitudes beyond 100 count as 100 where only the limit is left of them, so that an
+// infinity gives the limit instead of inf * 0.
+//   GELU is z Phi(z). With q = Phi(-|z|): max(z, 0) - |z| q, and its derivative 1/2 +- (1/2 - q) + z phi(z).
+// q comes from Abramowitz and Stegun's formula 7.1.26 for erfc (five terms in t = 1 / (1 + p x) times
+// exp(-x^2), at most 1.5e-7 off, so q is 7.5e-8 off and its terms' roundings), whose exponential is
+// phi's too: 14 and 17 instructions, where erff and a second exponential took about 45.
+//   Its tanh form is z sigma(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3), since (1 + tanh u) / 2 = sigma(2 u);
+// SiLU is z sigma(z). sigma(t) = 1 / (1 + 2^(-t log2 e)) by the hardware's exponential and reciprocal
+// (2^-22 and 2^-23 relative), the argument's rounding |t| 2^-24 on top. All of it is below a
+// hundredth of a 16-bit rounding.
 
+// min(|x|, |y|) with the product's sign (here: x clamped to +-y), a NaN kept.
+__device__ __forceinline__ float clamp_nan(float x, float y) {
+    float r;
+    asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float min_nan(float a, float b) {
+__device__ __forceinline__ float exp2_hw(float x) {
     float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_hw(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
-__device__ __forceinline__ float sigmoid(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
+constexpr float LOG2E = 1.44269504f, RSQRT_2PI = 0.39894228f;
+constexpr float GELU_C = 0.044715f, GELU_2K = 1.59576912f;  // 2 sqrt(2 / pi)
 
-constexpr float SQRT_HALF = 0.70710678f, SQRT_2_PI = 0.79788456f, RSQRT_2PI = 0.39894228f;
-constexpr float GELU_C = 0.044715f;
+// 1 / (1 + 2^w)
+__device__ __forceinline__ float sigma2(float w) { return rcp_hw(1.0f + exp2_hw(w)); }
+
+// Phi(-a) for 0 <= a <= 100, and e = exp(-a^2 / 2) = phi(a) sqrt(2 pi).
+__device__ __forceinline__ float normal_tail(float a, float& e) {
+    const float t = rcp_hw(fmaf(0.3275911f * 0.70710678f, a, 1.0f));
+    e = exp2_hw(a * a * (-0.5f * LOG2E));
+    float y = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    y = fmaf(y, t, 0.5f * 1.421413741f);
+    y = fmaf(y, t, 0.5f * -0.284496736f);
+    y = fmaf(y, t, 0.5f * 0.254829592f);
+    return y * t * e;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_value(float z, float slope) {
@@ -78,21 +109,20 @@ __device__ __forceinline__ float act_value(float z, float slope) {
     } else if constexpr (ACT == GK_ACT_LEAKY_RELU) {
         return fmaf(slope, z < 0.0f ? z : 0.0f, z > 0.0f ? z : 0.0f);
     } else if constexpr (ACT == GK_ACT_GELU) {
-        z = max_nan(z, -100.0f);
-        const float h = 0.5f * z;
-        return fmaf(h, erff(z * SQRT_HALF), h);
+        const float a = fabsf(clamp_nan(z, 100.0f));
+        float e;
+        return fmaf(-a, normal_tail(a, e), max_nan(z, 0.0f));
     } else if constexpr (ACT == GK_ACT_GELU_TANH) {
         z = max_nan(z, -100.0f);
-        return z * sigmoid(2.0f * SQRT_2_PI * fmaf(GELU_C * z * z, z, z));
+        return z * sigma2(-z * fmaf(GELU_2K * LOG2E * GELU_C, z * z, GELU_2K * LOG2E));
     } else if constexpr (ACT == GK_ACT_SILU) {
         z = max_nan(z, -100.0f);
-        return z * sigmoid(z);
+        return z * sigma2(z * -LOG2E);
     } else {
         return z;
     }
 }
 
-// The derivative. GELU and SiLU take arguments beyond +-100 as +-100 (the limits 0 and 1).
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z, float slope) {
     if constexpr (ACT == GK_ACT_RELU) {
@@ -100,17 +130,19 @@ __device__ __forceinline__ float act_slope(float z, float slope) {
     } else if constexpr (ACT == GK_ACT_LEAKY_RELU) {
         return z > 0.0f ? 1.0f : slope;
     } else if constexpr (ACT == GK_ACT_GELU) {
-        z = min_nan(max_nan(z, -100.0f), 100.0f);
-        return fmaf(z * RSQRT_2PI, __expf(-0.5f * z * z), fmaf(0.5f, erff(z * SQRT_HALF), 0.5f));
+        z = clamp_nan(z, 100.0f);
+        float e;
+        const float half = 0.5f - normal_tail(fabsf(z), e);
+        return fmaf(z * RSQRT_2PI, e, 0.5f + copysignf(half, z));
     } else if constexpr (ACT == GK_ACT_GELU_TANH) {
-        z = min_nan(max_nan(z, -100.0f), 100.0f);
+        z = clamp_nan(z, 100.0f);
         const float z2 = z * z;
-        const float s = sigmoid(2.0f * SQRT_2_PI * fmaf(GELU_C * z2, z, z));
-        return fmaf(z * s * (1.0f - s), 2.0f * SQRT_2_PI * fmaf(3.0f * GELU_C, z2, 1.0f), s);
+        const float s = sigma2(-z * fmaf(GELU_2K * LOG2E * GELU_C, z2, GELU_2K * LOG2E));
+        return fmaf(z * fmaf(-s, s, s), fmaf(3.0f * GELU_C * GELU_2K, z2, GELU_2K), s);
     } else if constexpr (ACT == GK_ACT_SILU) {
-        z = min_nan(max_nan(z, -100.0f), 100.0f);
-        const float s = sigmoid(z);
-        return fmaf(z * s, 1.0f - s, s);
+        z = clamp_nan(z, 100.0f);
+        const float s = sigma2(z * -LOG2E);
+        return fmaf(z, fmaf(-s, s, s), s);
     } else {
         return 1.0f;
     }
@@ -149,20 +181,25 @@ __device__ __forceinline__ float half_hi(uint32_t w, int f16) {
                : __uint_as_float(w & 0xFFFF0000u);
 }
 
-// The loads of store_pairs' layout, not yet exchanged: N words hold the 2 N columns of this lane pair.
+// The loads of that layout, not yet exchanged: N words hold the 2 N columns of this lane pair.
 template <int N>
 __device__ __forceinline__ void load_pairs(uint32_t (&w)[N], const uint16_t* c, int64_t ldq, int n,
                                            int pn, int lane) {
     const int odd = lane & 1;
     const uint16_t* q = c + (lane & 30) + odd * ldq;
+    if (n >= 2 * N && pn >= 32) {  // (the warp's; no predicates)
+#pragma unroll
+        for (int j = 0; j < N; ++j, q += 2 * ldq) w[j] = *reinterpret_cast<const uint32_t*>(q);
+        return;
+    }
     const int left = (lane & 30) < pn ? n - odd : 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-        w[j] = 2 * j < left ? *reinterpret_cast<const uint32_t*>(q + 2 * j * ldq) : 0u;
+    for (int j = 0; j < N; ++j, q += 2 * ldq)
+        w[j] = 2 * j < left ? *reinterpret_cast<const uint32_t*>(q) : 0u;
 }
 
-// The exchange: w[j] becomes columns 2 j and 2 j + 1 of this lane's own P row (store_pairs' exchange
-// undone, which is the same one).
+// The exchange: w[j] becomes columns 2 j and 2 j + 1 of this lane's own P row (and back: the exchange undoes
+// itself).
 template <int N>
 __device__ __forceinline__ void own_pairs(uint32_t (&w)[N], int lane) {
     const int odd = lane & 1;
@@ -174,6 +211,24 @@ __device__ __forceinline__ void own_pairs(uint32_t (&w)[N], int lane) {
         w[j] = __byte_perm(w[j], got, sel0);
         w[j + 1] = __byte_perm(w[j + 1], got, sel1);
     }
+}
+
+// 2 N columns of this lane's own P row, rounded, into a matrix that moves in pairs; w is used up.
+template <int N>
+__device__ __forceinline__ void put_pairs(uint32_t (&w)[N], uint16_t* c, int64_t ldq, int n, int pn,
+                                          int lane) {
+    own_pairs(w, lane);
+    const int odd = lane & 1;
+    uint16_t* q = c + (lane & 30) + odd * ldq;
+    if (n >= 2 * N && pn >= 32) {
+#pragma unroll
+        for (int j = 0; j < N; ++j, q += 2 * ldq) *reinterpret_cast<uint32_t*>(q) = w[j];
+        return;
+    }
+    const int left = (lane & 30) < pn ? n - odd : 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j, q += 2 * ldq)
+        if (2 * j < left) *reinterpret_cast<uint32_t*>(q) = w[j];
 }
 
 // ---- a warp's accumulators ----------------------------------------------------------------------------
@@ -195,7 +250,7 @@ struct EpiSide {
     // PAIRS: see EpiArgs; f32 sides are read where they are used.
     template <bool PAIRS>
     __device__ __forceinline__ void load(const EpiArgs& e, const EpiAt& at, bool f32, int lane) {
-        if (EPI == EPI_BWD && e.z8.codes) {
+        if (epi_bwd(EPI) && e.z8.codes) {
 #pragma unroll
             for (int j = 0; j < N / 4; ++j) {
                 const int c = 4 * j + (lane >> 3);
@@ -227,7 +282,7 @@ struct EpiSide {
     // After load(): the pairs' exchange, or this lane's byte positions.
     template <bool PAIRS>
     __device__ __forceinline__ void own(const EpiArgs& e, int lane) {
-        if (EPI == EPI_BWD && e.z8.codes) {
+        if (epi_bwd(EPI) && e.z8.codes) {
 #pragma unroll
             for (int j = 0; j < N / 4; ++j) w[j] ^= 0x80808080u;
             sb = __float_as_uint(act8_unit(sb));
@@ -241,46 +296,35 @@ struct EpiSide {
         const float unit = __uint_as_float(__shfl_sync(0xffffffffu, sb, c));
         return act8_code(x, lane & 3) * unit;
     }
-    __device__ __forceinline__ float half(int c, int f16) const {
-        return c & 1 ? half_hi(w[c / 2], f16) : half_lo(w[c / 2], f16);
+    __device__ __forceinline__ float half(int c) const {
+        return c & 1 ? half_hi(w[c / 2], epi_f16(EPI)) : half_lo(w[c / 2], epi_f16(EPI));
     }
 };
 
 // N accumulators of each lane (f32 bits), their side loaded and owned, through the activation and into
 // C: a row of C is 32 P rows of the warp. `sum` gains the stored columns (backward).
-template <int EPI, int ACT, int N, bool PAIRS>
-__device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_type, int f16,
+template <int EPI, int N, bool PAIRS>
+__device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_type,
                                             int64_t ldq, int64_t ldp, const EpiAt& at,
                                             const uint32_t (&v)[N], const EpiSide<EPI, N>& s,
                                             float alpha, float bias, float& sum, int lane) {
+    constexpr bool f16 = epi_f16(EPI);
     float y[N];
     const bool live = lane < at.pn;
     const int64_t own = (at.i0 + lane) * ldp + at.r * ldq;  // element by element
-    if constexpr (EPI == EPI_FWD) {
+    if constexpr (epi_fwd(EPI)) {
         uint32_t zw[N / 2];
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
             const float a = fmaf(alpha, __uint_as_float(v[j]), bias);
             const float b = fmaf(alpha, __uint_as_float(v[j + 1]), bias);
             zw[j / 2] = pack_half2(a, b, f16);
-            y[j] = act_value<ACT>(a, e.slope);
-            y[j + 1] = act_value<ACT>(b, e.slope);
-        }
-        if (e.side) {
-            if (PAIRS || out_type != GK_F32) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) y[j] += s.half(j, f16);
-            } else {
-                const float* r = static_cast<const float*>(e.side) + (at.i0 + lane) * e.sp +
-                                 at.r * e.sq;
-                const int n = live ? at.n : 0;
-#pragma unroll
-                for (int j = 0; j < N; ++j) y[j] += j < n ? r[j * e.sq] : 0.0f;
-            }
+            y[j] = a;
+            y[j + 1] = b;
         }
         if (e.z) {
             if constexpr (PAIRS) {
-                store_pairs(zw, e.z + at.r * e.zq + at.i0, e.zq, at.n, at.pn, lane);
+                put_pairs(zw, e.z + at.r * e.zq + at.i0, e.zq, at.n, at.pn, lane);
             } else {
                 uint16_t* z = e.z + (at.i0 + lane) * e.zp + at.r * e.zq;
 #pragma unroll
@@ -289,19 +333,46 @@ __device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_t
                         z[j * e.zq] = static_cast<uint16_t>(zw[j / 2] >> (16 * (j & 1)));
             }
         }
+        with_act(e.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) y[j] = act_value<decltype(act)::value>(y[j], e.slope);
+        });
+        if (e.side) {
+            if (PAIRS || out_type != GK_F32) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) y[j] += s.half(j);
+            } else {
+                const float* r = static_cast<const float*>(e.side) + (at.i0 + lane) * e.sp +
+                                 at.r * e.sq;
+                const int n = live ? at.n : 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) y[j] += j < n ? r[j * e.sq] : 0.0f;
+            }
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float z = e.z8.codes ? s.z8(j, lane) : s.half(j, f16);
-            y[j] = alpha * __uint_as_float(v[j]) * act_slope<ACT>(z, e.slope);
+        for (int j = 0; j < N; ++j) y[j] = alpha * __uint_as_float(v[j]);
+        with_act(e.act, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            if constexpr (ACT != GK_ACT_NONE) {
+                if (e.z8.codes) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) y[j] *= act_slope<ACT>(s.z8(j, lane), e.slope);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) y[j] *= act_slope<ACT>(s.half(j), e.slope);
+                }
+            }
+        });
+#pragma unroll
+        for (int j = 0; j < N; ++j)
             if (j < at.n) sum += y[j];
-        }
     }
     if constexpr (PAIRS) {
         uint32_t w[N / 2];
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) w[j] = pack_half2(y[2 * j], y[2 * j + 1], f16);
-        store_pairs(w, static_cast<uint16_t*>(c) + at.r * ldq + at.i0, ldq, at.n, at.pn, lane);
+        put_pairs(w, static_cast<uint16_t*>(c) + at.r * ldq + at.i0, ldq, at.n, at.pn, lane);
     } else if (out_type == GK_F32) {
 #pragma unroll
         for (int j = 0; j < N; ++j)

@@ -258,35 +258,32 @@ __device__ __forceinline__ void epi_tile(const GroupedParams& p, const GTile& t,
                                          uint32_t tb, int wcols, int cbase, int i0, int pn, int share,
                                          int shares, int lane) {
     const float alpha = tile_alpha(p, t);
-    const float bias = EPI == EPI_FWD ? epi_bias(p.e, t.g, i0, pn, lane) : 0.0f;
+    const float bias = epi_fwd(EPI) ? epi_bias(p.e, t.g, i0, pn, lane) : 0.0f;
     float sum = 0.0f;
-    with_act(p.e.act, [&](auto act) {
-        auto columns = [&](auto pairs) {
-            constexpr bool PAIRS = decltype(pairs)::value;
+    auto columns = [&](auto pairs) {
+        constexpr bool PAIRS = decltype(pairs)::value;
 #pragma unroll 1
-            for (int c = 0; c < wcols && cbase + c < t.qn; c += 16) {
-                const EpiAt at{i0, pn, t.qbase + cbase + c, t.qn - cbase - c};
-                EpiSide<EPI, 16> s;
-                s.template load<PAIRS>(p.e, at, EPI == EPI_FWD && p.out_type == GK_F32, lane);
-                uint32_t v[16];
-                if (t.nk > 0) {
-                    tmem_ld_cols16(tb + c, v);
-                } else {
+        for (int c = 0; c < wcols && cbase + c < t.qn; c += 16) {
+            const EpiAt at{i0, pn, t.qbase + cbase + c, t.qn - cbase - c};
+            EpiSide<EPI, 16> s;
+            s.template load<PAIRS>(p.e, at, epi_fwd(EPI) && p.out_type == GK_F32, lane);
+            uint32_t v[16];
+            if (t.nk > 0) {
+                tmem_ld_cols16(tb + c, v);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = 0u;
-                }
-                s.template own<PAIRS>(p.e, lane);
-                epi_columns<EPI, decltype(act)::value, 16, PAIRS>(p.e, p.c, p.out_type, p.f16, p.ldq,
-                                                                  p.ldp, at, v, s, alpha, bias, sum,
-                                                                  lane);
+                for (int i = 0; i < 16; ++i) v[i] = 0u;
             }
-        };
-        if (p.e.pairs)
-            columns(std::true_type{});
-        else
-            columns(std::false_type{});
-    });
-    if constexpr (EPI == EPI_BWD) epi_sum(p, t, tile0, i0, pn, share, shares, sum, lane);
+            s.template own<PAIRS>(p.e, lane);
+            epi_columns<EPI, 16, PAIRS>(p.e, p.c, p.out_type, p.ldq, p.ldp, at, v, s, alpha, bias,
+                                        sum, lane);
+        }
+    };
+    if (p.e.pairs)
+        columns(std::true_type{});
+    else
+        columns(std::false_type{});
+    if constexpr (epi_bwd(EPI)) epi_sum(p, t, tile0, i0, pn, share, shares, sum, lane);
 }
 
 template <int BN, int EPI>
@@ -547,8 +544,14 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
 template <int PB, int EPI>
 struct GPairCfg {
     static constexpr int BN = 256;
-    // PB = 2 holds a warp's accumulators in registers (see above): 64 where a whole epilogue follows
-    static constexpr int NEPI = EPI != EPI_STORE && PB == 2 ? 16 : 8;
+    static constexpr int NEPI = 8;
+    // A whole epilogue on tall tiles keeps 128 accumulators a lane in registers (epi_tall): the four
+    // other warps give theirs up for it (setmaxnreg). 128 x 56 + 256 x 224 registers are the
+    // 384 x 168 that the block is launched with.
+    static constexpr bool SPLIT_REGS = EPI != EPI_STORE && PB == 2;
+    static constexpr int REGS_OTHER = 56, REGS_EPI = 224;
+    static_assert(!SPLIT_REGS || 128 * REGS_OTHER + 32 * NEPI * REGS_EPI <= 32 * (4 + NEPI) * 168,
+                  "registers of the block");
     static constexpr int EPI_W0 = 4;
     static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
     static constexpr int WCOLS = BN / (NEPI / 4);
@@ -568,41 +571,46 @@ struct GPairCfg {
     static_assert(STAGES >= 4 && (4 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
 };
 
-// A warp's 64 columns of a tall tile's accumulator through the epilogue: all of them go to registers
+// A warp's 128 columns of a tall tile's accumulator through the epilogue: all of them go to registers
 // and the accumulator is handed back before any of the arithmetic, which then passes under the MMAs.
 // (C moves in pairs.)
 template <int EPI>
 __device__ __forceinline__ void epi_tall(const GroupedParams& p, const GTile& t, const int* tile0,
-                                         uint32_t tb, int cbase, int i0, int pn, int share,
+                                         uint32_t tb, int cbase, int i0, int pn, int share, int shares,
                                          uint32_t tempty, int lane) {
-    uint32_t lo[32], hi[32];
-    tmem_ld_x32_nowait(tb, lo);
-    tmem_ld_x32_nowait(tb + 32, hi);
+    uint32_t raw[8][16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tmem_ld_cols16_nowait(tb + 16 * i, raw[i]);
     tmem_wait_ld();
-    reg_fence<32>(lo);
-    reg_fence<32>(hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) frag_fence(raw[i]);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster_relaxed(tempty);
     if (pn <= 0) return;
-    const float bias = EPI == EPI_FWD ? epi_bias(p.e, t.g, i0, pn, lane) : 0.0f;
+    const float bias = epi_fwd(EPI) ? epi_bias(p.e, t.g, i0, pn, lane) : 0.0f;
     float sum = 0.0f;
-    with_act(p.e.act, [&](auto act) {
+    auto columns = [&](int c, const uint32_t(&v)[16]) {
+        const EpiAt at{i0, pn, t.qbase + cbase + c, t.qn - cbase - c};
+        if (at.n <= 0) return;
+        EpiSide<EPI, 16> s;
+        s.template load<true>(p.e, at, false, lane);
+        s.template own<true>(p.e, lane);
+        epi_columns<EPI, 16, true>(p.e, p.c, p.out_type, p.ldq, 1, at, v, s, p.alpha, bias, sum, lane);
+    };
+    // A loop, the accumulators moved up after each 32 columns: unrolled over all 128 the code left the
+    // instruction cache behind (8192 x 4096 -> 14336 with GELU and z kept: 926 us,
+    // now 680).
+#pragma unroll 1
+    for (int c = 0; c < 128 && cbase + c < t.qn; c += 32) {
+        columns(c, raw[0]);
+        columns(c + 16, raw[1]);
 #pragma unroll
-        for (int c = 0; c < 64; c += 16) {
-            const EpiAt at{i0, pn, t.qbase + cbase + c, t.qn - cbase - c};
-            if (at.n <= 0) break;
-            EpiSide<EPI, 16> s;
-            s.template load<true>(p.e, at, false, lane);
-            uint32_t v[16];
+        for (int i = 0; i < 6; ++i)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = c < 32 ? lo[(c & 16) + i] : hi[(c & 16) + i];
-            s.template own<true>(p.e, lane);
-            epi_columns<EPI, decltype(act)::value, 16, true>(p.e, p.c, p.out_type, p.f16, p.ldq, 1, at,
-                                                             v, s, p.alpha, bias, sum, lane);
-        }
-    });
-    if constexpr (EPI == EPI_BWD) epi_sum(p, t, tile0, i0, pn, share, 4, sum, lane);
+            for (int j = 0; j < 16; ++j) raw[i][j] = raw[i + 2][j];
+    }
+    if constexpr (epi_bwd(EPI)) epi_sum(p, t, tile0, i0, pn, share, shares, sum, lane);
 }
 
 template <int PB, int EPI>
@@ -668,7 +676,10 @@ __global__ void __launch_bounds__(GPairCfg<PB, EPI>::THREADS, 1)
     GroupWalk walk(off, tile0, p.groups, blockIdx.x >> 1, gridDim.x >> 1);
     GTile t;
 
+    // (Each role's branch sets its own registers: after a common point the compiler would have to
+    // count on the smaller number.)
     if (warp == 0) {
+        if constexpr (C::SPLIT_REGS) regs_dec<C::REGS_OTHER>();
         // ---------------- TMA producer (both CTAs; the whole warp, one lane issues) ------------
         int stage = 0;
         uint32_t phase = 0, issued = 0, last_par = 0;
@@ -739,6 +750,7 @@ __global__ void __launch_bounds__(GPairCfg<PB, EPI>::THREADS, 1)
                               GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp == 1) {
+        if constexpr (C::SPLIT_REGS) regs_dec<C::REGS_OTHER>();
         if (leader) {
             // ---------------- MMA issuer (leader; the whole warp, one lane issues) ----------------
             int stage = 0;
@@ -842,6 +854,7 @@ __global__ void __launch_bounds__(GPairCfg<PB, EPI>::THREADS, 1)
             mbar_wait(drain, 0, &dummy, p.status, GK_DEV_TIMEOUT_DRAIN, tmo);
         }
     } else if (warp == 2) {
+        if constexpr (C::SPLIT_REGS) regs_dec<C::REGS_OTHER>();
         // ---------------- the contraction's ragged end (both CTAs) ----------------
         // Each CTA's warp zeroes its own half; the leader's completes full[] once both have.
         if (p.wgrad) {
@@ -872,6 +885,7 @@ __global__ void __launch_bounds__(GPairCfg<PB, EPI>::THREADS, 1)
             }
         }
     } else if (warp >= C::EPI_W0) {
+        if constexpr (C::SPLIT_REGS) regs_inc<C::REGS_EPI>();
         // ---------------- epilogue (both CTAs) ----------------
         const int q = warp & 3;
         const int cbase = ((warp - C::EPI_W0) >> 2) * C::WCOLS;
@@ -894,7 +908,7 @@ __global__ void __launch_bounds__(GPairCfg<PB, EPI>::THREADS, 1)
                     const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
                     if constexpr (EPI != EPI_STORE) {
                         epi_tall<EPI>(p, t, tile0, tb, cbase, i0, pn, (warp - C::EPI_W0) >> 2,
-                                      tempty_l + 8u * b, lane);
+                                      C::NEPI / 4, tempty_l + 8u * b, lane);
                     } else {
                     uint32_t w[C::WCOLS / 2];
                     if (t.nk > 0) {
@@ -958,6 +972,8 @@ __global__ void __launch_bounds__(GPairCfg<PB, EPI>::THREADS, 1)
                 if (lane == 0) mbar_arrive_cluster_relaxed(tempty_l + 8u * acc);
             }
         }
+    } else {
+        if constexpr (C::SPLIT_REGS) regs_dec<C::REGS_OTHER>();
     }
 
     tc_fence_before();
@@ -1214,9 +1230,9 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
             default: return go(std::integral_constant<int, 256>{});
         }
     };
-    if constexpr (EPI == EPI_BWD) {
+    if constexpr (epi_bwd(EPI)) {
         if (p.e.dbias) {  // a slot for each share of each tile along the Q side
-            const int shares = tall ? GPairCfg<2, EPI>::NEPI / 4 : bn == 32 ? 1 : 2;
+            const int shares = bn == 32 ? 1 : 2;  // NEPI / 4 of each kernel
             const int64_t slots = ((static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups) * shares;
             void* part = nullptr;
             if ((rc = scratch_alloc(&part, static_cast<size_t>(slots * p.np) * 4, stream))) return rc;

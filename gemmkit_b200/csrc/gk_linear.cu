@@ -65,9 +65,11 @@ namespace {
 
 // ---- the gradient without a product -----------------------------------------------------------------------
 //
-// Bound by memory: dy and z are read and dz is written once. A block takes GR rows x 32 V columns, a
-// warp every eighth of the rows, with V consecutive columns a lane (16 bytes) where every matrix
-// allows that, else one; rows are read four at a time so that enough loads are in flight.
+// Bound by memory: dy and z are read and dz is written once. A block walks tiles of GR rows x 32 V
+// columns, a warp takes every eighth row, with V consecutive columns a lane (16 bytes) where every
+// matrix allows that, else one; rows are read two at a time, by 32 warps of an SM. The
+// grid is what is resident: a block per tile spent more on starting (the groups' table) than a tile
+// takes (57 us for 8192 x 4096 by 8 groups with SiLU, now 39).
 
 constexpr int GR = 64, GW = 8;
 
@@ -117,8 +119,8 @@ struct GradRow {
     }
 };
 
-template <int V>
-__global__ void __launch_bounds__(32 * GW) act_grad_kernel(const ActGrad p) {
+template <int V, bool F16>
+__global__ void __launch_bounds__(32 * GW, 4) act_grad_kernel(const ActGrad p) {
     __shared__ int off[GROUP_TABLE_INTS], tile0[GROUP_TABLE_INTS];
     __shared__ float red[GW][32 * V];
     griddep_wait();
@@ -126,49 +128,59 @@ __global__ void __launch_bounds__(32 * GW) act_grad_kernel(const ActGrad p) {
     load_groups(p.offsets, p.groups, p.rows, off, tile0,
                 blockIdx.x == 0 ? p.status : nullptr, [](int m) { return (m + GR - 1) / GR; });
     const unsigned blocks = static_cast<unsigned>((p.np + 32 * V - 1) / (32 * V));  // along the columns
-    const int t = static_cast<int>(blockIdx.x / blocks);
-    const int64_t c0 = static_cast<int64_t>(blockIdx.x % blocks) * 32 * V;
-    if (t >= tile0[p.groups]) return;
-    int lo = 0, hi = p.groups;  // the group of tile t: tile0[lo] <= t < tile0[lo + 1]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tile0[mid] <= t)
-            lo = mid;
-        else
-            hi = mid;
-    }
+    const unsigned total = static_cast<unsigned>(tile0[p.groups]) * blocks;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int r0 = off[lo] + (t - tile0[lo]) * GR, r1 = min(r0 + GR, off[lo + 1]);
-    const int64_t c = c0 + lane * V;
-    const bool live = c < p.np;
-    float sum[V];
+    for (unsigned u = blockIdx.x; u < total; u += gridDim.x) {
+        const int t = static_cast<int>(u / blocks);
+        const int64_t c0 = static_cast<int64_t>(u - t * blocks) * 32 * V;
+        int lo = 0, hi = p.groups;  // the group of tile t: tile0[lo] <= t < tile0[lo + 1]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (tile0[mid] <= t)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        const int r0 = off[lo] + (t - tile0[lo]) * GR, r1 = min(r0 + GR, off[lo + 1]);
+        const int64_t c = c0 + lane * V;
+        const bool live = c < p.np;
+        float sum[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = 0.0f;
-    with_act(p.e.act, [&](auto act) {
+        for (int i = 0; i < V; ++i) sum[i] = 0.0f;
 #pragma unroll 1
-        for (int r = r0 + w; live && r < r1; r += 4 * GW) {
-            GradRow<V> row[4];
+        for (int r = r0 + w; live && r < r1; r += 2 * GW) {
+            GradRow<V> row[2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 2; ++k)
                 if (r + k * GW < r1) row[k].load(p, r + k * GW, c);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 const int64_t at = r + k * GW;
                 if (at >= r1) break;
                 float d[V];
-                const float unit = p.e.z8.codes ? act8_unit(row[k].x) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const uint32_t yw = row[k].y[i / 2];
-                    const float y = i & 1 ? half_hi(yw, p.f16) : half_lo(yw, p.f16);
-                    float z;
-                    if (p.e.z8.codes)
-                        z = act8_code(row[k].z[i / 4] ^ 0x80808080u, i & 3) * unit;
-                    else
-                        z = i & 1 ? half_hi(row[k].z[i / 2], p.f16) : half_lo(row[k].z[i / 2], p.f16);
-                    d[i] = y * act_slope<decltype(act)::value>(z, p.e.slope);
-                    sum[i] += d[i];
+                    d[i] = i & 1 ? half_hi(yw, F16) : half_lo(yw, F16);
                 }
+                with_act(p.e.act, [&](auto act) {
+                    constexpr int ACT = decltype(act)::value;
+                    if constexpr (ACT != GK_ACT_NONE) {
+                        const float unit = p.e.z8.codes ? act8_unit(row[k].x) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            float z;
+                            if (p.e.z8.codes)
+                                z = act8_code(row[k].z[i / 4] ^ 0x80808080u, i & 3) * unit;
+                            else
+                                z = i & 1 ? half_hi(row[k].z[i / 2], F16)
+                                          : half_lo(row[k].z[i / 2], F16);
+                            d[i] *= act_slope<ACT>(z, p.e.slope);
+                        }
+                    }
+                });
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] += d[i];
                 if (!p.dz) continue;
                 const int64_t o = at * p.zq + c * p.zp;
                 if constexpr (V == 8) {
@@ -179,30 +191,30 @@ __global__ void __launch_bounds__(32 * GW) act_grad_kernel(const ActGrad p) {
                         st_global_v4(f + 4, __float_as_uint(d[4]), __float_as_uint(d[5]),
                                      __float_as_uint(d[6]), __float_as_uint(d[7]));
                     } else {
-                        st_global_v4(static_cast<uint16_t*>(p.dz) + o, pack_half2(d[0], d[1], p.f16),
-                                     pack_half2(d[2], d[3], p.f16), pack_half2(d[4], d[5], p.f16),
-                                     pack_half2(d[6], d[7], p.f16));
+                        st_global_v4(static_cast<uint16_t*>(p.dz) + o, pack_half2(d[0], d[1], F16),
+                                     pack_half2(d[2], d[3], F16), pack_half2(d[4], d[5], F16),
+                                     pack_half2(d[6], d[7], F16));
                     }
                 } else if (p.out_type == GK_F32) {
                     static_cast<float*>(p.dz)[o] = d[0];
                 } else {
                     static_cast<uint16_t*>(p.dz)[o] =
-                        static_cast<uint16_t>(pack_half2(d[0], 0.0f, p.f16));
+                        static_cast<uint16_t>(pack_half2(d[0], 0.0f, F16));
                 }
             }
         }
-    });
-    if (!p.part) return;
+        if (!p.part) continue;
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[w][i * 32 + lane] = sum[i];
-    __syncthreads();
-    // column lane + 32 * i of the block's 32 V: thread by thread, eight warps' sums each
-    for (int i = threadIdx.x; i < 32 * V; i += 32 * GW) {
-        float a = red[0][i];
+        for (int i = 0; i < V; ++i) red[w][i * 32 + lane] = sum[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 32 * V; i += 32 * GW) {  // column (i % 32) V + i / 32 of the tile
+            float a = red[0][i];
 #pragma unroll
-        for (int k = 1; k < GW; ++k) a += red[k][i];
-        const int64_t col = c0 + (i & 31) * V + (i >> 5);
-        if (col < p.np) p.part[static_cast<int64_t>(t) * p.np + col] = a;
+            for (int k = 1; k < GW; ++k) a += red[k][i];
+            const int64_t col = c0 + (i & 31) * V + (i >> 5);
+            if (col < p.np) p.part[static_cast<int64_t>(t) * p.np + col] = a;
+        }
+        __syncthreads();
     }
 }
 
@@ -413,7 +425,8 @@ int gk_gemm_half_epilogue(int is_f16, size_t groups, const int32_t* offsets, flo
     e.pairs = out_type != GK_F32 && in_pairs(c.data, c.rs, c.cs, c.rows, c.cols) &&
               (!e.side || in_pairs(e.side, e.sq, e.sp, c.rows, c.cols)) &&
               (!e.z || in_pairs(e.z, e.zq, e.zp, c.rows, c.cols));
-    return run_grouped<EPI_FWD>(p, static_cast<cudaStream_t>(stream));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return p.f16 ? run_grouped<EPI_FWD | EPI_F16>(p, st) : run_grouped<EPI_FWD>(p, st);
 }
 
 int gk_gemm_half_dact(int is_f16, size_t groups, const int32_t* offsets, float alpha, gk_matref a,
@@ -438,7 +451,7 @@ int gk_gemm_half_dact(int is_f16, size_t groups, const int32_t* offsets, float a
     if (!p.zero && (!a.data || !b.data)) return api_err(GK_EINVAL, "gemmkit: null A or B");
     p.e.pairs = out_type != GK_F32 && in_pairs(c.data, c.rs, c.cs, c.rows, c.cols) &&
                 (!p.e.side || in_pairs(p.e.side, p.e.sq, p.e.sp, c.rows, c.cols));
-    return run_grouped<EPI_BWD>(p, st);
+    return p.f16 ? run_grouped<EPI_BWD | EPI_F16>(p, st) : run_grouped<EPI_BWD>(p, st);
 }
 
 int gk_act_backward(int is_f16, size_t groups, const int32_t* offsets, gk_matref dy,
@@ -509,11 +522,14 @@ int gk_act_backward(int is_f16, size_t groups, const int32_t* offsets, gk_matref
                          (!p.e.side || whole(p.e.side, p.e.sq, p.e.sp, 2));
         const int v = vec ? 8 : 1;
         const int64_t blocks = tiles * ((p.np + 32 * v - 1) / (32 * v));
+        const int64_t most = 4ll * sm_count();
+        const auto kern = vec ? (p.f16 ? act_grad_kernel<8, true> : act_grad_kernel<8, false>)
+                              : (p.f16 ? act_grad_kernel<1, true> : act_grad_kernel<1, false>);
         if (blocks > INT32_MAX)
             rc = api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
         else
-            rc = launch_overlapped(vec ? act_grad_kernel<8> : act_grad_kernel<1>,
-                                   dim3(static_cast<unsigned>(blocks)), 32 * GW, st, p);
+            rc = launch_overlapped(kern, dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
+                                   32 * GW, st, p);
     }
     if (!rc && p.e.dbias)
         rc = launch_sum_parts(p.part, offsets, p.groups, rows, GR, 1, p.np, p.e, st);

@@ -328,6 +328,17 @@ __device__ __forceinline__ void tmem_ld_cols16(uint32_t taddr, uint32_t (&r)[16]
         : "r"(taddr));
 }
 
+__device__ __forceinline__ void tmem_ld_cols16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 // Non-blocking TMEM loads of a CH-column chunk (32 or 16); pair with tmem_wait_ld() and
 // reg_fence() before reading the registers.
 __device__ __forceinline__ void tmem_ld_x32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
@@ -427,6 +438,18 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t caddr, uint32_t a, uint32
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(caddr), "r"(a), "r"(b),
                  "r"(c), "r"(d)
                  : "memory");
+}
+
+// ---- registers between warpgroups (every warp of an aligned group of four executes it) --------------
+// What regs_inc takes must have been given up by regs_dec: the shares' sum stays within what the block
+// was launched with, or regs_inc would wait forever.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---- programmatic dependent launch ---------------------------------------------------------

@@ -1,8 +1,8 @@
 """The router's balance loss, counts and gradient against 64-bit forms.
 
-Bounds: expf is 2 units of 2^-24 off, a difference of logits half a unit (times its size: at most 2^-24
-|x - max|, below 100 here where p matters: p < e^-88 is below any bound), a softmax's sum and division
-at most 11 + 2 more steps: 128 2^-24 relative to p covers all. Sums over a warp's tokens (at most 64
+Bounds: the fast exponential is 4 units of 2^-24 off, a difference of logits and its product with log2 e one
+unit each times its size (at most 2^-24 |x - max|, below 50 here where p matters: p < e^-50 is below
+any bound), a softmax's sum and division at most 11 + 2 more steps: 128 2^-24 relative to p covers all. Sums over a warp's tokens (at most 64
 here) add 64 2^-24 of the sum; the blocks are added in 64 bits. dlogits: p's bound twice, the dot
 over at most 1024 experts in trees of 32 by at most 32 steps, and half a step of the type.
 """

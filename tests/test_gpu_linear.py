@@ -3,9 +3,10 @@
 Bounds. The accumulators: products of 16-bit floats are exact in f32, a step of the sum loses at most
 2^-23 of the sum of magnitudes, at most k + 32 steps; alpha and the bias add a rounding of 2^-24 each
 (counted as 4 steps). Activations and derivatives: |act'| < 1.13, |act''| < 1.2; their own evaluation in
-f32 is at most 2^-20 |z| off for values (erf to 2 units of 2^-24 times |z| / 2; sigma to 2^-21 relative, and
-sigma (1 - sigma) |t| < 0.23 for the error of its argument) and 2^-18 for derivatives, which add two such
-terms of |z| phi(z) and z sigma (1 - sigma) 2 u' < 0.6. R adds one rounding; the type half a step.
+f32 is at most 2^-20 |z| off for values (Phi to 7.5e-8, half of the 1.5e-7 that formula 7.1.26 of Abramowitz
+and Stegun leaves, and a few roundings; sigma to 2^-21 relative, and sigma (1 - sigma) |t| < 0.23 for the
+error of its argument) and 2^-18 for derivatives, which add two such terms of |z| phi(z) and z sigma
+(1 - sigma) 2 u' < 0.6. R adds one rounding; the type half a step.
 Small integers make the accumulators exact, and the piecewise linear activations then leave one rounding.
 Column sums: each value's bound, and 2^-24 of the sum of magnitudes for each of at most 256 + 16 steps.
 """
