@@ -27,8 +27,11 @@ __device__ __forceinline__ float act8_unit(uint32_t b) {
 // Code k (0 .. 3) of a word of four, each with its sign bit flipped (word ^ 0x80808080), as a float:
 // placed under the exponent of 2^23 it reads 2^23 + 128 + code. (Two instructions at full rate;
 // a conversion from an integer runs at a quarter of it.)
+__device__ __forceinline__ float act8_raw(uint32_t flipped, int k) {  // 2^23 + 128 + code
+    return __uint_as_float(__byte_perm(flipped, 0x4B000000u, 0x7650u | k));
+}
 __device__ __forceinline__ float act8_code(uint32_t flipped, int k) {
-    return __uint_as_float(__byte_perm(flipped, 0x4B000000u, 0x7650u | k)) - 8388736.0f;
+    return act8_raw(flipped, k) - 8388736.0f;
 }
 
 }  // namespace gk

@@ -57,7 +57,8 @@ struct EpiArgs {
 //   GELU is z Phi(z). With q = Phi(-|z|): max(z, 0) - |z| q, and its derivative 1/2 +- (1/2 - q) + z phi(z).
 // q comes from Abramowitz and Stegun's formula 7.1.26 for erfc (five terms in t = 1 / (1 + p x) times
 // exp(-x^2), at most 1.5e-7 off, so q is 7.5e-8 off and its terms' roundings), whose exponential is
-// phi's too: 14 and 17 instructions, where erff and a second exponential took about 45.
+// phi's too: 10 and 12 instructions an element, two elements at a time, where erff and a second
+// exponential took about 45.
 //   Its tanh form is z sigma(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3), since (1 + tanh u) / 2 = sigma(2 u);
 // SiLU is z sigma(z). sigma(t) = 1 / (1 + 2^(-t log2 e)) by the hardware's exponential and reciprocal
 // (2^-22 and 2^-23 relative), the argument's rounding |t| 2^-24 on top. All of it is below a
@@ -85,66 +86,110 @@ __device__ __forceinline__ float rcp_hw(float x) {
     return r;
 }
 
+// Two f32 in a register pair: Blackwell adds and multiplies both with one instruction.
+struct F2 {
+    uint64_t v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float a, float b) {
+        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    }
+    __device__ __forceinline__ explicit F2(float a) : F2(a, a) {}
+    __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
+    __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 clamp2(F2 x, float y) { return F2(clamp_nan(x.lo(), y), clamp_nan(x.hi(), y)); }
+__device__ __forceinline__ F2 max2(F2 x, float y) { return F2(max_nan(x.lo(), y), max_nan(x.hi(), y)); }
+__device__ __forceinline__ F2 exp2_2(F2 x) { return F2(exp2_hw(x.lo()), exp2_hw(x.hi())); }
+__device__ __forceinline__ F2 rcp2(F2 x) { return F2(rcp_hw(x.lo()), rcp_hw(x.hi())); }
+
 constexpr float LOG2E = 1.44269504f, RSQRT_2PI = 0.39894228f;
 constexpr float GELU_C = 0.044715f, GELU_2K = 1.59576912f;  // 2 sqrt(2 / pi)
 
 // 1 / (1 + 2^w)
-__device__ __forceinline__ float sigma2(float w) { return rcp_hw(1.0f + exp2_hw(w)); }
+__device__ __forceinline__ F2 sigma2(F2 w) { return rcp2(add2(exp2_2(w), F2(1.0f))); }
 
-// Phi(-a) for 0 <= a <= 100, and e = exp(-a^2 / 2) = phi(a) sqrt(2 pi).
-__device__ __forceinline__ float normal_tail(float a, float& e) {
-    const float t = rcp_hw(fmaf(0.3275911f * 0.70710678f, a, 1.0f));
-    e = exp2_hw(a * a * (-0.5f * LOG2E));
-    float y = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    y = fmaf(y, t, 0.5f * 1.421413741f);
-    y = fmaf(y, t, 0.5f * -0.284496736f);
-    y = fmaf(y, t, 0.5f * 0.254829592f);
-    return y * t * e;
+// Phi(-|z|) for |z| <= 100, from n = -|z|, and e = exp(-z^2 / 2) = phi(z) sqrt(2 pi).
+__device__ __forceinline__ F2 normal_tail(F2 n, F2& e) {
+    const F2 t = rcp2(fma2(n, F2(-0.3275911f * 0.70710678f), F2(1.0f)));
+    e = exp2_2(mul2(mul2(n, n), F2(-0.5f * LOG2E)));
+    F2 y = fma2(F2(0.5f * 1.061405429f), t, F2(0.5f * -1.453152027f));
+    y = fma2(y, t, F2(0.5f * 1.421413741f));
+    y = fma2(y, t, F2(0.5f * -0.284496736f));
+    y = fma2(y, t, F2(0.5f * 0.254829592f));
+    return mul2(mul2(y, t), e);
+}
+__device__ __forceinline__ F2 minus_abs(F2 z) {
+    F2 r;
+    r.v = z.v | 0x8000000080000000ull;
+    return r;
 }
 
 template <int ACT>
-__device__ __forceinline__ float act_value(float z, float slope) {
+__device__ __forceinline__ F2 act_value(F2 z, float slope) {
     if constexpr (ACT == GK_ACT_RELU) {
-        return z > 0.0f ? z : 0.0f;
+        return F2(z.lo() > 0.0f ? z.lo() : 0.0f, z.hi() > 0.0f ? z.hi() : 0.0f);
     } else if constexpr (ACT == GK_ACT_LEAKY_RELU) {
-        return fmaf(slope, z < 0.0f ? z : 0.0f, z > 0.0f ? z : 0.0f);
+        return fma2(F2(slope), F2(z.lo() < 0.0f ? z.lo() : 0.0f, z.hi() < 0.0f ? z.hi() : 0.0f),
+                    F2(z.lo() > 0.0f ? z.lo() : 0.0f, z.hi() > 0.0f ? z.hi() : 0.0f));
     } else if constexpr (ACT == GK_ACT_GELU) {
-        const float a = fabsf(clamp_nan(z, 100.0f));
-        float e;
-        return fmaf(-a, normal_tail(a, e), max_nan(z, 0.0f));
+        const F2 n = minus_abs(clamp2(z, 100.0f));
+        F2 e;
+        return fma2(n, normal_tail(n, e), max2(z, 0.0f));
     } else if constexpr (ACT == GK_ACT_GELU_TANH) {
-        z = max_nan(z, -100.0f);
-        return z * sigma2(-z * fmaf(GELU_2K * LOG2E * GELU_C, z * z, GELU_2K * LOG2E));
+        z = max2(z, -100.0f);
+        const F2 m = fma2(F2(-GELU_2K * LOG2E * GELU_C), mul2(z, z), F2(-GELU_2K * LOG2E));
+        return mul2(z, sigma2(mul2(z, m)));
     } else if constexpr (ACT == GK_ACT_SILU) {
-        z = max_nan(z, -100.0f);
-        return z * sigma2(z * -LOG2E);
+        z = max2(z, -100.0f);
+        return mul2(z, sigma2(mul2(z, F2(-LOG2E))));
     } else {
         return z;
     }
 }
 
+// s (1 - s)
+__device__ __forceinline__ F2 s_1_s(F2 s) { return mul2(s, fma2(s, F2(-1.0f), F2(1.0f))); }
+
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z, float slope) {
+__device__ __forceinline__ F2 act_slope(F2 z, float slope) {
     if constexpr (ACT == GK_ACT_RELU) {
-        return z > 0.0f ? 1.0f : 0.0f;
+        return F2(z.lo() > 0.0f ? 1.0f : 0.0f, z.hi() > 0.0f ? 1.0f : 0.0f);
     } else if constexpr (ACT == GK_ACT_LEAKY_RELU) {
-        return z > 0.0f ? 1.0f : slope;
+        return F2(z.lo() > 0.0f ? 1.0f : slope, z.hi() > 0.0f ? 1.0f : slope);
     } else if constexpr (ACT == GK_ACT_GELU) {
-        z = clamp_nan(z, 100.0f);
-        float e;
-        const float half = 0.5f - normal_tail(fabsf(z), e);
-        return fmaf(z * RSQRT_2PI, e, 0.5f + copysignf(half, z));
+        z = clamp2(z, 100.0f);
+        F2 e;
+        const F2 q = normal_tail(minus_abs(z), e);
+        const F2 half = fma2(q, F2(-1.0f), F2(0.5f));
+        return fma2(mul2(z, F2(RSQRT_2PI)), e,
+                    add2(F2(copysignf(half.lo(), z.lo()), copysignf(half.hi(), z.hi())), F2(0.5f)));
     } else if constexpr (ACT == GK_ACT_GELU_TANH) {
-        z = clamp_nan(z, 100.0f);
-        const float z2 = z * z;
-        const float s = sigma2(-z * fmaf(GELU_2K * LOG2E * GELU_C, z2, GELU_2K * LOG2E));
-        return fmaf(z * fmaf(-s, s, s), fmaf(3.0f * GELU_C * GELU_2K, z2, GELU_2K), s);
+        z = clamp2(z, 100.0f);
+        const F2 z2 = mul2(z, z);
+        const F2 m = fma2(F2(-GELU_2K * LOG2E * GELU_C), z2, F2(-GELU_2K * LOG2E));
+        const F2 s = sigma2(mul2(z, m));
+        return fma2(mul2(z, s_1_s(s)), fma2(F2(3.0f * GELU_C * GELU_2K), z2, F2(GELU_2K)), s);
     } else if constexpr (ACT == GK_ACT_SILU) {
-        z = clamp_nan(z, 100.0f);
-        const float s = sigma2(z * -LOG2E);
-        return fmaf(z, fmaf(-s, s, s), s);
+        z = clamp2(z, 100.0f);
+        const F2 s = sigma2(mul2(z, F2(-LOG2E)));
+        return fma2(z, s_1_s(s), s);
     } else {
-        return 1.0f;
+        return F2(1.0f);
     }
 }
 
@@ -188,8 +233,11 @@ __device__ __forceinline__ void load_pairs(uint32_t (&w)[N], const uint16_t* c, 
     const int odd = lane & 1;
     const uint16_t* q = c + (lane & 30) + odd * ldq;
     if (n >= 2 * N && pn >= 32) {  // (the warp's; no predicates)
+        const uint32_t step = static_cast<uint32_t>(ldq) * 4u;  // one multiply-add an address
 #pragma unroll
-        for (int j = 0; j < N; ++j, q += 2 * ldq) w[j] = *reinterpret_cast<const uint32_t*>(q);
+        for (int j = 0; j < N; ++j)
+            w[j] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(q) +
+                                                      static_cast<uint64_t>(step) * j);
         return;
     }
     const int left = (lane & 30) < pn ? n - odd : 0;
@@ -221,8 +269,11 @@ __device__ __forceinline__ void put_pairs(uint32_t (&w)[N], uint16_t* c, int64_t
     const int odd = lane & 1;
     uint16_t* q = c + (lane & 30) + odd * ldq;
     if (n >= 2 * N && pn >= 32) {
+        const uint32_t step = static_cast<uint32_t>(ldq) * 4u;
 #pragma unroll
-        for (int j = 0; j < N; ++j, q += 2 * ldq) *reinterpret_cast<uint32_t*>(q) = w[j];
+        for (int j = 0; j < N; ++j)
+            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(q) +
+                                         static_cast<uint64_t>(step) * j) = w[j];
         return;
     }
     const int left = (lane & 30) < pn ? n - odd : 0;
@@ -238,7 +289,6 @@ struct EpiAt {
     int i0, pn;
     int64_t r;
     int n;
-    __device__ __forceinline__ EpiAt plus(int c) const { return EpiAt{i0, pn, r + c, n - c}; }
 };
 
 // N columns of the matrix that the epilogue reads beside the accumulators, all loads issued together:
@@ -290,14 +340,19 @@ struct EpiSide {
             own_pairs(w, lane);
         }
     }
-    // Column c of this lane's P row.
-    __device__ __forceinline__ float z8(int c, int lane) const {
-        const uint32_t x = __shfl_sync(0xffffffffu, w[c / 4], (c % 4) * 8 + (lane >> 2));
-        const float unit = __uint_as_float(__shfl_sync(0xffffffffu, sb, c));
-        return act8_code(x, lane & 3) * unit;
+    // Columns c and c + 1 (c even) of this lane's P row.
+    __device__ __forceinline__ F2 z8(int c, int lane) const {
+        float v[2], unit[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t x = __shfl_sync(0xffffffffu, w[c / 4], ((c + i) % 4) * 8 + (lane >> 2));
+            v[i] = act8_raw(x, lane & 3);
+            unit[i] = __uint_as_float(__shfl_sync(0xffffffffu, sb, c + i));
+        }
+        return mul2(add2(F2(v[0], v[1]), F2(-8388736.0f)), F2(unit[0], unit[1]));
     }
-    __device__ __forceinline__ float half(int c) const {
-        return c & 1 ? half_hi(w[c / 2], epi_f16(EPI)) : half_lo(w[c / 2], epi_f16(EPI));
+    __device__ __forceinline__ F2 half(int c) const {
+        return F2(half_lo(w[c / 2], epi_f16(EPI)), half_hi(w[c / 2], epi_f16(EPI)));
     }
 };
 
@@ -309,20 +364,17 @@ __device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_t
                                             const uint32_t (&v)[N], const EpiSide<EPI, N>& s,
                                             float alpha, float bias, float& sum, int lane) {
     constexpr bool f16 = epi_f16(EPI);
-    float y[N];
+    F2 y[N / 2];  // two columns each
     const bool live = lane < at.pn;
     const int64_t own = (at.i0 + lane) * ldp + at.r * ldq;  // element by element
     if constexpr (epi_fwd(EPI)) {
-        uint32_t zw[N / 2];
 #pragma unroll
-        for (int j = 0; j < N; j += 2) {
-            const float a = fmaf(alpha, __uint_as_float(v[j]), bias);
-            const float b = fmaf(alpha, __uint_as_float(v[j + 1]), bias);
-            zw[j / 2] = pack_half2(a, b, f16);
-            y[j] = a;
-            y[j + 1] = b;
-        }
+        for (int j = 0; j < N / 2; ++j)
+            y[j] = fma2(F2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), F2(alpha), F2(bias));
         if (e.z) {
+            uint32_t zw[N / 2];
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) zw[j] = pack_half2(y[j].lo(), y[j].hi(), f16);
             if constexpr (PAIRS) {
                 put_pairs(zw, e.z + at.r * e.zq + at.i0, e.zq, at.n, at.pn, lane);
             } else {
@@ -335,52 +387,65 @@ __device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_t
         }
         with_act(e.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) y[j] = act_value<decltype(act)::value>(y[j], e.slope);
+            for (int j = 0; j < N / 2; ++j) y[j] = act_value<decltype(act)::value>(y[j], e.slope);
         });
         if (e.side) {
             if (PAIRS || out_type != GK_F32) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) y[j] += s.half(j);
+                for (int j = 0; j < N / 2; ++j) y[j] = add2(y[j], s.half(2 * j));
             } else {
                 const float* r = static_cast<const float*>(e.side) + (at.i0 + lane) * e.sp +
                                  at.r * e.sq;
                 const int n = live ? at.n : 0;
 #pragma unroll
-                for (int j = 0; j < N; ++j) y[j] += j < n ? r[j * e.sq] : 0.0f;
+                for (int j = 0; j < N; j += 2)
+                    y[j / 2] = add2(y[j / 2], F2(j < n ? r[j * e.sq] : 0.0f,
+                                                 j + 1 < n ? r[(j + 1) * e.sq] : 0.0f));
             }
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) y[j] = alpha * __uint_as_float(v[j]);
+        for (int j = 0; j < N / 2; ++j)
+            y[j] = mul2(F2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), F2(alpha));
         with_act(e.act, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
             if constexpr (ACT != GK_ACT_NONE) {
                 if (e.z8.codes) {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) y[j] *= act_slope<ACT>(s.z8(j, lane), e.slope);
+                    for (int j = 0; j < N / 2; ++j)
+                        y[j] = mul2(y[j], act_slope<ACT>(s.z8(2 * j, lane), e.slope));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < N; ++j) y[j] *= act_slope<ACT>(s.half(j), e.slope);
+                    for (int j = 0; j < N / 2; ++j)
+                        y[j] = mul2(y[j], act_slope<ACT>(s.half(2 * j), e.slope));
                 }
             }
         });
+        if (at.n >= N) {  // (rows past the tile hold anything)
+            F2 a = y[0];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < at.n) sum += y[j];
+            for (int j = 1; j < N / 2; ++j) a = add2(a, y[j]);
+            sum += a.lo() + a.hi();
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < at.n) sum += j & 1 ? y[j / 2].hi() : y[j / 2].lo();
+        }
     }
     if constexpr (PAIRS) {
         uint32_t w[N / 2];
 #pragma unroll
-        for (int j = 0; j < N / 2; ++j) w[j] = pack_half2(y[2 * j], y[2 * j + 1], f16);
+        for (int j = 0; j < N / 2; ++j) w[j] = pack_half2(y[j].lo(), y[j].hi(), f16);
         put_pairs(w, static_cast<uint16_t*>(c) + at.r * ldq + at.i0, ldq, at.n, at.pn, lane);
     } else if (out_type == GK_F32) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (live && j < at.n) static_cast<float*>(c)[own + j * ldq] = y[j];
+            if (live && j < at.n)
+                static_cast<float*>(c)[own + j * ldq] = j & 1 ? y[j / 2].hi() : y[j / 2].lo();
     } else {
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
-            const uint32_t w = pack_half2(y[j], y[j + 1], f16);
+            const uint32_t w = pack_half2(y[j / 2].lo(), y[j / 2].hi(), f16);
             uint16_t* o = static_cast<uint16_t*>(c) + own + j * ldq;
             if (live && j < at.n) *o = static_cast<uint16_t>(w);
             if (live && j + 1 < at.n) o[ldq] = static_cast<uint16_t>(w >> 16);

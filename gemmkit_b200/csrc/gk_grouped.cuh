@@ -544,14 +544,13 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
 template <int PB, int EPI>
 struct GPairCfg {
     static constexpr int BN = 256;
-    static constexpr int NEPI = 8;
-    // A whole epilogue on tall tiles keeps 128 accumulators a lane in registers (epi_tall): the four
-    // other warps give theirs up for it (setmaxnreg). 128 x 56 + 256 x 224 registers are the
-    // 384 x 168 that the block is launched with.
+    // A whole epilogue on tall tiles keeps 64 accumulators a lane in registers (epi_tall); sixteen warps
+    // do it, and the four others give up registers for it (setmaxnreg): 128 x 56 + 512 x 104 are 60416
+    // of the 640 x 96 that the block is launched with.
     static constexpr bool SPLIT_REGS = EPI != EPI_STORE && PB == 2;
-    static constexpr int REGS_OTHER = 56, REGS_EPI = 224;
-    static_assert(!SPLIT_REGS || 128 * REGS_OTHER + 32 * NEPI * REGS_EPI <= 32 * (4 + NEPI) * 168,
-                  "registers of the block");
+    static constexpr int NEPI = SPLIT_REGS ? 16 : 8;
+    static constexpr int REGS_OTHER = 56, REGS_EPI = 104;
+    static_assert(128 * REGS_OTHER + 32 * 16 * REGS_EPI <= 32 * 20 * 96, "registers of the block");
     static constexpr int EPI_W0 = 4;
     static constexpr int THREADS = 32 * (EPI_W0 + NEPI);
     static constexpr int WCOLS = BN / (NEPI / 4);
@@ -571,19 +570,19 @@ struct GPairCfg {
     static_assert(STAGES >= 4 && (4 * STAGES + 6) * 8 <= BAR_BYTES, "barrier area");
 };
 
-// A warp's 128 columns of a tall tile's accumulator through the epilogue: all of them go to registers
+// A warp's 64 columns of a tall tile's accumulator through the epilogue: all of them go to registers
 // and the accumulator is handed back before any of the arithmetic, which then passes under the MMAs.
 // (C moves in pairs.)
 template <int EPI>
 __device__ __forceinline__ void epi_tall(const GroupedParams& p, const GTile& t, const int* tile0,
                                          uint32_t tb, int cbase, int i0, int pn, int share, int shares,
                                          uint32_t tempty, int lane) {
-    uint32_t raw[8][16];
+    uint32_t raw[4][16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tmem_ld_cols16_nowait(tb + 16 * i, raw[i]);
+    for (int i = 0; i < 4; ++i) tmem_ld_cols16_nowait(tb + 16 * i, raw[i]);
     tmem_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) frag_fence(raw[i]);
+    for (int i = 0; i < 4; ++i) frag_fence(raw[i]);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster_relaxed(tempty);
@@ -602,11 +601,11 @@ __device__ __forceinline__ void epi_tall(const GroupedParams& p, const GTile& t,
     // instruction cache behind (8192 x 4096 -> 14336 with GELU and z kept: 926 us,
     // now 680).
 #pragma unroll 1
-    for (int c = 0; c < 128 && cbase + c < t.qn; c += 32) {
+    for (int c = 0; c < 64 && cbase + c < t.qn; c += 32) {
         columns(c, raw[0]);
         columns(c + 16, raw[1]);
 #pragma unroll
-        for (int i = 0; i < 6; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) raw[i][j] = raw[i + 2][j];
     }
@@ -1232,7 +1231,7 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
     };
     if constexpr (epi_bwd(EPI)) {
         if (p.e.dbias) {  // a slot for each share of each tile along the Q side
-            const int shares = bn == 32 ? 1 : 2;  // NEPI / 4 of each kernel
+            const int shares = tall ? GPairCfg<2, EPI>::NEPI / 4 : bn == 32 ? 1 : 2;
             const int64_t slots = ((static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups) * shares;
             void* part = nullptr;
             if ((rc = scratch_alloc(&part, static_cast<size_t>(slots * p.np) * 4, stream))) return rc;

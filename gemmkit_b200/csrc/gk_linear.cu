@@ -144,9 +144,9 @@ __global__ void __launch_bounds__(32 * GW, 4) act_grad_kernel(const ActGrad p) {
         const int r0 = off[lo] + (t - tile0[lo]) * GR, r1 = min(r0 + GR, off[lo + 1]);
         const int64_t c = c0 + lane * V;
         const bool live = c < p.np;
-        float sum[V];
+        F2 sum[(V + 1) / 2];
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+        for (int i = 0; i < (V + 1) / 2; ++i) sum[i] = F2(0.0f);
 #pragma unroll 1
         for (int r = r0 + w; live && r < r1; r += 2 * GW) {
             GradRow<V> row[2];
@@ -157,55 +157,57 @@ __global__ void __launch_bounds__(32 * GW, 4) act_grad_kernel(const ActGrad p) {
             for (int k = 0; k < 2; ++k) {
                 const int64_t at = r + k * GW;
                 if (at >= r1) break;
-                float d[V];
+                F2 d[(V + 1) / 2];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const uint32_t yw = row[k].y[i / 2];
-                    d[i] = i & 1 ? half_hi(yw, F16) : half_lo(yw, F16);
-                }
+                for (int i = 0; i < (V + 1) / 2; ++i)
+                    d[i] = F2(half_lo(row[k].y[i], F16), V == 1 ? 0.0f : half_hi(row[k].y[i], F16));
                 with_act(p.e.act, [&](auto act) {
                     constexpr int ACT = decltype(act)::value;
                     if constexpr (ACT != GK_ACT_NONE) {
                         const float unit = p.e.z8.codes ? act8_unit(row[k].x) : 0.0f;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            float z;
-                            if (p.e.z8.codes)
-                                z = act8_code(row[k].z[i / 4] ^ 0x80808080u, i & 3) * unit;
-                            else
-                                z = i & 1 ? half_hi(row[k].z[i / 2], F16)
-                                          : half_lo(row[k].z[i / 2], F16);
-                            d[i] *= act_slope<ACT>(z, p.e.slope);
+                        for (int i = 0; i < (V + 1) / 2; ++i) {
+                            F2 z;
+                            if (p.e.z8.codes) {
+                                const uint32_t w = row[k].z[i / 2] ^ 0x80808080u;
+                                z = mul2(add2(F2(act8_raw(w, 2 * (i & 1)), act8_raw(w, 2 * (i & 1) + 1)),
+                                              F2(-8388736.0f)),
+                                         F2(unit));
+                            } else {
+                                z = F2(half_lo(row[k].z[i], F16), half_hi(row[k].z[i], F16));
+                            }
+                            d[i] = mul2(d[i], act_slope<ACT>(z, p.e.slope));
                         }
                     }
                 });
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum[i] += d[i];
+                for (int i = 0; i < (V + 1) / 2; ++i) sum[i] = add2(sum[i], d[i]);
                 if (!p.dz) continue;
                 const int64_t o = at * p.zq + c * p.zp;
                 if constexpr (V == 8) {
                     if (p.out_type == GK_F32) {
                         float* f = static_cast<float*>(p.dz) + o;
-                        st_global_v4(f, __float_as_uint(d[0]), __float_as_uint(d[1]),
-                                     __float_as_uint(d[2]), __float_as_uint(d[3]));
-                        st_global_v4(f + 4, __float_as_uint(d[4]), __float_as_uint(d[5]),
-                                     __float_as_uint(d[6]), __float_as_uint(d[7]));
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2)
+                            st_global_v4(f + 2 * i, __float_as_uint(d[i].lo()), __float_as_uint(d[i].hi()),
+                                         __float_as_uint(d[i + 1].lo()), __float_as_uint(d[i + 1].hi()));
                     } else {
-                        st_global_v4(static_cast<uint16_t*>(p.dz) + o, pack_half2(d[0], d[1], F16),
-                                     pack_half2(d[2], d[3], F16), pack_half2(d[4], d[5], F16),
-                                     pack_half2(d[6], d[7], F16));
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = pack_half2(d[i].lo(), d[i].hi(), F16);
+                        st_global_v4(static_cast<uint16_t*>(p.dz) + o, w[0], w[1], w[2], w[3]);
                     }
                 } else if (p.out_type == GK_F32) {
-                    static_cast<float*>(p.dz)[o] = d[0];
+                    static_cast<float*>(p.dz)[o] = d[0].lo();
                 } else {
                     static_cast<uint16_t*>(p.dz)[o] =
-                        static_cast<uint16_t>(pack_half2(d[0], 0.0f, F16));
+                        static_cast<uint16_t>(pack_half2(d[0].lo(), 0.0f, F16));
                 }
             }
         }
         if (!p.part) continue;
 #pragma unroll
-        for (int i = 0; i < V; ++i) red[w][i * 32 + lane] = sum[i];
+        for (int i = 0; i < V; ++i) red[w][i * 32 + lane] = i & 1 ? sum[i / 2].hi() : sum[i / 2].lo();
         __syncthreads();
         for (int i = threadIdx.x; i < 32 * V; i += 32 * GW) {  // column (i % 32) V + i / 32 of the tile
             float a = red[0][i];
@@ -297,7 +299,7 @@ int check_apart(const Span& w, const char* name, std::initializer_list<Span> oth
 
 // Whether a 16-bit matrix can move in pairs: unit column stride, even rows of whole words.
 bool in_pairs(const void* data, int64_t rs, int64_t cs, size_t rows, size_t cols) {
-    return cols % 2 == 0 && cs == 1 && (rows <= 1 || rs % 2 == 0) &&
+    return cols % 2 == 0 && cs == 1 && (rows <= 1 || (rs % 2 == 0 && rs < (int64_t{1} << 30))) &&
            (reinterpret_cast<uintptr_t>(data) & 3) == 0;
 }
 
