@@ -966,11 +966,17 @@ class Act8Matrix:
     @property
     def codes(self):
         """The codes (rows x cols, int8)."""
+        if self._codes is None:  # parts of one buffer (empty), cut when they are asked for
+            n = self.c.codes_len
+            self._codes = self._where[:n].view(_cuda[0].int8).view(self.rows, -1 if n else 0)[:, :self.cols]
         return self._codes
 
     @property
     def exponents(self):
         """The exponent bytes (rows x ceil(cols / 32), uint8): 127 is a largest magnitude in [1, 2)."""
+        if self._exps is None:
+            part = self._where[self.c.codes_len:]
+            self._exps = part.view(self.rows, -1 if part.numel() else 0)[:, :(self.cols + 31) // 32]
         return self._exps
 
     @staticmethod
@@ -994,8 +1000,7 @@ class Act8Matrix:
                 buf = torch.empty(n + rows * pitch, dtype=torch.uint8, device=device)
         q = Act8Matrix.__new__(Act8Matrix)
         q.rows, q.cols, q._where = rows, cols, buf
-        q._codes = buf[:n].view(torch.int8).view(rows, nb * 32)[:, :cols]
-        q._exps = buf[n:].view(rows, pitch)[:, :nb]
+        q._codes = q._exps = None
         at = buf.data_ptr()
         q.c = _lib.Act8MatrixC(rows, cols, at, n, nb * 32, at + n, rows * pitch, pitch)
         return q
@@ -1006,7 +1011,7 @@ class Act8Matrix:
             raise GemmkitError(GK_EINVAL, f"gemmkit: no rows {first} to {last} of {self.rows}")
         q = Act8Matrix.__new__(Act8Matrix)
         q.rows, q.cols, q._where = last - first, self.cols, self._where
-        q._codes, q._exps = self._codes[first:last], self._exps[first:last]
+        q._codes, q._exps = self.codes[first:last], self.exponents[first:last]
         c = self.c
         a, b = first * c.codes_ld, first * c.exps_ld
         q.c = _lib.Act8MatrixC(q.rows, q.cols, (c.codes or 0) + a, max(0, c.codes_len - a), c.codes_ld,
@@ -1068,7 +1073,27 @@ class MoeBalance:
     moe_balance_backward)."""
 
     def __init__(self, loss, counts, offsets, rates):
-        self.loss, self.counts, self.offsets, self.rates = loss, counts, offsets, rates
+        e = counts.numel()
+        for name, t, dt, n in (("loss", loss, "torch.float32", 1), ("counts", counts, "torch.int32", e),
+                               ("offsets", offsets, "torch.int32", e + 1),
+                               ("rates", rates, "torch.float32", e)):
+            if str(t.dtype) != dt or t.numel() != n or not t.is_contiguous():
+                raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold {n} contiguous {dt[6:]}")
+        self.experts, self._parts = e, [loss, counts, offsets, rates]
+        self._where = _one_device("loss", loss, "counts", counts, "offsets", offsets, "rates", rates)
+        self._at = [t.data_ptr() for t in self._parts]
+
+    def _part(self, i):
+        if self._parts is None:  # parts of one buffer (empty), cut when they are asked for
+            e, f32 = self.experts, _cuda[0].float32
+            loss, counts, offsets, rates = self._where.split_with_sizes((1, e, e + 1, e))
+            self._parts = [loss.view(f32), counts, offsets, rates.view(f32)]
+        return self._parts[i]
+
+    loss = property(lambda self: self._part(0))
+    counts = property(lambda self: self._part(1))
+    offsets = property(lambda self: self._part(2))
+    rates = property(lambda self: self._part(3))
 
     @staticmethod
     def empty(experts: int, stream=None) -> "MoeBalance":
@@ -1078,27 +1103,28 @@ class MoeBalance:
             raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
         torch = calls[0]
         device = torch.device("cuda", calls[1]())
-
-        def make():
-            return torch.empty(3 * experts + 2, dtype=torch.int32, device=device)
+        n = 3 * experts + 2
         if stream is None:
-            buf = make()
-        else:
+            buf = torch.empty(n, dtype=torch.int32, device=device)
+        else:  # not what the current stream may still be writing
             with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
-                buf = make()
-        e = experts
-        return MoeBalance(buf[:1].view(torch.float32), buf[1:1 + e], buf[1 + e:2 + 2 * e],
-                          buf[2 + 2 * e:].view(torch.float32))
+                buf = torch.empty(n, dtype=torch.int32, device=device)
+        b = MoeBalance.__new__(MoeBalance)
+        b.experts, b._where, b._parts = experts, buf, None
+        at = buf.data_ptr()
+        b._at = [at, at + 4, at + 4 * (experts + 1), at + 4 * (2 * experts + 2)]
+        return b
 
 
 def _ids(ids, tokens):
     """(pointer, length, ids a token, 64-bit) of a tokens x top tensor."""
-    kinds = {"torch.int32": 0, "torch.int64": 1}
-    if str(ids.dtype) not in kinds or ids.dim() != 2 or ids.shape[0] != tokens or \
-            not ids.is_contiguous():
+    torch = (_cuda or _cuda_calls() or (None,))[0]
+    wide = 0 if torch and ids.dtype is torch.int32 else 1 if torch and ids.dtype is torch.int64 else None
+    shape = ids.shape
+    if wide is None or len(shape) != 2 or shape[0] != tokens or not ids.is_contiguous():
         raise GemmkitError(GK_EINVAL, f"gemmkit: ids must be a contiguous {tokens} x top tensor of int32 "
                                       "or int64")
-    return ids.data_ptr(), ids.numel(), ids.shape[1], kinds[str(ids.dtype)]
+    return ids.data_ptr(), shape[0] * shape[1], shape[1], wide
 
 
 def moe_balance(logits: MatRef, ids, coef: float = 1.0, out: Optional[MoeBalance] = None,
@@ -1107,43 +1133,37 @@ def moe_balance(logits: MatRef, ids, coef: float = 1.0, out: Optional[MoeBalance
     experts, f32, f16 or bf16), `ids` (tokens x top, int32 or int64, contiguous) the experts that each
     token goes to, a negative id for none; a token without any is padding. loss = coef * experts *
     sum_e (counts_e / routed) * (mean of softmax(logits)_e over the live tokens)."""
-    o = out
-    _same_device("logits", logits.data, "ids", ids,
-                 *(() if o is None else ("loss", o.loss, "counts", o.counts, "offsets", o.offsets,
-                                         "rates", o.rates)))
+    _same_device("logits", logits.data, "ids", ids, "out", None if out is None else out._where)
     i = _ids(ids, logits.rows)
-    if o is None:
-        o = MoeBalance.empty(logits.cols, stream=stream)
-    elif o.counts.numel() != logits.cols or o.offsets.numel() != logits.cols + 1 or \
-            o.rates.numel() != logits.cols:
+    if out is None:
+        out = MoeBalance.empty(logits.cols, stream=stream)
+    elif out.experts != logits.cols:
         raise GemmkitError(GK_EINVAL, f"gemmkit: the results are not of {logits.cols} experts")
     if x_type is None:
         x_type = _elem_type(logits.data, -1)
-    _check(_lib.load().gk_moe_balance(logits.c(), x_type, *i, float(coef), o.loss.data_ptr(),
-                                      o.counts.data_ptr(), o.offsets.data_ptr(), o.rates.data_ptr(),
-                                      _stream(stream)))
+    _check(_lib.load().gk_moe_balance(logits.c(), x_type, *i, float(coef), *out._at, _stream(stream)))
     if sync:
         _sync(stream)
-    return o
+    return out
 
 
 def moe_balance_backward(logits: MatRef, ids, balance: MoeBalance, dloss, dlogits: MatMut,
                          x_type: Optional[int] = None, stream=None, sync: bool = True) -> None:
     """The loss's gradient by the logits (extension), times `dloss` (one f32 on the device); padding
     gets zeros. dlogits has the logits' type and may be the logits themselves."""
-    _same_device("logits", logits.data, "ids", ids, "rates", balance.rates, "dloss", dloss, "dlogits",
-                 dlogits.data)
+    _same_device("logits", logits.data, "ids", ids, "balance", balance._where, "dloss", dloss,
+                 "dlogits", dlogits.data)
     i = _ids(ids, logits.rows)
-    if balance.rates.numel() != logits.cols:
+    if balance.experts != logits.cols:
         raise GemmkitError(GK_EINVAL, f"gemmkit: the results are not of {logits.cols} experts")
-    if str(dloss.dtype) != "torch.float32" or dloss.numel() != 1:
+    if dloss.dtype is not _cuda[0].float32 or dloss.numel() != 1:
         raise GemmkitError(GK_EINVAL, "gemmkit: dloss must be one f32")
     if x_type is None:
         x_type = _elem_type(logits.data, -1)
     if _elem_type(dlogits.data, x_type) != x_type:
         raise GemmkitError(GK_EINVAL, "gemmkit: dlogits must have the logits' type")
-    _check(_lib.load().gk_moe_balance_backward(logits.c(), x_type, *i, balance.rates.data_ptr(),
-                                               dloss.data_ptr(), dlogits.c(), _stream(stream)))
+    _check(_lib.load().gk_moe_balance_backward(logits.c(), x_type, *i, balance._at[3], dloss.data_ptr(),
+                                               dlogits.c(), _stream(stream)))
     if sync:
         _sync(stream)
 

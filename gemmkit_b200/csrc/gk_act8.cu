@@ -10,16 +10,20 @@
 //
 // Both kernels move each byte once and are bound by memory. The matrix is a run of pieces of E elements,
 // row after row; a lane takes AU of them, 32 pieces apart, all of their loads issued together (so short
-// rows fill warps too). E is 16 where the elements have 16 bits, 8 in f32: 16-byte loads and stores
-// either way, and a block's maximum over two or four lanes. (With E = 8 for 16 bits, and pieces that ended
-// with a row's 1024 elements, 8192 x 8192 of bf16 took 44 and 47 us; now 45 and 34.)
+// rows fill warps too). Quantising, E is 16 where the elements have 16 bits, 8 in f32: 16-byte loads, a
+// block's maximum over two or four lanes. The other way E makes 16 bytes of output, so that a warp's
+// store writes whole sectors (with 16 elements a lane, two half sectors each, 8192 x 8192 of bf16 took 45
+// instead of 36 us; quantising it takes 36).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "gemmkit_cuda.h"
 #include "gk_act8.cuh"
 #include "gk_engine.h"
+#include "gk_f2.cuh"
 #include "gk_launch.h"
 #include "gk_sm100.cuh"
 #include "gk_store.cuh"
@@ -71,6 +75,24 @@ struct Piece {  // its elements as they lie in memory
     }
 };
 
+// The largest magnitude of a piece, as f32 bits; 16-bit magnitudes compare as integers, two at a time.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(const Piece<T>& x) {
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < Piece<T>::W; ++k) m = max(m, x.w[k] & 0x7FFFFFFFu);
+    } else {
+#pragma unroll
+        for (int k = 0; k < Piece<T>::W; ++k) m = __vmaxu2(m, x.w[k] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+        m = std::is_same_v<T, __half>
+                ? __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))))
+                : m << 16;
+    }
+    return m;
+}
+
 // x clamped to +-127 (one instruction: the smaller magnitude with the product's sign).
 __device__ __forceinline__ float clamp_127(float x) {
     float r;
@@ -78,14 +100,22 @@ __device__ __forceinline__ float clamp_127(float x) {
     return r;
 }
 
-// Where piece i lies: `per` of them make the whole blocks of a row. (Divided in 64 bits only where 32 do not
-// hold the pieces.)
+// Where a lane's pieces lie, 32 apart: `per` of them make the whole blocks of a row. Divided once, in 64
+// bits only where 32 do not hold the pieces.
 struct At {
     int64_t r;
-    int c;
-    __device__ __forceinline__ At(uint64_t i, uint32_t per, bool wide, int e) {
-        r = wide ? i / per : static_cast<uint32_t>(i) / per;
-        c = static_cast<int>(i - r * per) * e;
+    uint32_t i;  // piece of the row
+    __device__ __forceinline__ At(uint64_t piece, uint32_t per, bool wide) {
+        r = wide ? piece / per : static_cast<uint32_t>(piece) / per;
+        i = static_cast<uint32_t>(piece - r * per);
+    }
+    __device__ __forceinline__ void next(uint32_t per, uint32_t rows32, uint32_t rest32) {
+        r += rows32;
+        i += rest32;
+        if (i >= per) {
+            i -= per;
+            ++r;
+        }
     }
 };
 
@@ -99,7 +129,7 @@ struct Act8Out {
 
 // vec: rows of x are contiguous and start on 16-byte boundaries.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
     quantize_act8_kernel(const T* x, int64_t rs, int64_t cs, int vec, Act8Out q) {
     griddep_wait();
     griddep_launch_dependents();
@@ -108,61 +138,68 @@ __global__ void __launch_bounds__(256)
     const uint32_t per = static_cast<uint32_t>((q.cols + 31) / 32 * LANES);
     const uint64_t pieces = static_cast<uint64_t>(q.rows) * per;
     const bool wide = pieces + 32 * AU > 0xFFFFFFFFull;
+    const uint32_t rows32 = 32 / per, rest32 = 32 % per;
     const uint64_t step = static_cast<uint64_t>(gridDim.x) * (blockDim.x >> 5) * (32 * AU);
     for (uint64_t u = static_cast<uint64_t>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (32 * AU);
          u < pieces; u += step) {
         Piece<T> raw[AU];
+        At at(u + lane, per, wide);
+        const At first = at;
 #pragma unroll
-        for (int i = 0; i < AU; ++i) {
-            const At at(u + 32 * i + lane, per, wide, E);
+        for (int i = 0; i < AU; ++i, at.next(per, rows32, rest32)) {
+            const int c = static_cast<int>(at.i) * E;
             const T* src = x + at.r * rs;
-            if (at.r < q.rows) {
-                if (vec && at.c + E <= q.cols)
-                    raw[i].load(src + at.c);
-                else
-                    raw[i].load(src + at.c * cs, cs, q.cols - at.c);
-            } else {
-                raw[i].load(src, cs, 0);
-            }
+            if (at.r < q.rows && vec && c + E <= q.cols)
+                raw[i].load(src + c);
+            else
+                raw[i].load(src + c * cs, cs, at.r < q.rows ? q.cols - c : 0);
         }
+        at = first;
 #pragma unroll
-        for (int i = 0; i < AU; ++i) {
+        for (int i = 0; i < AU; ++i, at.next(per, rows32, rest32)) {
             if (u + 32 * i >= pieces) break;  // the whole warp
-            float v[E];
-            uint32_t m = 0;
-#pragma unroll
-            for (int k = 0; k < E; ++k) {
-                v[k] = raw[i].value(k);
-                m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
-            }
+            uint32_t m = largest(raw[i]);
 #pragma unroll
             for (int d = 1; d < LANES; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
             const uint32_t b = m >> 23;  // the biased exponent is e + 127; 255: an infinity or a NaN
+            float v[E];
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] = raw[i].value(k);
             // x 2^(6 - e), in two exact steps where 2^(6 - e) would not be a normal number
             if (__any_sync(0xffffffffu, b < 64)) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) v[k] = b < 64 ? v[k] * 0x1p64f : v[k];
             }
-            const float mul = __uint_as_float((b < 64 ? 196u - b : 260u - b) << 23);
-            uint32_t y[E], w[E / 4];
+            const F2 mul(__uint_as_float((b < 64 ? 196u - b : 260u - b) << 23));
+            F2 s[E / 2];
 #pragma unroll
-            for (int k = 0; k < E; ++k)
-                // below 128 in magnitude; 1.5 2^23 + s: rounded to an integer, half to even, its low
-                // byte the code
-                y[k] = __float_as_uint(clamp_127(v[k] * mul) + 12582912.0f);
+            for (int k = 0; k < E / 2; ++k) s[k] = mul2(F2(v[2 * k], v[2 * k + 1]), mul);
+            // Below 128 in magnitude: only a block whose largest value's digits begin 1.9921875 holds one
+            // that would round to 128.
+            if (__any_sync(0xffffffffu, (m & 0x7FFFFFu) >= 0x7F0000u)) {
 #pragma unroll
-            for (int h = 0; h < E / 4; ++h)
+                for (int k = 0; k < E / 2; ++k) s[k] = F2(clamp_127(s[k].lo()), clamp_127(s[k].hi()));
+            }
+            // 1.5 2^23 + s: rounded to an integer, half to even, its low byte the code
+            uint32_t w[E / 4];
+#pragma unroll
+            for (int h = 0; h < E / 4; ++h) {
+                const F2 y0 = add2(s[2 * h], F2(12582912.0f)), y1 = add2(s[2 * h + 1], F2(12582912.0f));
                 w[h] = b == 255 ? 0u
-                                : __byte_perm(__byte_perm(y[4 * h], y[4 * h + 1], 0x0040),
-                                              __byte_perm(y[4 * h + 2], y[4 * h + 3], 0x0040), 0x5410);
-            const At at(u + 32 * i + lane, per, wide, E);
+                                : __byte_perm(__byte_perm(__float_as_uint(y0.lo()),
+                                                          __float_as_uint(y0.hi()), 0x0040),
+                                              __byte_perm(__float_as_uint(y1.lo()),
+                                                          __float_as_uint(y1.hi()), 0x0040),
+                                              0x5410);
+            }
             if (at.r >= q.rows) continue;
-            int8_t* dst = q.codes + at.r * q.codes_ld + at.c;
+            const int c = static_cast<int>(at.i) * E;
+            int8_t* dst = q.codes + at.r * q.codes_ld + c;
             if constexpr (E == 16)
                 st_global_v4(dst, w[0], w[1], w[2], w[3]);
             else
                 *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-            if (lane % LANES == 0) q.exps[at.r * q.exps_ld + (at.c >> 5)] = static_cast<uint8_t>(b);
+            if (lane % LANES == 0) q.exps[at.r * q.exps_ld + (c >> 5)] = static_cast<uint8_t>(b);
         }
     }
 }
@@ -174,39 +211,49 @@ __global__ void __launch_bounds__(256)
                            int vec) {
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int E = piece<T>();
+    constexpr int E = 16 / sizeof(T), AU = 8;  // whole sectors are stored
     const int lane = threadIdx.x & 31;
     const uint32_t per = static_cast<uint32_t>((cols + E - 1) / E);
     const uint64_t pieces = static_cast<uint64_t>(rows) * per;
     const bool wide = pieces + 32 * AU > 0xFFFFFFFFull;
+    const uint32_t rows32 = 32 / per, rest32 = 32 % per;
     const uint64_t step = static_cast<uint64_t>(gridDim.x) * (blockDim.x >> 5) * (32 * AU);
     for (uint64_t u = static_cast<uint64_t>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (32 * AU);
          u < pieces; u += step) {
         uint32_t w[AU][E / 4], b[AU];
+        At at(u + lane, per, wide);
+        const At first = at;
 #pragma unroll
-        for (int i = 0; i < AU; ++i) {
-            const At at(u + 32 * i + lane, per, wide, E);
-            if (at.r >= rows) continue;
-            const int8_t* src = q.codes + at.r * q.codes_ld + at.c;
-            if constexpr (E == 16) {
-                const uint4 v = ld_global_v4(src);
-                w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
-            } else {
+        for (int i = 0; i < AU; ++i, at.next(per, rows32, rest32)) {
+            // (past the end the first piece again: no branch between the loads)
+            const bool in = at.r < rows;
+            const int c = in ? static_cast<int>(at.i) * E : 0;
+            const int64_t r = in ? at.r : 0;
+            const int8_t* src = q.codes + r * q.codes_ld + c;
+            if constexpr (E == 8) {
                 const uint2 v = *reinterpret_cast<const uint2*>(src);
                 w[i][0] = v.x, w[i][1] = v.y;
+            } else {
+                w[i][0] = *reinterpret_cast<const uint32_t*>(src);
             }
-            b[i] = q.exps[at.r * q.exps_ld + (at.c >> 5)];
+            b[i] = q.exps[r * q.exps_ld + (c >> 5)];
         }
+        at = first;
 #pragma unroll
-        for (int i = 0; i < AU; ++i) {
-            const At at(u + 32 * i + lane, per, wide, E);
+        for (int i = 0; i < AU; ++i, at.next(per, rows32, rest32)) {
             if (at.r >= rows) break;
-            const int n = cols - at.c;
-            const float unit = act8_unit(b[i]);
+            const int c = static_cast<int>(at.i) * E, n = cols - c;
+            const F2 unit(act8_unit(b[i]));
             float v[E];
 #pragma unroll
-            for (int k = 0; k < E; ++k) v[k] = act8_code(w[i][k / 4] ^ 0x80808080u, k & 3) * unit;
-            T* o = out + at.r * rs + at.c * cs;
+            for (int k = 0; k < E; k += 2) {
+                const uint32_t x = w[i][k / 4] ^ 0x80808080u;
+                const F2 y = mul2(add2(F2(act8_raw(x, k & 3), act8_raw(x, (k & 3) + 1)), F2(-8388736.0f)),
+                                  unit);
+                v[k] = y.lo();
+                v[k + 1] = y.hi();
+            }
+            T* o = out + at.r * rs + c * cs;
             if (vec && n >= E) {
                 uint32_t p[E * sizeof(T) / 4];
 #pragma unroll
@@ -229,8 +276,9 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-dim3 piece_grid(int64_t rows, int64_t cols, int e) {
-    const int64_t blocks = (rows * ((cols + 31) / 32 * (32 / e)) + 256 * AU - 1) / (256 * AU);
+// Blocks for pieces of e elements, `au` a lane.
+dim3 piece_grid(int64_t rows, int64_t cols, int e, int au) {
+    const int64_t blocks = (rows * ((cols + 31) / 32 * (32 / e)) + 256 * au - 1) / (256 * au);
     const int64_t most = static_cast<int64_t>(sm_count()) * 4;  // what is resident
     return dim3(static_cast<unsigned>(blocks < most ? blocks : most));
 }
@@ -242,7 +290,7 @@ bool whole_rows(const void* p, int64_t rows, int64_t rs, int64_t cs, size_t es) 
 
 template <typename T>
 int quantize(const gk_matref& x, const Act8Out& q, cudaStream_t st) {
-    return launch_overlapped(quantize_act8_kernel<T>, piece_grid(q.rows, q.cols, piece<T>()), 256, st,
+    return launch_overlapped(quantize_act8_kernel<T>, piece_grid(q.rows, q.cols, piece<T>(), AU), 256, st,
                              static_cast<const T*>(x.data), static_cast<int64_t>(x.rs),
                              static_cast<int64_t>(x.cs),
                              whole_rows(x.data, q.rows, x.rs, x.cs, sizeof(T)) ? 1 : 0, q);
@@ -252,7 +300,7 @@ template <typename T>
 int dequantize(const gk_act8_matrix& q, void* out, int64_t rs, int64_t cs, cudaStream_t st) {
     const Act8View v{q.codes, q.exps, static_cast<int64_t>(q.codes_ld), static_cast<int64_t>(q.exps_ld)};
     const int64_t rows = static_cast<int64_t>(q.rows);
-    return launch_overlapped(dequantize_act8_kernel<T>, piece_grid(rows, static_cast<int64_t>(q.cols), piece<T>()),
+    return launch_overlapped(dequantize_act8_kernel<T>, piece_grid(rows, static_cast<int64_t>(q.cols), 16 / sizeof(T), 8),
                              256, st, v, rows, static_cast<int32_t>(q.cols), static_cast<T*>(out), rs, cs,
                              whole_rows(out, rows, rs, cs, sizeof(T)) ? 1 : 0);
 }

@@ -17,6 +17,7 @@
 
 #include "gemmkit_cuda.h"
 #include "gk_engine.h"
+#include "gk_f2.cuh"
 #include "gk_launch.h"
 #include "gk_sm100.cuh"
 #include "gk_store.cuh"
@@ -43,19 +44,23 @@ template <int T, int V, int J>
 struct Logits {
     uint32_t w[J * V];  // f32 bits, or 16-bit values two a word (V == 4), or one a word (V == 1)
     __device__ __forceinline__ void load(const Router& p, int64_t t, int lane) {
+        constexpr int ES = T == GK_F32 ? 4 : 2;
+        const uint8_t* row = static_cast<const uint8_t*>(p.x) + (t * p.rs + (V == 4 ? lane * V : 0)) * ES;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int e = (32 * j + lane) * V;
             if (e >= p.experts) continue;
-            const int64_t at = t * p.rs + e * p.cs;
             if constexpr (V == 1) {
-                w[j] = T == GK_F32 ? static_cast<const uint32_t*>(p.x)[at]
-                                        : static_cast<const uint16_t*>(p.x)[at];
+                const uint8_t* at = row + e * p.cs * ES;
+                if (T == GK_F32)
+                    w[j] = *reinterpret_cast<const uint32_t*>(at);
+                else
+                    w[j] = *reinterpret_cast<const uint16_t*>(at);
             } else if (T == GK_F32) {
-                const uint4 v = ld_global_v4(static_cast<const float*>(p.x) + at);
+                const uint4 v = ld_global_v4(row + 32 * j * V * ES);
                 w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
             } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.x) + at);
+                const uint2 v = *reinterpret_cast<const uint2*>(row + 32 * j * V * ES);
                 w[4 * j] = v.x, w[4 * j + 1] = v.y;
             }
         }
@@ -66,32 +71,34 @@ struct Logits {
         return T == GK_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xFFFFu)))
                            : __uint_as_float(h << 16);
     }
-    // The softmax; 0 everywhere where every logit is minus infinity.
-    __device__ __forceinline__ void softmax(const Router& p, int lane, float (&y)[J * V]) const {
+    // The softmax is y times the value returned; 0 everywhere where every logit is minus infinity.
+    __device__ __forceinline__ float softmax(const Router& p, int lane, F2 (&y)[(J * V + 1) / 2]) const {
+        float x[(J * V + 1) / 2 * 2];
+        x[(J * V + 1) / 2 * 2 - 1] = -INFINITY;
         float m = -INFINITY;
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                y[V * j + v] = (32 * j + lane) * V < p.experts ? value(j, v) : -INFINITY;
-                m = fmaxf(m, y[V * j + v]);
+                x[V * j + v] = (32 * j + lane) * V < p.experts ? value(j, v) : -INFINITY;
+                m = fmaxf(m, x[V * j + v]);
             }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
         const bool none = m == -INFINITY;
-        const float base = none ? 0.0f : m;
-        float s = 0.0f;
+        // (the difference first: logits of the type's lowest value stay apart from infinities)
+        const F2 scale(1.44269504f), base(none ? 0.0f : -m);
+        F2 s2(0.0f);
 #pragma unroll
-        for (int i = 0; i < J * V; ++i) {
-            y[i] = __expf(y[i] - base);
-            s += y[i];
+        for (int i = 0; i < (J * V + 1) / 2; ++i) {
+            const F2 t = mul2(add2(F2(x[2 * i], x[2 * i + 1]), base), scale);
+            y[i] = F2(exp2_hw(t.lo()), exp2_hw(t.hi()));
+            s2 = add2(s2, y[i]);
         }
+        float s = s2.lo() + s2.hi();
 #pragma unroll
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         // (a row of NaN also has no maximum: its sum is NaN, and stays so)
-        const float inv = none && s == 0.0f ? 0.0f : 1.0f / s;
-#pragma unroll
-        for (int i = 0; i < J * V; ++i) y[i] *= inv;
+        return none && s == 0.0f ? 0.0f : __frcp_rn(s);
     }
 };
 
@@ -194,7 +201,7 @@ __device__ __forceinline__ void finish(S sum, N count, int tokens, int experts, 
 }
 
 template <int T, int V, int J>
-__global__ void __launch_bounds__(32 * BW)
+__global__ void __launch_bounds__(32 * BW, V * J <= 8 ? 2 : 1)
     balance_kernel(const Router p, uint32_t* part, const BalanceOut o) {
     constexpr int U = together<V, J>();
     extern __shared__ float smem[];  // BW x experts sums, then the block's part
@@ -205,9 +212,9 @@ __global__ void __launch_bounds__(32 * BW)
     griddep_wait();
     griddep_launch_dependents();
     __syncthreads();
-    float sum[J * V];
+    F2 sum[(J * V + 1) / 2];
 #pragma unroll
-    for (int i = 0; i < J * V; ++i) sum[i] = 0.0f;
+    for (int i = 0; i < (J * V + 1) / 2; ++i) sum[i] = F2(0.0f);
     int live = 0;
     const int64_t step = static_cast<int64_t>(gridDim.x) * BW * U;
     for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * BW + w) * U; t0 < p.tokens; t0 += step) {
@@ -221,10 +228,10 @@ __global__ void __launch_bounds__(32 * BW)
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             if (!(has >> k & 1)) continue;
-            float y[J * V];
-            x[k].softmax(p, lane, y);
+            F2 y[(J * V + 1) / 2];
+            const F2 inv(x[k].softmax(p, lane, y));
 #pragma unroll
-            for (int i = 0; i < J * V; ++i) sum[i] += y[i];
+            for (int i = 0; i < (J * V + 1) / 2; ++i) sum[i] = fma2(y[i], inv, sum[i]);
         }
     }
 #pragma unroll
@@ -232,7 +239,8 @@ __global__ void __launch_bounds__(32 * BW)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int e = (32 * j + lane) * V + v;
-            if (e < p.experts) smem[w * p.experts + e] = sum[V * j + v];
+            const F2 pair = sum[(V * j + v) / 2];
+            if (e < p.experts) smem[w * p.experts + e] = (V * j + v) & 1 ? pair.hi() : pair.lo();
         }
     if (lane == 0 && live) atomicAdd(&hist[p.experts], live);
     __syncthreads();
@@ -315,22 +323,25 @@ __global__ void __launch_bounds__(32 * FW)
 }
 
 template <int T, int V, int J>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, V * J <= 8 ? 4 : 1)
     balance_backward_kernel(const Router p, const float* rates, const float* dloss, void* dx,
                             int64_t ds, int64_t dc) {
     constexpr int U = together<V, J>();
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    float rate[J * V];
+    F2 rate[(J * V + 1) / 2];
     const float scale = *dloss;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int i = 0; i < (J * V + 1) / 2; ++i) {
+        float r[2];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = (32 * j + lane) * V + v;
-            rate[V * j + v] = e < p.experts ? rates[e] : 0.0f;
+        for (int k = 0; k < 2; ++k) {
+            const int at = 2 * i + k, e = (32 * (at / V) + lane) * V + at % V;
+            r[k] = at < J * V && e < p.experts ? rates[e] : 0.0f;
         }
+        rate[i] = F2(r[0], r[1]);
+    }
     const int64_t step = static_cast<int64_t>(gridDim.x) * warps * U;
     for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + w) * U; t0 < p.tokens; t0 += step) {
         const int n = static_cast<int>(min(static_cast<int64_t>(U), p.tokens - t0));
@@ -342,19 +353,21 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             if (k >= n) break;
-            float y[J * V];
+            F2 y[(J * V + 1) / 2];
             if (has >> k & 1) {
-                x[k].softmax(p, lane, y);
-                float dot = 0.0f;
+                const float inv = x[k].softmax(p, lane, y);
+                F2 dot2(0.0f);
 #pragma unroll
-                for (int i = 0; i < J * V; ++i) dot = fmaf(y[i], rate[i], dot);
+                for (int i = 0; i < (J * V + 1) / 2; ++i) dot2 = fma2(y[i], rate[i], dot2);
+                float dot = dot2.lo() + dot2.hi();
 #pragma unroll
                 for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+                const F2 less(-(dot * inv)), f(scale * inv);
 #pragma unroll
-                for (int i = 0; i < J * V; ++i) y[i] = scale * y[i] * (rate[i] - dot);
+                for (int i = 0; i < (J * V + 1) / 2; ++i) y[i] = mul2(mul2(y[i], f), add2(rate[i], less));
             } else {
 #pragma unroll
-                for (int i = 0; i < J * V; ++i) y[i] = 0.0f;
+                for (int i = 0; i < (J * V + 1) / 2; ++i) y[i] = F2(0.0f);
             }
 #pragma unroll
             for (int j = 0; j < J; ++j) {
@@ -362,16 +375,20 @@ __global__ void __launch_bounds__(256)
                 if (e >= p.experts) continue;
                 const int64_t at = (t0 + k) * ds + e * dc;
                 if constexpr (V == 1) {
+                    const float g = j & 1 ? y[j / 2].hi() : y[j / 2].lo();
                     if (T == GK_F32)
-                        to_out(static_cast<float*>(dx) + at, y[j]);
+                        to_out(static_cast<float*>(dx) + at, g);
                     else if (T == GK_F16)
-                        to_out(static_cast<__half*>(dx) + at, y[j]);
+                        to_out(static_cast<__half*>(dx) + at, g);
                     else
-                        to_out(static_cast<__nv_bfloat16*>(dx) + at, y[j]);
+                        to_out(static_cast<__nv_bfloat16*>(dx) + at, g);
                 } else {
                     uint32_t b[4];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) b[v] = __float_as_uint(y[4 * j + v]);
+                    for (int v = 0; v < 4; ++v) {
+                        const F2 pair = y[(4 * j + v) / 2];
+                        b[v] = __float_as_uint(v & 1 ? pair.hi() : pair.lo());
+                    }
                     if (T == GK_F32)
                         st_global_v4(static_cast<float*>(dx) + at, b[0], b[1], b[2], b[3]);
                     else

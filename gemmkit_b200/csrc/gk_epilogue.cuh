@@ -21,6 +21,7 @@
 
 #include "gemmkit_cuda.h"
 #include "gk_act8.cuh"
+#include "gk_f2.cuh"
 #include "gk_sm100.cuh"
 #include "gk_store.cuh"
 
@@ -75,43 +76,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float exp2_hw(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ float rcp_hw(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
-// Two f32 in a register pair: Blackwell adds and multiplies both with one instruction.
-struct F2 {
-    uint64_t v;
-    __device__ __forceinline__ F2() {}
-    __device__ __forceinline__ F2(float a, float b) {
-        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    }
-    __device__ __forceinline__ explicit F2(float a) : F2(a, a) {}
-    __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
-    __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-};
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
 __device__ __forceinline__ F2 clamp2(F2 x, float y) { return F2(clamp_nan(x.lo(), y), clamp_nan(x.hi(), y)); }
 __device__ __forceinline__ F2 max2(F2 x, float y) { return F2(max_nan(x.lo(), y), max_nan(x.hi(), y)); }
 __device__ __forceinline__ F2 exp2_2(F2 x) { return F2(exp2_hw(x.lo()), exp2_hw(x.hi())); }

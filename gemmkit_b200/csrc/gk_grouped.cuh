@@ -64,9 +64,9 @@ int realign(GOperand* o, int64_t rows, int64_t len, int64_t groups, bool mn, int
             cudaStream_t st, void** scratch);
 
 // dbias[g] from the sums of the tiles of `tile` rows that a backward epilogue left in `part`, `shares`
-// slots of np columns each (gk_linear.cu).
+// slots of np columns each (gk_linear.cu; slice: see there).
 int launch_sum_parts(const float* part, const int32_t* offsets, int groups, int rows, int tile,
-                     int shares, int64_t np, const EpiArgs& e, cudaStream_t st);
+                     int shares, int slice, int64_t np, const EpiArgs& e, cudaStream_t st);
 
 namespace {
 
@@ -1239,7 +1239,7 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
             if ((rc = launch()))
                 set_last_error(rc, err);
             else
-                rc = launch_sum_parts(p.e.part, p.offsets, p.groups, p.rows, bn, shares, p.np, p.e,
+                rc = launch_sum_parts(p.e.part, p.offsets, p.groups, p.rows, bn, shares, 0, p.np, p.e,
                                       stream);
             const int fr = scratch_free(part, stream);
             return rc ? rc : fr;

@@ -13,28 +13,35 @@ namespace {
 
 // ---- column sums ----------------------------------------------------------------------------------------
 //
-// Whoever computes the gradient leaves the sums of each of its tiles in slots of np f32: the tiles of `tile`
-// rows of a group one after the other, `shares` slots each. No atomics, so the sums repeat bit for
-// bit. A warp of the second kernel takes 32 columns of a group and adds an eighth of the slots in f64.
+// Whoever computes the gradient leaves the sums of its parts of a group in consecutive slots of np f32: the
+// tiles of `tile` rows of a group, `shares` slots each; or, with `slice`, the pieces of slices of that many
+// rows that lie in the group, slice s of group g in slot s + g (two pieces that meet in a slice or in a
+// group never share one). No atomics, so the sums repeat bit for bit. A warp of the second kernel takes
+// 32 columns of a group and adds an eighth of the slots in f64.
 
 constexpr int SUM_WARPS = 8;
 
 __global__ void __launch_bounds__(32 * SUM_WARPS)
     sum_parts_kernel(const float* part, const int32_t* offsets, int groups, int rows, int tile,
-                     int shares, int64_t np, void* out, int64_t gs, int type) {
+                     int shares, int slice, int64_t np, void* out, int64_t gs, int type) {
     __shared__ int off[GROUP_TABLE_INTS], tile0[GROUP_TABLE_INTS];
     __shared__ double s[SUM_WARPS][32];
     griddep_wait();
     griddep_launch_dependents();
     load_groups(offsets, groups, rows, off, tile0, nullptr,
-                [&](int m) { return (m + tile - 1) / tile; });
+                [&](int m) { return slice ? 0 : (m + tile - 1) / tile; });
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = blockIdx.y;
+    int64_t first = static_cast<int64_t>(tile0[g]) * shares,
+            end = static_cast<int64_t>(tile0[g + 1]) * shares;
+    if (slice && off[g] < off[g + 1]) {
+        first = off[g] / slice + g;
+        end = (off[g + 1] - 1) / slice + g + 1;
+    }
     const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     double a = 0.0;
     if (col < np) {
-        const int64_t end = static_cast<int64_t>(tile0[g + 1]) * shares;
 #pragma unroll 4
-        for (int64_t i = static_cast<int64_t>(tile0[g]) * shares + w; i < end; i += SUM_WARPS)
+        for (int64_t i = first + w; i < end; i += SUM_WARPS)
             a += static_cast<double>(part[i * np + col]);
     }
     s[w][lane] = a;
@@ -55,23 +62,24 @@ __global__ void __launch_bounds__(32 * SUM_WARPS)
 }  // namespace
 
 int launch_sum_parts(const float* part, const int32_t* offsets, int groups, int rows, int tile,
-                     int shares, int64_t np, const EpiArgs& e, cudaStream_t st) {
+                     int shares, int slice, int64_t np, const EpiArgs& e, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>((np + 31) / 32), static_cast<unsigned>(groups));
     return launch_overlapped(sum_parts_kernel, grid, 32 * SUM_WARPS, st, part, offsets, groups, rows,
-                             tile, shares, np, e.dbias, e.dbias_gs, e.bias_type);
+                             tile, shares, slice, np, e.dbias, e.dbias_gs, e.bias_type);
 }
 
 namespace {
 
 // ---- the gradient without a product -----------------------------------------------------------------------
 //
-// Bound by memory: dy and z are read and dz is written once. A block walks tiles of GR rows x 32 V
-// columns, a warp takes every eighth row, with V consecutive columns a lane (16 bytes) where every
-// matrix allows that, else one; rows are read two at a time, by 32 warps of an SM. The
-// grid is what is resident: a block per tile spent more on starting (the groups' table) than a tile
-// takes (57 us for 8192 x 4096 by 8 groups with SiLU, now 39).
+// Bound by memory: dy and z are read and dz is written once. The rows are cut into as many equal slices as
+// make the grid what is resident; a block walks one slice's 32 V columns, group by group, a warp every
+// eighth row, with V consecutive columns a lane (16 bytes) where every matrix allows that, else one. Rows
+// are read four at a time so that enough loads are in flight. A block's sums stay in registers to the end of a group. (Tiles of 64
+// rows, their sums added in shared memory after each: 49 to 65 us for 8192 x 4096 by 8 groups with
+// SiLU, now 35.)
 
-constexpr int GR = 64, GW = 8;
+constexpr int GW = 8, GU = 4;  // warps, rows of a warp at a time
 
 struct ActGrad {
     const uint16_t* dy;
@@ -81,6 +89,7 @@ struct ActGrad {
     int64_t np;
     const int32_t* offsets;
     int groups, rows, f16, out_type;
+    int slice;            // rows of a block
     float* part;
     unsigned int* status;
     EpiArgs e;
@@ -90,133 +99,168 @@ struct ActGrad {
 template <int V>
 struct GradRow {
     uint32_t y[(V + 1) / 2], z[(V + 1) / 2], x;
-    __device__ __forceinline__ void load(const ActGrad& p, int64_t r, int64_t c) {
-        const uint16_t* yp = p.dy + r * p.yq + c * p.yp;
+    __device__ __forceinline__ static void pieces(uint32_t (&w)[(V + 1) / 2], const uint8_t* p) {
         if constexpr (V == 8) {
-            const uint4 a = ld_global_v4(yp);
-            y[0] = a.x, y[1] = a.y, y[2] = a.z, y[3] = a.w;
+            const uint4 a = ld_global_v4(p);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
         } else {
-            y[0] = *yp;
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
         }
-        if (p.e.z8.codes) {
-            const int8_t* q = p.e.z8.codes + r * p.e.z8.codes_ld + c;
-            if constexpr (V == 8) {
-                const uint2 a = *reinterpret_cast<const uint2*>(q);
-                z[0] = a.x, z[1] = a.y;
-            } else {
-                z[0] = static_cast<uint8_t>(*q);
-            }
-            x = p.e.z8.exps[r * p.e.z8.exps_ld + (c >> 5)];
-        } else if (p.e.side) {
-            const uint16_t* s = static_cast<const uint16_t*>(p.e.side) + r * p.e.sq + c * p.e.sp;
-            if constexpr (V == 8) {
-                const uint4 a = ld_global_v4(s);
-                z[0] = a.x, z[1] = a.y, z[2] = a.z, z[3] = a.w;
-            } else {
-                z[0] = *s;
-            }
+    }
+    __device__ __forceinline__ void codes(const uint8_t* p) {
+        if constexpr (V == 8) {
+            const uint2 a = *reinterpret_cast<const uint2*>(p);
+            z[0] = a.x, z[1] = a.y;
+        } else {
+            z[0] = *p;
         }
     }
 };
 
-template <int V, bool F16>
-__global__ void __launch_bounds__(32 * GW, 4) act_grad_kernel(const ActGrad p) {
-    __shared__ int off[GROUP_TABLE_INTS], tile0[GROUP_TABLE_INTS];
+// ACT: the activation, or -1 for the one that p names.
+template <int V, bool F16, int ACT>
+__global__ void __launch_bounds__(32 * GW, 3) act_grad_kernel(const ActGrad p) {
+    constexpr int W = (V + 1) / 2;
+    __shared__ int off[GROUP_TABLE_INTS], unused[GROUP_TABLE_INTS];
     __shared__ float red[GW][32 * V];
     griddep_wait();
     griddep_launch_dependents();
-    load_groups(p.offsets, p.groups, p.rows, off, tile0,
-                blockIdx.x == 0 ? p.status : nullptr, [](int m) { return (m + GR - 1) / GR; });
-    const unsigned blocks = static_cast<unsigned>((p.np + 32 * V - 1) / (32 * V));  // along the columns
-    const unsigned total = static_cast<unsigned>(tile0[p.groups]) * blocks;
+    load_groups(p.offsets, p.groups, p.rows, off, unused, blockIdx.x == 0 ? p.status : nullptr,
+                [](int) { return 0; });
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    for (unsigned u = blockIdx.x; u < total; u += gridDim.x) {
-        const int t = static_cast<int>(u / blocks);
-        const int64_t c0 = static_cast<int64_t>(u - t * blocks) * 32 * V;
-        int lo = 0, hi = p.groups;  // the group of tile t: tile0[lo] <= t < tile0[lo + 1]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (tile0[mid] <= t)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        const int r0 = off[lo] + (t - tile0[lo]) * GR, r1 = min(r0 + GR, off[lo + 1]);
-        const int64_t c = c0 + lane * V;
-        const bool live = c < p.np;
-        F2 sum[(V + 1) / 2];
+    const unsigned blocks = static_cast<unsigned>((p.np + 32 * V - 1) / (32 * V));  // along the columns
+    const int s = static_cast<int>(blockIdx.x / blocks);
+    const int64_t c0 = static_cast<int64_t>(blockIdx.x % blocks) * 32 * V, c = c0 + lane * V;
+    const int s0 = s * p.slice, s1 = min(s0 + p.slice, p.rows);
+    int g = 0, hi = p.groups;  // the first group that ends behind the slice's first row
+    while (g < hi) {
+        const int mid = (g + hi) >> 1;
+        if (off[mid + 1] > s0)
+            hi = mid;
+        else
+            g = mid + 1;
+    }
+    const int osize = p.out_type == GK_F32 ? 4 : 2;
+    const bool z8 = p.e.z8.codes != nullptr;
+    const int64_t ystep = p.yq * 2 * GW, ostep = p.zq * osize * GW, xstep = p.e.z8.exps_ld * GW,
+                  zstep = (z8 ? p.e.z8.codes_ld : p.e.sq * 2) * GW;
+    for (; g < p.groups && off[g] < s1; ++g) {
+        const int r0 = max(off[g], s0), r1 = min(off[g + 1], s1);
+        if (r0 >= r1) continue;
+        // this lane's place in its first row
+        const int64_t r = r0 + w;
+        const uint8_t* yp = reinterpret_cast<const uint8_t*>(p.dy + r * p.yq + c * p.yp);
+        const uint8_t* zp = z8 ? reinterpret_cast<const uint8_t*>(p.e.z8.codes + r * p.e.z8.codes_ld + c)
+                               : static_cast<const uint8_t*>(p.e.side) + (r * p.e.sq + c * p.e.sp) * 2;
+        const uint8_t* xp = p.e.z8.exps + r * p.e.z8.exps_ld + (c >> 5);
+        uint8_t* op = static_cast<uint8_t*>(p.dz) + (r * p.zq + c * p.zp) * osize;
+        int left = c < p.np && r0 + w < r1 ? (r1 - r0 - w + GW - 1) / GW : 0;  // rows of this warp
+        F2 sum[W];
 #pragma unroll
-        for (int i = 0; i < (V + 1) / 2; ++i) sum[i] = F2(0.0f);
+        for (int i = 0; i < W; ++i) sum[i] = F2(0.0f);
 #pragma unroll 1
-        for (int r = r0 + w; live && r < r1; r += 2 * GW) {
-            GradRow<V> row[2];
+        for (; left > 0; left -= GU) {
+            // (no branch between the loads: where a row is missing, the first again)
+            GradRow<V> row[GU];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                if (r + k * GW < r1) row[k].load(p, r + k * GW, c);
+            for (int k = 0; k < GU; ++k) GradRow<V>::pieces(row[k].y, yp + (k < left ? k : 0) * ystep);
+            if (z8) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int64_t at = r + k * GW;
-                if (at >= r1) break;
-                F2 d[(V + 1) / 2];
+                for (int k = 0; k < GU; ++k) {
+                    row[k].codes(zp + (k < left ? k : 0) * zstep);
+                    row[k].x = xp[(k < left ? k : 0) * xstep];
+                }
+            } else if (ACT != GK_ACT_NONE && p.e.side) {
 #pragma unroll
-                for (int i = 0; i < (V + 1) / 2; ++i)
-                    d[i] = F2(half_lo(row[k].y[i], F16), V == 1 ? 0.0f : half_hi(row[k].y[i], F16));
-                with_act(p.e.act, [&](auto act) {
-                    constexpr int ACT = decltype(act)::value;
-                    if constexpr (ACT != GK_ACT_NONE) {
-                        const float unit = p.e.z8.codes ? act8_unit(row[k].x) : 0.0f;
+                for (int k = 0; k < GU; ++k)
+                    GradRow<V>::pieces(row[k].z, zp + (k < left ? k : 0) * zstep);
+            }
+            yp += GU * ystep;
+            zp += GU * zstep;
+            xp += GU * xstep;
+            auto rows = [&](auto in8, auto act) {
+                constexpr int A = decltype(act)::value;
 #pragma unroll
-                        for (int i = 0; i < (V + 1) / 2; ++i) {
+                for (int k = 0; k < GU; ++k) {
+                    if (k >= left) break;
+                    F2 d[W];
+                    const F2 unit(decltype(in8)::value ? act8_unit(row[k].x) : 0.0f);
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        d[i] = F2(half_lo(row[k].y[i], F16), V == 1 ? 0.0f : half_hi(row[k].y[i], F16));
+                        if constexpr (A != GK_ACT_NONE) {
                             F2 z;
-                            if (p.e.z8.codes) {
-                                const uint32_t w = row[k].z[i / 2] ^ 0x80808080u;
-                                z = mul2(add2(F2(act8_raw(w, 2 * (i & 1)), act8_raw(w, 2 * (i & 1) + 1)),
+                            if constexpr (decltype(in8)::value) {
+                                const uint32_t x = row[k].z[i / 2] ^ 0x80808080u;
+                                z = mul2(add2(F2(act8_raw(x, 2 * (i & 1)), act8_raw(x, 2 * (i & 1) + 1)),
                                               F2(-8388736.0f)),
-                                         F2(unit));
+                                         unit);
                             } else {
                                 z = F2(half_lo(row[k].z[i], F16), half_hi(row[k].z[i], F16));
                             }
-                            d[i] = mul2(d[i], act_slope<ACT>(z, p.e.slope));
+                            d[i] = mul2(d[i], act_slope<A>(z, p.e.slope));
                         }
+                        sum[i] = add2(sum[i], d[i]);
                     }
-                });
+                    if (!p.dz) continue;
+                    if constexpr (V == 8) {
+                        if (p.out_type == GK_F32) {
 #pragma unroll
-                for (int i = 0; i < (V + 1) / 2; ++i) sum[i] = add2(sum[i], d[i]);
-                if (!p.dz) continue;
-                const int64_t o = at * p.zq + c * p.zp;
-                if constexpr (V == 8) {
-                    if (p.out_type == GK_F32) {
-                        float* f = static_cast<float*>(p.dz) + o;
+                            for (int i = 0; i < W; i += 2)
+                                st_global_v4(op + 8 * i, __float_as_uint(d[i].lo()),
+                                             __float_as_uint(d[i].hi()), __float_as_uint(d[i + 1].lo()),
+                                             __float_as_uint(d[i + 1].hi()));
+                        } else {
+                            uint32_t x[W];
 #pragma unroll
-                        for (int i = 0; i < 4; i += 2)
-                            st_global_v4(f + 2 * i, __float_as_uint(d[i].lo()), __float_as_uint(d[i].hi()),
-                                         __float_as_uint(d[i + 1].lo()), __float_as_uint(d[i + 1].hi()));
+                            for (int i = 0; i < W; ++i) x[i] = pack_half2(d[i].lo(), d[i].hi(), F16);
+                            st_global_v4(op, x[0], x[1], x[2], x[3]);
+                        }
+                    } else if (p.out_type == GK_F32) {
+                        *reinterpret_cast<float*>(op) = d[0].lo();
                     } else {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = pack_half2(d[i].lo(), d[i].hi(), F16);
-                        st_global_v4(static_cast<uint16_t*>(p.dz) + o, w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint16_t*>(op) =
+                            static_cast<uint16_t>(pack_half2(d[0].lo(), 0.0f, F16));
                     }
-                } else if (p.out_type == GK_F32) {
-                    static_cast<float*>(p.dz)[o] = d[0].lo();
-                } else {
-                    static_cast<uint16_t*>(p.dz)[o] =
-                        static_cast<uint16_t>(pack_half2(d[0].lo(), 0.0f, F16));
+                    op += ostep;
                 }
-            }
+            };
+            auto kinds = [&](auto act) {
+                if (z8)
+                    rows(std::true_type{}, act);
+                else
+                    rows(std::false_type{}, act);
+            };
+            if constexpr (ACT >= 0)
+                kinds(std::integral_constant<int, ACT>{});
+            else
+                with_act(p.e.act, kinds);
         }
         if (!p.part) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i) red[w][i * 32 + lane] = i & 1 ? sum[i / 2].hi() : sum[i / 2].lo();
         __syncthreads();
-        for (int i = threadIdx.x; i < 32 * V; i += 32 * GW) {  // column (i % 32) V + i / 32 of the tile
+        for (int i = threadIdx.x; i < 32 * V; i += 32 * GW) {  // column (i % 32) V + i / 32 of the block
             float a = red[0][i];
 #pragma unroll
             for (int k = 1; k < GW; ++k) a += red[k][i];
             const int64_t col = c0 + (i & 31) * V + (i >> 5);
-            if (col < p.np) p.part[static_cast<int64_t>(t) * p.np + col] = a;
+            if (col < p.np) p.part[static_cast<int64_t>(s + g) * p.np + col] = a;
         }
         __syncthreads();
+    }
+}
+
+template <bool F16>
+void (*act_grad_for(bool vec, int act))(const ActGrad) {
+    if (!vec) return act_grad_kernel<1, F16, -1>;
+    switch (act) {
+        case GK_ACT_RELU: return act_grad_kernel<8, F16, GK_ACT_RELU>;
+        case GK_ACT_LEAKY_RELU: return act_grad_kernel<8, F16, GK_ACT_LEAKY_RELU>;
+        case GK_ACT_GELU: return act_grad_kernel<8, F16, GK_ACT_GELU>;
+        case GK_ACT_GELU_TANH: return act_grad_kernel<8, F16, GK_ACT_GELU_TANH>;
+        case GK_ACT_SILU: return act_grad_kernel<8, F16, GK_ACT_SILU>;
+        default: return act_grad_kernel<8, F16, GK_ACT_NONE>;
     }
 }
 
@@ -447,7 +491,7 @@ int gk_gemm_half_dact(int is_f16, size_t groups, const int32_t* offsets, float a
         if (!p.e.dbias) return GK_OK;
         int dev = 0;
         if ((rc = api_check_device(&dev))) return rc;
-        return launch_sum_parts(nullptr, nullptr, p.groups, 0, 1, 1, p.np, p.e, st);
+        return launch_sum_parts(nullptr, nullptr, p.groups, 0, 1, 1, 0, p.np, p.e, st);
     }
     if (!c.data) return api_err(GK_EINVAL, "gemmkit: null C");
     if (!p.zero && (!a.data || !b.data)) return api_err(GK_EINVAL, "gemmkit: null A or B");
@@ -508,13 +552,8 @@ int gk_act_backward(int is_f16, size_t groups, const int32_t* offsets, gk_matref
     p.f16 = is_f16 != 0;
     p.out_type = out_type;
     p.status = device_status_ptr();
-    // tiles of GR rows; a group may end inside one
-    const int64_t tiles = (static_cast<int64_t>(rows) + GR - 1) / GR + (offsets ? p.groups : 0);
     void* scratch = nullptr;
     if (rows) {
-        if (p.e.dbias && (rc = scratch_alloc(&scratch, static_cast<size_t>(tiles) * p.np * 4, st)))
-            return rc;
-        p.part = static_cast<float*>(scratch);
         auto whole = [&](const void* d, int64_t rs, int64_t cs, size_t es) {
             return cs == 1 && (rows == 1 || rs * es % 16 == 0) &&
                    (reinterpret_cast<uintptr_t>(d) & 15) == 0;
@@ -522,19 +561,22 @@ int gk_act_backward(int is_f16, size_t groups, const int32_t* offsets, gk_matref
         const bool vec = p.np % 8 == 0 && whole(p.dy, p.yq, p.yp, 2) &&
                          (!p.dz || whole(p.dz, p.zq, p.zp, so)) &&
                          (!p.e.side || whole(p.e.side, p.e.sq, p.e.sp, 2));
-        const int v = vec ? 8 : 1;
-        const int64_t blocks = tiles * ((p.np + 32 * v - 1) / (32 * v));
-        const int64_t most = 4ll * sm_count();
-        const auto kern = vec ? (p.f16 ? act_grad_kernel<8, true> : act_grad_kernel<8, false>)
-                              : (p.f16 ? act_grad_kernel<1, true> : act_grad_kernel<1, false>);
-        if (blocks > INT32_MAX)
-            rc = api_err(GK_EINVAL, "gemmkit: problem dimensions exceed the engine's limits");
-        else
-            rc = launch_overlapped(kern, dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
-                                   32 * GW, st, p);
+        const int64_t wide = vec ? 256 : 32, blocks = (p.np + wide - 1) / wide;
+        // slices: what makes the grid resident at once, of 32 rows at least
+        int64_t slices = 3ll * sm_count() / blocks;
+        if (slices < 1) slices = 1;
+        int64_t slice = (rows + slices - 1) / slices;
+        slice = slice < 32 ? 32 : slice;
+        slices = (rows + slice - 1) / slice;
+        p.slice = static_cast<int>(slice);
+        if (p.e.dbias && (rc = scratch_alloc(&scratch, static_cast<size_t>(slices + p.groups) * p.np * 4, st)))
+            return rc;
+        p.part = static_cast<float*>(scratch);
+        rc = launch_overlapped(p.f16 ? act_grad_for<true>(vec, p.e.act) : act_grad_for<false>(vec, p.e.act),
+                               dim3(static_cast<unsigned>(slices * blocks)), 32 * GW, st, p);
     }
     if (!rc && p.e.dbias)
-        rc = launch_sum_parts(p.part, offsets, p.groups, rows, GR, 1, p.np, p.e, st);
+        rc = launch_sum_parts(p.part, offsets, p.groups, rows, 1, 1, p.slice, p.np, p.e, st);
     const int fr = scratch_free(scratch, st);
     return rc ? rc : fr;
 }
