@@ -267,7 +267,7 @@ template <int EPI, int N>
 struct EpiSide {
     uint32_t w[N / 2];
     uint32_t sb;  // z in 8 bits: lane e holds the exponent byte of column e
-    // PAIRS: see EpiArgs; f32 sides are read where they are used.
+    // PAIRS: see EpiArgs; an f32 R (f32: C is) is read where it is used.
     template <bool PAIRS>
     __device__ __forceinline__ void load(const EpiArgs& e, const EpiAt& at, bool f32, int lane) {
         if (epi_bwd(EPI) && e.z8.codes) {
@@ -286,7 +286,7 @@ struct EpiSide {
             if constexpr (PAIRS) {
                 load_pairs(w, static_cast<const uint16_t*>(e.side) + at.r * e.sq + at.i0, e.sq, at.n,
                            at.pn, lane);
-            } else if (!f32) {
+            } else if (!f32 || epi_bwd(EPI)) {
                 const uint16_t* s = static_cast<const uint16_t*>(e.side) + at.r * e.sq +
                                     (at.i0 + lane) * e.sp;
                 const int n = lane < at.pn ? at.n : 0;

@@ -266,7 +266,7 @@ __device__ __forceinline__ void epi_tile(const GroupedParams& p, const GTile& t,
         for (int c = 0; c < wcols && cbase + c < t.qn; c += 16) {
             const EpiAt at{i0, pn, t.qbase + cbase + c, t.qn - cbase - c};
             EpiSide<EPI, 16> s;
-            s.template load<PAIRS>(p.e, at, epi_fwd(EPI) && p.out_type == GK_F32, lane);
+            s.template load<PAIRS>(p.e, at, p.out_type == GK_F32, lane);
             uint32_t v[16];
             if (t.nk > 0) {
                 tmem_ld_cols16(tb + c, v);
@@ -286,7 +286,12 @@ __device__ __forceinline__ void epi_tile(const GroupedParams& p, const GTile& t,
     if constexpr (epi_bwd(EPI)) epi_sum(p, t, tile0, i0, pn, share, shares, sum, lane);
 }
 
-template <int BN, int EPI>
+// SPLIT: a cluster of up to eight CTAs computes one tile, each a run of its stages. Their accumulators are
+// exchanged through shared memory once the ring is idle: 16 Q rows (a unit) go to CTA unit % cluster
+// size, which adds them in the CTAs' order and runs the epilogue. For products with fewer tiles than the
+// SMs hold: one row, 14336 -> 4096 in 32 tiles streams its weights through 128 SMs instead of 32 (83 ->
+// 26 us).
+template <int BN, int EPI, bool SPLIT = false>
 __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     grouped_half_kernel(const __grid_constant__ CUtensorMap tmP,
                         const __grid_constant__ CUtensorMap tmQ, const GroupedParams p) {
@@ -340,8 +345,16 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    GroupWalk walk(off, tile0, p.groups, blockIdx.x, gridDim.x);
+    const int ctas = SPLIT ? static_cast<int>(cluster_ctas()) : 1;
+    const int rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+    GroupWalk walk(off, tile0, p.groups, blockIdx.x / ctas, gridDim.x / ctas);
     GTile t;
+    // the contraction indices of this CTA (a cluster's tile has more stages than the cluster CTAs)
+    auto first_k = [&](int r) {
+        return SPLIT ? (t.nk + GBK - 1) / GBK * r / ctas * GBK : 0;
+    };
+    auto last_k = [&]() { return SPLIT ? min(first_k(rank + 1), t.nk) : t.nk; };
+    bool tile = false;  // SPLIT: this CTA's part of a tile is ready
 
     if (warp == 0) {
         // ---------------- TMA producer (the whole warp, one lane issues) ----------------
@@ -351,7 +364,8 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
         while (ok && next_tile<BN>(walk, p, t)) {
             const int pz = p.p_z ? t.g : 0;
             const int qb = static_cast<int>(t.qbase);
-            for (int kb = 0; kb < t.nk; kb += GBK) {
+            const int kend = last_k();
+            for (int kb = first_k(rank); kb < kend; kb += GBK) {
                 if (!warp_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
                                GK_DEV_TIMEOUT_PRODUCER, tmo)) {
                     ok = false;
@@ -435,7 +449,8 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                                    (static_cast<uint32_t>(p.p_mn) << 15) |
                                    (static_cast<uint32_t>(p.q_mn) << 16);
             const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-            for (int kb = 0; kb < t.nk; kb += GBK) {
+            const int kb0 = first_k(rank), kend = last_k();
+            for (int kb = kb0; kb < kend; kb += GBK) {
                 if (!warp_wait(&full[stage], phase, abort_flag, p.status, GK_DEV_TIMEOUT_MMA, tmo)) {
                     ok = false;
                     break;
@@ -448,11 +463,11 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
                     if (cut) {
                         const int steps = (t.nk - kb + 15) >> 4;
                         for (int ks = 0; ks < steps; ++ks)
-                            mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, (kb | ks) != 0 ? 1u : 0u);
+                            mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, ((kb - kb0) | ks) != 0 ? 1u : 0u);
                     } else {
 #pragma unroll
                         for (int ks = 0; ks < GBK / 16; ++ks)
-                            mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, (kb | ks) != 0 ? 1u : 0u);
+                            mma_f16(d, dP.at(po, ks), dQ.at(qo, ks), idesc, ((kb - kb0) | ks) != 0 ? 1u : 0u);
                     }
                     mma_commit(&empty[stage]);
                 }
@@ -481,6 +496,10 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
             if (!warp_wait(&tfull[acc], aph, abort_flag, p.status, GK_DEV_TIMEOUT_EPILOGUE, tmo))
                 break;
             tc_fence_after();
+            if constexpr (SPLIT) {
+                tile = true;
+                break;
+            }
             const int i0 = t.p0 + q * 32;  // the warp's first P row
             const int64_t at = (p.wgrad ? t.g * p.gsc : 0) + t.qbase * p.ldq + i0 * p.ldp;
             const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
@@ -510,6 +529,71 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[acc]);
+        }
+    }
+
+    if constexpr (SPLIT) {
+        static_assert(EPI != EPI_STORE && BN <= 128, "the epilogues that a cluster shares");
+        tc_fence_before();
+        __syncwarp();
+        cluster_sync();  // every CTA's MMAs are done, its ring is idle
+        tc_fence_after();
+        const int q = warp & 3, sets = C::NEPI / 4, set = (warp - C::EPI_W0) >> 2;
+        const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+        const int units = tile ? (min(BN, t.qn) + 15) >> 4 : 0;
+        // unit u of CTA r lies at ((u / ctas) * ctas + r) * UNIT of its owner's shared memory
+        constexpr int UNIT = 16 * BM * 4;
+        if (warp >= C::EPI_W0) {
+            for (int u = set; u < units; u += sets) {
+                const int owner = u % ctas;
+                if (owner == rank) continue;
+                uint32_t v[16];
+                tmem_ld_cols16(tb + 16 * u, v);
+                const uint32_t at =
+                    mapa_shared(smem_u32(smem) + static_cast<uint32_t>((u - owner + rank) * UNIT), owner) +
+                    static_cast<uint32_t>(q * 32 + lane) * 4u;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) st_cluster_u32(at + e * BM * 4, v[e]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // the units have arrived
+        if (warp >= C::EPI_W0) {
+            const int i0 = t.p0 + q * 32;
+            const int pn = static_cast<int>(min(static_cast<int64_t>(32), p.np - i0));
+            const float bias = tile && epi_fwd(EPI) ? epi_bias(p.e, t.g, i0, pn, lane) : 0.0f;
+            float sum = 0.0f;
+            for (int u = set * ctas + rank; u < units; u += sets * ctas) {
+                const EpiAt at{i0, pn, t.qbase + 16 * u, t.qn - 16 * u};
+                uint32_t v[16];
+                tmem_ld_cols16(tb + 16 * u, v);
+                float a[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) a[e] = 0.0f;
+                for (int r = 0; r < ctas; ++r) {
+                    const float* part = reinterpret_cast<const float*>(
+                        smem + (u - rank + r) * UNIT + (q * 32 + lane) * 4);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        a[e] += r == rank ? __uint_as_float(v[e]) : part[e * BM];
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(a[e]);
+                EpiSide<EPI, 16> s;
+                auto columns = [&](auto pairs) {
+                    constexpr bool PAIRS = decltype(pairs)::value;
+                    s.template load<PAIRS>(p.e, at, p.out_type == GK_F32, lane);
+                    s.template own<PAIRS>(p.e, lane);
+                    epi_columns<EPI, 16, PAIRS>(p.e, p.c, p.out_type, p.ldq, p.ldp, at, v, s, p.alpha, bias,
+                                                sum, lane);
+                };
+                if (p.e.pairs)
+                    columns(std::true_type{});
+                else
+                    columns(std::false_type{});
+            }
+            if (epi_bwd(EPI) && tile)
+                epi_sum(p, t, tile0, i0, pn, set * ctas + rank, sets * ctas, sum, lane);
         }
     }
 
@@ -1016,11 +1100,12 @@ int launch_grouped_pair(const CUtensorMap& tp, const CUtensorMap& tq, const Grou
     return GK_OK;
 }
 
-template <int BN, int EPI>
+// ctas > 1: clusters that split the contraction (SPLIT).
+template <int BN, int EPI, bool SPLIT = false>
 int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedParams& p, int grid,
-                   int pdl, cudaStream_t stream, char* err, size_t errlen) {
+                   int ctas, int pdl, cudaStream_t stream, char* err, size_t errlen) {
     using C = GroupedCfg<BN>;
-    auto kern = grouped_half_kernel<BN, EPI>;
+    auto kern = grouped_half_kernel<BN, EPI, SPLIT>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kern, C::SMEM, done);
     if (e == cudaSuccess) {
@@ -1030,11 +1115,20 @@ int launch_grouped(const CUtensorMap& tp, const CUtensorMap& tq, const GroupedPa
         cfg.blockDim = dim3(C::THREADS);
         cfg.dynamicSmemBytes = C::SMEM;
         cfg.stream = stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchAttribute attr[2];
+        int n = 0;
+        if (SPLIT) {
+            attr[n].id = cudaLaunchAttributeClusterDimension;
+            attr[n].val.clusterDim.x = static_cast<unsigned>(ctas);
+            attr[n].val.clusterDim.y = 1;
+            attr[n++].val.clusterDim.z = 1;
+        }
+        if (pdl) {
+            attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[n++].val.programmaticStreamSerializationAllowed = 1;
+        }
         cfg.attrs = attr;
-        cfg.numAttrs = pdl ? 1 : 0;
+        cfg.numAttrs = static_cast<unsigned>(n);
         e = cudaLaunchKernelEx(&cfg, kern, tp, tq, p);
     }
     if (e == cudaSuccess) e = cudaGetLastError();
@@ -1100,6 +1194,43 @@ int pair_clusters() {
         }
         return c;
     });
+}
+
+// How many CTAs share a tile's contraction: the most (8, 4 or 2) for which all clusters are resident at once
+// and each CTA keeps four stages, else 1.
+template <int BN, int EPI>
+int split_ctas(int64_t tiles, int64_t stages) {
+    for (int ctas = 8; ctas > 1; ctas /= 2) {
+        if (stages < 4 * ctas || tiles * ctas > sm_count()) continue;
+        static PerDevice<int> cache[3];
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const int clusters = cache[ctas == 8 ? 0 : ctas == 4 ? 1 : 2].get(dev, [ctas] {
+            auto kern = grouped_half_kernel<BN, EPI, true>;
+            cudaLaunchConfig_t q;
+            memset(&q, 0, sizeof(q));
+            q.gridDim = dim3(static_cast<unsigned>(sm_count() / ctas * ctas));
+            q.blockDim = dim3(GroupedCfg<BN>::THREADS);
+            q.dynamicSmemBytes = GroupedCfg<BN>::SMEM;
+            cudaLaunchAttribute a[1];
+            a[0].id = cudaLaunchAttributeClusterDimension;
+            a[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+            a[0].val.clusterDim.y = 1;
+            a[0].val.clusterDim.z = 1;
+            q.attrs = a;
+            q.numAttrs = 1;
+            int c = 0;
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     GroupedCfg<BN>::SMEM) != cudaSuccess ||
+                cudaOccupancyMaxActiveClusters(&c, kern, &q) != cudaSuccess || c <= 0) {
+                cudaGetLastError();
+                c = -1;
+            }
+            return c;
+        });
+        if (tiles <= clusters) return ctas;
+    }
+    return 1;
 }
 
 template <int EPI>
@@ -1208,6 +1339,17 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
                                  sizeof(err));
         if (rc) return set_last_error(rc, err);
     }
+    // Products with few tiles share them between clusters of CTAs; `few`: no more tiles than that, whatever
+    // the groups are.
+    const int64_t few = (p.np + BM - 1) / BM * ((p.rows + static_cast<int64_t>(p.groups) * (bn - 1)) / bn);
+    int ctas = 1;
+    if constexpr (EPI != EPI_STORE) {
+        const int64_t stages = (plen + GBK - 1) / GBK;
+        if (tma && !pair && bn <= 128)
+            ctas = bn == 32   ? split_ctas<32, EPI>(few, stages)
+                   : bn == 64 ? split_ctas<64, EPI>(few, stages)
+                              : split_ctas<128, EPI>(few, stages);
+    }
     auto launch = [&]() -> int {
         if (pair) {
             // (tall tiles may be walked in halves)
@@ -1220,7 +1362,11 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
         const int grid = static_cast<int>(tiles < sms ? tiles : sms);
         auto go = [&](auto bn_tag) {
             constexpr int BN = decltype(bn_tag)::value;
-            return launch_grouped<BN, EPI>(tmp, tmq, p, grid, pdl, stream, err, sizeof(err));
+            if constexpr (EPI != EPI_STORE && BN <= 128)
+                if (ctas > 1)
+                    return launch_grouped<BN, EPI, true>(tmp, tmq, p, static_cast<int>(few) * ctas, ctas, pdl,
+                                                         stream, err, sizeof(err));
+            return launch_grouped<BN, EPI>(tmp, tmq, p, grid, 1, pdl, stream, err, sizeof(err));
         };
         switch (bn) {
             case 32: return go(std::integral_constant<int, 32>{});
@@ -1231,7 +1377,7 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
     };
     if constexpr (epi_bwd(EPI)) {
         if (p.e.dbias) {  // a slot for each share of each tile along the Q side
-            const int shares = tall ? GPairCfg<2, EPI>::NEPI / 4 : bn == 32 ? 1 : 2;
+            const int shares = tall ? GPairCfg<2, EPI>::NEPI / 4 : (bn == 32 ? 1 : 2) * ctas;
             const int64_t slots = ((static_cast<int64_t>(p.rows) + bn - 1) / bn + p.groups) * shares;
             void* part = nullptr;
             if ((rc = scratch_alloc(&part, static_cast<size_t>(slots * p.np) * 4, stream))) return rc;

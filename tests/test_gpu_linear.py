@@ -181,6 +181,29 @@ def test_forward_pairs(sizes, rows, k, n, out, act):
     assert torch.equal(c, again)
 
 
+# few tiles and a long contraction: clusters that share a tile, of 8, 4 and 2 CTAs
+SHARED = [(None, 1, 4096, 300), (None, 17, 1000, 264), (None, 33, 2050, 512), (None, 100, 600, 1100),
+          (None, 128, 4100, 7000), ([3, 0, 20, 9], 40, 777, 250), ([70, 58], 128, 1030, 1024)]
+
+
+@pytest.mark.parametrize("sizes,rows,k,n", SHARED)
+@pytest.mark.parametrize("act,out", [("relu", "bf16"), ("leaky", "f32"), ("gelu", "f16")])
+def test_forward_shared_tiles(sizes, rows, k, n, act, out):
+    torch = torch_cuda()
+    dtype, exact = ("f16" if out == "f16" else "bf16"), act != "gelu"
+    a, b, off, groups = problem(sizes, rows, k, n, dtype, "k" if n % 8 else "n", 25, exact)
+    bias = numbers(28, (groups, n), dtype, exact)
+    r = numbers(29, (rows, n), out, exact)
+    c0 = torch.full((rows, n), 7.0, dtype=tdt(out), device="cuda")
+    z0 = c0.to(tdt(dtype))
+    c, z = c0.clone(), z0.clone()
+    forward(a, b, off, dtype, act, bias, r, c, z)
+    check_forward(a, b, off, dtype, act, bias, r, c, z, c0, z0, out=out, exact=exact)
+    again = c0.clone()
+    forward(a, b, off, dtype, act, bias, r, again)
+    assert torch.equal(c, again)
+
+
 @pytest.mark.parametrize("rows,k,n", [(3, 40, 24), (150, 64, 130), (2048, 64, 4096)])
 def test_forward_onto_the_residual(rows, k, n):
     """C is the residual itself."""
@@ -343,6 +366,27 @@ def test_backward_pairs(sizes, rows, k, n, out, act, zform):
     a, b, off, groups = problem(sizes, rows, k, n, dtype, "k" if act == "relu" else "n", 80, exact)
     z = numbers(83, (rows, n), dtype, exact, 2.0)
     q = {"act8": lambda: gk.quantize_act8(ref(z)), "half": lambda: z, None: lambda: None}[zform]()
+    z64 = act8_values(q) if zform == "act8" else z.double()
+    c0 = torch.full((rows, n), 7.0, dtype=tdt(out), device="cuda")
+    c = c0.clone()
+    dbias = torch.empty(groups, n, dtype=torch.float32, device="cuda")
+    backward(a, b, off, dtype, q, act, c, dbias)
+    d, mag = product64(a, b, off)
+    check_backward(d, (k + 36) * 2.0 ** -23 * mag, z64, off, dtype, act, c, c0, dbias, out, exact)
+    again = torch.empty_like(dbias)
+    backward(a, b, off, dtype, q, act, c, again)
+    assert torch.equal(dbias, again)
+
+
+@pytest.mark.parametrize("sizes,rows,k,n", SHARED)
+@pytest.mark.parametrize("act,zform,out", [("relu", "act8", "bf16"), ("leaky", "half", "f32"),
+                                           ("silu", "act8", "f16")])
+def test_backward_shared_tiles(sizes, rows, k, n, act, zform, out):
+    torch = torch_cuda()
+    dtype, exact = ("f16" if out == "f16" else "bf16"), act != "silu"
+    a, b, off, groups = problem(sizes, rows, k, n, dtype, "k" if n % 8 else "n", 85, exact)
+    z = numbers(88, (rows, n), dtype, exact, 2.0)
+    q = gk.quantize_act8(ref(z)) if zform == "act8" else z
     z64 = act8_values(q) if zform == "act8" else z.double()
     c0 = torch.full((rows, n), 7.0, dtype=tdt(out), device="cuda")
     c = c0.clone()
