@@ -112,9 +112,9 @@ def _sync(stream) -> None:
 
 def _flat(data):
     """(pointer, length in elements) of a flat tensor / (ptr, len) pair."""
-    if isinstance(data, tuple):
+    if type(data) is tuple:
         return int(data[0]), int(data[1])
-    return int(data.data_ptr()), int(data.numel())
+    return data.data_ptr(), data.numel()
 
 
 class MatRef:

@@ -4,11 +4,10 @@
 //   loss = coef E sum_e f_e P_e;   dloss/dlogit_te = rates_e-weighted:  p_te (rates_e - sum_j p_tj rates_j),
 //   rates_e = coef E f_e / live
 //
-// Bound by memory: the logits are read once in each direction. A warp takes a token, its logits in
-// registers (V consecutive ones a lane, J times), and in the forward pass adds its p to sums that stay
-// in registers over all of its tokens; counts are integers in shared memory. Each block leaves its sums
+// Bound by memory: the logits are read once in each direction. A few lanes take a token, its logits in
+// registers, and in the forward pass add its p to sums that stay in registers over all of their tokens; counts are integers in shared memory. Each block leaves its sums
 // and counts, a last block adds them (one block does all of it where there are few tokens). No
-// floating atomics: which token a warp takes depends on the sizes alone, and so does every sum.
+// floating atomics: which token a warp takes depends on the sizes (and the SMs) alone, and so does every sum.
 // Differences of logits go through the fast exponential (2^-22, and 2^-24 of the difference: the large p
 // come from small differences), sums over blocks through f64.
 #include <cuda_bf16.h>
@@ -28,7 +27,6 @@ namespace {
 
 constexpr int MAX_EXPERTS = 1024;
 constexpr int BW = 16;           // warps of a block
-constexpr int TOKENS_A_WARP = 4; // before another block is added
 
 struct Router {
     const void* x;
@@ -39,16 +37,26 @@ struct Router {
     unsigned int* status;
 };
 
-// A token's logits as they lie: lane l holds elements (32 j + l) V .. + V - 1.
-template <int T, int V, int J>
+// How a warp takes tokens: L lanes a token, 32 / L tokens at a time, and lane q of a token's holds the logits
+// (L j + q) V .. + V - 1 for j < J, as they lie: f32 bits, or 16-bit values two a word (V = 4) or one.
+// (A whole warp a token spends most of its instructions on reductions over lanes: 155 a token of 256
+// experts forward and 220 backward.)
+template <int T_, int V_, int J_, int L_>
+struct Layout {
+    static constexpr int T = T_, V = V_, J = J_, L = L_, N = J * V, G = 32 / L;
+    static constexpr int U = 1;  // tokens of a lane at a time, their loads in flight
+};
+
+template <typename C>
 struct Logits {
-    uint32_t w[J * V];  // f32 bits, or 16-bit values two a word (V == 4), or one a word (V == 1)
-    __device__ __forceinline__ void load(const Router& p, int64_t t, int lane) {
+    static constexpr int T = C::T, V = C::V, J = C::J;
+    uint32_t w[C::N];
+    __device__ __forceinline__ void load(const Router& p, int64_t t, int q) {
         constexpr int ES = T == GK_F32 ? 4 : 2;
-        const uint8_t* row = static_cast<const uint8_t*>(p.x) + (t * p.rs + (V == 4 ? lane * V : 0)) * ES;
+        const uint8_t* row = static_cast<const uint8_t*>(p.x) + (t * p.rs + (V == 4 ? q * V : 0)) * ES;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int e = (32 * j + lane) * V;
+            const int e = (C::L * j + q) * V;
             if (e >= p.experts) continue;
             if constexpr (V == 1) {
                 const uint8_t* at = row + e * p.cs * ES;
@@ -57,10 +65,10 @@ struct Logits {
                 else
                     w[j] = *reinterpret_cast<const uint16_t*>(at);
             } else if (T == GK_F32) {
-                const uint4 v = ld_global_v4(row + 32 * j * V * ES);
+                const uint4 v = ld_global_v4(row + C::L * j * V * ES);
                 w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
             } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(row + 32 * j * V * ES);
+                const uint2 v = *reinterpret_cast<const uint2*>(row + C::L * j * V * ES);
                 w[4 * j] = v.x, w[4 * j + 1] = v.y;
             }
         }
@@ -72,61 +80,56 @@ struct Logits {
                            : __uint_as_float(h << 16);
     }
     // The softmax is y times the value returned; 0 everywhere where every logit is minus infinity.
-    __device__ __forceinline__ float softmax(const Router& p, int lane, F2 (&y)[(J * V + 1) / 2]) const {
-        float x[(J * V + 1) / 2 * 2];
-        x[(J * V + 1) / 2 * 2 - 1] = -INFINITY;
-        float m = -INFINITY;
+    __device__ __forceinline__ float softmax(const Router& p, int q, F2 (&y)[C::N / 2]) const {
+        float x[C::N], m = -INFINITY;
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                x[V * j + v] = (32 * j + lane) * V < p.experts ? value(j, v) : -INFINITY;
+                x[V * j + v] = (C::L * j + q) * V < p.experts ? value(j, v) : -INFINITY;
                 m = fmaxf(m, x[V * j + v]);
             }
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
+#pragma unroll
+        for (int d = C::L / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         const bool none = m == -INFINITY;
         // (the difference first: logits of the type's lowest value stay apart from infinities)
         const F2 scale(1.44269504f), base(none ? 0.0f : -m);
         F2 s2(0.0f);
 #pragma unroll
-        for (int i = 0; i < (J * V + 1) / 2; ++i) {
+        for (int i = 0; i < C::N / 2; ++i) {
             const F2 t = mul2(add2(F2(x[2 * i], x[2 * i + 1]), base), scale);
             y[i] = F2(exp2_hw(t.lo()), exp2_hw(t.hi()));
             s2 = add2(s2, y[i]);
         }
         float s = s2.lo() + s2.hi();
 #pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        for (int d = C::L / 2; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         // (a row of NaN also has no maximum: its sum is NaN, and stays so)
         return none && s == 0.0f ? 0.0f : __frcp_rn(s);
     }
 };
 
-// Tokens that a warp takes at a time: as many as keep its loads in flight.
-template <int V, int J>
-constexpr int together() {
-    return V * J <= 8 ? 4 : 1;
-}
-
-// The ids of n tokens from t0 on (they lie one after the other) into `hist`, when there is one; a bit for
-// each token that has any.
-__device__ __forceinline__ uint32_t token_ids(const Router& p, int64_t t0, int n, int* hist, int lane) {
-    uint32_t live = 0;
-    bool bad = false;
-    for (int i = lane; i < n * p.top; i += 32) {
-        const int64_t at = t0 * p.top + i;
+// A token's ids into `hist` (when there is one), its L lanes together; whether it has any. All lanes of the
+// warp call it, with on == false where they have no token.
+template <int L>
+__device__ __forceinline__ bool token_ids(const Router& p, int64_t t, bool on, int* hist, int lane) {
+    const int q = lane % L;
+    bool any = false, bad = false;
+    for (int i = q; on && i < p.top; i += L) {
+        const int64_t at = t * p.top + i;
         const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at]
                                    : static_cast<const int32_t*>(p.ids)[at];
         if (id >= 0 && id < p.experts) {
-            const int k = (i >= p.top) + (i >= 2 * p.top) + (i >= 3 * p.top);
-            live |= 1u << k;
+            any = true;
             if (hist) atomicAdd(&hist[id], 1);
         } else if (id >= 0) {
             bad = true;
         }
     }
     if (hist && bad) atomicOr(p.status, GK_DEV_BAD_OFFSETS);
-    return __reduce_or_sync(0xffffffffu, live);
+    const uint32_t who = __ballot_sync(0xffffffffu, any);
+    constexpr uint32_t mine = L == 32 ? 0xffffffffu : (1u << (L & 31)) - 1u;
+    return (who >> (lane - q) & mine) != 0;
 }
 
 // What a block leaves, in words: experts sums (f32), experts counts and the live tokens. Behind all
@@ -200,47 +203,55 @@ __device__ __forceinline__ void finish(S sum, N count, int tokens, int experts, 
     }
 }
 
-template <int T, int V, int J>
-__global__ void __launch_bounds__(32 * BW, V * J <= 8 ? 2 : 1)
+template <typename C>
+__global__ void __launch_bounds__(32 * BW, C::N <= 16 ? 2 : 1)
     balance_kernel(const Router p, uint32_t* part, const BalanceOut o) {
-    constexpr int U = together<V, J>();
     extern __shared__ float smem[];  // BW x experts sums, then the block's part
     uint32_t* own = reinterpret_cast<uint32_t*>(smem + BW * p.experts);
     int* hist = reinterpret_cast<int*>(own + p.experts);
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, q = lane % C::L;
     for (int i = threadIdx.x; i <= p.experts; i += blockDim.x) hist[i] = 0;  // counts, live tokens
     griddep_wait();
     griddep_launch_dependents();
     __syncthreads();
-    F2 sum[(J * V + 1) / 2];
+    F2 sum[C::N / 2];
 #pragma unroll
-    for (int i = 0; i < (J * V + 1) / 2; ++i) sum[i] = F2(0.0f);
+    for (int i = 0; i < C::N / 2; ++i) sum[i] = F2(0.0f);
     int live = 0;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * BW * U;
-    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * BW + w) * U; t0 < p.tokens; t0 += step) {
-        const int n = static_cast<int>(min(static_cast<int64_t>(U), p.tokens - t0));
-        Logits<T, V, J> x[U];
+    const int64_t step = static_cast<int64_t>(gridDim.x) * BW * C::G * C::U;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * BW + w) * C::G * C::U; t0 < p.tokens; t0 += step) {
+        Logits<C> x[C::U];
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (k < n) x[k].load(p, t0 + k, lane);
-        const uint32_t has = token_ids(p, t0, n, hist, lane);
-        live += __popc(has);
+        for (int k = 0; k < C::U; ++k) {
+            const int64_t t = t0 + k * C::G + lane / C::L;
+            if (t < p.tokens) x[k].load(p, t, q);
+        }
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            if (!(has >> k & 1)) continue;
-            F2 y[(J * V + 1) / 2];
-            const F2 inv(x[k].softmax(p, lane, y));
+        for (int k = 0; k < C::U; ++k) {
+            const int64_t t = t0 + k * C::G + lane / C::L;
+            const bool has = token_ids<C::L>(p, t, t < p.tokens, hist, lane);
+            live += has && q == 0;
+            if (!__any_sync(0xffffffffu, has)) continue;
+            F2 y[C::N / 2];
+            const float inv = x[k].softmax(p, q, y);
+            if (has) {  // (padding may hold anything)
 #pragma unroll
-            for (int i = 0; i < (J * V + 1) / 2; ++i) sum[i] = fma2(y[i], inv, sum[i]);
+                for (int i = 0; i < C::N / 2; ++i) sum[i] = fma2(y[i], F2(inv), sum[i]);
+            }
         }
     }
+    live = __reduce_add_sync(0xffffffffu, live);
+    // the warp's sums: the tokens that it took at one time lie L lanes apart
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < C::J; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = (32 * j + lane) * V + v;
-            const F2 pair = sum[(V * j + v) / 2];
-            if (e < p.experts) smem[w * p.experts + e] = (V * j + v) & 1 ? pair.hi() : pair.lo();
+        for (int v = 0; v < C::V; ++v) {
+            const F2 pair = sum[(C::V * j + v) / 2];
+            float a = (C::V * j + v) & 1 ? pair.hi() : pair.lo();
+#pragma unroll
+            for (int d = C::L; d < 32; d <<= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+            const int e = (C::L * j + q) * C::V + v;
+            if (lane < C::L && e < p.experts) smem[w * p.experts + e] = a;
         }
     if (lane == 0 && live) atomicAdd(&hist[p.experts], live);
     __syncthreads();
@@ -322,106 +333,113 @@ __global__ void __launch_bounds__(32 * FW)
            __ldcg(counts + experts), experts, o);
 }
 
-template <int T, int V, int J>
-__global__ void __launch_bounds__(256, V * J <= 8 ? 4 : 1)
+template <typename C>
+__global__ void __launch_bounds__(256, C::N <= 16 ? 4 : 2)
     balance_backward_kernel(const Router p, const float* rates, const float* dloss, void* dx,
                             int64_t ds, int64_t dc) {
-    constexpr int U = together<V, J>();
     griddep_wait();
     griddep_launch_dependents();
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    F2 rate[(J * V + 1) / 2];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5, q = lane % C::L;
+    F2 rate[C::N / 2];
     const float scale = *dloss;
 #pragma unroll
-    for (int i = 0; i < (J * V + 1) / 2; ++i) {
+    for (int i = 0; i < C::N / 2; ++i) {
         float r[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int at = 2 * i + k, e = (32 * (at / V) + lane) * V + at % V;
-            r[k] = at < J * V && e < p.experts ? rates[e] : 0.0f;
+            const int at = 2 * i + k, e = (C::L * (at / C::V) + q) * C::V + at % C::V;
+            r[k] = e < p.experts ? rates[e] : 0.0f;
         }
         rate[i] = F2(r[0], r[1]);
     }
-    const int64_t step = static_cast<int64_t>(gridDim.x) * warps * U;
-    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + w) * U; t0 < p.tokens; t0 += step) {
-        const int n = static_cast<int>(min(static_cast<int64_t>(U), p.tokens - t0));
-        Logits<T, V, J> x[U];
+    constexpr int ES = C::T == GK_F32 ? 4 : 2;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps * C::G * C::U;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + w) * C::G * C::U; t0 < p.tokens; t0 += step) {
+        Logits<C> x[C::U];
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (k < n) x[k].load(p, t0 + k, lane);
-        const uint32_t has = token_ids(p, t0, n, nullptr, lane);
+        for (int k = 0; k < C::U; ++k) {
+            const int64_t t = t0 + k * C::G + lane / C::L;
+            if (t < p.tokens) x[k].load(p, t, q);
+        }
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            if (k >= n) break;
-            F2 y[(J * V + 1) / 2];
-            if (has >> k & 1) {
-                const float inv = x[k].softmax(p, lane, y);
-                F2 dot2(0.0f);
+        for (int k = 0; k < C::U; ++k) {
+            const int64_t t = t0 + k * C::G + lane / C::L;
+            const bool has = token_ids<C::L>(p, t, t < p.tokens, nullptr, lane);
+            F2 y[C::N / 2];
+            const float inv = x[k].softmax(p, q, y);
+            F2 dot2(0.0f);
 #pragma unroll
-                for (int i = 0; i < (J * V + 1) / 2; ++i) dot2 = fma2(y[i], rate[i], dot2);
-                float dot = dot2.lo() + dot2.hi();
+            for (int i = 0; i < C::N / 2; ++i) dot2 = fma2(y[i], rate[i], dot2);
+            float dot = dot2.lo() + dot2.hi();
 #pragma unroll
-                for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-                const F2 less(-(dot * inv)), f(scale * inv);
+            for (int d = C::L / 2; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+            const F2 less(-(dot * inv)), f(scale * inv);
 #pragma unroll
-                for (int i = 0; i < (J * V + 1) / 2; ++i) y[i] = mul2(mul2(y[i], f), add2(rate[i], less));
-            } else {
+            for (int i = 0; i < C::N / 2; ++i)  // (padding may hold anything)
+                y[i] = has ? mul2(mul2(y[i], f), add2(rate[i], less)) : F2(0.0f);
+            if (t >= p.tokens) continue;
+            uint8_t* row = static_cast<uint8_t*>(dx) + (t * ds + (C::V == 4 ? q * C::V : 0)) * ES;
 #pragma unroll
-                for (int i = 0; i < (J * V + 1) / 2; ++i) y[i] = F2(0.0f);
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int e = (32 * j + lane) * V;
+            for (int j = 0; j < C::J; ++j) {
+                const int e = (C::L * j + q) * C::V;
                 if (e >= p.experts) continue;
-                const int64_t at = (t0 + k) * ds + e * dc;
-                if constexpr (V == 1) {
+                if constexpr (C::V == 1) {
                     const float g = j & 1 ? y[j / 2].hi() : y[j / 2].lo();
-                    if (T == GK_F32)
-                        to_out(static_cast<float*>(dx) + at, g);
-                    else if (T == GK_F16)
-                        to_out(static_cast<__half*>(dx) + at, g);
+                    uint8_t* at = row + e * dc * ES;
+                    if (C::T == GK_F32)
+                        to_out(reinterpret_cast<float*>(at), g);
+                    else if (C::T == GK_F16)
+                        to_out(reinterpret_cast<__half*>(at), g);
                     else
-                        to_out(static_cast<__nv_bfloat16*>(dx) + at, g);
+                        to_out(reinterpret_cast<__nv_bfloat16*>(at), g);
                 } else {
+                    uint8_t* at = row + C::L * j * C::V * ES;
                     uint32_t b[4];
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         const F2 pair = y[(4 * j + v) / 2];
                         b[v] = __float_as_uint(v & 1 ? pair.hi() : pair.lo());
                     }
-                    if (T == GK_F32)
-                        st_global_v4(static_cast<float*>(dx) + at, b[0], b[1], b[2], b[3]);
+                    if (C::T == GK_F32)
+                        st_global_v4(at, b[0], b[1], b[2], b[3]);
                     else
-                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dx) + at) =
-                            make_uint2(round_pair(b[0], b[1], 1.0f, T),
-                                       round_pair(b[2], b[3], 1.0f, T));
+                        *reinterpret_cast<uint2*>(at) = make_uint2(round_pair(b[0], b[1], 1.0f, C::T),
+                                                                   round_pair(b[2], b[3], 1.0f, C::T));
                 }
             }
         }
     }
 }
 
-// f(type, V, J) as constants: V = 4 where a row's logits are whole 4-element pieces, J the smallest of
-// those compiled that holds the experts (up to 8 in pieces, 32 otherwise).
+// f(a Layout): V = 4 where a row's logits are whole 4-element pieces, sixteen logits a lane where the
+// experts allow that (fewer lanes a token mean fewer steps over lanes), 32 at most.
 template <typename F>
 int with_layout(int type, bool vec, int experts, F f) {
     auto pick = [&](auto t) {
-        auto go = [&](auto v, auto j) { return f(t, v, j); };
-        using std::integral_constant;
+        constexpr int T = decltype(t)::value;
         if (vec) {
-            integral_constant<int, 4> v;
-            if (experts <= 128) return go(v, integral_constant<int, 1>{});
-            if (experts <= 256) return go(v, integral_constant<int, 2>{});
-            return go(v, integral_constant<int, 8>{});
+            if (experts <= 16) return f(Layout<T, 4, 4, 1>{});
+            if (experts <= 64) return f(Layout<T, 4, 4, 4>{});
+            if (experts <= 256) return f(Layout<T, 4, 4, 16>{});
+            if (experts <= 512) return f(Layout<T, 4, 4, 32>{});
+            return f(Layout<T, 4, 8, 32>{});
         }
-        integral_constant<int, 1> v;
-        if (experts <= 32) return go(v, integral_constant<int, 1>{});
-        if (experts <= 256) return go(v, integral_constant<int, 8>{});
-        return go(v, integral_constant<int, 32>{});
+        if (experts <= 64) return f(Layout<T, 1, 16, 4>{});
+        if (experts <= 256) return f(Layout<T, 1, 16, 16>{});
+        if (experts <= 512) return f(Layout<T, 1, 16, 32>{});
+        return f(Layout<T, 1, 32, 32>{});
     };
     if (type == GK_F32) return pick(std::integral_constant<int, GK_F32>{});
     if (type == GK_F16) return pick(std::integral_constant<int, GK_F16>{});
     return pick(std::integral_constant<int, GK_BF16>{});
+}
+
+// Tokens of a warp at a time.
+int tokens_a_step(int type, bool vec, int experts) {
+    return with_layout(type, vec, experts, [](auto layout) {
+        using C = decltype(layout);
+        return C::G * C::U;
+    });
 }
 
 bool in_fours(const void* p, int64_t rows, int64_t cols, int64_t rs, int64_t cs, size_t es) {
@@ -489,17 +507,19 @@ int gk_moe_balance(gk_matref logits, int x_type, const void* ids, size_t ids_len
     if ((rc = api_check_device(&dev))) return rc;
     p.status = device_status_ptr();
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t want = (static_cast<int64_t>(p.tokens) + BW * TOKENS_A_WARP - 1) / (BW * TOKENS_A_WARP);
-    const int64_t most = 2ll * sm_count();  // resident with up to 256 experts
+    const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es);
+    // a block more for each step of tokens, up to what is resident
+    const int64_t step = BW * tokens_a_step(x_type, vec, p.experts), most = 2ll * sm_count();
+    const int64_t want = (p.tokens + step - 1) / step;
     const int blocks = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
     const BalanceOut o{coef, loss, counts, offsets, rates};
     void* part = nullptr;
     if (blocks > 1 &&
         (rc = scratch_alloc(&part, static_cast<size_t>(part_words(blocks, p.experts)) * 4, st)))
         return rc;
-    const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es);
-    rc = with_layout(x_type, vec, p.experts, [&](auto t, auto v, auto j) {
-        auto kern = balance_kernel<decltype(t)::value, decltype(v)::value, decltype(j)::value>;
+    rc = with_layout(x_type, vec, p.experts, [&](auto layout) {
+        using C = decltype(layout);
+        auto kern = balance_kernel<C>;
         const int smem = ((BW + 2) * p.experts + 1) * 4;
         static std::atomic<uint64_t> done{0};
         const cudaError_t e = allow_smem(kern, ((BW + 2) * MAX_EXPERTS + 1) * 4, done);
@@ -546,11 +566,13 @@ int gk_moe_balance_backward(gk_matref logits, int x_type, const void* ids, size_
     int dev = 0;
     if ((rc = api_check_device(&dev))) return rc;
     p.status = device_status_ptr();
-    const int64_t want = (static_cast<int64_t>(p.tokens) + 31) / 32, most = 4ll * sm_count();
     const bool vec = in_fours(logits.data, p.tokens, p.experts, p.rs, p.cs, es) &&
                      in_fours(dlogits.data, p.tokens, p.experts, dlogits.rs, dlogits.cs, es);
-    return with_layout(x_type, vec, p.experts, [&](auto t, auto v, auto j) {
-        return launch_overlapped(balance_backward_kernel<decltype(t)::value, decltype(v)::value, decltype(j)::value>,
+    const int64_t step = 8 * tokens_a_step(x_type, vec, p.experts), most = 4ll * sm_count();
+    const int64_t want = (p.tokens + step - 1) / step;
+    return with_layout(x_type, vec, p.experts, [&](auto layout) {
+        using C = decltype(layout);
+        return launch_overlapped(balance_backward_kernel<C>,
                                  dim3(static_cast<unsigned>(want < most ? want : most)), 256,
                                  static_cast<cudaStream_t>(stream), p, rates, dloss, dlogits.data,
                                  static_cast<int64_t>(dlogits.rs), static_cast<int64_t>(dlogits.cs));
