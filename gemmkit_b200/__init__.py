@@ -136,8 +136,10 @@ class MatRef:
         return cls(data, rows, cols, 1, rows)
 
     def c(self) -> MatRefC:
-        p, n = _flat(self.data)
-        return MatRefC(p, n, self.rows, self.cols, self.rs, self.cs)
+        d = self.data
+        if type(d) is tuple:
+            return MatRefC(int(d[0]), int(d[1]), self.rows, self.cols, self.rs, self.cs)
+        return MatRefC(d.data_ptr(), d.numel(), self.rows, self.cols, self.rs, self.cs)
 
     def ptr(self) -> int:
         return _flat(self.data)[0]
@@ -147,8 +149,10 @@ class MatMut(MatRef):
     """A mutable strided view (gemmkit MatMut), the output C."""
 
     def c(self) -> MatMutC:
-        p, n = _flat(self.data)
-        return MatMutC(p, n, self.rows, self.cols, self.rs, self.cs)
+        d = self.data
+        if type(d) is tuple:
+            return MatMutC(int(d[0]), int(d[1]), self.rows, self.cols, self.rs, self.cs)
+        return MatMutC(d.data_ptr(), d.numel(), self.rows, self.cols, self.rs, self.cs)
 
 
 class Workspace:
@@ -819,10 +823,13 @@ def gemm_fp4(alpha: float, a: Fp4Matrix, b: Fp4Matrix, beta: float, c: MatMut,
 
 # ---- feed-forward layers, dense or by expert ---------------------------------------------------
 
-_NO_REF, _NO_MUT = MatRefC(), MatMutC()
+_NO_MUT = MatMutC()
 
 
 def _half_type(name: str, data, half: int, f32_too: bool = False) -> int:
+    t = half if type(data) is tuple else _elem.get(data.dtype, -1)
+    if t == half:
+        return t
     t = _elem_type(data, half)
     if t != half and not (f32_too and t == _lib.DT_F32):
         raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must hold "
@@ -839,11 +846,9 @@ def _groups_of(offsets):
     return ptr, max(groups, 0)
 
 
-def _vector(name, t, half, groups, n, gs):
+def _vector(name, t, half, n, gs):
     """(pointer, length, group stride, type) of a bias or its gradient."""
-    if t is None:
-        return None, 0, 0, half
-    if not isinstance(t, tuple) and not t.is_contiguous():
+    if type(t) is not tuple and not t.is_contiguous():
         raise GemmkitError(GK_EINVAL, f"gemmkit: {name} must be contiguous")
     return (*_flat(t), n if gs is None else int(gs), _half_type(name, t, half, True))
 
@@ -864,16 +869,23 @@ def gemm_half_epilogue(alpha: float, a: MatRef, b: MatRef, c: MatMut, bias=None,
     rd, zd = residual and residual.data, z and z.data
     _same_device("A", a.data, "B", b.data, "C", c.data, "offsets", offsets, "bias", bias,
                  "residual", rd, "z", zd)
-    for name, d in (("A", a.data), ("B", b.data), ("z", zd)):
-        if d is not None:
-            _half_type(name, d, half)
+    _half_type("A", a.data, half)
+    _half_type("B", b.data, half)
+    if zd is not None:
+        _half_type("z", zd, half)
     out = _elem_type(c.data, half)
     if rd is not None and _elem_type(rd, out) != out:
         raise GemmkitError(GK_EINVAL, "gemmkit: the residual must have C's type")
     ptr, groups = _groups_of(offsets)
-    epi = _lib.EpilogueC(act.kind if act else _lib.ACT_NONE, act.slope if act else 0.0,
-                         *_vector("bias", bias, half, groups, c.cols, bias_gs),
-                         residual.c() if residual else _NO_REF, z.c() if z else _NO_MUT)
+    epi = _lib.EpilogueC()  # (no activation, bias, residual or z)
+    if act:
+        epi.act, epi.slope = act.kind, act.slope
+    if bias is not None:
+        epi.bias, epi.bias_len, epi.bias_gs, epi.bias_type = _vector("bias", bias, half, c.cols, bias_gs)
+    if residual:
+        epi.residual = residual.c()
+    if z:
+        epi.z = z.c()
     _check(_lib.load().gk_gemm_half_epilogue(int(is_f16), groups, ptr, float(alpha), a.c(), b.c(),
                                              int(b_gs), C.byref(epi), c.c(), out, par.c(),
                                              _stream(stream)))
@@ -881,16 +893,19 @@ def gemm_half_epilogue(alpha: float, a: MatRef, b: MatRef, c: MatMut, bias=None,
         _sync(stream)
 
 
-def _epilogue_bwd(z, act, dbias, dbias_gs, half, groups, n):
-    kind, slope = (act.kind, act.slope) if act else (_lib.ACT_NONE, 0.0)
-    z16, z8 = _NO_REF, None
+def _epilogue_bwd(z, act, dbias, dbias_gs, half, n):
+    epi = _lib.EpilogueBwdC()  # (no activation, z or dbias)
+    if act:
+        epi.act, epi.slope = act.kind, act.slope
     if isinstance(z, Act8Matrix):
-        z8 = C.pointer(z.c)
+        epi.z8 = C.pointer(z.c)
     elif z is not None:
         _half_type("z", z.data, half)
-        z16 = z.c()
-    return _lib.EpilogueBwdC(kind, slope, z16, z8,
-                             *_vector("dbias", dbias, half, groups, n, dbias_gs))
+        epi.z = z.c()
+    if dbias is not None:
+        epi.dbias, epi.dbias_len, epi.dbias_gs, epi.dbias_type = \
+            _vector("dbias", dbias, half, n, dbias_gs)
+    return epi
 
 
 def _z_data(z):
@@ -908,10 +923,10 @@ def gemm_half_dact(alpha: float, a: MatRef, b: MatRef, z, act: Optional[Activati
     half = _lib.DT_F16 if is_f16 else _lib.DT_BF16
     _same_device("A", a.data, "B", b.data, "C", c.data, "offsets", offsets, "z", _z_data(z),
                  "dbias", dbias)
-    for name, d in (("A", a.data), ("B", b.data)):
-        _half_type(name, d, half)
+    _half_type("A", a.data, half)
+    _half_type("B", b.data, half)
     ptr, groups = _groups_of(offsets)
-    epi = _epilogue_bwd(z, act, dbias, dbias_gs, half, groups, c.cols)
+    epi = _epilogue_bwd(z, act, dbias, dbias_gs, half, c.cols)
     _check(_lib.load().gk_gemm_half_dact(int(is_f16), groups, ptr, float(alpha), a.c(), b.c(),
                                          int(b_gs), C.byref(epi), c.c(), _elem_type(c.data, half),
                                          par.c(), _stream(stream)))
@@ -931,11 +946,27 @@ def act_backward(dy: MatRef, z, act: Optional[Activation], dz: Optional[MatMut],
     _half_type("dY", dy.data, half)
     out = half if dzd is None else _elem_type(dzd, half)
     ptr, groups = _groups_of(offsets)
-    epi = _epilogue_bwd(z, act, dbias, dbias_gs, half, groups, dy.cols)
+    epi = _epilogue_bwd(z, act, dbias, dbias_gs, half, dy.cols)
     _check(_lib.load().gk_act_backward(int(is_f16), groups, ptr, dy.c(), C.byref(epi),
                                        dz.c() if dz else _NO_MUT, out, _stream(stream)))
     if sync:
         _sync(stream)
+
+
+_devices = {}  # torch.device objects by index
+
+
+def _buffer(n, dtype, stream):
+    """n unwritten elements on the current device, for torch's current stream or for `stream`."""
+    torch, current = _cuda[0], _cuda[1]()
+    device = _devices.get(current)
+    if device is None:
+        device = _devices[current] = torch.device("cuda", current)
+    if stream is None:
+        return torch.empty(n, dtype=dtype, device=device)
+    # not what the current stream may still be writing
+    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
+        return torch.empty(n, dtype=dtype, device=device)
 
 
 class Act8Matrix:
@@ -989,15 +1020,10 @@ class Act8Matrix:
         if rows < 0 or cols < 0:
             raise GemmkitError(GK_EINVAL, f"gemmkit: no 8-bit matrix of {rows}x{cols}")
         torch = calls[0]
-        device = torch.device("cuda", calls[1]())
         nb = (cols + 31) // 32
         pitch = (nb + 15) // 16 * 16  # of the exponents: whole 16-byte pieces, as the codes' rows
         n = rows * nb * 32
-        if stream is None:
-            buf = torch.empty(n + rows * pitch, dtype=torch.uint8, device=device)
-        else:  # not what the current stream may still be writing
-            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
-                buf = torch.empty(n + rows * pitch, dtype=torch.uint8, device=device)
+        buf = _buffer(n + rows * pitch, torch.uint8, stream)
         q = Act8Matrix.__new__(Act8Matrix)
         q.rows, q.cols, q._where = rows, cols, buf
         q._codes = q._exps = None
@@ -1101,14 +1127,7 @@ class MoeBalance:
         calls = _cuda or _cuda_calls()
         if calls is None:
             raise GemmkitError(GK_ENODEV, "gemmkit: no CUDA device")
-        torch = calls[0]
-        device = torch.device("cuda", calls[1]())
-        n = 3 * experts + 2
-        if stream is None:
-            buf = torch.empty(n, dtype=torch.int32, device=device)
-        else:  # not what the current stream may still be writing
-            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
-                buf = torch.empty(n, dtype=torch.int32, device=device)
+        buf = _buffer(3 * experts + 2, calls[0].int32, stream)
         b = MoeBalance.__new__(MoeBalance)
         b.experts, b._where, b._parts = experts, buf, None
         at = buf.data_ptr()

@@ -423,6 +423,16 @@ __device__ __forceinline__ void epi_columns(const EpiArgs& e, void* c, int out_t
     }
 }
 
+// A column's sum to element `at` of the sums.
+__device__ __forceinline__ void store_sum(const EpiArgs& e, int64_t at, float y) {
+    if (e.bias_type == GK_F32)
+        to_out(static_cast<float*>(e.dbias) + at, y);
+    else if (e.bias_type == GK_F16)
+        to_out(static_cast<__half*>(e.dbias) + at, y);
+    else
+        to_out(static_cast<__nv_bfloat16*>(e.dbias) + at, y);
+}
+
 // The bias of this lane's P row.
 __device__ __forceinline__ float epi_bias(const EpiArgs& e, int g, int i0, int pn, int lane) {
     if (!e.bias || lane >= pn) return 0.0f;
