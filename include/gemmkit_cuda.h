@@ -99,7 +99,7 @@ const char *gk_version(void);
 const char *gk_last_error(void);
 /* Read (and with clear != 0 reset) the device status word of `device`. GK_STATUS_OFFSETS means a
  * grouped call's offsets did not ascend inside its rows (the call ran on the offsets made safe,
- * see gk_gemm_half_grouped); any other bit that a bounded in-kernel wait gave up (GK_ETIMEOUT).
+ * see gk_gemm_half_grouped), or that a router's id named no expert (gk_moe_balance); any other bit that a bounded in-kernel wait gave up (GK_ETIMEOUT).
  * Synchronizes the device. */
 #define GK_STATUS_OFFSETS (1u << 5)
 int gk_device_status(int device, int clear, uint32_t *status);

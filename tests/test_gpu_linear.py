@@ -458,6 +458,27 @@ def test_act_backward_strides_and_places():
     assert torch.equal(odd, want)
 
 
+def test_broadcast_rows():
+    """R, z and dY whose rows are all the same memory (row stride 0), as a sum's gradient arrives."""
+    torch = torch_cuda()
+    for rows, k, n in ((70, 48, 66), (2048, 64, 4096)):
+        a, b, _, _ = problem(None, rows, k, n, "bf16", "n", 35)
+        one = numbers(38, (1, n), "bf16")
+        many = one.expand(rows, n)
+        row = gk.MatRef(one.reshape(-1), rows, n, 0, 1)
+        c0 = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+        c = c0.clone()
+        bv, gs = stack_ref(b)
+        gk.gemm_half_epilogue(1.0, ref(a), bv, mut(c), act=act_of("relu"), residual=row)
+        check_forward(a, b, None, "bf16", "relu", None, many, c, None, c0, None, exact=True)
+        gk.gemm_half_dact(1.0, ref(a), bv, row, act_of("relu"), mut(c))
+        d, mag = product64(a, b, None)
+        check_backward(d, 0 * mag, many.double(), None, "bf16", "relu", c, c0, None, exact=True)
+        dbias = torch.empty(n, device="cuda")
+        gk.act_backward(row, ref(c), None, None, dbias=dbias)
+        assert torch.equal(dbias.double(), rows * one[0].double())
+
+
 def test_derivatives_at_special_values():
     torch = torch_cuda()
     inf = float("inf")
