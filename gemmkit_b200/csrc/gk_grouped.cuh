@@ -267,21 +267,21 @@ __device__ __forceinline__ void epi_tile(const GroupedParams& p, const GTile& t,
     float sum = 0.0f;
     auto columns = [&](auto pairs) {
         constexpr bool PAIRS = decltype(pairs)::value;
+        constexpr int N = 32;  // (with 16 the latencies of a block show: 1024 -> 8192 over 8192 rows 164 us, 153)
 #pragma unroll 1
-        for (int c = 0; c < wcols && cbase + c < t.qn; c += 16) {
+        for (int c = 0; c < wcols && cbase + c < t.qn; c += N) {
             const EpiAt at{i0, pn, t.qbase + cbase + c, t.qn - cbase - c};
-            EpiSide<EPI, 16> s;
+            EpiSide<EPI, N> s;
             s.template load<PAIRS>(p.e, at, p.out_type == GK_F32, lane);
-            uint32_t v[16];
+            uint32_t v[N];
             if (t.nk > 0) {
-                tmem_ld_cols16(tb + c, v);
+                tmem_ld_x32(tb + c, v);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = 0u;
+                for (int i = 0; i < N; ++i) v[i] = 0u;
             }
             s.template own<PAIRS>(p.e, lane);
-            epi_columns<EPI, 16, PAIRS>(p.e, p.c, p.out_type, p.ldq, p.ldp, at, v, s, alpha, bias,
-                                        sum, lane);
+            epi_columns<EPI, N, PAIRS>(p.e, p.c, p.out_type, p.ldq, p.ldp, at, v, s, alpha, bias, sum, lane);
         }
     };
     if (p.e.pairs)
@@ -1306,7 +1306,13 @@ int run_planned(GroupedParams p, int64_t gp, int64_t plen, int64_t qrows, cudaSt
     const int64_t waves = ((p.np + 2 * BM - 1) / (2 * BM) * q_tiles + clusters - 1) / clusters;
     const int64_t tall_tiles = (p.np + 4 * BM - 1) / (4 * BM) * q_tiles, rest = tall_tiles % clusters;
     const int64_t half_waves = tall_tiles / clusters * 2 + (rest == 0 ? 0 : 2 * rest <= clusters ? 1 : 2);
-    const bool tall = pair && p.pieces && p.np > 2 * BM && 11 * half_waves <= 12 * waves;
+    // A whole epilogue holds the next tile's second accumulator back (epi_tall): about 11000 to 13000 cycles a
+    // tile forward and 22000 backward, where square tiles cost 184 cycles more a stage of 64. Measured
+    // over 8192 rows, in tall and in square tiles: 1024 -> 8192 with GELU and z kept 172 and 153 us,
+    // 4096 -> 14336 796 and 806, 8192 -> 8192 840 and 915; the gradient 2048 -> 8192 295 and 265,
+    // 4096 -> 14336 835 and 800, 8192 -> 8192 885 and 944.
+    const bool long_enough = EPI == EPI_STORE || plen >= (epi_fwd(EPI) ? 4096 : 8192);
+    const bool tall = pair && long_enough && p.pieces && p.np > 2 * BM && 11 * half_waves <= 12 * waves;
     const int tm = tall ? 4 * BM : pair ? 2 * BM : BM;
     const int64_t tiles = tiles_bound(tm, bn);
     if (tiles > INT32_MAX / 2)
