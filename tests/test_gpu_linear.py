@@ -181,6 +181,28 @@ def test_forward_pairs(sizes, rows, k, n, out, act):
     assert torch.equal(c, again)
 
 
+# long contractions: tall tiles, whole and ragged
+TALL = [(None, 2047, 4096, "bf16"), ([700, 0, 1500, 257], 2460, 4098, "f16"), (None, 2048, 4102, "bf16")]
+
+
+@pytest.mark.parametrize("sizes,rows,n,dtype", TALL)
+@pytest.mark.parametrize("act", ["none", "leaky", "silu"])
+def test_forward_tall(sizes, rows, n, dtype, act):
+    torch = torch_cuda()
+    k, exact = 4168, act != "silu"
+    a, b, off, groups = problem(sizes, rows, k, n, dtype, "k" if act == "none" else "n", 26, exact)
+    bias = numbers(27, (groups, n), dtype, exact)
+    r = numbers(28, (rows, n), dtype, exact)
+    c0 = torch.full((rows, n), 7.0, dtype=tdt(dtype), device="cuda")
+    c, z = c0.clone(), c0.clone()
+    forward(a, b, off, dtype, act, bias, r, c, z)
+    check_forward(a, b, off, dtype, act, bias, r, c, z, c0, c0, exact=exact)
+    onto = r.clone()  # C is the residual itself
+    forward(a, b, off, dtype, act, bias, onto, onto)
+    live = in_groups(off, rows)
+    assert torch.equal(onto[live], c[live]) and torch.equal(onto[~live], r[~live])
+
+
 # few tiles and a long contraction: clusters that share a tile, of 8, 4 and 2 CTAs
 SHARED = [(None, 1, 4096, 300), (None, 17, 1000, 264), (None, 33, 2050, 512), (None, 100, 600, 1100),
           (None, 128, 4100, 7000), ([3, 0, 20, 9], 40, 777, 250), ([70, 58], 128, 1030, 1024)]
@@ -373,6 +395,28 @@ def test_backward_pairs(sizes, rows, k, n, out, act, zform):
     backward(a, b, off, dtype, q, act, c, dbias)
     d, mag = product64(a, b, off)
     check_backward(d, (k + 36) * 2.0 ** -23 * mag, z64, off, dtype, act, c, c0, dbias, out, exact)
+    again = torch.empty_like(dbias)
+    backward(a, b, off, dtype, q, act, c, again)
+    assert torch.equal(dbias, again)
+
+
+@pytest.mark.parametrize("sizes,rows,n,dtype", TALL)
+@pytest.mark.parametrize("act,zform", [("none", None), ("relu", "act8"), ("gelu", "half"), ("gelu_tanh", "act8")])
+def test_backward_tall(sizes, rows, n, dtype, act, zform):
+    torch = torch_cuda()
+    k, exact = 8200, act in ("none", "relu")
+    a, b, off, groups = problem(sizes, rows, k, n, dtype, "k" if act == "relu" else "n", 86, exact)
+    if exact:  # sums over k and the rows stay below 2^24
+        a = a.clamp(-1, 1)
+    z = numbers(87, (rows, n), dtype, exact, 2.0)
+    q = {"act8": lambda: gk.quantize_act8(ref(z)), "half": lambda: z, None: lambda: None}[zform]()
+    z64 = act8_values(q) if zform == "act8" else z.double()
+    c0 = torch.full((rows, n), 7.0, dtype=tdt(dtype), device="cuda")
+    c = c0.clone()
+    dbias = torch.empty(groups, n, dtype=torch.float32, device="cuda")
+    backward(a, b, off, dtype, q, act, c, dbias)
+    d, mag = product64(a, b, off)
+    check_backward(d, (k + 36) * 2.0 ** -23 * mag, z64, off, dtype, act, c, c0, dbias, exact=exact)
     again = torch.empty_like(dbias)
     backward(a, b, off, dtype, q, act, c, again)
     assert torch.equal(dbias, again)
