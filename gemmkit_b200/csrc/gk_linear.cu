@@ -400,6 +400,10 @@ int take_bwd(const gk_epilogue_bwd* d, int is_f16, size_t groups, const gk_matmu
     } else if (d->act != GK_ACT_NONE) {
         return api_err(GK_EINVAL, "gemmkit: null z");
     }
+    if (d->act == GK_ACT_NONE) {  // act' is 1: z is not read
+        e->side = nullptr;
+        e->z8 = Act8View{nullptr, nullptr, 0, 0};
+    }
     if (d->dbias) {
         if ((rc = check_vector(d->dbias, d->dbias_len, d->dbias_gs, d->dbias_type, groups, c.cols, is_f16,
                                true, "dbias")))

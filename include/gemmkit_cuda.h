@@ -472,7 +472,7 @@ int gk_dequantize_act8(const gk_act8_matrix *q, gk_matmut out, int out_type, gk_
 
 /* What the backward pass of such a layer needs besides the products: act'(z), with z in 16 bits (rows x n,
  * the operands' type), or in 8 bits (z8 != NULL; z is then not looked at), or nothing for
- * GK_ACT_NONE (z.data NULL); and the bias's gradient, the sums over each group's rows, n elements
+ * GK_ACT_NONE (z.data NULL; a z that is given is not read); and the bias's gradient, the sums over each group's rows, n elements
  * a group, dbias_gs apart, f32 or the operands' type (NULL: not wanted). The sums are of the f32
  * values, in f32 over a tile's rows and in f64 over the tiles, in an order that only the sizes set:
  * they repeat bit for bit. An empty group's are 0. act' is the limit at infinities; ReLU's is 0 and
