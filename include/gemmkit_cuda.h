@@ -491,8 +491,8 @@ typedef struct {
 /* C[i, :] <- alpha * A[i, :] * B[g] * act'(z[i, :]): the gradient by z of the layer before, A the
  * gradient that reaches this layer's output and B its weights viewed transposed; dbias[g] the sums
  * of C (before its rounding) over the group's rows. C may be z itself, the same view. Everything
- * else as in gk_gemm_half_epilogue; the sums take scratch of 4 bytes for each 64 or more elements
- * of C. */
+ * else as in gk_gemm_half_epilogue; the sums take scratch of 4 bytes for each 64 to 128 elements of a
+ * large C (for each 4 at least of one of few tiles; none where up to 16 rows form one group). */
 int gk_gemm_half_dact(int is_f16, size_t groups, const int32_t *offsets, float alpha, gk_matref a,
                       gk_matref b, ptrdiff_t b_gs, const gk_epilogue_bwd *epi, gk_matmut c,
                       int out_type, gk_parallelism par, gk_stream_t stream);
