@@ -5,9 +5,10 @@
 //   rates_e = coef E f_e / live
 //
 // Bound by memory: the logits are read once in each direction. A few lanes take a token, its logits in
-// registers, and in the forward pass add its p to sums that stay in registers over all of their tokens; counts are integers in shared memory. Each block leaves its sums
-// and counts, a last block adds them (one block does all of it where there are few tokens). No
-// floating atomics: which token a warp takes depends on the sizes (and the SMs) alone, and so does every sum.
+// registers, and in the forward pass add its p to sums that stay in registers over all of their tokens;
+// counts are integers in shared memory. Each block leaves its sums and counts, and a second kernel adds
+// them (one block does all of it where there are few tokens). No floating atomics: which token a warp
+// takes depends on the sizes (and the SMs) alone, and so does every sum.
 // Differences of logits go through the fast exponential (2^-22, and 2^-24 of the difference: the large p
 // come from small differences), sums over blocks through f64.
 #include <cuda_bf16.h>
